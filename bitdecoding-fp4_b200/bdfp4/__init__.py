@@ -50,6 +50,10 @@ EXPORTS = (
     "bdfp4_peer_close",
     "bdfp4_peer_free",
     "bdfp4_exchange_merge",
+    "bdfp4_tree_workspace_bytes",
+    "bdfp4_tree_decode",
+    "bdfp4_verify_drafts",
+    "bdfp4_commit_drafts",
 )
 
 
@@ -178,6 +182,78 @@ class ExchangeArgs(Structure):
     ]
 
 
+class TreeArgs(Structure):
+    """``struct bdfp4_tree_args``."""
+
+    _fields_ = [
+        ("rows", c_int32), ("nodes", c_int32), ("heads_q", c_int32), ("heads_kv", c_int32),
+        ("query", c_void_p), ("query_row_stride", c_int64), ("query_node_stride", c_int64),
+        ("draft_key", c_void_p), ("draft_value", c_void_p),
+        ("draft_key_row_stride", c_int64), ("draft_key_node_stride", c_int64),
+        ("draft_value_row_stride", c_int64), ("draft_value_node_stride", c_int64),
+        ("parents", c_void_p), ("parents_row_stride", c_int64),
+        ("node_counts", c_void_p),
+        ("key_codes", c_void_p), ("key_scales", c_void_p),
+        ("value_codes", c_void_p), ("value_scales", c_void_p),
+        ("key_codes_pitch", c_int64), ("key_scales_pitch", c_int64),
+        ("value_codes_pitch", c_int64), ("value_scales_pitch", c_int64),
+        ("pages", c_int32), ("page_tokens", c_int32),
+        ("page_table", c_void_p), ("page_table_stride", c_int64), ("max_pages_per_row", c_int32),
+        ("rotate", c_int32),
+        ("seqused_fp4", c_void_p),
+        ("tail_key", c_void_p), ("tail_value", c_void_p), ("tail_slot_stride", c_int64),
+        ("tail_slots", c_int32),
+        ("softmax_scale", c_float),
+        ("tail_slot_ids", c_void_p), ("seqused_residual", c_void_p), ("seqused_sink", c_void_p),
+        ("key_shift", c_void_p),
+        ("key_tensor_scale", c_float), ("value_tensor_scale", c_float),
+        ("out", c_void_p), ("out_row_stride", c_int64), ("out_node_stride", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+        ("error_word", c_void_p),
+    ]
+
+
+class VerifyArgs(Structure):
+    """``struct bdfp4_verify_args``."""
+
+    _fields_ = [
+        ("rows", c_int32), ("nodes", c_int32), ("vocab", c_int32), ("bf16", c_int32),
+        ("target_probs", c_void_p), ("target_row_stride", c_int64), ("target_node_stride", c_int64),
+        ("draft_probs", c_void_p), ("draft_row_stride", c_int64), ("draft_node_stride", c_int64),
+        ("tokens", c_void_p), ("tokens_row_stride", c_int64),
+        ("parents", c_void_p), ("parents_row_stride", c_int64),
+        ("uniforms", c_void_p), ("uniforms_row_stride", c_int64),
+        ("node_counts", c_void_p),
+        ("accepted", c_void_p), ("accepted_counts", c_void_p), ("next_tokens", c_void_p),
+    ]
+
+
+COMMIT_ALL, COMMIT_HEAD, COMMIT_REST = 0, 1, 2
+
+
+class CommitArgs(Structure):
+    """``struct bdfp4_commit_args``."""
+
+    _fields_ = [
+        ("layers", c_int32), ("rows", c_int32), ("nodes", c_int32), ("heads_kv", c_int32),
+        ("draft_key", c_void_p), ("draft_value", c_void_p),
+        ("key_layer_stride", c_int64), ("key_row_stride", c_int64), ("key_node_stride", c_int64),
+        ("value_layer_stride", c_int64), ("value_row_stride", c_int64), ("value_node_stride", c_int64),
+        ("accepted", c_void_p), ("accepted_row_stride", c_int64),
+        ("accepted_counts", c_void_p), ("seq_lens", c_void_p), ("row_to_slot", c_void_p),
+        ("tail_key", c_void_p), ("tail_value", c_void_p),
+        ("tail_layer_stride", c_int64), ("tail_slot_stride", c_int64),
+        ("tail_slots", c_int32), ("sink_tokens", c_int32), ("rotate", c_int32), ("part", c_int32),
+        ("key_shift", c_void_p),
+        ("page_table", c_void_p), ("page_table_stride", c_int64),
+        ("max_pages_per_row", c_int32), ("pages", c_int32), ("page_tokens", c_int32), ("reserved", c_int32),
+        ("new_seq_lens", c_void_p), ("seqused_fp4", c_void_p), ("seqused_residual", c_void_p),
+        ("seqused_sink", c_void_p),
+        ("source_tokens", c_void_p), ("destination_pages", c_void_p),
+        ("error_word", c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -246,6 +322,14 @@ def library() -> ctypes.CDLL:
     lib.bdfp4_exchange_merge.restype = c_int32
     lib.bdfp4_exchange_merge.argtypes = [POINTER(ExchangeArgs), c_void_p]
     lib.bdfp4_mla_combine.argtypes = [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]
+    lib.bdfp4_tree_workspace_bytes.restype = c_int64
+    lib.bdfp4_tree_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32]
+    lib.bdfp4_tree_decode.restype = c_int32
+    lib.bdfp4_tree_decode.argtypes = [POINTER(TreeArgs), c_void_p]
+    lib.bdfp4_verify_drafts.restype = c_int32
+    lib.bdfp4_verify_drafts.argtypes = [POINTER(VerifyArgs), c_void_p]
+    lib.bdfp4_commit_drafts.restype = c_int32
+    lib.bdfp4_commit_drafts.argtypes = [POINTER(CommitArgs), c_void_p]
     lib.bdfp4_decode_split_static.restype = c_int32
     lib.bdfp4_decode_split_static.argtypes = [POINTER(DecodeArgs), c_void_p]
     _lib = lib
@@ -384,6 +468,18 @@ def mla_decode(args: MlaDecodeArgs, stream: int) -> None:
 def mla_combine(partial_out, partial_lse, parts: int, rows: int, heads_q: int, out, stream: int) -> None:
     check("bdfp4_mla_combine",
           library().bdfp4_mla_combine(ptr(partial_out), ptr(partial_lse), parts, rows, heads_q, ptr(out), stream))
+
+
+def tree_decode(args: TreeArgs, stream: int) -> None:
+    check("bdfp4_tree_decode", library().bdfp4_tree_decode(ctypes.byref(args), stream))
+
+
+def verify_drafts(args: VerifyArgs, stream: int) -> None:
+    check("bdfp4_verify_drafts", library().bdfp4_verify_drafts(ctypes.byref(args), stream))
+
+
+def commit_drafts(args: CommitArgs, stream: int) -> None:
+    check("bdfp4_commit_drafts", library().bdfp4_commit_drafts(ctypes.byref(args), stream))
 
 
 def control_step(args: ControlArgs, stream: int) -> None:

@@ -568,6 +568,142 @@ int bdfp4_mla_decode(const bdfp4_mla_decode_args* args, void* stream);
 int bdfp4_mla_combine(const float* partial_out, const float* partial_lse, int32_t parts, int32_t rows,
                       int32_t heads_q, void* out, void* stream);
 
+/*
+ * Speculative decoding over the NVFP4 cache (no counterpart in the reference, whose plugin refuses it:
+ * src/nvfp4_vllm/guards.py): attention of a tree of drafted tokens, verification of the tree against
+ * the target's probabilities, and the accepted path's way into the cache.
+ */
+#define BDFP4_MAX_TREE_NODES 64
+
+/*
+ * Attention of `nodes` drafted tokens per row. Node i sees the row's cache (FP4 pages, BF16 rolling tail,
+ * BF16 sink, as bdfp4_decode sees them) and, among the drafts, itself and its ancestors: parents[i] < i is
+ * the parent's number, anything else makes node i a root. Queries and probabilities are not quantized to
+ * FP4: K and V enter the MMAs exactly (E2M1 x E4M3 fits FP16; tail, sink and drafts keep BF16 values),
+ * probabilities as FP16 (pages) or BF16. `rotate` applies the Hadamard rotation to the queries and to the
+ * draft keys, and `key_shift` (FP32 [heads_kv][128], in the rotated basis) is subtracted from the draft
+ * keys, which are then rounded to BF16: what the cache would hold of them. Rows of node_counts[r] nodes
+ * (0..nodes) leave the output of the nodes behind them as it was. A node that sees nothing gets zeros.
+ */
+typedef struct bdfp4_tree_args {
+  int32_t rows, nodes, heads_q, heads_kv;
+  const void* query;        /* BF16 [rows][nodes][heads_q][128], dense within a node; strides in elements */
+  int64_t query_row_stride, query_node_stride;
+  const void* draft_key;    /* BF16 [rows][nodes][heads_kv][128], dense within a node */
+  const void* draft_value;
+  int64_t draft_key_row_stride, draft_key_node_stride, draft_value_row_stride, draft_value_node_stride;
+  const int32_t* parents;   /* [rows][nodes], row stride in elements (0: one tree for all rows) */
+  int64_t parents_row_stride;
+  const int32_t* node_counts; /* [rows], or null: `nodes` everywhere */
+  const void* key_codes;    /* the four cache regions, as bdfp4_decode takes them (NVFP4) */
+  const void* key_scales;
+  const void* value_codes;
+  const void* value_scales;
+  int64_t key_codes_pitch, key_scales_pitch, value_codes_pitch, value_scales_pitch;
+  int32_t pages, page_tokens; /* page_tokens 128 or 64 (0 means 128) */
+  const int32_t* page_table;
+  int64_t page_table_stride;
+  int32_t max_pages_per_row;
+  int32_t rotate;
+  const int32_t* seqused_fp4;
+  const void* tail_key;     /* BF16 [slots][tail_slot_stride elements], or null: no tail and no sink */
+  const void* tail_value;
+  int64_t tail_slot_stride;
+  int32_t tail_slots;
+  float softmax_scale;
+  const int32_t* tail_slot_ids;
+  const int32_t* seqused_residual;
+  const int32_t* seqused_sink; /* or null */
+  const float* key_shift;   /* or null */
+  float key_tensor_scale, value_tensor_scale; /* of the pages; 0 means 1 */
+  void* out;                /* BF16 [rows][nodes][heads_q][128], dense within a node */
+  int64_t out_row_stride, out_node_stride;
+  void* workspace;          /* bdfp4_tree_workspace_bytes bytes, 16-byte aligned; contents do not matter, and
+                               calls that may overlap on the GPU need one each */
+  int64_t workspace_bytes;
+  int32_t* error_word;
+} bdfp4_tree_args;
+
+int64_t bdfp4_tree_workspace_bytes(int32_t rows, int32_t nodes, int32_t heads_q, int32_t heads_kv);
+int bdfp4_tree_decode(const bdfp4_tree_args* args, void* stream);
+
+/*
+ * Verification of a drafted tree, one walk per row from node 0 (which is already decided). At the current
+ * node n the weights are w = target_probs[n] and their mass W = 1. Its children c (parents[c] == n) are
+ * tried in order: c with token x is accepted when uniforms[c] * q(x) * W < w(x), and the walk moves to c;
+ * refused, it changes the weights. With draft_probs (q = draft_probs[n], the distribution n's children were
+ * drawn from) w becomes max(w / W - q, 0) and W its sum, unless that sum is zero; without (q(x) = 1) w(x)
+ * becomes 0 and W becomes max(W - w(x), 0). When no child is left the row's next token is the first index
+ * whose cumulative w exceeds uniforms[0] times its total (the last index of positive weight if none does;
+ * target_probs[n] stands in when nothing is left of w). Products, sums and quotients are in FP64. A token
+ * outside the vocabulary is never accepted. A row of node_counts 0 gets accepted -1, count 0, token -1.
+ */
+typedef struct bdfp4_verify_args {
+  int32_t rows, nodes, vocab;
+  int32_t bf16;             /* element type of both probability tensors: 0 FP32, 1 BF16 */
+  const void* target_probs; /* [rows][nodes][vocab], dense along the vocabulary; strides in elements */
+  int64_t target_row_stride, target_node_stride;
+  const void* draft_probs;  /* the same, or null */
+  int64_t draft_row_stride, draft_node_stride;
+  const int32_t* tokens;    /* [rows][nodes] */
+  int64_t tokens_row_stride;
+  const int32_t* parents;   /* [rows][nodes] */
+  int64_t parents_row_stride;
+  const float* uniforms;    /* [rows][nodes] in [0, 1): entry c >= 1 tries node c, entry 0 draws the next token */
+  int64_t uniforms_row_stride;
+  const int32_t* node_counts; /* [rows], or null */
+  int32_t* accepted;        /* [rows][nodes]: the accepted path's node numbers from 0 on, then -1 */
+  int32_t* accepted_counts; /* [rows] */
+  int32_t* next_tokens;     /* [rows] */
+} bdfp4_verify_args;
+
+int bdfp4_verify_drafts(const bdfp4_verify_args* args, void* stream);
+
+/*
+ * The accepted path's K/V into the BF16 tail and sink of every layer: accepted node i of row r becomes
+ * token seq_lens[r] + i of the row and goes to row (seq_lens[r] + i) % 128 of its slot, and to row
+ * 128 + seq_lens[r] + i while that token lies in the sink; K is rotated, shifted (FP32
+ * [layers][heads_kv][128]) and rounded to BF16 on the way like the cache's other keys. part BDFP4_COMMIT_ALL
+ * writes every token; BDFP4_COMMIT_HEAD only those that belong to a page the row fills now (all of them
+ * where it fills none), BDFP4_COMMIT_REST the others: between the two a caller seals the filled pages out of
+ * the tail with the work table (source_tokens, destination_pages: [rows * 128 / page_tokens], -1 where the row
+ * fills no page). ALL and HEAD also write the new lengths. A row with a negative slot is left alone (its
+ * lengths are those of seq_lens). A filled page without a valid destination sets BDFP4_DEV_BAD_PAGE.
+ */
+#define BDFP4_COMMIT_ALL 0
+#define BDFP4_COMMIT_HEAD 1
+#define BDFP4_COMMIT_REST 2
+
+typedef struct bdfp4_commit_args {
+  int32_t layers, rows, nodes, heads_kv;
+  const void* draft_key;    /* BF16 [layers][rows][nodes][heads_kv][128], dense within a node; strides in elements */
+  const void* draft_value;
+  int64_t key_layer_stride, key_row_stride, key_node_stride;
+  int64_t value_layer_stride, value_row_stride, value_node_stride;
+  const int32_t* accepted;  /* [rows][nodes] node numbers */
+  int64_t accepted_row_stride;
+  const int32_t* accepted_counts; /* [rows], 0..nodes */
+  const int32_t* seq_lens;  /* [rows], before the step */
+  const int32_t* row_to_slot; /* [rows] */
+  void* tail_key;           /* BF16 [layers][slots][128 + sink_tokens][heads_kv][128] */
+  void* tail_value;
+  int64_t tail_layer_stride, tail_slot_stride;
+  int32_t tail_slots, sink_tokens, rotate, part;
+  const float* key_shift;
+  const int32_t* page_table; /* or null: no page is sealed */
+  int64_t page_table_stride;
+  int32_t max_pages_per_row, pages, page_tokens, reserved;
+  int32_t* new_seq_lens;    /* [rows] each */
+  int32_t* seqused_fp4;
+  int32_t* seqused_residual;
+  int32_t* seqused_sink;
+  int32_t* source_tokens;   /* or null without page_table */
+  int32_t* destination_pages;
+  int32_t* error_word;
+} bdfp4_commit_args;
+
+int bdfp4_commit_drafts(const bdfp4_commit_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
