@@ -77,9 +77,10 @@ static bool encode_cache_maps(EncodeTiledFn encode, const CacheMapKey& c, CUtens
   return true;
 }
 
-static bool cached_cache_maps(EncodeTiledFn encode, const void* key_codes, const void* value_codes, int heads_kv,
-                              int page_tokens, int pages, int64_t key_pitch, int64_t value_pitch, CUtensorMap* k_map,
-                              CUtensorMap* v_map) {
+bool cache_tensor_maps(const void* key_codes, const void* value_codes, int heads_kv, int page_tokens, int pages,
+                       int64_t key_pitch, int64_t value_pitch, CUtensorMap* k_map, CUtensorMap* v_map) {
+  EncodeTiledFn encode = encode_tiled();
+  if (!encode) return false;
   // A tensor map holds a device address, which means the same thing in every context of the
   // process's unified address space, so the device is not part of the key.
   static thread_local CacheMapEntry entries[kCacheMapEntries];
@@ -157,14 +158,13 @@ extern "C" int bdfp4_decode(const bdfp4_decode_args* a, void* stream_handle) {
   } else if (!a->partial_out || !a->partial_lse) {
     return BDFP4_E_ARG;
   }
-  EncodeTiledFn encode = encode_tiled();
-  if (!encode) return BDFP4_E_CUDA;
+  if (!encode_tiled()) return BDFP4_E_CUDA;
 
   // The two tensor maps depend only on the cache regions and their geometry, which a serving layer
   // keeps for its whole life: they are encoded once per distinct cache and looked up afterwards.
   CUtensorMap k_map, v_map;
-  if (!cached_cache_maps(encode, a->key_codes, a->value_codes, a->heads_kv, page_tokens, a->pages,
-                         a->key_codes_pitch, a->value_codes_pitch, &k_map, &v_map))
+  if (!cache_tensor_maps(a->key_codes, a->value_codes, a->heads_kv, page_tokens, a->pages, a->key_codes_pitch,
+                         a->value_codes_pitch, &k_map, &v_map))
     return BDFP4_E_ARG;
 
   DecodeParams p{};

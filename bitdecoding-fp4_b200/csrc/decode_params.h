@@ -56,6 +56,11 @@ struct DecodeParams {
   const int32_t* row_splits;  // parts per row (1..num_splits), or null: num_splits for every row
 };
 
+// The tensor maps of a cache's K and V codes (128-token pages; the maps of 64-token pages are encoded but not
+// read): encoded once per distinct cache and host thread, looked up afterwards. False when encoding fails.
+bool cache_tensor_maps(const void* key_codes, const void* value_codes, int heads_kv, int page_tokens, int pages,
+                       int64_t key_pitch, int64_t value_pitch, CUtensorMap* k_map, CUtensorMap* v_map);
+
 // One launch of decode_kernel<GP, TERMS, STAGES, PT, MX> with GP the smallest of 4, 8, 16 that holds
 // `p.ratio` query heads per KV head, TERMS = 2 when `two_terms`, and the ring depth chosen from the
 // grid size. Defined in decode_nvfp4_p128.cu, decode_nvfp4_p64.cu and decode_mxfp4.cu.
