@@ -37,25 +37,47 @@ namespace tree {
 
 constexpr int kStage = 18432;  // K codes 8192, V codes 8192, K scales 1024, V scales 1024
 constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
-constexpr int kDraftPitch = 272;  // bytes per staged draft key: 16-byte chunks of 8 rows on distinct banks
+// A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
+// 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
+constexpr int kBf16Pitch = 272, kBf16Rows = 64;
+// Named barriers: one per softmax group (four at most), all softmax threads, the key threads.
+constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kKeysBarrier = 6;
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
 constexpr float kGrowth = 8.0f;     // a maximum is renewed when a score exceeds it by more than this (log2)
 
+// A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (128
+// threads for NT = 64, 256 for 128) the kernel spilled, into an L1 that shared memory has left 24 KB of.
 template <int NT>
 struct Shape {
-  static constexpr int kGroups = NT > 64 ? 2 : 1;           // softmax groups of 128 threads, NT / kGroups queries each
-  static constexpr int kColumns = NT / kGroups;             // queries per softmax thread
+  static constexpr int kColumns = NT < 32 ? NT : 32;        // queries per softmax thread
+  static constexpr int kGroups = NT / kColumns;             // softmax groups of 128 threads
   static constexpr int kBlocks = (NT + 63) / 64;            // 128-byte rows of P per token
   static constexpr int kKBuffers = NT > 96 ? 1 : 2;         // operand buffers in tensor memory, as many as it holds
   static constexpr int kVBuffers = NT > 64 ? 1 : 2;
   static constexpr int kStages = NT > 96 ? 5 : NT > 64 ? 6 : 8;
   static constexpr int kSoftmaxThreads = 128 * kGroups;
-  static constexpr int kThreads = 256 + kSoftmaxThreads + 64;
+  static constexpr int kThreads = 256 + kSoftmaxThreads + 128;  // keys, values, softmax, control (two of its warps idle)
+  // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
+  // must not exceed what the launch was given.
+  static constexpr int kLaunchRegs = kGroups == 4 ? 72 : kGroups == 3 ? 80 : kGroups == 2 ? 96 : 128;
+  static constexpr int kSoftmaxRegs = kGroups == 4 ? 80 : kGroups == 3 ? 96 : kGroups == 2 ? 112 : 144;
+  static constexpr int kKeyRegs = kGroups == 4 ? 80 : kGroups == 3 ? 88 : kGroups == 2 ? 112 : 152;
+  static constexpr int kValueRegs = kGroups == 4 ? 64 : kGroups == 3 ? 64 : kGroups == 2 ? 88 : 128;
+  static constexpr int kControlRegs = kGroups == 4 ? 40 : kGroups == 3 ? 40 : kGroups == 2 ? 56 : 88;
+  static_assert(kSoftmaxRegs * kGroups + kKeyRegs + kValueRegs + kControlRegs <= kLaunchRegs * (3 + kGroups), "registers");
+  static_assert(kLaunchRegs * kThreads <= 65536, "registers");
+  static constexpr bool kHold = kGroups <= 2;  // a thread's scores stay in registers between the vote and the exponentials
   // tensor memory columns
   static constexpr int kS = 0, kO = 2 * NT, kK = 3 * NT, kV = kK + 64 * kKBuffers;
   static_assert(kV + 64 * kVBuffers <= 512, "tensor memory");
 };
+
+template <int FROM, int TO>
+__device__ __forceinline__ void trade_registers() {
+  if constexpr (TO > FROM) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TO));
+  if constexpr (TO < FROM) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
+}
 
 template <int NT>
 struct Smem {
@@ -63,7 +85,6 @@ struct Smem {
   alignas(1024) uint8_t ring[Sh::kStages][kStage];
   alignas(1024) uint8_t q[2][NT * 128];  // two halves of 64 channels, K-major, 128-byte swizzle
   alignas(1024) uint8_t p[2][Sh::kBlocks * 16384];  // MN-major: 128-byte rows of 64 queries per token, swizzled
-  alignas(16) uint8_t draft[BDFP4_MAX_TREE_NODES * kDraftPitch];
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
@@ -72,13 +93,13 @@ struct Smem {
   float col_max[4][NT];
   float col_sum[4][NT];
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
-  float q_max[8];
+  float q_max[16];
   int parents[BDFP4_MAX_TREE_NODES];
   uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
   uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];
   uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
   uint64_t q_full, o_full, o_empty, drained;
-  long long sums[32];
+  long long sums[Sh::kThreads / 32];
   int start_row;
   long long start_offset, first, last, per_cta;
   uint32_t tmem;
@@ -126,14 +147,12 @@ __host__ __device__ constexpr uint32_t f16_idesc(int n, int format, bool b_mn_ma
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void st32(uint32_t address, const uint32_t* v) {
+__device__ __forceinline__ void st16(uint32_t address, const uint32_t* v) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(address),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::
+          "r"(address),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 
@@ -217,45 +236,42 @@ enum StepKind { kStepPage, kStepTail, kStepDraft };
 __device__ __forceinline__ StepKind step_kind(const RowInfo& r, int step) {
   return step < r.pages ? kStepPage : (step == r.pages && r.residual > 0) ? kStepTail : kStepDraft;
 }
+// Token places of a BF16 step: the tail's tokens, or 16 places of the sink and the drafts behind them.
+__device__ __forceinline__ int bf16_places(const RowInfo& r, StepKind kind) {
+  return kind == kStepTail ? r.residual : BDFP4_MAX_SINK + r.count;
+}
 // 16-token slices of a step that hold anything.
 __device__ __forceinline__ int step_slices(const RowInfo& r, StepKind kind) {
-  return kind == kStepPage ? 8 : kind == kStepTail ? (r.residual + 15) / 16 : 1 + (r.count + 15) / 16;
+  return kind == kStepPage ? 8 : (bf16_places(r, kind) + 15) / 16;
 }
 
-// The units of this CTA in order; every role walks them on its own.
+// The units of this CTA in order; every role walks them on its own. Steps are counted in 32 bits within a
+// row (the host refuses larger rows).
 struct Walker {
   const TreeParams& p;
-  int row, page_tokens;
-  long long offset, left;
-  bool loaded;
-  RowInfo info;
-  __device__ Walker(const TreeParams& params, int start_row, long long start_offset, long long steps, int pt)
-      : p(params), row(start_row), page_tokens(pt), offset(start_offset), left(steps), loaded(false) {}
-  __device__ bool next(Unit& u) {
-    while (left > 0 && row < p.rows) {
-      if (!loaded) {
-        info = row_info(p, row, page_tokens);
-        loaded = true;
-      }
-      const long long whole = (long long)info.steps * info.tiles * p.heads_kv;
-      if (offset >= whole) {
-        offset -= whole;
-        ++row;
-        loaded = false;
-        continue;
-      }
-      const int unit = (int)(offset / info.steps);
-      u.info = info;
-      u.row = row;
-      u.head = unit / info.tiles;
-      u.tile = unit % info.tiles;
-      u.begin = (int)(offset % info.steps);
-      u.end = (int)min((long long)info.steps, u.begin + left);
-      left -= u.end - u.begin;
-      offset += u.end - u.begin;
-      return true;
+  int row, page_tokens, offset, left;
+  __device__ Walker(const TreeParams& params, int start_row, int start_offset, int steps, int pt)
+      : p(params), row(start_row), page_tokens(pt), offset(start_offset), left(steps) {}
+  // `known`: u is a unit of this walk, so its row's lengths need not be read again.
+  __device__ __forceinline__ bool next(Unit& u, bool known) {
+    if (left <= 0) return false;
+    while (true) {
+      if (!known || u.row != row) u.info = row_info(p, row, page_tokens);
+      const int whole = u.info.steps * u.info.tiles * p.heads_kv;
+      if (offset < whole) break;
+      offset -= whole;
+      known = false;
+      if (++row >= p.rows) return false;
     }
-    return false;
+    const int unit = offset / u.info.steps;
+    u.row = row;
+    u.head = unit / u.info.tiles;
+    u.tile = unit - u.head * u.info.tiles;
+    u.begin = offset - unit * u.info.steps;
+    u.end = min(u.info.steps, u.begin + left);
+    left -= u.end - u.begin;
+    offset += u.end - u.begin;
+    return true;
   }
 };
 
@@ -266,11 +282,16 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
                                         const CUtensorMap* v_map, int lane) {
   using Sh = Shape<NT>;
   constexpr int kEntries = kPage / PT;
-  int slot = 0;
+  const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
+  int slot = 0, issued = 0;
   uint32_t turn = 0;
-  int issued = 0;
+  auto advance = [&] {
+    ++issued;
+    if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+  };
   Unit u;
-  while (walker.next(u)) {
+  bool known = false;
+  for (; walker.next(u, known); known = true) {
     const int32_t* table = p.table + u.row * p.table_stride;
     const int stop = min(u.end, u.info.pages);
     for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
@@ -310,10 +331,40 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
                             &sm.full_v[slot]);
             }
           }
-          ++issued;
         }
         __syncwarp();
-        if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+        advance();
+      }
+    }
+    for (int step = max(u.begin, u.info.pages); step < u.end; ++step) {
+      const StepKind kind = step_kind(u.info, step);
+      const int places = bf16_places(u.info, kind);
+      for (int side = 0; side < 2; ++side) {
+        const __nv_bfloat16* tail = (side ? p.tail_value : p.tail_key) + u.info.slot * p.tail_slot + u.head * kHeadDim;
+        const __nv_bfloat16* draft = side ? p.draft_value + u.row * p.draft_value_row + u.head * kHeadDim
+                                          : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
+        const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
+        for (int first = 0; first < places; first += kBf16Rows) {
+          const int end = min(first + kBf16Rows, places);
+          uint64_t* full = side ? &sm.full_v[slot] : &sm.full_k[slot];
+          if (lane == 0) {
+            tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+            // the sink's places behind its length stay empty
+            const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
+            tc::mbar_expect_tx(full, (end - first - absent) * 256);
+            tc::mbar_arrive(side ? &sm.full_k[slot] : &sm.full_v[slot]);  // the other side only passes the stage on
+          }
+          __syncwarp();
+          for (int i = first + lane; i < end; i += 32) {
+            const __nv_bfloat16* source = nullptr;
+            if (kind == kStepTail) source = tail + i * tail_row;
+            else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
+            else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
+            if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, full);
+          }
+          __syncwarp();
+          advance();
+        }
       }
     }
   }
@@ -337,7 +388,8 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p);
   int n = 0, unit = 0;
   Unit u;
-  while (walker.next(u)) {
+  bool known = false;
+  for (; walker.next(u, known); known = true) {
     auto output = [&](int step, int j) {  // O^T += V^T P^T of step `step` of the unit, the CTA's j-th
       const StepKind kind = step_kind(u.info, step);
       const int slices = step_slices(u.info, kind);
@@ -377,25 +429,45 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   tc::mbar_wait(&sm.drained, 0, &ignore);
 }
 
-// Sixteen code words (128 values) and the scales of their eight groups, in four passes of two groups.
+// Sixteen code words (128 values) and the scales of their eight groups.
 __device__ __forceinline__ void store_dequantized(uint32_t a, const uint4* chunk, uint32_t scales0, uint32_t scales1) {
-  __half2 scale[8];
-  scale_pairs(scales0, scale);
-  scale_pairs(scales1, scale + 4);
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t v[32];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint4 c = chunk[2 * half + j];
-      dequantize8(c.x, scale[4 * half + 2 * j], v + 16 * j);
-      dequantize8(c.y, scale[4 * half + 2 * j], v + 16 * j + 4);
-      dequantize8(c.z, scale[4 * half + 2 * j + 1], v + 16 * j + 8);
-      dequantize8(c.w, scale[4 * half + 2 * j + 1], v + 16 * j + 12);
-    }
-    st32(a + 32 * half, v);
+  for (int j = 0; j < 4; ++j) {
+    __half2 scale[4];
+    scale_pairs(j < 2 ? scales0 : scales1, scale);
+    uint32_t v[16];
+    dequantize8(chunk[j].x, scale[2 * (j & 1)], v);
+    dequantize8(chunk[j].y, scale[2 * (j & 1)], v + 4);
+    dequantize8(chunk[j].z, scale[2 * (j & 1) + 1], v + 8);
+    dequantize8(chunk[j].w, scale[2 * (j & 1) + 1], v + 12);
+    st16(a + 16 * j, v);
   }
 }
+
+// One side of the ring as its consumers (four warps) see it.
+template <int NT>
+struct Ring {
+  Smem<NT>& sm;
+  uint64_t* full;
+  int lane, slot;
+  uint32_t turn;
+  __device__ Ring(Smem<NT>& s, uint64_t* f, int l) : sm(s), full(f), lane(l), slot(0), turn(0) {}
+  __device__ __forceinline__ const uint8_t* wait() {
+    tc::mbar_wait(&full[slot], turn, &sm.abort_flag);
+    return sm.ring[slot];
+  }
+  __device__ __forceinline__ void release() {
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
+    if (++slot == Shape<NT>::kStages) slot = 0, turn ^= 1;
+  }
+  __device__ __forceinline__ void pass(int stages) {
+    for (int i = 0; i < stages; ++i) {
+      wait();
+      release();
+    }
+  }
+};
 
 // Keys: thread t holds token t of every step.
 template <int NT, int PT>
@@ -403,18 +475,18 @@ __device__ __forceinline__ void keys(const TreeParams& p, Smem<NT>& sm, Walker w
   using Sh = Shape<NT>;
   const int lane = t & 31;
   const uint32_t tmem = sm.tmem + Sh::kK + ((uint32_t)(t & ~31) << 16);
-  const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
-  int slot = 0, n = 0;
-  uint32_t turn = 0;
+  Ring<NT> ring(sm, sm.full_k, lane);
+  int n = 0;
   Unit u;
-  while (walker.next(u)) {
+  bool known = false;
+  for (; walker.next(u, known); known = true) {
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const int a = n % Sh::kKBuffers;
+      const uint32_t operand = tmem + (n % Sh::kKBuffers) * 64;
+      uint64_t* operand_empty = &sm.ka_empty[n % Sh::kKBuffers];
       const uint32_t empty_parity = ((n / Sh::kKBuffers) & 1) ^ 1;
       if (kind == kStepPage) {
-        tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);
-        const uint8_t* stage = sm.ring[slot];
+        const uint8_t* stage = ring.wait();
         uint4 chunk[4];
         const uint8_t* row = stage + t * 64;
 #pragma unroll
@@ -423,78 +495,89 @@ __device__ __forceinline__ void keys(const TreeParams& p, Smem<NT>& sm, Walker w
                                       : stage + kKsOffset + (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4;
         const uint32_t s0 = *reinterpret_cast<const uint32_t*>(at);
         const uint32_t s1 = *reinterpret_cast<const uint32_t*>(at + (PT == 128 ? 512 : 256));
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
-        if (++slot == Sh::kStages) slot = 0, turn ^= 1;
-        tc::mbar_wait(&sm.ka_empty[a], empty_parity, &sm.abort_flag);
+        ring.release();
+        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-        store_dequantized(tmem + a * 64, chunk, s0, s1);
+        store_dequantized(operand, chunk, s0, s1);
       } else {
-        // BF16 rows: the rolling tail, or the sink (16 places) and the drafts behind it
-        const uint4* source = nullptr;
-        bool staged = false;
-        if (kind == kStepTail) {
-          if (t < u.info.residual)
-            source = reinterpret_cast<const uint4*>(p.tail_key + u.info.slot * p.tail_slot + t * tail_row + u.head * kHeadDim);
-        } else {
-          staged = p.rotate || p.key_shift;
-          if (t < BDFP4_MAX_SINK) {
-            if (t < u.info.sink)
-              source = reinterpret_cast<const uint4*>(p.tail_key + u.info.slot * p.tail_slot + (kPage + t) * tail_row +
-                                                      u.head * kHeadDim);
-          } else if (t - BDFP4_MAX_SINK < u.info.count) {
-            const int node = t - BDFP4_MAX_SINK;
-            source = staged ? reinterpret_cast<const uint4*>(sm.draft + node * kDraftPitch)
-                            : reinterpret_cast<const uint4*>(p.draft_key + u.row * p.draft_key_row + node * p.draft_key_node +
-                                                             u.head * kHeadDim);
-          }
-          if (staged) {  // eight threads bring one draft key into the cache's basis
-            bar_sync(4, 128);  // the last unit's keys have been read
+        const int places = bf16_places(u.info, kind);
+        const int stages = (places + kBf16Rows - 1) / kBf16Rows;
+        // a step's stages are held together; both have arrived when each has been waited for
+        ring.wait();
+        uint8_t* const stage0 = sm.ring[ring.slot];
+        uint8_t* stage1 = stage0;
+        if (stages > 1) {
+          const bool wraps = ring.slot + 1 == Sh::kStages;
+          const int next = wraps ? 0 : ring.slot + 1;
+          tc::mbar_wait(&sm.full_k[next], ring.turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
+          stage1 = sm.ring[next];
+        }
+        auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
+        bool there = t < places;
+        if (kind == kStepDraft) {
+          if (t < BDFP4_MAX_SINK) there = t < u.info.sink;
+          if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
             const int group = t & 7;
+            const int64_t shift_at = u.head * kHeadDim + group * kGroup;
             for (int first = 0; first < u.info.count; first += 16) {
-              const int node = first + (t >> 3);
-              const int64_t shift_at = u.head * kHeadDim + group * kGroup;
+              // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
+              const int node = min(first + (t >> 3), u.info.count - 1);
+              uint4* at = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + node) + group * 32);
+              const uint4 raw[2] = {at[0], at[1]};
+              const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
               float v[16];
-              load_bf16x16(p.draft_key + u.row * p.draft_key_row + min(node, u.info.count - 1) * p.draft_key_node +
-                               u.head * kHeadDim + group * kGroup, v);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+              }
               if (p.rotate && p.key_shift) cache_basis16<BDFP4_SHIFT_F32, true>(v, group, p.key_shift, shift_at);
               else if (p.rotate) cache_basis16<BDFP4_SHIFT_NONE, true>(v, group, nullptr, 0);
               else cache_basis16<BDFP4_SHIFT_F32, false>(v, group, p.key_shift, shift_at);
-              if (node < u.info.count)
-                store_bf16x16(reinterpret_cast<__nv_bfloat16*>(sm.draft + node * kDraftPitch) + group * kGroup, v);
+              if (first + (t >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
             }
-            bar_sync(4, 128);
+            tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
+            bar_sync(kKeysBarrier, 128);
           }
         }
-        uint32_t raw[64];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (source) w = source[j];
-          raw[4 * j] = w.x;
-          raw[4 * j + 1] = w.y;
-          raw[4 * j + 2] = w.z;
-          raw[4 * j + 3] = w.w;
-        }
+        const uint4* row = reinterpret_cast<const uint4*>(row_of(min(t, places - 1)));
         float amax = 0.0f;
+        if (there) {
+#pragma unroll 4
+          for (int j = 0; j < 16; ++j) {
+            const uint4 r = row[j];
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int j = 0; j < 64; ++j)
-          amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(raw[j] << 16)), fabsf(__uint_as_float(raw[j] & 0xffff0000u))));
+            for (int i = 0; i < 4; ++i)
+              amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+          }
+        }
         float inverse;
         const float scale = fp16_scale(amax, &inverse);
         sm.key_factor[n & 7][t] = inverse;
-#pragma unroll
-        for (int j = 0; j < 64; ++j)
-          raw[j] = h2(__floats2half2_rn(__uint_as_float(raw[j] << 16) * scale, __uint_as_float(raw[j] & 0xffff0000u) * scale));
-        tc::mbar_wait(&sm.ka_empty[a], empty_parity, &sm.abort_flag);
+        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-        st32(tmem + a * 64, raw);
-        st32(tmem + a * 64 + 32, raw + 32);
+#pragma unroll 1
+        for (int quarter = 0; quarter < 4; ++quarter) {
+          uint32_t v[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint4 r = make_uint4(0, 0, 0, 0);
+            if (there) r = row[quarter * 4 + j];
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
+          }
+          st16(operand + quarter * 16, v);
+        }
+        for (int i = 0; i < stages; ++i) ring.release();
+        ring.pass(stages);  // the values'
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.ka_full[a]);
+      if (lane == 0) tc::mbar_arrive(&sm.ka_full[n % Sh::kKBuffers]);
     }
   }
 }
@@ -505,18 +588,18 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
   using Sh = Shape<NT>;
   const int lane = c & 31;
   const uint32_t tmem = sm.tmem + Sh::kV + ((uint32_t)(c & ~31) << 16);
-  const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
-  int slot = 0, n = 0;
-  uint32_t turn = 0;
+  Ring<NT> ring(sm, sm.full_v, lane);
+  int n = 0;
   Unit u;
-  while (walker.next(u)) {
+  bool known = false;
+  for (; walker.next(u, known); known = true) {
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const int a = n % Sh::kVBuffers;
+      const uint32_t operand = tmem + (n % Sh::kVBuffers) * 64;
+      uint64_t* operand_empty = &sm.va_empty[n % Sh::kVBuffers];
       const uint32_t empty_parity = ((n / Sh::kVBuffers) & 1) ^ 1;
       if (kind == kStepPage) {
-        tc::mbar_wait(&sm.full_v[slot], turn, &sm.abort_flag);
-        const uint8_t* stage = sm.ring[slot];
+        const uint8_t* stage = ring.wait();
         uint4 chunk[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -527,43 +610,38 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
         const uint8_t* at = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
         const uint32_t s0 = *reinterpret_cast<const uint32_t*>(at);
         const uint32_t s1 = *reinterpret_cast<const uint32_t*>(at + 512);
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
-        if (++slot == Sh::kStages) slot = 0, turn ^= 1;
-        tc::mbar_wait(&sm.va_empty[a], empty_parity, &sm.abort_flag);
+        ring.release();
+        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-        store_dequantized(tmem + a * 64, chunk, s0, s1);
+        store_dequantized(operand, chunk, s0, s1);
       } else {
-        tc::mbar_wait(&sm.va_empty[a], empty_parity, &sm.abort_flag);
+        const int places = bf16_places(u.info, kind);
+        ring.pass((places + kBf16Rows - 1) / kBf16Rows);  // the keys'
+        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-        const int slices = step_slices(u.info, kind);
-        const __nv_bfloat16* tail = p.tail_value + u.info.slot * p.tail_slot + u.head * kHeadDim + c;
-        const __nv_bfloat16* draft = p.draft_value + u.row * p.draft_value_row + u.head * kHeadDim + c;
-        for (int s = 0; s < slices; ++s) {
-          uint16_t w[16];
+        for (int first = 0; first < places; first += kBf16Rows) {
+          const uint8_t* stage = ring.wait() + 2 * c;
+          const int slices = (min(places - first, kBf16Rows) + 15) / 16;
+          for (int s = 0; s < slices; ++s) {
+            const int place = first + s * 16;
+            const int stop = kind == kStepDraft && place == 0 ? u.info.sink : places;
+            uint32_t v[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int t = s * 16 + i;
-            const __nv_bfloat16* at = nullptr;
-            if (kind == kStepTail) {
-              if (t < u.info.residual) at = tail + t * tail_row;
-            } else if (s == 0) {
-              if (t < u.info.sink) at = tail + (kPage + t) * tail_row;
-            } else if (t - BDFP4_MAX_SINK < u.info.count) {
-              at = draft + (t - BDFP4_MAX_SINK) * p.draft_value_node;
+            for (int i = 0; i < 8; ++i) {
+              uint32_t lo = 0, hi = 0;
+              if (place + 2 * i < stop) lo = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i) * kBf16Pitch);
+              if (place + 2 * i + 1 < stop) hi = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i + 1) * kBf16Pitch);
+              v[i] = lo | (hi << 16);
             }
-            w[i] = at ? __ldg(reinterpret_cast<const unsigned short*>(at)) : (uint16_t)0;
+            st8(operand + (place >> 4) * 8, v);
           }
-          uint32_t v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = (uint32_t)w[2 * i] | ((uint32_t)w[2 * i + 1] << 16);
-          st8(tmem + a * 64 + s * 8, v);
+          ring.release();
         }
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.va_full[a]);
+      if (lane == 0) tc::mbar_arrive(&sm.va_full[n % Sh::kVBuffers]);
     }
   }
 }
@@ -601,7 +679,7 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
   }
   amax = warp_max(amax);
   if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
-  bar_sync(3, Sh::kSoftmaxThreads);
+  bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);
 #pragma unroll
   for (int w = 0; w < Sh::kSoftmaxThreads / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
   float inverse;
@@ -618,7 +696,7 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
     *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
   }
   tc::fence_proxy_async_smem();
-  bar_sync(3, Sh::kSoftmaxThreads);
+  bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);
   if (thread == 0) tc::mbar_arrive(&sm.q_full);
   return inverse;
 }
@@ -651,14 +729,14 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
   constexpr int C = Sh::kColumns;
   const int t = thread & 127, lane = thread & 31, warp = t >> 5, group = thread >> 7;
   const int first_column = group * C;
-  const int barrier = 1 + group;
+  const int barrier = kGroupBarrier + group;
   const uint32_t lanes = (uint32_t)(t & ~31) << 16;
   float* base = sm.base + first_column;
   float* top = sm.top + first_column;
   int n = 0, unit = 0;
-  Unit u, following;
-  bool more = walker.next(u);
-  if (!more) return;
+  Unit u;
+  if (!walker.next(u, false)) return;
+  bool more = true;
   float q_inverse = load_queries<NT>(p, sm, u, thread);
   while (more) {
     for (int j = t; j < C; j += 128) {
@@ -693,7 +771,6 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       if (kind != kStepPage) f = p.scale_log2 * q_inverse * sm.key_factor[n & 7][t];
       const float2 f2 = make_float2(f, f);
       const uint32_t scores = sm.tmem + Sh::kS + (n & 1) * NT + first_column + lanes;
-      // sixteen scores in log2 units, on top of `add`
       auto load16 = [&](int j, float* s) {
         tc::tmem_ld16(scores + j, s);
         tc::tmem_wait_ld();
@@ -703,20 +780,27 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
             if (!((sm.family[first_column + j + i] >> node) & 1)) s[i] = -INFINITY;
         }
       };
-      bool grows = false;
-#pragma unroll
-      for (int j = 0; j < C; j += 16) {
-        float s[16];
-        load16(j, s);
+      // scores -> log2 units above the maxima, plus kShift
+      auto above16 = [&](int j, float* s) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const float4 b = *reinterpret_cast<const float4*>(base + j + i);
           const float2 y0 = __ffma2_rn(make_float2(s[i], s[i + 1]), f2, make_float2(b.x, b.y));
           const float2 y1 = __ffma2_rn(make_float2(s[i + 2], s[i + 3]), f2, make_float2(b.z, b.w));
-          grows |= fmaxf(fmaxf(y0.x, y0.y), fmaxf(y1.x, y1.y)) > kGrowth + kShift;
+          s[i] = y0.x, s[i + 1] = y0.y, s[i + 2] = y1.x, s[i + 3] = y1.y;
         }
+      };
+      float held[Sh::kHold ? C : 16];
+      float highest = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < C; j += 16) {
+        float* s = Sh::kHold ? held + j : held;
+        load16(j, s);
+        above16(j, s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) highest = fmaxf(highest, s[i]);
       }
-      if (bar_any(barrier, grows && !dead)) {
+      if (bar_any(barrier, highest > kGrowth + kShift && !dead)) {
 #pragma unroll
         for (int j = 0; j < C; j += 16) {
           float s[16];
@@ -748,7 +832,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
         if (step > u.begin) {  // what O^T holds is of the old maxima
           tc::mbar_wait(&sm.p_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, &sm.abort_flag);
           tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < C; j += 16) {
             float o[16];
             const uint32_t at = sm.tmem + Sh::kO + first_column + j + lanes;
@@ -760,31 +844,44 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
           }
           tc::tmem_wait_st();
         }
+        if constexpr (Sh::kHold) {
+#pragma unroll
+          for (int j = 0; j < C; j += 16) {
+            load16(j, held + j);
+            above16(j, held + j);
+          }
+        }
+      }
+      if constexpr (Sh::kHold) {  // the scores are in registers: the next but one may come
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.s_empty[n & 1]);
       }
       // P of this step goes where the one before the last was
       tc::mbar_wait(&sm.p_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
-      const float value_factor = p.inverse_value_scale;
 #pragma unroll
       for (int j = 0; j < C; j += 16) {
-        float s[16];
-        load16(j, s);
+        float* s = Sh::kHold ? held + j : held;
+        if constexpr (!Sh::kHold) {
+          load16(j, s);
+          above16(j, s);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = ex2(s[i]);
+        if (dead) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+        }
         uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(base + j + i);
-          const float2 y0 = __ffma2_rn(make_float2(s[i], s[i + 1]), f2, make_float2(b.x, b.y));
-          const float2 y1 = __ffma2_rn(make_float2(s[i + 2], s[i + 3]), f2, make_float2(b.z, b.w));
-          float2 e0 = make_float2(ex2(y0.x), ex2(y0.y)), e1 = make_float2(ex2(y1.x), ex2(y1.y));
-          if (dead) e0 = e1 = make_float2(0.0f, 0.0f);
-          sum[(j + i) / 2] = __fadd2_rn(sum[(j + i) / 2], e0);
-          sum[(j + i) / 2 + 1] = __fadd2_rn(sum[(j + i) / 2 + 1], e1);
-          if (kind == kStepPage) {
-            w[i / 2] = h2(__floats2half2_rn(e0.x, e0.y));
-            w[i / 2 + 1] = h2(__floats2half2_rn(e1.x, e1.y));
-          } else {
-            w[i / 2] = pack_bf16x2(e0.x * value_factor, e0.y * value_factor);
-            w[i / 2 + 1] = pack_bf16x2(e1.x * value_factor, e1.y * value_factor);
-          }
+        for (int i = 0; i < 8; ++i) sum[j / 2 + i] = __fadd2_rn(sum[j / 2 + i], make_float2(s[2 * i], s[2 * i + 1]));
+        if (kind == kStepPage) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = h2(__floats2half2_rn(s[2 * i], s[2 * i + 1]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            w[i] = pack_bf16x2(s[2 * i] * p.inverse_value_scale, s[2 * i + 1] * p.inverse_value_scale);
         }
         const int column = first_column + j;
         uint8_t* row = sm.p[n & 1] + (column >> 6) * 16384 + t * 128;
@@ -796,7 +893,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        tc::mbar_arrive(&sm.s_empty[n & 1]);
+        if constexpr (!Sh::kHold) tc::mbar_arrive(&sm.s_empty[n & 1]);
         tc::mbar_arrive(&sm.p_full[n & 1]);
       }
     }
@@ -808,9 +905,10 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col_sum[warp][first_column + j] = total; });
     }
     // the next unit's queries go in while this one's last product runs: all its scores are done
-    more = walker.next(following);
+    Unit following = u;
+    more = walker.next(following, true);
     float next_inverse = 1.0f;
-    bar_sync(3, Sh::kSoftmaxThreads);  // both groups have seen their last scores; the parents are free
+    bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);  // both groups have seen their last scores; the parents are free
     if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
     bar_sync(barrier, 128);
     const bool whole = u.begin == 0 && u.end == u.info.steps;
@@ -955,17 +1053,20 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   __syncthreads();
   tc::fence_after_sync();
   if (sm.first < sm.last) {
-    const Walker walker(p, sm.start_row, sm.start_offset, sm.last - sm.first, PT);
+    const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
     if (warp < 4) {
+      trade_registers<Sh::kLaunchRegs, Sh::kKeyRegs>();
       keys<NT, PT>(p, sm, walker, thread);
     } else if (warp < 8) {
+      trade_registers<Sh::kLaunchRegs, Sh::kValueRegs>();
       values<NT, PT>(p, sm, walker, thread - 128);
     } else if (warp < 8 + 4 * Sh::kGroups) {
+      trade_registers<Sh::kLaunchRegs, Sh::kSoftmaxRegs>();
       softmax<NT>(p, sm, walker, thread - 256);
-    } else if (warp == 8 + 4 * Sh::kGroups) {
-      produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
     } else {
-      if (lane == 0) issue<NT>(sm, walker);
+      trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
+      if (warp == 8 + 4 * Sh::kGroups) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
+      if (warp == 9 + 4 * Sh::kGroups && lane == 0) issue<NT>(sm, walker);
       __syncwarp();
     }
   }
