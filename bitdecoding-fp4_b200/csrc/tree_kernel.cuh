@@ -380,11 +380,21 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
   __syncwarp();
 }
 
+// One thread of a converged warp. tcgen05.mma takes its descriptors from uniform registers: behind an elected
+// predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32 (N = 64) to 64
+// cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its size.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(elected));
+  return elected != 0;
+}
+
+// The whole warp walks and waits; one thread of it issues.
 template <int NT>
 __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   using Sh = Shape<NT>;
   constexpr uint32_t kScores = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
-  const uint32_t tmem = sm.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p);
   int n = 0, unit = 0;
   Unit u;
@@ -392,19 +402,28 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   for (; walker.next(u, known); known = true) {
     auto output = [&](int step, int j) {  // O^T += V^T P^T of step `step` of the unit, the CTA's j-th
       const StepKind kind = step_kind(u.info, step);
-      const int slices = step_slices(u.info, kind);
       const int a = j % Sh::kVBuffers;
       tc::mbar_wait(&sm.va_full[a], (j / Sh::kVBuffers) & 1, &sm.abort_flag);
       tc::mbar_wait(&sm.p_full[j & 1], (j >> 1) & 1, &sm.abort_flag);
       const bool first = step == u.begin;
       if (first) tc::mbar_wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
       tc::fence_after_sync();
-      const uint32_t tile = prob + (j & 1) * Sh::kBlocks * 16384;
-      for (int s = 0; s < slices; ++s)
-        mma_ts(tmem + Sh::kO, tmem + Sh::kV + a * 64 + s * 8, tc::smem_desc(tile + s * 2048, tc::kSwizzle128B, 1024, 16384),
-               kind == kStepPage ? kPages : kBf16, !(first && s == 0));
-      tc::commit(&sm.va_empty[a]);
-      tc::commit(&sm.p_empty[j & 1]);
+      const uint64_t tile = tc::smem_desc(prob + (j & 1) * Sh::kBlocks * 16384, tc::kSwizzle128B, 1024, 16384);
+      const uint32_t operand = tmem + Sh::kV + a * 64;
+      if (elect_one()) {
+        if (kind == kStepPage) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
+            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kPages, !(first && s == 0));
+        } else {
+          const int slices = step_slices(u.info, kind);
+          for (int s = 0; s < slices; ++s)
+            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kBf16, !(first && s == 0));
+        }
+        tc::commit(&sm.va_empty[a]);
+        tc::commit(&sm.p_empty[j & 1]);
+      }
+      __syncwarp();
     };
     tc::mbar_wait(&sm.q_full, unit & 1, &sm.abort_flag);
     for (int step = u.begin; step < u.end; ++step, ++n) {
@@ -412,20 +431,25 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
       tc::mbar_wait(&sm.ka_full[a], (n / Sh::kKBuffers) & 1, &sm.abort_flag);
       tc::mbar_wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
       tc::fence_after_sync();
+      if (elect_one()) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
-        mma_ts(tmem + Sh::kS + (n & 1) * NT, tmem + Sh::kK + a * 64 + s * 8,
-               tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
-      tc::commit(&sm.s_full[n & 1]);
-      tc::commit(&sm.ka_empty[a]);
+        for (int s = 0; s < 8; ++s)
+          mma_ts(tmem + Sh::kS + (n & 1) * NT, tmem + Sh::kK + a * 64 + s * 8,
+                 tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
+        tc::commit(&sm.s_full[n & 1]);
+        tc::commit(&sm.ka_empty[a]);
+      }
+      __syncwarp();
       if (step > u.begin) output(step - 1, n - 1);
     }
     output(u.end - 1, n - 1);
-    tc::commit(&sm.o_full);
+    if (elect_one()) tc::commit(&sm.o_full);
+    __syncwarp();
     ++unit;
   }
   int ignore = 0;  // also after an abort: tensor memory is freed behind the last product
-  tc::commit(&sm.drained);
+  if (elect_one()) tc::commit(&sm.drained);
+  __syncwarp();
   tc::mbar_wait(&sm.drained, 0, &ignore);
 }
 
@@ -1066,8 +1090,7 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     } else {
       trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
       if (warp == 8 + 4 * Sh::kGroups) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
-      if (warp == 9 + 4 * Sh::kGroups && lane == 0) issue<NT>(sm, walker);
-      __syncwarp();
+      if (warp == 9 + 4 * Sh::kGroups) issue<NT>(sm, walker);
     }
   }
   tc::fence_before_sync();
