@@ -15,7 +15,7 @@ namespace bdfp4 {
 static int tree_tile(int queries) {
   const int tiles = (queries + kTreeMaxTile - 1) / kTreeMaxTile;
   const int each = (queries + tiles - 1) / tiles;
-  for (int tile : {16, 32, 64, 96})
+  for (int tile : {16, 32})
     if (each <= tile) return tile;
   return kTreeMaxTile;
 }

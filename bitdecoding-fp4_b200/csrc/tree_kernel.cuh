@@ -11,9 +11,9 @@
 // through shared memory. P is stored as the softmax threads hold it, one token per thread with its queries
 // contiguous, which is the MN-major form of B.
 //
-// Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: a step votes
-// whether any score exceeds its query's maximum by more than 2^8, and only then are the maxima taken anew
-// (across threads) and O^T rescaled. Sums stay per thread until the unit ends. Probabilities carry a factor
+// Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: probabilities are
+// formed against them at once, and only when one comes out more than 2^8 above its maximum (the barrier
+// that ends a step carries that vote) are the maxima taken anew, O^T rescaled and the step formed again. Sums stay per thread until the unit ends. Probabilities carry a factor
 // 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
 //
 // The rolling tail and the drafts with the sink are two more steps of the same form over BF16 values: K is
@@ -40,34 +40,32 @@ constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
 // A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
 // 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
 constexpr int kBf16Pitch = 272, kBf16Rows = 64;
-// Named barriers: one per softmax group (four at most), all softmax threads, the key threads.
+// Named barriers: one per softmax group (four ids), all softmax threads, the key threads.
 constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kKeysBarrier = 6;
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
-constexpr float kGrowth = 8.0f;     // a maximum is renewed when a score exceeds it by more than this (log2)
+constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renewed when one exceeds this, 2^8 above
 
-// A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (128
-// threads for NT = 64, 256 for 128) the kernel spilled, into an L1 that shared memory has left 24 KB of.
+// A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 the
+// kernel spilled, into an L1 that shared memory has left 24 KB of.
 template <int NT>
 struct Shape {
   static constexpr int kColumns = NT < 32 ? NT : 32;        // queries per softmax thread
   static constexpr int kGroups = NT / kColumns;             // softmax groups of 128 threads
   static constexpr int kBlocks = (NT + 63) / 64;            // 128-byte rows of P per token
-  static constexpr int kKBuffers = NT > 96 ? 1 : 2;         // operand buffers in tensor memory, as many as it holds
-  static constexpr int kVBuffers = NT > 64 ? 1 : 2;
-  static constexpr int kStages = NT > 96 ? 5 : NT > 64 ? 6 : 8;
+  static constexpr int kKBuffers = 2, kVBuffers = 2;        // operand buffers in tensor memory
+  static constexpr int kStages = 8;
   static constexpr int kSoftmaxThreads = 128 * kGroups;
   static constexpr int kThreads = 256 + kSoftmaxThreads + 128;  // keys, values, softmax, control (two of its warps idle)
   // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
   // must not exceed what the launch was given.
-  static constexpr int kLaunchRegs = kGroups == 4 ? 72 : kGroups == 3 ? 80 : kGroups == 2 ? 96 : 128;
-  static constexpr int kSoftmaxRegs = kGroups == 4 ? 80 : kGroups == 3 ? 96 : kGroups == 2 ? 112 : 144;
-  static constexpr int kKeyRegs = kGroups == 4 ? 80 : kGroups == 3 ? 88 : kGroups == 2 ? 112 : 152;
-  static constexpr int kValueRegs = kGroups == 4 ? 64 : kGroups == 3 ? 64 : kGroups == 2 ? 88 : 128;
-  static constexpr int kControlRegs = kGroups == 4 ? 40 : kGroups == 3 ? 40 : kGroups == 2 ? 56 : 88;
+  static constexpr int kLaunchRegs = kGroups == 2 ? 96 : 128;
+  static constexpr int kSoftmaxRegs = kGroups == 2 ? 128 : 152;
+  static constexpr int kKeyRegs = kGroups == 2 ? 88 : 128;
+  static constexpr int kValueRegs = kGroups == 2 ? 80 : 128;
+  static constexpr int kControlRegs = kGroups == 2 ? 56 : 104;
   static_assert(kSoftmaxRegs * kGroups + kKeyRegs + kValueRegs + kControlRegs <= kLaunchRegs * (3 + kGroups), "registers");
   static_assert(kLaunchRegs * kThreads <= 65536, "registers");
-  static constexpr bool kHold = kGroups <= 2;  // a thread's scores stay in registers between the vote and the exponentials
   // tensor memory columns
   static constexpr int kS = 0, kO = 2 * NT, kK = 3 * NT, kV = kK + 64 * kKBuffers;
   static_assert(kV + 64 * kVBuffers <= 512, "tensor memory");
@@ -162,6 +160,12 @@ __device__ __forceinline__ void st8(uint32_t address, const uint32_t* v) {
                : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t address, float* v) {
+#pragma unroll
+  for (int j = 0; j < N; j += 16) tc::tmem_ld16(address + j, v + j);
+}
+
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
 // Eight E2M1 codes times one FP16 scale -> eight FP16 values in four words, in code order. Exact.
@@ -175,17 +179,13 @@ __device__ __forceinline__ void dequantize8(uint32_t codes, __half2 scale, uint3
   for (int i = 0; i < 4; ++i) out[i] = h2(__hmul2(*reinterpret_cast<__half2*>(&v[i]), scale));
 }
 
-// Four E4M3 bytes -> four FP16 pairs (scale, scale).
+// Two E4M3 bytes -> two FP16 pairs (scale, scale).
 __device__ __forceinline__ void scale_pairs(uint32_t bytes, __half2* out) {
-  uint32_t lo, hi;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(bytes));
-  const __half2 a = *reinterpret_cast<__half2*>(&lo), b = *reinterpret_cast<__half2*>(&hi);
-  out[0] = __low2half2(a);
-  out[1] = __high2half2(a);
-  out[2] = __low2half2(b);
-  out[3] = __high2half2(b);
+  uint32_t both;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(both) : "r"(bytes));
+  const __half2 pair = *reinterpret_cast<__half2*>(&both);
+  out[0] = __low2half2(pair);
+  out[1] = __high2half2(pair);
 }
 
 // The power of two that brings `amax` into [2^14, 2^15), and its inverse. Zero, infinite or NaN: 1.
@@ -453,19 +453,18 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   tc::mbar_wait(&sm.drained, 0, &ignore);
 }
 
-// Sixteen code words (128 values) and the scales of their eight groups.
-__device__ __forceinline__ void store_dequantized(uint32_t a, const uint4* chunk, uint32_t scales0, uint32_t scales1) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    __half2 scale[4];
-    scale_pairs(j < 2 ? scales0 : scales1, scale);
-    uint32_t v[16];
-    dequantize8(chunk[j].x, scale[2 * (j & 1)], v);
-    dequantize8(chunk[j].y, scale[2 * (j & 1)], v + 4);
-    dequantize8(chunk[j].z, scale[2 * (j & 1) + 1], v + 8);
-    dequantize8(chunk[j].w, scale[2 * (j & 1) + 1], v + 12);
-    st16(a + 16 * j, v);
-  }
+// Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane. The callers'
+// loops over a row's four chunks stay rolled: four roles run side by side on every scheduler, and unrolled
+// (300 instructions each for keys and values) they waited for instructions a third of the time.
+__device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint32_t scales) {
+  __half2 scale[2];
+  scale_pairs(scales, scale);
+  uint32_t v[16];
+  dequantize8(chunk.x, scale[0], v);
+  dequantize8(chunk.y, scale[0], v + 4);
+  dequantize8(chunk.z, scale[1], v + 8);
+  dequantize8(chunk.w, scale[1], v + 12);
+  st16(a, v);
 }
 
 // One side of the ring as its consumers (four warps) see it.
@@ -511,18 +510,16 @@ __device__ __forceinline__ void keys(const TreeParams& p, Smem<NT>& sm, Walker w
       const uint32_t empty_parity = ((n / Sh::kKBuffers) & 1) ^ 1;
       if (kind == kStepPage) {
         const uint8_t* stage = ring.wait();
-        uint4 chunk[4];
         const uint8_t* row = stage + t * 64;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) chunk[j] = *reinterpret_cast<const uint4*>(row + ((j ^ ((t >> 1) & 3)) * 16));
-        const uint8_t* at = PT == 128 ? stage + kKsOffset + (t & 31) * 16 + (t >> 5) * 4
-                                      : stage + kKsOffset + (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4;
-        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(at);
-        const uint32_t s1 = *reinterpret_cast<const uint32_t*>(at + (PT == 128 ? 512 : 256));
-        ring.release();
+        const uint8_t* scales = PT == 128 ? stage + kKsOffset + (t & 31) * 16 + (t >> 5) * 4
+                                          : stage + kKsOffset + (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4;
         tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-        store_dequantized(operand, chunk, s0, s1);
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j)
+          store_dequantized(operand + 16 * j, *reinterpret_cast<const uint4*>(row + ((j ^ ((t >> 1) & 3)) * 16)),
+                            *reinterpret_cast<const uint16_t*>(scales + (j >> 1) * (PT == 128 ? 512 : 256) + (j & 1) * 2));
+        ring.release();
       } else {
         const int places = bf16_places(u.info, kind);
         const int stages = (places + kBf16Rows - 1) / kBf16Rows;
@@ -624,20 +621,17 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
       const uint32_t empty_parity = ((n / Sh::kVBuffers) & 1) ^ 1;
       if (kind == kStepPage) {
         const uint8_t* stage = ring.wait();
-        uint4 chunk[4];
-#pragma unroll
+        const uint8_t* scales = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
+        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
+        tc::fence_after_sync();
+#pragma unroll 1
         for (int j = 0; j < 4; ++j) {
           const uint8_t* at = PT == 128 ? stage + kVOffset + c * 64 + ((j ^ ((c >> 1) & 3)) * 16)
                                         : stage + kVOffset + (j >> 1) * 4096 + c * 32 + (((j & 1) ^ ((c >> 2) & 1)) * 16);
-          chunk[j] = *reinterpret_cast<const uint4*>(at);
+          store_dequantized(operand + 16 * j, *reinterpret_cast<const uint4*>(at),
+                            *reinterpret_cast<const uint16_t*>(scales + (j >> 1) * 512 + (j & 1) * 2));
         }
-        const uint8_t* at = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
-        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(at);
-        const uint32_t s1 = *reinterpret_cast<const uint32_t*>(at + 512);
         ring.release();
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-        store_dequantized(operand, chunk, s0, s1);
       } else {
         const int places = bf16_places(u.info, kind);
         ring.pass((places + kBf16Rows - 1) / kBf16Rows);  // the keys'
@@ -787,64 +781,85 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       if (kind == kStepPage) dead = step == 0 && t < u.info.sink;
       else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
       else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
+      const bool special = kind != kStepPage || (step == 0 && u.info.sink > 0);  // the same in the whole group
       const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
       const int node = t - BDFP4_MAX_SINK;
+      // P of this step goes where the one before the last was
+      tc::mbar_wait(&sm.p_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
       tc::mbar_wait(&sm.s_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
       tc::fence_after_sync();
       float f = page_factor;
       if (kind != kStepPage) f = p.scale_log2 * q_inverse * sm.key_factor[n & 7][t];
       const float2 f2 = make_float2(f, f);
       const uint32_t scores = sm.tmem + Sh::kS + (n & 1) * NT + first_column + lanes;
-      auto load16 = [&](int j, float* s) {
-        tc::tmem_ld16(scores + j, s);
+      uint8_t* const p_row = sm.p[n & 1] + (first_column >> 6) * 16384 + t * 128;
+
+      float s[C];
+      auto load = [&] {
+        tmem_load<C>(scores, s);
         tc::tmem_wait_ld();
-        if (masked) {
+        if (special) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!((sm.family[first_column + j + i] >> node) & 1)) s[i] = -INFINITY;
+          for (int j = 0; j < C; ++j)
+            if (dead || (masked && !((sm.family[first_column + j] >> node) & 1))) s[j] = -INFINITY;
         }
       };
-      // scores -> log2 units above the maxima, plus kShift
-      auto above16 = [&](int j, float* s) {
+      // The step's probabilities into s and, rounded, into shared memory. True when one of this thread's
+      // exceeds 2^(kShift + kGrowth): its query's maximum has to be renewed, and the step formed again.
+      auto form = [&]() -> bool {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(base + j + i);
-          const float2 y0 = __ffma2_rn(make_float2(s[i], s[i + 1]), f2, make_float2(b.x, b.y));
-          const float2 y1 = __ffma2_rn(make_float2(s[i + 2], s[i + 3]), f2, make_float2(b.z, b.w));
-          s[i] = y0.x, s[i + 1] = y0.y, s[i + 2] = y1.x, s[i + 3] = y1.y;
+        for (int j = 0; j < C; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(base + j);
+          const float2 y0 = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, make_float2(b.x, b.y));
+          const float2 y1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), f2, make_float2(b.z, b.w));
+          s[j] = ex2(y0.x), s[j + 1] = ex2(y0.y), s[j + 2] = ex2(y1.x), s[j + 3] = ex2(y1.y);
         }
-      };
-      float held[Sh::kHold ? C : 16];
-      float highest = -INFINITY;
+        uint32_t w[C / 2];
+        bool high;
+        if (kind == kStepPage) {
+          __half2 most = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
-      for (int j = 0; j < C; j += 16) {
-        float* s = Sh::kHold ? held + j : held;
-        load16(j, s);
-        above16(j, s);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) highest = fmaxf(highest, s[i]);
-      }
-      if (bar_any(barrier, highest > kGrowth + kShift && !dead)) {
-#pragma unroll
-        for (int j = 0; j < C; j += 16) {
-          float s[16];
-          load16(j, s);
-          float mine = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float m = warp_max(dead ? -INFINITY : s[i] * f);
-            if (lane == i) mine = m;
+          for (int j = 0; j < C / 2; ++j) {
+            const __half2 pair = __floats2half2_rn(s[2 * j], s[2 * j + 1]);
+            most = __hmax2(most, pair);
+            w[j] = h2(pair);
           }
-          if (lane < 16) sm.col_max[warp][first_column + j + lane] = mine;
+          high = __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
+        } else {
+          float most = 0.0f;
+#pragma unroll
+          for (int j = 0; j < C / 2; ++j) {
+            most = fmaxf(most, fmaxf(s[2 * j], s[2 * j + 1]));
+            w[j] = pack_bf16x2(s[2 * j] * p.inverse_value_scale, s[2 * j + 1] * p.inverse_value_scale);
+          }
+          high = most > kHighest;
         }
+#pragma unroll
+        for (int j = 0; j < C / 8; ++j)
+          *reinterpret_cast<uint4*>(p_row + (((((first_column & 63) >> 3) + j) ^ (t & 7)) * 16)) =
+              make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        tc::fence_before_sync();
+        tc::fence_proxy_async_smem();
+        return high;
+      };
+      load();
+      if (bar_any(barrier, form())) {
+        load();
+        float mine = 0.0f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          const float m = warp_max(s[j] * f);
+          if (lane == j) mine = m;
+        }
+        if (lane < C) sm.col_max[warp][first_column + lane] = mine;
         bar_sync(barrier, 128);
-        for (int j = t; j < C; j += 128) {
-          const int col = first_column + j;
-          const float before = top[j];
+        if (t < C) {
+          const int col = first_column + t;
+          const float before = top[t];
           const float now = fmaxf(fmaxf(fmaxf(sm.col_max[0][col], sm.col_max[1][col]),
                                         fmaxf(sm.col_max[2][col], sm.col_max[3][col])), before);
-          top[j] = now;
-          base[j] = kShift - now;
+          top[t] = now;
+          base[t] = kShift - now;
           sm.factor[col] = ex2(before - now);
         }
         bar_sync(barrier, 128);
@@ -853,6 +868,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
           sum[j].x *= sm.factor[first_column + 2 * j];
           sum[j].y *= sm.factor[first_column + 2 * j + 1];
         }
+        form();
         if (step > u.begin) {  // what O^T holds is of the old maxima
           tc::mbar_wait(&sm.p_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, &sm.abort_flag);
           tc::fence_after_sync();
@@ -867,59 +883,17 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
             tc::tmem_st16(at, o);
           }
           tc::tmem_wait_st();
+          tc::fence_before_sync();
         }
-        if constexpr (Sh::kHold) {
-#pragma unroll
-          for (int j = 0; j < C; j += 16) {
-            load16(j, held + j);
-            above16(j, held + j);
-          }
-        }
+        bar_sync(barrier, 128);
       }
-      if constexpr (Sh::kHold) {  // the scores are in registers: the next but one may come
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.s_empty[n & 1]);
-      }
-      // P of this step goes where the one before the last was
-      tc::mbar_wait(&sm.p_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
-#pragma unroll
-      for (int j = 0; j < C; j += 16) {
-        float* s = Sh::kHold ? held + j : held;
-        if constexpr (!Sh::kHold) {
-          load16(j, s);
-          above16(j, s);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = ex2(s[i]);
-        if (dead) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-        }
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[j / 2 + i] = __fadd2_rn(sum[j / 2 + i], make_float2(s[2 * i], s[2 * i + 1]));
-        if (kind == kStepPage) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = h2(__floats2half2_rn(s[2 * i], s[2 * i + 1]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = pack_bf16x2(s[2 * i] * p.inverse_value_scale, s[2 * i + 1] * p.inverse_value_scale);
-        }
-        const int column = first_column + j;
-        uint8_t* row = sm.p[n & 1] + (column >> 6) * 16384 + t * 128;
-        const int chunk = (column & 63) >> 3;
-        *reinterpret_cast<uint4*>(row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-      tc::fence_before_sync();
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (!Sh::kHold) tc::mbar_arrive(&sm.s_empty[n & 1]);
+      // the group's barrier stands behind every thread's scores read and probabilities written
+      if (t == 0) {
         tc::mbar_arrive(&sm.p_full[n & 1]);
+        tc::mbar_arrive(&sm.s_empty[n & 1]);
       }
+#pragma unroll
+      for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
     }
 
     {  // each query's weight: first over a warp's 32 tokens, then (below) over the four warps
@@ -1021,8 +995,8 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       tc::mbar_init(&sm.ka_empty[i], 1);
       tc::mbar_init(&sm.va_empty[i], 1);
       tc::mbar_init(&sm.s_full[i], 1);
-      tc::mbar_init(&sm.s_empty[i], 4 * Sh::kGroups);
-      tc::mbar_init(&sm.p_full[i], 4 * Sh::kGroups);
+      tc::mbar_init(&sm.s_empty[i], Sh::kGroups);
+      tc::mbar_init(&sm.p_full[i], Sh::kGroups);
       tc::mbar_init(&sm.p_empty[i], 1);
     }
     tc::mbar_init(&sm.q_full, 1);
@@ -1119,9 +1093,7 @@ static cudaError_t launch_tile(const CUtensorMap& k_map, const CUtensorMap& v_ma
   switch (p.tile) {
     case 16: return launch<16, PT>(k_map, v_map, p, stream);
     case 32: return launch<32, PT>(k_map, v_map, p, stream);
-    case 64: return launch<64, PT>(k_map, v_map, p, stream);
-    case 96: return launch<96, PT>(k_map, v_map, p, stream);
-    default: return launch<128, PT>(k_map, v_map, p, stream);
+    default: return launch<64, PT>(k_map, v_map, p, stream);
   }
 }
 
