@@ -4,21 +4,27 @@
 // tokens at a time,
 //     S^T [token, query]   = K   [token, channel]  * Q^T
 //     O^T [channel, query] = V^T [channel, token] * P^T
-// both as tcgen05.mma.kind::f16 with the cache operand A in tensor memory and the query-side operand B in
-// shared memory. E2M1 x E4M3 has at most six significant bits and lies in [2^-10, 2688], so a page's values
-// are exact in FP16: a thread reads its own token's (K) or channel's (V) 64 code bytes, converts and scales
-// them in registers and stores them straight into its tensor-memory lane; the dequantized tile never passes
-// through shared memory. P is stored as the softmax threads hold it, one token per thread with its queries
-// contiguous, which is the MN-major form of B.
+//
+// S^T over a page is the block-scaled FP4 product of the codes as they lie in the cache (kind::mxf4nvf4, no
+// dequantization) with the query written as a sum of four FP4 terms, each the rounding of what the ones
+// before left: a term leaves at most 0.177 of its group's largest value (half a step of 2/6, the E4M3
+// scale's rounding included), four leave 10^-3, less than the BF16 rounding the query came with. Four terms
+// of K = 64 take the tensor time of one FP16 product.
+//
+// O^T over a page is a kind::f16 product with V^T in tensor memory: E2M1 x E4M3 has at most six significant
+// bits and lies in [2^-10, 2688], so a page's values are exact in FP16. A thread reads its own channel's 64
+// code bytes, converts and scales them in registers and stores them straight into its tensor-memory lane; the
+// dequantized tile never passes through shared memory. P is stored as the softmax threads hold it, one token
+// per thread with its queries contiguous, which is the MN-major form of operand B.
 //
 // Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: probabilities are
 // formed against them at once, and only when one comes out more than 2^8 above its maximum (the barrier
 // that ends a step carries that vote) are the maxima taken anew, O^T rescaled and the step formed again. Sums stay per thread until the unit ends. Probabilities carry a factor
 // 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
 //
-// The rolling tail and the drafts with the sink are two more steps of the same form over BF16 values: K is
-// scaled per token by a power of two into FP16's range (the softmax thread of the token undoes it), V and
-// P are BF16. Queries are scaled per tile the same way.
+// The rolling tail and the drafts with the sink are two more steps over BF16 values, both products kind::f16
+// with the cache side in tensor memory: K is scaled per token by a power of two into FP16's range (the softmax
+// thread of the token undoes it), V and P are BF16. Queries are scaled per tile the same way.
 //
 // Work is the sequence of all steps of all (row, head, tile) units, cut into equal runs, one per CTA, so any
 // mix of lengths is balanced; a unit that straddles CTAs leaves unnormalised parts that a second kernel adds.
@@ -40,8 +46,9 @@ constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
 // A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
 // 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
 constexpr int kBf16Pitch = 272, kBf16Rows = 64;
-// Named barriers: one per softmax group (four ids), all softmax threads, the key threads.
-constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kKeysBarrier = 6;
+// Named barriers: one per softmax group (four ids), all softmax threads, the values' threads.
+constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kValuesBarrier = 6;
+constexpr int kTerms = 4;             // FP4 terms of a query
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
 constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renewed when one exceeds this, 2^8 above
@@ -50,39 +57,25 @@ constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renew
 // kernel spilled, into an L1 that shared memory has left 24 KB of.
 template <int NT>
 struct Shape {
-  static constexpr int kColumns = NT < 32 ? NT : 32;        // queries per softmax thread
-  static constexpr int kGroups = NT / kColumns;             // softmax groups of 128 threads
-  static constexpr int kBlocks = (NT + 63) / 64;            // 128-byte rows of P per token
-  static constexpr int kKBuffers = 2, kVBuffers = 2;        // operand buffers in tensor memory
-  static constexpr int kStages = 8;
+  static constexpr int kColumns = NT < 32 ? NT : 32;  // queries per softmax thread
+  static constexpr int kGroups = NT / kColumns;       // softmax groups of 128 threads
+  static constexpr int kStages = NT > 32 ? 7 : 8;
   static constexpr int kSoftmaxThreads = 128 * kGroups;
-  static constexpr int kThreads = 256 + kSoftmaxThreads + 128;  // keys, values, softmax, control (two of its warps idle)
-  // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
-  // must not exceed what the launch was given.
-  static constexpr int kLaunchRegs = kGroups == 2 ? 96 : 128;
-  static constexpr int kSoftmaxRegs = kGroups == 2 ? 128 : 152;
-  static constexpr int kKeyRegs = kGroups == 2 ? 88 : 128;
-  static constexpr int kValueRegs = kGroups == 2 ? 80 : 128;
-  static constexpr int kControlRegs = kGroups == 2 ? 56 : 104;
-  static_assert(kSoftmaxRegs * kGroups + kKeyRegs + kValueRegs + kControlRegs <= kLaunchRegs * (3 + kGroups), "registers");
-  static_assert(kLaunchRegs * kThreads <= 65536, "registers");
-  // tensor memory columns
-  static constexpr int kS = 0, kO = 2 * NT, kK = 3 * NT, kV = kK + 64 * kKBuffers;
-  static_assert(kV + 64 * kVBuffers <= 512, "tensor memory");
+  static constexpr int kThreads = 128 + kSoftmaxThreads + 128;  // values, softmax, control
+  // tensor memory columns: scores (two steps), output, a BF16 step's keys, values (two steps), scales of the
+  // keys (two steps) and of the query terms
+  static constexpr int kS = 0, kO = 2 * NT, kK = 3 * NT, kV = kK + 64, kKs = kV + 128, kQs = kKs + 16;
+  static_assert(kQs + 8 * kTerms <= 512, "tensor memory");
 };
-
-template <int FROM, int TO>
-__device__ __forceinline__ void trade_registers() {
-  if constexpr (TO > FROM) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TO));
-  if constexpr (TO < FROM) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
-}
 
 template <int NT>
 struct Smem {
   using Sh = Shape<NT>;
   alignas(1024) uint8_t ring[Sh::kStages][kStage];
-  alignas(1024) uint8_t q[2][NT * 128];  // two halves of 64 channels, K-major, 128-byte swizzle
-  alignas(1024) uint8_t p[2][Sh::kBlocks * 16384];  // MN-major: 128-byte rows of 64 queries per token, swizzled
+  alignas(1024) uint8_t q[2][NT * 128];          // FP16: two halves of 64 channels, K-major, 128-byte swizzle
+  alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
+  alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
+  alignas(1024) uint8_t p[2][16384];               // MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
@@ -94,7 +87,8 @@ struct Smem {
   float q_max[16];
   int parents[BDFP4_MAX_TREE_NODES];
   uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
-  uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];
+  uint64_t k_ready[Sh::kStages];  // 64-token pages: the stage's key scales are whole atoms
+  uint64_t ka_full, ka_empty, va_full[2], va_empty[2];
   uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
   uint64_t q_full, o_full, o_empty, drained;
   long long sums[Sh::kThreads / 32];
@@ -188,14 +182,15 @@ __device__ __forceinline__ void scale_pairs(uint32_t bytes, __half2* out) {
   out[1] = __high2half2(pair);
 }
 
-// The power of two that brings `amax` into [2^14, 2^15), and its inverse. Zero, infinite or NaN: 1.
+// The power of two that brings `amax` into [2^10, 2^11), where FP16 has 25 binades below and the FP4 terms'
+// E4M3 scales (up to 448 = 2688 / 6) reach their fourth, and its inverse. Zero, infinite or NaN: 1.
 __device__ __forceinline__ float fp16_scale(float amax, float* inverse) {
   const int e = (int)((__float_as_uint(amax) >> 23) & 0xffu);
   if (e == 0 || e == 255) {
     *inverse = 1.0f;
     return 1.0f;
   }
-  const int field = min(127 + 14 + 127 - e, 253);
+  const int field = min(127 + 10 + 127 - e, 253);
   *inverse = __uint_as_float((uint32_t)(254 - field) << 23);
   return __uint_as_float((uint32_t)field << 23);
 }
@@ -346,13 +341,12 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
         const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
         for (int first = 0; first < places; first += kBf16Rows) {
           const int end = min(first + kBf16Rows, places);
-          uint64_t* full = side ? &sm.full_v[slot] : &sm.full_k[slot];
           if (lane == 0) {
             tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
             // the sink's places behind its length stay empty
             const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
-            tc::mbar_expect_tx(full, (end - first - absent) * 256);
-            tc::mbar_arrive(side ? &sm.full_k[slot] : &sm.full_v[slot]);  // the other side only passes the stage on
+            tc::mbar_expect_tx(&sm.full_v[slot], (end - first - absent) * 256);
+            tc::mbar_arrive(&sm.full_k[slot]);  // nothing for the FP4 product here
           }
           __syncwarp();
           for (int i = first + lane; i < end; i += 32) {
@@ -360,7 +354,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
             if (kind == kStepTail) source = tail + i * tail_row;
             else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
             else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
-            if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, full);
+            if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, &sm.full_v[slot]);
           }
           __syncwarp();
           advance();
@@ -390,25 +384,28 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // The whole warp walks and waits; one thread of it issues.
-template <int NT>
+template <int NT, int PT>
 __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   using Sh = Shape<NT>;
-  constexpr uint32_t kScores = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
+  constexpr uint32_t kScoresFp4 = tc::nvf4_idesc(128, NT);
+  constexpr uint32_t kScoresF16 = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p);
-  int n = 0, unit = 0;
+  const uint32_t q_codes = tc::smem_u32(sm.q_codes), q_scales = tc::smem_u32(sm.q_scales), ring = tc::smem_u32(sm.ring);
+  int n = 0, unit = 0, slot = 0, bf16_steps = 0;
+  uint32_t turn = 0;
   Unit u;
   bool known = false;
   for (; walker.next(u, known); known = true) {
     auto output = [&](int step, int j) {  // O^T += V^T P^T of step `step` of the unit, the CTA's j-th
       const StepKind kind = step_kind(u.info, step);
-      const int a = j % Sh::kVBuffers;
-      tc::mbar_wait(&sm.va_full[a], (j / Sh::kVBuffers) & 1, &sm.abort_flag);
-      tc::mbar_wait(&sm.p_full[j & 1], (j >> 1) & 1, &sm.abort_flag);
+      const int a = j & 1;
+      tc::mbar_wait(&sm.va_full[a], (j >> 1) & 1, &sm.abort_flag);
+      tc::mbar_wait(&sm.p_full[a], (j >> 1) & 1, &sm.abort_flag);
       const bool first = step == u.begin;
       if (first) tc::mbar_wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
       tc::fence_after_sync();
-      const uint64_t tile = tc::smem_desc(prob + (j & 1) * Sh::kBlocks * 16384, tc::kSwizzle128B, 1024, 16384);
+      const uint64_t tile = tc::smem_desc(prob + a * 16384, tc::kSwizzle128B, 1024, 16384);
       const uint32_t operand = tmem + Sh::kV + a * 64;
       if (elect_one()) {
         if (kind == kStepPage) {
@@ -421,25 +418,60 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
             mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kBf16, !(first && s == 0));
         }
         tc::commit(&sm.va_empty[a]);
-        tc::commit(&sm.p_empty[j & 1]);
+        tc::commit(&sm.p_empty[a]);
       }
       __syncwarp();
     };
     tc::mbar_wait(&sm.q_full, unit & 1, &sm.abort_flag);
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const int a = n % Sh::kKBuffers;
-      tc::mbar_wait(&sm.ka_full[a], (n / Sh::kKBuffers) & 1, &sm.abort_flag);
-      tc::mbar_wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      if (elect_one()) {
+    tc::fence_after_sync();
+    if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          mma_ts(tmem + Sh::kS + (n & 1) * NT, tmem + Sh::kK + a * 64 + s * 8,
-                 tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
-        tc::commit(&sm.s_full[n & 1]);
-        tc::commit(&sm.ka_empty[a]);
+      for (int i = 0; i < 2 * kTerms; ++i)
+        tc::cp_sf_atom(tmem + Sh::kQs + i * 4, tc::sf_atom_desc(q_scales + i * 512));
+    }
+    __syncwarp();
+    for (int step = u.begin; step < u.end; ++step, ++n) {
+      const StepKind kind = step_kind(u.info, step);
+      const uint32_t scores = tmem + Sh::kS + (n & 1) * NT;
+      tc::mbar_wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
+      if (kind == kStepPage) {
+        tc::mbar_wait(PT == 64 ? &sm.k_ready[slot] : &sm.full_k[slot], turn, &sm.abort_flag);
+        tc::fence_after_sync();
+        const uint32_t stage = ring + slot * kStage;
+        const uint32_t scales = tmem + Sh::kKs + (n & 1) * 8;
+        if (elect_one()) {
+          tc::cp_sf_atom(scales, tc::sf_atom_desc(stage + kKsOffset));
+          tc::cp_sf_atom(scales + 4, tc::sf_atom_desc(stage + kKsOffset + 512));
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term)
+              tc::mma_nvf4(scores, tc::fp4_tile_desc(stage, s), tc::fp4_tile_desc(q_codes + term * NT * 64, s), kScoresFp4,
+                           scales + 4 * s, tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
+          }
+          tc::commit(&sm.s_full[n & 1]);
+          tc::commit(&sm.empty[slot]);
+        }
+        __syncwarp();
+        if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+      } else {
+        for (int i = 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows); i > 0; --i) {
+          tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);  // the stage is not this product's
+          if (elect_one()) tc::mbar_arrive(&sm.empty[slot]);
+          __syncwarp();
+          if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+        }
+        tc::mbar_wait(&sm.ka_full, bf16_steps++ & 1, &sm.abort_flag);
+        tc::fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+            mma_ts(scores, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScoresF16, s > 0);
+          tc::commit(&sm.s_full[n & 1]);
+          tc::commit(&sm.ka_empty);
+        }
+        __syncwarp();
       }
-      __syncwarp();
       if (step > u.begin) output(step - 1, n - 1);
     }
     output(u.end - 1, n - 1);
@@ -453,9 +485,50 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   tc::mbar_wait(&sm.drained, 0, &ignore);
 }
 
-// Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane. The callers'
-// loops over a row's four chunks stay rolled: four roles run side by side on every scheduler, and unrolled
-// (300 instructions each for keys and values) they waited for instructions a third of the time.
+// 64-token pages: the key scales of a step's two pages come as half atoms (32 rows of 8 bytes); one warp
+// interleaves them, in place, into the two whole atoms the MMA reads.
+template <int NT>
+__device__ __forceinline__ void interleave_scales(Smem<NT>& sm, Walker walker, int lane) {
+  int slot = 0;
+  uint32_t turn = 0;
+  auto advance = [&] {
+    if (++slot == Shape<NT>::kStages) slot = 0, turn ^= 1;
+  };
+  Unit u;
+  bool known = false;
+  for (; walker.next(u, known); known = true) {
+    for (int step = u.begin; step < u.end; ++step) {
+      const StepKind kind = step_kind(u.info, step);
+      if (kind == kStepPage) {
+        tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);
+        uint8_t* scales = sm.ring[slot] + kKsOffset;
+        uint2 half[2][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) half[i & 1][i >> 1] = *reinterpret_cast<const uint2*>(scales + (i >> 1) * 512 + (i & 1) * 256 + lane * 8);
+        __syncwarp();
+#pragma unroll
+        for (int atom = 0; atom < 2; ++atom)
+          *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) =
+              make_uint4(half[atom][0].x, half[atom][0].y, half[atom][1].x, half[atom][1].y);
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
+        advance();
+      } else {
+        for (int i = 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows); i > 0; --i) {
+          tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);
+          if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
+          __syncwarp();
+          advance();
+        }
+      }
+    }
+  }
+}
+
+// Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane. The caller's
+// loop over a channel's four chunks stays rolled: three roles run side by side on every scheduler, and with
+// the 300 instructions of the unrolled form the warps waited for instructions a third of the time.
 __device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint32_t scales) {
   __half2 scale[2];
   scale_pairs(scales, scale);
@@ -467,160 +540,33 @@ __device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint3
   st16(a, v);
 }
 
-// One side of the ring as its consumers (four warps) see it.
-template <int NT>
-struct Ring {
-  Smem<NT>& sm;
-  uint64_t* full;
-  int lane, slot;
-  uint32_t turn;
-  __device__ Ring(Smem<NT>& s, uint64_t* f, int l) : sm(s), full(f), lane(l), slot(0), turn(0) {}
-  __device__ __forceinline__ const uint8_t* wait() {
-    tc::mbar_wait(&full[slot], turn, &sm.abort_flag);
-    return sm.ring[slot];
-  }
-  __device__ __forceinline__ void release() {
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
-    if (++slot == Shape<NT>::kStages) slot = 0, turn ^= 1;
-  }
-  __device__ __forceinline__ void pass(int stages) {
-    for (int i = 0; i < stages; ++i) {
-      wait();
-      release();
-    }
-  }
-};
-
-// Keys: thread t holds token t of every step.
-template <int NT, int PT>
-__device__ __forceinline__ void keys(const TreeParams& p, Smem<NT>& sm, Walker walker, int t) {
-  using Sh = Shape<NT>;
-  const int lane = t & 31;
-  const uint32_t tmem = sm.tmem + Sh::kK + ((uint32_t)(t & ~31) << 16);
-  Ring<NT> ring(sm, sm.full_k, lane);
-  int n = 0;
-  Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const StepKind kind = step_kind(u.info, step);
-      const uint32_t operand = tmem + (n % Sh::kKBuffers) * 64;
-      uint64_t* operand_empty = &sm.ka_empty[n % Sh::kKBuffers];
-      const uint32_t empty_parity = ((n / Sh::kKBuffers) & 1) ^ 1;
-      if (kind == kStepPage) {
-        const uint8_t* stage = ring.wait();
-        const uint8_t* row = stage + t * 64;
-        const uint8_t* scales = PT == 128 ? stage + kKsOffset + (t & 31) * 16 + (t >> 5) * 4
-                                          : stage + kKsOffset + (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4;
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-#pragma unroll 1
-        for (int j = 0; j < 4; ++j)
-          store_dequantized(operand + 16 * j, *reinterpret_cast<const uint4*>(row + ((j ^ ((t >> 1) & 3)) * 16)),
-                            *reinterpret_cast<const uint16_t*>(scales + (j >> 1) * (PT == 128 ? 512 : 256) + (j & 1) * 2));
-        ring.release();
-      } else {
-        const int places = bf16_places(u.info, kind);
-        const int stages = (places + kBf16Rows - 1) / kBf16Rows;
-        // a step's stages are held together; both have arrived when each has been waited for
-        ring.wait();
-        uint8_t* const stage0 = sm.ring[ring.slot];
-        uint8_t* stage1 = stage0;
-        if (stages > 1) {
-          const bool wraps = ring.slot + 1 == Sh::kStages;
-          const int next = wraps ? 0 : ring.slot + 1;
-          tc::mbar_wait(&sm.full_k[next], ring.turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
-          stage1 = sm.ring[next];
-        }
-        auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
-        bool there = t < places;
-        if (kind == kStepDraft) {
-          if (t < BDFP4_MAX_SINK) there = t < u.info.sink;
-          if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
-            const int group = t & 7;
-            const int64_t shift_at = u.head * kHeadDim + group * kGroup;
-            for (int first = 0; first < u.info.count; first += 16) {
-              // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
-              const int node = min(first + (t >> 3), u.info.count - 1);
-              uint4* at = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + node) + group * 32);
-              const uint4 raw[2] = {at[0], at[1]};
-              const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-              float v[16];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-              }
-              if (p.rotate && p.key_shift) cache_basis16<BDFP4_SHIFT_F32, true>(v, group, p.key_shift, shift_at);
-              else if (p.rotate) cache_basis16<BDFP4_SHIFT_NONE, true>(v, group, nullptr, 0);
-              else cache_basis16<BDFP4_SHIFT_F32, false>(v, group, p.key_shift, shift_at);
-              if (first + (t >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
-            }
-            tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
-            bar_sync(kKeysBarrier, 128);
-          }
-        }
-        const uint4* row = reinterpret_cast<const uint4*>(row_of(min(t, places - 1)));
-        float amax = 0.0f;
-        if (there) {
-#pragma unroll 4
-          for (int j = 0; j < 16; ++j) {
-            const uint4 r = row[j];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-          }
-        }
-        float inverse;
-        const float scale = fp16_scale(amax, &inverse);
-        sm.key_factor[n & 7][t] = inverse;
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-#pragma unroll 1
-        for (int quarter = 0; quarter < 4; ++quarter) {
-          uint32_t v[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 r = make_uint4(0, 0, 0, 0);
-            if (there) r = row[quarter * 4 + j];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
-          }
-          st16(operand + quarter * 16, v);
-        }
-        for (int i = 0; i < stages; ++i) ring.release();
-        ring.pass(stages);  // the values'
-      }
-      tc::tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.ka_full[n % Sh::kKBuffers]);
-    }
-  }
-}
-
-// Values: thread c holds channel c of every step.
+// The values' warps: thread c holds channel c of every step's V^T, and token c of a BF16 step's K.
 template <int NT, int PT>
 __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker walker, int c) {
   using Sh = Shape<NT>;
   const int lane = c & 31;
-  const uint32_t tmem = sm.tmem + Sh::kV + ((uint32_t)(c & ~31) << 16);
-  Ring<NT> ring(sm, sm.full_v, lane);
-  int n = 0;
+  const uint32_t lanes = (uint32_t)(c & ~31) << 16;
+  int slot = 0, n = 0, bf16_steps = 0;
+  uint32_t turn = 0;
+  auto arrived = [&]() -> uint8_t* {
+    tc::mbar_wait(&sm.full_v[slot], turn, &sm.abort_flag);
+    return sm.ring[slot];
+  };
+  auto release = [&] {
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
+    if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+  };
   Unit u;
   bool known = false;
   for (; walker.next(u, known); known = true) {
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const uint32_t operand = tmem + (n % Sh::kVBuffers) * 64;
-      uint64_t* operand_empty = &sm.va_empty[n % Sh::kVBuffers];
-      const uint32_t empty_parity = ((n / Sh::kVBuffers) & 1) ^ 1;
+      const uint32_t operand = sm.tmem + Sh::kV + (n & 1) * 64 + lanes;
+      uint64_t* operand_empty = &sm.va_empty[n & 1];
+      const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
       if (kind == kStepPage) {
-        const uint8_t* stage = ring.wait();
+        const uint8_t* stage = arrived();
         const uint8_t* scales = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
         tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
@@ -631,14 +577,89 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
           store_dequantized(operand + 16 * j, *reinterpret_cast<const uint4*>(at),
                             *reinterpret_cast<const uint16_t*>(scales + (j >> 1) * 512 + (j & 1) * 2));
         }
-        ring.release();
+        release();
       } else {
         const int places = bf16_places(u.info, kind);
-        ring.pass((places + kBf16Rows - 1) / kBf16Rows);  // the keys'
+        const int stages = (places + kBf16Rows - 1) / kBf16Rows;
+        {  // keys; a step's stages are held together
+          uint8_t* const stage0 = arrived();
+          uint8_t* stage1 = stage0;
+          if (stages > 1) {
+            const bool wraps = slot + 1 == Sh::kStages;
+            const int next = wraps ? 0 : slot + 1;
+            tc::mbar_wait(&sm.full_v[next], turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
+            stage1 = sm.ring[next];
+          }
+          auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
+          bool there = c < places;
+          if (kind == kStepDraft) {
+            if (c < BDFP4_MAX_SINK) there = c < u.info.sink;
+            if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
+              const int group = c & 7;
+              const int64_t shift_at = u.head * kHeadDim + group * kGroup;
+              for (int first = 0; first < u.info.count; first += 16) {
+                // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
+                const int node = min(first + (c >> 3), u.info.count - 1);
+                uint4* at = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + node) + group * 32);
+                const uint4 raw[2] = {at[0], at[1]};
+                const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  v[2 * i] = __uint_as_float(w[i] << 16);
+                  v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                }
+                if (p.rotate && p.key_shift) cache_basis16<BDFP4_SHIFT_F32, true>(v, group, p.key_shift, shift_at);
+                else if (p.rotate) cache_basis16<BDFP4_SHIFT_NONE, true>(v, group, nullptr, 0);
+                else cache_basis16<BDFP4_SHIFT_F32, false>(v, group, p.key_shift, shift_at);
+                if (first + (c >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
+              }
+              tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
+              bar_sync(kValuesBarrier, 128);
+            }
+          }
+          const uint4* row = reinterpret_cast<const uint4*>(row_of(min(c, places - 1)));
+          float amax = 0.0f;
+          if (there) {
+#pragma unroll 4
+            for (int j = 0; j < 16; ++j) {
+              const uint4 r = row[j];
+              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+            }
+          }
+          float inverse;
+          const float scale = fp16_scale(amax, &inverse);
+          sm.key_factor[n & 7][c] = inverse;
+          tc::mbar_wait(&sm.ka_empty, (bf16_steps & 1) ^ 1, &sm.abort_flag);
+          tc::fence_after_sync();
+#pragma unroll 1
+          for (int quarter = 0; quarter < 4; ++quarter) {
+            uint32_t v[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint4 r = make_uint4(0, 0, 0, 0);
+              if (there) r = row[quarter * 4 + j];
+              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
+            }
+            st16(sm.tmem + Sh::kK + lanes + quarter * 16, v);
+          }
+          for (int i = 0; i < stages; ++i) release();
+          tc::tmem_wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sm.ka_full);
+          ++bf16_steps;
+        }
         tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
         for (int first = 0; first < places; first += kBf16Rows) {
-          const uint8_t* stage = ring.wait() + 2 * c;
+          const uint8_t* stage = arrived() + 2 * c;
           const int slices = (min(places - first, kBf16Rows) + 15) / 16;
           for (int s = 0; s < slices; ++s) {
             const int place = first + s * 16;
@@ -653,19 +674,20 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
             }
             st8(operand + (place >> 4) * 8, v);
           }
-          ring.release();
+          release();
         }
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.va_full[n % Sh::kVBuffers]);
+      if (lane == 0) tc::mbar_arrive(&sm.va_full[n & 1]);
     }
   }
 }
 
-// The tile's queries into shared memory: rotated if asked, scaled by one power of two into FP16's range
-// (rows of the tile whose largest value is 2^-29 of the tile's keep full precision). Returns what undoes it.
+// The tile's queries into shared memory: rotated if asked, scaled by one power of two, as FP16 for the BF16 steps
+// and as FP4 terms for the pages. One scale for the tile: a query whose largest value is 2^-8 of the tile's
+// still has all four terms above E4M3's smallest scale. Returns what undoes the scaling.
 template <int NT>
 __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
   using Sh = Shape<NT>;
@@ -712,6 +734,26 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
     const int chunk = (group & 3) * 2;
     *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+    float left[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) left[j] = v[i][j] * scale;
+    const int at = r * 64 + group * 8;
+#pragma unroll 1
+    for (int term = 0; term < kTerms; ++term) {
+      float largest = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(left[j]));
+      const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
+      GroupCodes codes;
+      codes.scale = e4m3_to_float(byte);
+      encode16(left, codes.scale, codes.lo, codes.hi);
+      *reinterpret_cast<uint2*>(sm.q_codes[term] + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
+      sm.q_scales[term][scale_tile_offset(r, group)] = (uint8_t)byte;
+      float rest[16];
+      group_residual16(left, codes, rest);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) left[j] = rest[j];
+    }
   }
   tc::fence_proxy_async_smem();
   bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);
@@ -792,7 +834,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       if (kind != kStepPage) f = p.scale_log2 * q_inverse * sm.key_factor[n & 7][t];
       const float2 f2 = make_float2(f, f);
       const uint32_t scores = sm.tmem + Sh::kS + (n & 1) * NT + first_column + lanes;
-      uint8_t* const p_row = sm.p[n & 1] + (first_column >> 6) * 16384 + t * 128;
+      uint8_t* const p_row = sm.p[n & 1] + t * 128;
 
       float s[C];
       auto load = [&] {
@@ -836,7 +878,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
         }
 #pragma unroll
         for (int j = 0; j < C / 8; ++j)
-          *reinterpret_cast<uint4*>(p_row + (((((first_column & 63) >> 3) + j) ^ (t & 7)) * 16)) =
+          *reinterpret_cast<uint4*>(p_row + ((((first_column >> 3) + j) ^ (t & 7)) * 16)) =
               make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
         tc::fence_before_sync();
         tc::fence_proxy_async_smem();
@@ -987,18 +1029,19 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     for (int i = 0; i < Sh::kStages; ++i) {
       tc::mbar_init(&sm.full_k[i], 1);
       tc::mbar_init(&sm.full_v[i], 1);
-      tc::mbar_init(&sm.empty[i], 8);
+      tc::mbar_init(&sm.empty[i], 5);  // the values' four warps and the score product
+      tc::mbar_init(&sm.k_ready[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&sm.ka_full[i], 4);
       tc::mbar_init(&sm.va_full[i], 4);
-      tc::mbar_init(&sm.ka_empty[i], 1);
       tc::mbar_init(&sm.va_empty[i], 1);
       tc::mbar_init(&sm.s_full[i], 1);
       tc::mbar_init(&sm.s_empty[i], Sh::kGroups);
       tc::mbar_init(&sm.p_full[i], Sh::kGroups);
       tc::mbar_init(&sm.p_empty[i], 1);
     }
+    tc::mbar_init(&sm.ka_full, 4);
+    tc::mbar_init(&sm.ka_empty, 1);
     tc::mbar_init(&sm.q_full, 1);
     tc::mbar_init(&sm.o_full, 1);
     tc::mbar_init(&sm.o_empty, 4 * Sh::kGroups);
@@ -1053,18 +1096,15 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   if (sm.first < sm.last) {
     const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
     if (warp < 4) {
-      trade_registers<Sh::kLaunchRegs, Sh::kKeyRegs>();
-      keys<NT, PT>(p, sm, walker, thread);
-    } else if (warp < 8) {
-      trade_registers<Sh::kLaunchRegs, Sh::kValueRegs>();
-      values<NT, PT>(p, sm, walker, thread - 128);
-    } else if (warp < 8 + 4 * Sh::kGroups) {
-      trade_registers<Sh::kLaunchRegs, Sh::kSoftmaxRegs>();
-      softmax<NT>(p, sm, walker, thread - 256);
-    } else {
-      trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
-      if (warp == 8 + 4 * Sh::kGroups) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
-      if (warp == 9 + 4 * Sh::kGroups) issue<NT>(sm, walker);
+      values<NT, PT>(p, sm, walker, thread);
+    } else if (warp < 4 + 4 * Sh::kGroups) {
+      softmax<NT>(p, sm, walker, thread - 128);
+    } else if (warp == 4 + 4 * Sh::kGroups) {
+      produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
+    } else if (warp == 5 + 4 * Sh::kGroups) {
+      issue<NT, PT>(sm, walker);
+    } else if (PT == 64 && warp == 6 + 4 * Sh::kGroups) {
+      interleave_scales<NT>(sm, walker, lane);
     }
   }
   tc::fence_before_sync();

@@ -49,8 +49,13 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
     relative); each probability's rounding to BF16 (2^-8; FP16 pages round by 2^-11); and the scores' errors. A
     score is a sum of 128 products in FP32 whose terms add up to A = sum |q||k| * scale: 2^-16 A covers the
     products' and sums' rounding (128 additions of 2^-24), its scaling and the exponential's argument; a rotated
-    query is rounded to FP16 (2^-11), so its scores carry 2^-11 A more. An error d in a score is a relative error d
-    of its probability, and sum p v / sum p moves by at most sum p_t (d_t + mean d) |v_t|."""
+    query is rounded to FP16 (2^-11), so its scores carry 2^-11 A more. Against FP4 pages a query is four FP4
+    terms, each the rounding of what is left: the E4M3 scale of a group is at most 2^-4 off amax / 6, and half
+    the widest E2M1 step is one scale, so a term leaves at most 17/16 / 6 < 0.178 of the group's largest value (a
+    value clipped at six scales leaves less), four leave 0.178^4. Scaled so that the head's largest query value
+    lies in [2^10, 2^11), a term whose scale falls below E4M3's smallest (2^-9) leaves at most 6 x 2^-9, under
+    2^-16 of that value. An error d in a score is a relative error d of its probability, and sum p v / sum p
+    moves by at most sum p_t (d_t + mean d) |v_t|."""
     nodes, hq, _ = query.shape
     h = draft_key.shape[1]
     g = hq // h
@@ -78,6 +83,9 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
             torch.ones(nodes, sink, dtype=torch.bool))
     add(dk, draft_value.double(), ancestors(parents))
     k, v, mask = torch.cat(keys), torch.cat(values), torch.cat(seen, 1)
+    tile = q.abs().reshape(nodes, h, -1).amax((0, 2))  # the largest query value of each KV head
+    left = q.abs().reshape(nodes, hq, 8, 16).amax(3) * 0.178 ** 4
+    left = torch.maximum(left, 2.0 ** -16 * tile.repeat_interleave(g)[None, :, None])
     out = torch.empty(nodes, hq, 128, dtype=torch.float64)
     allowed = torch.empty_like(out)
     for head in range(hq):
@@ -86,6 +94,7 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
         p = torch.softmax(s, 1)
         terms = q[:, head].abs() @ kh.abs().T * softmax_scale
         d = terms * (2.0 ** -16 + (2.0 ** -11 if rotate else 0.0))
+        d[:, :fp4] += left[:, head] @ kh[:fp4].abs().reshape(fp4, 8, 16).sum(2).T * softmax_scale
         d = torch.where(mask, d, 0.0)
         out[:, head] = p @ vh
         weight = p * (d + (p * d).sum(1, keepdim=True) + 2.0 ** -8)
