@@ -46,27 +46,39 @@ constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
 // A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
 // 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
 constexpr int kBf16Pitch = 272, kBf16Rows = 64;
-// Named barriers: one per softmax group (four ids), all softmax threads, the values' threads.
-constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kValuesBarrier = 6;
+// Named barriers: the softmax threads, the two halves of the values' threads.
+constexpr int kSoftmaxBarrier = 1, kValuesBarrier = 2;
 constexpr int kTerms = 4;             // FP4 terms of a query
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
 constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renewed when one exceeds this, 2^8 above
 
-// A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 the
-// kernel spilled, into an L1 that shared memory has left 24 KB of.
+// Two warpgroups of softmax and two of values. With 64 queries the softmax halves take 32 queries each (sums
+// stay in registers for a whole unit; 64 spilled, into an L1 that shared memory has left 24 KB of); with 32 or
+// 16, where a step is all latency, they take the two steps of a block. The values' halves take even and odd steps.
 template <int NT>
 struct Shape {
-  static constexpr int kColumns = NT < 32 ? NT : 32;  // queries per softmax thread
-  static constexpr int kGroups = NT / kColumns;       // softmax groups of 128 threads
-  static constexpr int kStages = NT > 32 ? 7 : 8;
-  static constexpr int kSoftmaxThreads = 128 * kGroups;
-  static constexpr int kThreads = 128 + kSoftmaxThreads + 128;  // values, softmax, control
-  // tensor memory columns: scores (two steps), output, a BF16 step's keys, values (two steps), scales of the
-  // keys (two steps) and of the query terms
-  static constexpr int kS = 0, kO = 2 * NT, kK = 3 * NT, kV = kK + 64, kKs = kV + 128, kQs = kKs + 16;
+  static constexpr bool kByStep = NT <= 32;
+  static constexpr int kColumns = kByStep ? NT : NT / 2;  // queries per softmax thread
+  static constexpr int kOut = NT / 2;                     // queries whose output a half rescales and writes
+  static constexpr int kStages = NT > 32 ? 6 : 7;
+  static constexpr int kThreads = 256 + 256 + 128;  // values, softmax, control
+  // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
+  // must not exceed what the launch was given.
+  static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 136, kValueRegs = 72, kControlRegs = 64;
+  static_assert(2 * kSoftmaxRegs + 2 * kValueRegs + kControlRegs <= 5 * kLaunchRegs, "registers");
+  static_assert(kLaunchRegs * kThreads <= 65536, "registers");
+  // tensor memory columns: scores (two blocks of two steps), output, values (two steps; a BF16 step's keys before
+  // its values), scales of the keys (two steps) and of the query terms
+  static constexpr int kS = 0, kO = 4 * NT, kV = kO + NT, kKs = kV + 128, kQs = kKs + 16;
   static_assert(kQs + 8 * kTerms <= 512, "tensor memory");
 };
+
+template <int FROM, int TO>
+__device__ __forceinline__ void trade_registers() {
+  if constexpr (TO > FROM) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TO));
+  if constexpr (TO < FROM) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
+}
 
 template <int NT>
 struct Smem {
@@ -75,21 +87,21 @@ struct Smem {
   alignas(1024) uint8_t q[2][NT * 128];          // FP16: two halves of 64 channels, K-major, 128-byte swizzle
   alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
   alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
-  alignas(1024) uint8_t p[2][16384];               // MN-major: 128-byte rows of 64 queries per token, swizzled
+  alignas(1024) uint8_t p[2][2][16384];            // [block][step] MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
   float factor[NT];
   float total[NT];
-  float col_max[4][NT];
-  float col_sum[4][NT];
+  float col_max[8][NT];
+  float col_sum[8][NT];
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
-  float q_max[16];
+  float q_max[8];
   int parents[BDFP4_MAX_TREE_NODES];
   uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
   uint64_t k_ready[Sh::kStages];  // 64-token pages: the stage's key scales are whole atoms
-  uint64_t ka_full, ka_empty, va_full[2], va_empty[2];
-  uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
+  uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];  // by step
+  uint64_t s_full[2][2], s_empty[2], p_full[2], p_empty[2];  // [block][step] and [block]
   uint64_t q_full, o_full, o_empty, drained;
   long long sums[Sh::kThreads / 32];
   int start_row;
@@ -114,12 +126,14 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-__device__ __forceinline__ bool bar_any(int id, bool pred) {
+__device__ __forceinline__ void softmax_sync() { bar_sync(kSoftmaxBarrier, 256); }
+
+__device__ __forceinline__ bool softmax_any(bool pred) {
   uint32_t out;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(out)
-      : "r"((uint32_t)pred), "r"(id)
+      : "r"((uint32_t)pred), "n"(kSoftmaxBarrier)
       : "memory");
   return out != 0;
 }
@@ -152,12 +166,6 @@ __device__ __forceinline__ void st8(uint32_t address, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(address), "r"(v[0]),
                "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
-}
-
-template <int N>
-__device__ __forceinline__ void tmem_load(uint32_t address, float* v) {
-#pragma unroll
-  for (int j = 0; j < N; j += 16) tc::tmem_ld16(address + j, v + j);
 }
 
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
@@ -272,6 +280,16 @@ struct Walker {
 
 // ---- roles -----------------------------------------------------------------------------------------
 
+// One thread of a converged warp. tcgen05.mma and the bulk copies take their operands from uniform registers:
+// behind an elected predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32
+// (N = 64) to 64 cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its
+// size, and the copies of a step were longer than its HBM time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(elected));
+  return elected != 0;
+}
+
 template <int NT, int PT>
 __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* k_map,
                                         const CUtensorMap* v_map, int lane) {
@@ -304,8 +322,8 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
         int page[kEntries];
 #pragma unroll
         for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
-        if (lane == 0) {
-          tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+        tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+        if (elect_one()) {
           uint8_t* stage = sm.ring[slot];
           tc::mbar_expect_tx(&sm.full_k[slot], 9216);
           tc::mbar_expect_tx(&sm.full_v[slot], 9216);
@@ -374,82 +392,51 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
   __syncwarp();
 }
 
-// One thread of a converged warp. tcgen05.mma takes its descriptors from uniform registers: behind an elected
-// predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32 (N = 64) to 64
-// cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its size.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t elected;
-  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(elected));
-  return elected != 0;
-}
-
-// The whole warp walks and waits; one thread of it issues.
+// The products are issued by two warps, one for the scores and one for the output: an MMA keeps its issuer
+// for 40 to 60 cycles, and the sixteen of a step one after another were longer than the step's HBM time. The
+// whole warp walks and waits; one thread of it issues.
 template <int NT, int PT>
-__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
+__device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
   using Sh = Shape<NT>;
-  constexpr uint32_t kScoresFp4 = tc::nvf4_idesc(128, NT);
-  constexpr uint32_t kScoresF16 = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
+  constexpr uint32_t kFp4 = tc::nvf4_idesc(128, NT), kF16 = f16_idesc(NT, 0, false);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-  const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p);
-  const uint32_t q_codes = tc::smem_u32(sm.q_codes), q_scales = tc::smem_u32(sm.q_scales), ring = tc::smem_u32(sm.ring);
-  int n = 0, unit = 0, slot = 0, bf16_steps = 0;
-  uint32_t turn = 0;
+  const uint32_t q = tc::smem_u32(sm.q), ring = tc::smem_u32(sm.ring);
+  const uint64_t q_codes = tc::fp4_tile_desc(tc::smem_u32(sm.q_codes), 0);
+  const uint64_t q_scales = tc::sf_atom_desc(tc::smem_u32(sm.q_scales));
+  int n = 0, block = 0, unit = 0, slot = 0;
+  uint32_t turn = 0, bf16_turn = 0;  // bf16_turn: one bit per half of the values' threads
   Unit u;
   bool known = false;
   for (; walker.next(u, known); known = true) {
-    auto output = [&](int step, int j) {  // O^T += V^T P^T of step `step` of the unit, the CTA's j-th
-      const StepKind kind = step_kind(u.info, step);
-      const int a = j & 1;
-      tc::mbar_wait(&sm.va_full[a], (j >> 1) & 1, &sm.abort_flag);
-      tc::mbar_wait(&sm.p_full[a], (j >> 1) & 1, &sm.abort_flag);
-      const bool first = step == u.begin;
-      if (first) tc::mbar_wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      const uint64_t tile = tc::smem_desc(prob + a * 16384, tc::kSwizzle128B, 1024, 16384);
-      const uint32_t operand = tmem + Sh::kV + a * 64;
-      if (elect_one()) {
-        if (kind == kStepPage) {
-#pragma unroll
-          for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
-            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kPages, !(first && s == 0));
-        } else {
-          const int slices = step_slices(u.info, kind);
-          for (int s = 0; s < slices; ++s)
-            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kBf16, !(first && s == 0));
-        }
-        tc::commit(&sm.va_empty[a]);
-        tc::commit(&sm.p_empty[a]);
-      }
-      __syncwarp();
-    };
     tc::mbar_wait(&sm.q_full, unit & 1, &sm.abort_flag);
     tc::fence_after_sync();
     if (elect_one()) {
 #pragma unroll
-      for (int i = 0; i < 2 * kTerms; ++i)
-        tc::cp_sf_atom(tmem + Sh::kQs + i * 4, tc::sf_atom_desc(q_scales + i * 512));
+      for (int i = 0; i < 2 * kTerms; ++i) tc::cp_sf_atom(tmem + Sh::kQs + i * 4, q_scales + i * 32);
     }
     __syncwarp();
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const uint32_t scores = tmem + Sh::kS + (n & 1) * NT;
-      tc::mbar_wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
+      const int within = (step - u.begin) & 1, set = block & 1;
+      const uint32_t scores = tmem + Sh::kS + (2 * set + within) * NT;
+      if (within == 0) tc::mbar_wait(&sm.s_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
       if (kind == kStepPage) {
         tc::mbar_wait(PT == 64 ? &sm.k_ready[slot] : &sm.full_k[slot], turn, &sm.abort_flag);
         tc::fence_after_sync();
         const uint32_t stage = ring + slot * kStage;
+        const uint64_t codes = tc::fp4_tile_desc(stage, 0), atoms = tc::sf_atom_desc(stage + kKsOffset);
         const uint32_t scales = tmem + Sh::kKs + (n & 1) * 8;
         if (elect_one()) {
-          tc::cp_sf_atom(scales, tc::sf_atom_desc(stage + kKsOffset));
-          tc::cp_sf_atom(scales + 4, tc::sf_atom_desc(stage + kKsOffset + 512));
+          tc::cp_sf_atom(scales, atoms);
+          tc::cp_sf_atom(scales + 4, atoms + 32);
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
+          for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
 #pragma unroll
             for (int term = 0; term < kTerms; ++term)
-              tc::mma_nvf4(scores, tc::fp4_tile_desc(stage, s), tc::fp4_tile_desc(q_codes + term * NT * 64, s), kScoresFp4,
-                           scales + 4 * s, tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
+              tc::mma_nvf4(scores, codes + 2 * s, q_codes + term * NT * 4 + 2 * s, kFp4, scales + 4 * s,
+                           tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
           }
-          tc::commit(&sm.s_full[n & 1]);
+          tc::commit(&sm.s_full[set][within]);
           tc::commit(&sm.empty[slot]);
         }
         __syncwarp();
@@ -461,25 +448,72 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
           __syncwarp();
           if (++slot == Sh::kStages) slot = 0, turn ^= 1;
         }
-        tc::mbar_wait(&sm.ka_full, bf16_steps++ & 1, &sm.abort_flag);
+        tc::mbar_wait(&sm.ka_full[n & 1], (bf16_turn >> (n & 1)) & 1, &sm.abort_flag);
+        bf16_turn ^= 1u << (n & 1);
         tc::fence_after_sync();
         if (elect_one()) {
 #pragma unroll
           for (int s = 0; s < 8; ++s)
-            mma_ts(scores, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScoresF16, s > 0);
-          tc::commit(&sm.s_full[n & 1]);
-          tc::commit(&sm.ka_empty);
+            mma_ts(scores, tmem + Sh::kV + (n & 1) * 64 + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kF16, s > 0);
+          tc::commit(&sm.s_full[set][within]);
+          tc::commit(&sm.ka_empty[n & 1]);
         }
         __syncwarp();
       }
-      if (step > u.begin) output(step - 1, n - 1);
+      if (within == 1 || step + 1 == u.end) {
+        if (within == 0 && elect_one()) tc::mbar_arrive(&sm.s_full[set][1]);  // a block of one step
+        __syncwarp();
+        ++block;
+      }
     }
-    output(u.end - 1, n - 1);
-    if (elect_one()) tc::commit(&sm.o_full);
-    __syncwarp();
     ++unit;
   }
   int ignore = 0;  // also after an abort: tensor memory is freed behind the last product
+  if (elect_one()) tc::commit(&sm.drained);
+  __syncwarp();
+  tc::mbar_wait(&sm.drained, 0, &ignore);
+}
+
+template <int NT>
+__device__ __forceinline__ void issue_output(Smem<NT>& sm, Walker walker) {
+  using Sh = Shape<NT>;
+  constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  const uint64_t prob = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
+  int n = 0, block = 0, unit = 0;
+  Unit u;
+  bool known = false;
+  for (; walker.next(u, known); known = true) {
+    tc::mbar_wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
+    for (int step = u.begin; step < u.end; ++step, ++n) {
+      const StepKind kind = step_kind(u.info, step);
+      const int within = (step - u.begin) & 1, set = block & 1;
+      tc::mbar_wait(&sm.va_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
+      if (within == 0) tc::mbar_wait(&sm.p_full[set], (block >> 1) & 1, &sm.abort_flag);
+      tc::fence_after_sync();
+      const bool first = step == u.begin, closes = within == 1 || step + 1 == u.end;
+      const uint64_t tile = prob + (2 * set + within) * 1024;
+      const uint32_t operand = tmem + Sh::kV + (n & 1) * 64;
+      if (elect_one()) {
+        if (kind == kStepPage) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
+            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kPages, !(first && s == 0));
+        } else {
+          const int slices = step_slices(u.info, kind);
+          for (int s = 0; s < slices; ++s)
+            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kBf16, !(first && s == 0));
+        }
+        tc::commit(&sm.va_empty[n & 1]);
+        if (closes) tc::commit(&sm.p_empty[set]);
+        if (step + 1 == u.end) tc::commit(&sm.o_full);
+      }
+      __syncwarp();
+      if (closes) ++block;
+    }
+    ++unit;
+  }
+  int ignore = 0;
   if (elect_one()) tc::commit(&sm.drained);
   __syncwarp();
   tc::mbar_wait(&sm.drained, 0, &ignore);
@@ -540,14 +574,18 @@ __device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint3
   st16(a, v);
 }
 
-// The values' warps: thread c holds channel c of every step's V^T, and token c of a BF16 step's K.
+// The values' warps: thread c of a half holds channel c of its steps' V^T, and token c of a BF16 step's K.
 template <int NT, int PT>
-__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker walker, int c) {
+__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
+  const int c = thread & 127, lane = c & 31, half = thread >> 7;
   using Sh = Shape<NT>;
-  const int lane = c & 31;
   const uint32_t lanes = (uint32_t)(c & ~31) << 16;
-  int slot = 0, n = 0, bf16_steps = 0;
-  uint32_t turn = 0;
+  int slot = 0, n = 0;
+  uint32_t turn = 0, bf16_turn = 0;
+  auto pass = [&](int stages) {  // the other half's
+    slot += stages;
+    if (slot >= Sh::kStages) slot -= Sh::kStages, turn ^= 1;
+  };
   auto arrived = [&]() -> uint8_t* {
     tc::mbar_wait(&sm.full_v[slot], turn, &sm.abort_flag);
     return sm.ring[slot];
@@ -555,13 +593,17 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
   auto release = [&] {
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
-    if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+    pass(1);
   };
   Unit u;
   bool known = false;
   for (; walker.next(u, known); known = true) {
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
+      if ((n & 1) != half) {
+        pass(kind == kStepPage ? 1 : 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows));
+        continue;
+      }
       const uint32_t operand = sm.tmem + Sh::kV + (n & 1) * 64 + lanes;
       uint64_t* operand_empty = &sm.va_empty[n & 1];
       const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
@@ -570,7 +612,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
         const uint8_t* scales = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
         tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-#pragma unroll 1
+#pragma unroll 2
         for (int j = 0; j < 4; ++j) {
           const uint8_t* at = PT == 128 ? stage + kVOffset + c * 64 + ((j ^ ((c >> 1) & 3)) * 16)
                                         : stage + kVOffset + (j >> 1) * 4096 + c * 32 + (((j & 1) ^ ((c >> 2) & 1)) * 16);
@@ -581,7 +623,10 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
       } else {
         const int places = bf16_places(u.info, kind);
         const int stages = (places + kBf16Rows - 1) / kBf16Rows;
-        {  // keys; a step's stages are held together
+        // keys first, through the buffer that takes the values after the score product
+        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
+        tc::fence_after_sync();
+        {  // a step's stages are held together
           uint8_t* const stage0 = arrived();
           uint8_t* stage1 = stage0;
           if (stages > 1) {
@@ -615,7 +660,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
                 if (first + (c >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
               }
               tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
-              bar_sync(kValuesBarrier, 128);
+              bar_sync(kValuesBarrier + half, 128);
             }
           }
           const uint4* row = reinterpret_cast<const uint4*>(row_of(min(c, places - 1)));
@@ -633,8 +678,6 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
           float inverse;
           const float scale = fp16_scale(amax, &inverse);
           sm.key_factor[n & 7][c] = inverse;
-          tc::mbar_wait(&sm.ka_empty, (bf16_steps & 1) ^ 1, &sm.abort_flag);
-          tc::fence_after_sync();
 #pragma unroll 1
           for (int quarter = 0; quarter < 4; ++quarter) {
             uint32_t v[16];
@@ -647,17 +690,17 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
               for (int i = 0; i < 4; ++i)
                 v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
             }
-            st16(sm.tmem + Sh::kK + lanes + quarter * 16, v);
+            st16(operand + quarter * 16, v);
           }
           for (int i = 0; i < stages; ++i) release();
           tc::tmem_wait_st();
           tc::fence_before_sync();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&sm.ka_full);
-          ++bf16_steps;
+          if (lane == 0) tc::mbar_arrive(&sm.ka_full[half]);
+          tc::mbar_wait(&sm.ka_empty[half], bf16_turn, &sm.abort_flag);
+          tc::fence_after_sync();
+          bf16_turn ^= 1;
         }
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
         for (int first = 0; first < places; first += kBf16Rows) {
           const uint8_t* stage = arrived() + 2 * c;
           const int slices = (min(places - first, kBf16Rows) + 15) / 16;
@@ -690,8 +733,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
 // still has all four terms above E4M3's smallest scale. Returns what undoes the scaling.
 template <int NT>
 __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
-  using Sh = Shape<NT>;
-  constexpr int kPerPass = Sh::kSoftmaxThreads / 8, kPasses = NT / kPerPass;
+  constexpr int kPerPass = 32, kPasses = (NT + kPerPass - 1) / kPerPass;
   const int group = thread & 7;
   const int queries = u.info.count * p.ratio;
   float v[kPasses][16];
@@ -701,7 +743,7 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
     const int query = u.tile * NT + i * kPerPass + (thread >> 3);
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[i][j] = 0.0f;
-    if (query < queries)
+    if (query < queries && i * kPerPass + (thread >> 3) < NT)
       load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
                        (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
   }
@@ -719,14 +761,15 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
   }
   amax = warp_max(amax);
   if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
-  bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);
+  softmax_sync();
 #pragma unroll
-  for (int w = 0; w < Sh::kSoftmaxThreads / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
+  for (int w = 0; w < 8; ++w) amax = fmaxf(amax, sm.q_max[w]);
   float inverse;
   const float scale = fp16_scale(amax, &inverse);
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = i * kPerPass + (thread >> 3);
+    if (NT < kPerPass && r >= NT) break;
     uint8_t* row = sm.q[group >> 2] + r * 128;
     uint32_t w[8];
 #pragma unroll
@@ -756,7 +799,7 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
     }
   }
   tc::fence_proxy_async_smem();
-  bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);
+  softmax_sync();
   if (thread == 0) tc::mbar_arrive(&sm.q_full);
   return inverse;
 }
@@ -787,158 +830,210 @@ template <int NT>
 __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
   using Sh = Shape<NT>;
   constexpr int C = Sh::kColumns;
-  const int t = thread & 127, lane = thread & 31, warp = t >> 5, group = thread >> 7;
-  const int first_column = group * C;
-  const int barrier = kGroupBarrier + group;
+  const int t = thread & 127, lane = thread & 31, warp = thread >> 5, half = thread >> 7;
+  const int first_column = Sh::kByStep ? 0 : half * C;
   const uint32_t lanes = (uint32_t)(t & ~31) << 16;
-  float* base = sm.base + first_column;
-  float* top = sm.top + first_column;
-  int n = 0, unit = 0;
+  const float* base = sm.base + first_column;
+  int n = 0, block = 0, unit = 0;
   Unit u;
   if (!walker.next(u, false)) return;
   bool more = true;
   float q_inverse = load_queries<NT>(p, sm, u, thread);
   while (more) {
-    for (int j = t; j < C; j += 128) {
-      top[j] = kNoMax;
-      base[j] = kShift - kNoMax;
-      // the draft nodes the query of column j sees
-      const int query = u.tile * NT + first_column + j;
+    if (thread < NT) {
+      sm.top[thread] = kNoMax;
+      sm.base[thread] = kShift - kNoMax;
+      // the draft nodes that this query sees
+      const int query = u.tile * NT + thread;
       uint64_t seen = 0;
       for (int node = min(query / p.ratio, u.info.count - 1); node >= 0;) {
         seen |= 1ull << node;
         const int parent = sm.parents[node];
         node = parent < node ? parent : -1;
       }
-      sm.family[first_column + j] = seen;
+      sm.family[thread] = seen;
     }
     float2 sum[C / 2];
 #pragma unroll
     for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
-    bar_sync(barrier, 128);
+    softmax_sync();
     const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const StepKind kind = step_kind(u.info, step);
-      bool dead;  // no query sees this thread's token
-      if (kind == kStepPage) dead = step == 0 && t < u.info.sink;
-      else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
-      else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-      const bool special = kind != kStepPage || (step == 0 && u.info.sink > 0);  // the same in the whole group
-      const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
-      const int node = t - BDFP4_MAX_SINK;
-      // P of this step goes where the one before the last was
-      tc::mbar_wait(&sm.p_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
-      tc::mbar_wait(&sm.s_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      float f = page_factor;
-      if (kind != kStepPage) f = p.scale_log2 * q_inverse * sm.key_factor[n & 7][t];
-      const float2 f2 = make_float2(f, f);
-      const uint32_t scores = sm.tmem + Sh::kS + (n & 1) * NT + first_column + lanes;
-      uint8_t* const p_row = sm.p[n & 1] + t * 128;
-
-      float s[C];
-      auto load = [&] {
-        tmem_load<C>(scores, s);
-        tc::tmem_wait_ld();
-        if (special) {
+    for (int block_begin = u.begin; block_begin < u.end; block_begin += 2, ++block) {
+      const int steps = min(2, u.end - block_begin), set = block & 1;
+      // this half's steps of the block
+      const int from = Sh::kByStep ? half : 0, to = Sh::kByStep ? min(half + 1, steps) : steps;
+      // One step of the block: its scores in log2 units above the maxima (plus kShift) are f * score + base.
+      struct Step {
+        StepKind kind;
+        bool dead, special, masked;  // special is the same for all tokens
+        float f;
+        uint32_t scores;
+        uint8_t* row;
+      };
+      auto open = [&](int i) {
+        Step k;
+        k.kind = step_kind(u.info, block_begin + i);
+        if (k.kind == kStepPage) k.dead = block_begin + i == 0 && t < u.info.sink;  // no query sees this thread's token
+        else if (k.kind == kStepTail) k.dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
+        else k.dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
+        k.special = k.kind != kStepPage || (block_begin + i == 0 && u.info.sink > 0);
+        k.masked = k.kind == kStepDraft && t >= BDFP4_MAX_SINK && !k.dead;
+        k.f = k.kind == kStepPage ? page_factor : p.scale_log2 * q_inverse * sm.key_factor[(n + i) & 7][t];
+        k.scores = sm.tmem + Sh::kS + (2 * set + i) * NT + first_column + lanes;
+        k.row = sm.p[set][i] + t * 128;
+        return k;
+      };
+      auto mask16 = [&](const Step& k, int j, float* v) {
+        if (k.special) {
 #pragma unroll
-          for (int j = 0; j < C; ++j)
-            if (dead || (masked && !((sm.family[first_column + j] >> node) & 1))) s[j] = -INFINITY;
+          for (int i = 0; i < 16; ++i)
+            if (k.dead || (k.masked && !((sm.family[first_column + j + i] >> (t - BDFP4_MAX_SINK)) & 1))) v[i] = -INFINITY;
         }
       };
-      // The step's probabilities into s and, rounded, into shared memory. True when one of this thread's
-      // exceeds 2^(kShift + kGrowth): its query's maximum has to be renewed, and the step formed again.
-      auto form = [&]() -> bool {
+      // The step's probabilities, added to s in FP32 and stored rounded. True when one of this thread's exceeds
+      // kHighest: its query's maximum has to be renewed, and the block formed again.
+      float s[C];
+      auto form = [&](int i) -> bool {
+        const Step k = open(i);
+        const float2 f2 = make_float2(k.f, k.f);
+        bool high = false;
+        float all[Sh::kByStep ? C : 16];
+        if constexpr (Sh::kByStep) {
 #pragma unroll
-        for (int j = 0; j < C; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(base + j);
-          const float2 y0 = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, make_float2(b.x, b.y));
-          const float2 y1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), f2, make_float2(b.z, b.w));
-          s[j] = ex2(y0.x), s[j + 1] = ex2(y0.y), s[j + 2] = ex2(y1.x), s[j + 3] = ex2(y1.y);
-        }
-        uint32_t w[C / 2];
-        bool high;
-        if (kind == kStepPage) {
-          __half2 most = __floats2half2_rn(0.0f, 0.0f);
-#pragma unroll
-          for (int j = 0; j < C / 2; ++j) {
-            const __half2 pair = __floats2half2_rn(s[2 * j], s[2 * j + 1]);
-            most = __hmax2(most, pair);
-            w[j] = h2(pair);
-          }
-          high = __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
-        } else {
-          float most = 0.0f;
-#pragma unroll
-          for (int j = 0; j < C / 2; ++j) {
-            most = fmaxf(most, fmaxf(s[2 * j], s[2 * j + 1]));
-            w[j] = pack_bf16x2(s[2 * j] * p.inverse_value_scale, s[2 * j + 1] * p.inverse_value_scale);
-          }
-          high = most > kHighest;
+          for (int j = 0; j < C; j += 16) tc::tmem_ld16(k.scores + j, all + j);
+          tc::tmem_wait_ld();
         }
 #pragma unroll
-        for (int j = 0; j < C / 8; ++j)
-          *reinterpret_cast<uint4*>(p_row + ((((first_column >> 3) + j) ^ (t & 7)) * 16)) =
-              make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-        tc::fence_before_sync();
-        tc::fence_proxy_async_smem();
+        for (int j = 0; j < C; j += 16) {
+          float* v = Sh::kByStep ? all + j : all;
+          if constexpr (!Sh::kByStep) {
+            tc::tmem_ld16(k.scores + j, v);
+            tc::tmem_wait_ld();
+          }
+          mask16(k, j, v);
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(base + j + c);
+            const float2 y0 = __ffma2_rn(make_float2(v[c], v[c + 1]), f2, make_float2(b.x, b.y));
+            const float2 y1 = __ffma2_rn(make_float2(v[c + 2], v[c + 3]), f2, make_float2(b.z, b.w));
+            v[c] = ex2(y0.x), v[c + 1] = ex2(y0.y), v[c + 2] = ex2(y1.x), v[c + 3] = ex2(y1.y);
+          }
+          uint32_t w[8];
+          if (k.kind == kStepPage) {
+            __half2 most = __floats2half2_rn(0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const __half2 pair = __floats2half2_rn(v[2 * c], v[2 * c + 1]);
+              most = __hmax2(most, pair);
+              w[c] = h2(pair);
+            }
+            high |= __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
+          } else {
+            float most = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              most = fmaxf(most, fmaxf(v[2 * c], v[2 * c + 1]));
+              w[c] = pack_bf16x2(v[2 * c] * p.inverse_value_scale, v[2 * c + 1] * p.inverse_value_scale);
+            }
+            high |= most > kHighest;
+          }
+          const int chunk = (first_column + j) >> 3;
+          *reinterpret_cast<uint4*>(k.row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(k.row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {
+            const float2 both = __fadd2_rn(make_float2(s[j + c], s[j + c + 1]), make_float2(v[c], v[c + 1]));
+            s[j + c] = both.x, s[j + c + 1] = both.y;
+          }
+        }
         return high;
       };
-      load();
-      if (bar_any(barrier, form())) {
-        load();
-        float mine = 0.0f;
+      auto fence = [&] {
+        tc::fence_before_sync();
+        tc::fence_proxy_async_smem();
+      };
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-          const float m = warp_max(s[j] * f);
-          if (lane == j) mine = m;
+      for (int j = 0; j < C; ++j) s[j] = 0.0f;
+      // P of this block goes where the one before the last was
+      tc::mbar_wait(&sm.p_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
+      bool high = false;
+#pragma unroll 1
+      for (int i = from; i < to; ++i) {
+        tc::mbar_wait(&sm.s_full[set][i], (block >> 1) & 1, &sm.abort_flag);
+        tc::fence_after_sync();
+        high |= form(i);
+      }
+      fence();
+      if (softmax_any(high)) {
+        float mine = -INFINITY;
+#pragma unroll 1
+        for (int i = from; i < to; ++i) {
+          const Step k = open(i);
+#pragma unroll
+          for (int j = 0; j < C; j += 16) {
+            float v[16];
+            tc::tmem_ld16(k.scores + j, v);
+            tc::tmem_wait_ld();
+            mask16(k, j, v);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float m = warp_max(v[c] * k.f);
+              if (lane == j + c) mine = fmaxf(mine, m);
+            }
+          }
         }
         if (lane < C) sm.col_max[warp][first_column + lane] = mine;
-        bar_sync(barrier, 128);
-        if (t < C) {
-          const int col = first_column + t;
-          const float before = top[t];
-          const float now = fmaxf(fmaxf(fmaxf(sm.col_max[0][col], sm.col_max[1][col]),
-                                        fmaxf(sm.col_max[2][col], sm.col_max[3][col])), before);
-          top[t] = now;
-          base[t] = kShift - now;
-          sm.factor[col] = ex2(before - now);
+        softmax_sync();
+        if (thread < NT) {
+          const float before = sm.top[thread];
+          float now = before;
+          const int w0 = Sh::kByStep ? 0 : thread / C * 4;
+#pragma unroll
+          for (int w = 0; w < (Sh::kByStep ? 8 : 4); ++w) now = fmaxf(now, sm.col_max[w0 + w][thread]);
+          sm.top[thread] = now;
+          sm.base[thread] = kShift - now;
+          sm.factor[thread] = ex2(before - now);
         }
-        bar_sync(barrier, 128);
+        softmax_sync();
 #pragma unroll
         for (int j = 0; j < C / 2; ++j) {
           sum[j].x *= sm.factor[first_column + 2 * j];
           sum[j].y *= sm.factor[first_column + 2 * j + 1];
         }
-        form();
-        if (step > u.begin) {  // what O^T holds is of the old maxima
-          tc::mbar_wait(&sm.p_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, &sm.abort_flag);
+#pragma unroll
+        for (int j = 0; j < C; ++j) s[j] = 0.0f;
+#pragma unroll 1
+        for (int i = from; i < to; ++i) form(i);
+        if (block_begin > u.begin) {  // what O^T holds is of the old maxima
+          tc::mbar_wait(&sm.p_empty[set ^ 1], ((block - 1) >> 1) & 1, &sm.abort_flag);
           tc::fence_after_sync();
 #pragma unroll 1
-          for (int j = 0; j < C; j += 16) {
-            float o[16];
-            const uint32_t at = sm.tmem + Sh::kO + first_column + j + lanes;
-            tc::tmem_ld16(at, o);
+          for (int j = half * Sh::kOut; j < (half + 1) * Sh::kOut; j += 8) {
+            float o[8];
+            uint32_t r[8];
+            const uint32_t at = sm.tmem + Sh::kO + j + lanes;
+            tc::tmem_ld8(at, o);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= sm.factor[first_column + j + i];
-            tc::tmem_st16(at, o);
+            for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(o[i] * sm.factor[j + i]);
+            st8(at, r);
           }
           tc::tmem_wait_st();
-          tc::fence_before_sync();
         }
-        bar_sync(barrier, 128);
+        fence();
+        softmax_sync();
       }
-      // the group's barrier stands behind every thread's scores read and probabilities written
-      if (t == 0) {
-        tc::mbar_arrive(&sm.p_full[n & 1]);
-        tc::mbar_arrive(&sm.s_empty[n & 1]);
+      // the barrier stands behind every thread's scores read and probabilities written
+      if (thread == 0) {
+        tc::mbar_arrive(&sm.p_full[set]);
+        tc::mbar_arrive(&sm.s_empty[set]);
       }
 #pragma unroll
       for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
+      n += steps;
     }
 
-    {  // each query's weight: first over a warp's 32 tokens, then (below) over the four warps
+    {  // each query's weight: first over a warp's 32 tokens, then (below) over the warps
       float v[C];
 #pragma unroll
       for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
@@ -948,40 +1043,42 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     Unit following = u;
     more = walker.next(following, true);
     float next_inverse = 1.0f;
-    bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);  // both groups have seen their last scores; the parents are free
-    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
-    bar_sync(barrier, 128);
+    softmax_sync();  // the column sums are there; the parents are free
     const bool whole = u.begin == 0 && u.end == u.info.steps;
     // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
     const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
-    for (int j = t; j < C; j += 128) {
-      const int col = first_column + j;
-      const float total = (sm.col_sum[0][col] + sm.col_sum[1][col]) + (sm.col_sum[2][col] + sm.col_sum[3][col]);
+    if (thread < NT) {
+      const int w0 = Sh::kByStep ? 0 : thread / C * 4;
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < (Sh::kByStep ? 8 : 4); ++w) total += sm.col_sum[w0 + w][thread];
       if (whole) {
-        sm.total[col] = total > 0.0f ? p.value_scale / total : 0.0f;
+        sm.total[thread] = total > 0.0f ? p.value_scale / total : 0.0f;
       } else {
-        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[j];
-        p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
+        p.partial_stat[(int64_t)(2 * part) * NT + thread] = sm.top[thread];
+        p.partial_stat[(int64_t)(2 * part + 1) * NT + thread] = total;
       }
     }
-    bar_sync(barrier, 128);
+    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
+    softmax_sync();
     tc::mbar_wait(&sm.o_full, unit & 1, &sm.abort_flag);
     tc::fence_after_sync();
-    const int queries = min(u.info.count * p.ratio - u.tile * NT - first_column, C);
-    int query = u.tile * NT + first_column;
+    const int out_first = half * Sh::kOut;
+    const int queries = min(u.info.count * p.ratio - u.tile * NT - out_first, Sh::kOut);
+    const int query = u.tile * NT + out_first;
     int out_node = query / p.ratio, out_head = query % p.ratio;
     __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
-    float* partial = p.partial + ((int64_t)part * NT + first_column) * kHeadDim + t;
-#pragma unroll
-    for (int j = 0; j < C; j += 16) {
-      float o[16];
-      tc::tmem_ld16(sm.tmem + Sh::kO + first_column + j + lanes, o);
+    float* partial = p.partial + ((int64_t)part * NT + out_first) * kHeadDim + t;
+#pragma unroll 1
+    for (int j = 0; j < Sh::kOut; j += 8) {
+      float o[8];
+      tc::tmem_ld8(sm.tmem + Sh::kO + out_first + j + lanes, o);
       tc::tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         if (j + i < queries) {
           if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[first_column + j + i]);
+            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[out_first + j + i]);
             if (++out_head == p.ratio) out_head = 0, ++out_node;
           } else {
             partial[(int64_t)(j + i) * kHeadDim] = o[i];
@@ -990,9 +1087,8 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       }
     }
     tc::fence_before_sync();
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.o_empty);
-    bar_sync(barrier, 128);  // base, top and total are written anew
+    softmax_sync();  // the output has been read; base, top and total are written anew
+    if (thread == 0) tc::mbar_arrive(&sm.o_empty);
     if (!whole && u.begin == 0 && thread == 0) {
       TreeSplit split;
       split.row = u.row;
@@ -1033,19 +1129,20 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       tc::mbar_init(&sm.k_ready[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&sm.ka_full[i], 4);
+      tc::mbar_init(&sm.ka_empty[i], 1);
       tc::mbar_init(&sm.va_full[i], 4);
       tc::mbar_init(&sm.va_empty[i], 1);
-      tc::mbar_init(&sm.s_full[i], 1);
-      tc::mbar_init(&sm.s_empty[i], Sh::kGroups);
-      tc::mbar_init(&sm.p_full[i], Sh::kGroups);
+      tc::mbar_init(&sm.s_full[i][0], 1);
+      tc::mbar_init(&sm.s_full[i][1], 1);
+      tc::mbar_init(&sm.s_empty[i], 1);
+      tc::mbar_init(&sm.p_full[i], 1);
       tc::mbar_init(&sm.p_empty[i], 1);
     }
-    tc::mbar_init(&sm.ka_full, 4);
-    tc::mbar_init(&sm.ka_empty, 1);
     tc::mbar_init(&sm.q_full, 1);
     tc::mbar_init(&sm.o_full, 1);
-    tc::mbar_init(&sm.o_empty, 4 * Sh::kGroups);
-    tc::mbar_init(&sm.drained, 1);
+    tc::mbar_init(&sm.o_empty, 1);
+    tc::mbar_init(&sm.drained, 2);
     tc::fence_barrier_init();
     sm.abort_flag = 0;
     TreeSplit none;
@@ -1095,16 +1192,18 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   tc::fence_after_sync();
   if (sm.first < sm.last) {
     const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
-    if (warp < 4) {
+    if (warp < 8) {
+      trade_registers<Sh::kLaunchRegs, Sh::kValueRegs>();
       values<NT, PT>(p, sm, walker, thread);
-    } else if (warp < 4 + 4 * Sh::kGroups) {
-      softmax<NT>(p, sm, walker, thread - 128);
-    } else if (warp == 4 + 4 * Sh::kGroups) {
-      produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
-    } else if (warp == 5 + 4 * Sh::kGroups) {
-      issue<NT, PT>(sm, walker);
-    } else if (PT == 64 && warp == 6 + 4 * Sh::kGroups) {
-      interleave_scales<NT>(sm, walker, lane);
+    } else if (warp < 16) {
+      trade_registers<Sh::kLaunchRegs, Sh::kSoftmaxRegs>();
+      softmax<NT>(p, sm, walker, thread - 256);
+    } else {
+      trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
+      if (warp == 16) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
+      if (warp == 17) issue_scores<NT, PT>(sm, walker);
+      if (warp == 18) issue_output<NT>(sm, walker);
+      if (PT == 64 && warp == 19) interleave_scales<NT>(sm, walker, lane);
     }
   }
   tc::fence_before_sync();
