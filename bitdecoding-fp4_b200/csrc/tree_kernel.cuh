@@ -290,12 +290,15 @@ __device__ __forceinline__ bool elect_one() {
   return elected != 0;
 }
 
-template <int NT, int PT>
-__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* k_map,
-                                        const CUtensorMap* v_map, int lane) {
+// One side's copies: SIDE 0 brings a page's key codes and scales, SIDE 1 its values' and the rows of the BF16
+// steps. Two warps, because a copy keeps its issuer for 80 cycles and a step of 64-token pages has eight.
+template <int NT, int PT, int SIDE>
+__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* map, int lane) {
   using Sh = Shape<NT>;
   constexpr int kEntries = kPage / PT;
   const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
+  const int64_t codes_pitch = p.codes_pitch[SIDE], scales_pitch = p.scales_pitch[SIDE];
+  uint64_t* full = SIDE ? sm.full_v : sm.full_k;
   int slot = 0, issued = 0;
   uint32_t turn = 0;
   auto advance = [&] {
@@ -306,6 +309,8 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
   bool known = false;
   for (; walker.next(u, known); known = true) {
     const int32_t* table = p.table + u.row * p.table_stride;
+    const uint8_t* codes = p.codes[SIDE] + u.head * (PT == 128 ? 8192 : 4096);
+    const uint8_t* scales = p.scales[SIDE] + u.head * (PT == 128 ? 1024 : 512);
     const int stop = min(u.end, u.info.pages);
     for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
       const int entry = batch * kEntries + lane;
@@ -325,23 +330,16 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
         tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
         if (elect_one()) {
           uint8_t* stage = sm.ring[slot];
-          tc::mbar_expect_tx(&sm.full_k[slot], 9216);
-          tc::mbar_expect_tx(&sm.full_v[slot], 9216);
+          tc::mbar_expect_tx(&full[slot], 9216);
           if constexpr (PT == 128) {
-            tc::tma_load_4d(stage, k_map, &sm.full_k[slot], 0, u.head, 0, page[0]);
-            tc::bulk_load(stage + kKsOffset, p.scales[0] + page[0] * p.scales_pitch[0] + u.head * 1024, 1024, &sm.full_k[slot]);
-            tc::tma_load_3d(stage + kVOffset, v_map, &sm.full_v[slot], 0, u.head * kHeadDim, page[0]);
-            tc::bulk_load(stage + kVsOffset, p.scales[1] + page[0] * p.scales_pitch[1] + u.head * 1024, 1024, &sm.full_v[slot]);
+            if constexpr (SIDE == 0) tc::tma_load_4d(stage, map, &full[slot], 0, u.head, 0, page[0]);
+            else tc::tma_load_3d(stage + kVOffset, map, &full[slot], 0, u.head * kHeadDim, page[0]);
+            tc::bulk_load(stage + (SIDE ? kVsOffset : kKsOffset), scales + page[0] * scales_pitch, 1024, &full[slot]);
           } else {
 #pragma unroll
             for (int e = 0; e < kEntries; ++e) {
-              tc::bulk_load(stage + e * 4096, p.codes[0] + page[e] * p.codes_pitch[0] + u.head * 4096, 4096, &sm.full_k[slot]);
-              tc::bulk_load(stage + kKsOffset + e * 512, p.scales[0] + page[e] * p.scales_pitch[0] + u.head * 512, 512,
-                            &sm.full_k[slot]);
-              tc::bulk_load(stage + kVOffset + e * 4096, p.codes[1] + page[e] * p.codes_pitch[1] + u.head * 4096, 4096,
-                            &sm.full_v[slot]);
-              tc::bulk_load(stage + kVsOffset + e * 512, p.scales[1] + page[e] * p.scales_pitch[1] + u.head * 512, 512,
-                            &sm.full_v[slot]);
+              tc::bulk_load(stage + (SIDE ? kVOffset : 0) + e * 4096, codes + page[e] * codes_pitch, 4096, &full[slot]);
+              tc::bulk_load(stage + (SIDE ? kVsOffset : kKsOffset) + e * 512, scales + page[e] * scales_pitch, 512, &full[slot]);
             }
           }
         }
@@ -358,21 +356,22 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
                                           : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
         const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
         for (int first = 0; first < places; first += kBf16Rows) {
-          const int end = min(first + kBf16Rows, places);
-          if (lane == 0) {
-            tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+          tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+          if (SIDE == 0) {
+            if (lane == 0) tc::mbar_arrive(&full[slot]);  // nothing for the FP4 product here
+          } else {
+            const int end = min(first + kBf16Rows, places);
             // the sink's places behind its length stay empty
             const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
-            tc::mbar_expect_tx(&sm.full_v[slot], (end - first - absent) * 256);
-            tc::mbar_arrive(&sm.full_k[slot]);  // nothing for the FP4 product here
-          }
-          __syncwarp();
-          for (int i = first + lane; i < end; i += 32) {
-            const __nv_bfloat16* source = nullptr;
-            if (kind == kStepTail) source = tail + i * tail_row;
-            else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
-            else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
-            if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, &sm.full_v[slot]);
+            if (lane == 0) tc::mbar_expect_tx(&full[slot], (end - first - absent) * 256);
+            __syncwarp();
+            for (int i = first + lane; i < end; i += 32) {
+              const __nv_bfloat16* source = nullptr;
+              if (kind == kStepTail) source = tail + i * tail_row;
+              else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
+              else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
+              if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, &full[slot]);
+            }
           }
           __syncwarp();
           advance();
@@ -385,8 +384,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
     int ignore = 0;
     for (int back = min(issued, Sh::kStages); back > 0; --back) {
       const int at = issued - back;
-      tc::mbar_wait(&sm.full_k[at % Sh::kStages], (at / Sh::kStages) & 1, &ignore);
-      tc::mbar_wait(&sm.full_v[at % Sh::kStages], (at / Sh::kStages) & 1, &ignore);
+      tc::mbar_wait(&full[at % Sh::kStages], (at / Sh::kStages) & 1, &ignore);
     }
   }
   __syncwarp();
@@ -521,43 +519,16 @@ __device__ __forceinline__ void issue_output(Smem<NT>& sm, Walker walker) {
 
 // 64-token pages: the key scales of a step's two pages come as half atoms (32 rows of 8 bytes); one warp
 // interleaves them, in place, into the two whole atoms the MMA reads.
-template <int NT>
-__device__ __forceinline__ void interleave_scales(Smem<NT>& sm, Walker walker, int lane) {
-  int slot = 0;
-  uint32_t turn = 0;
-  auto advance = [&] {
-    if (++slot == Shape<NT>::kStages) slot = 0, turn ^= 1;
-  };
-  Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
-    for (int step = u.begin; step < u.end; ++step) {
-      const StepKind kind = step_kind(u.info, step);
-      if (kind == kStepPage) {
-        tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);
-        uint8_t* scales = sm.ring[slot] + kKsOffset;
-        uint2 half[2][2];
+__device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
+  uint2 part[2][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) half[i & 1][i >> 1] = *reinterpret_cast<const uint2*>(scales + (i >> 1) * 512 + (i & 1) * 256 + lane * 8);
-        __syncwarp();
+  for (int i = 0; i < 4; ++i) part[i & 1][i >> 1] = *reinterpret_cast<const uint2*>(scales + (i >> 1) * 512 + (i & 1) * 256 + lane * 8);
+  __syncwarp();
 #pragma unroll
-        for (int atom = 0; atom < 2; ++atom)
-          *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) =
-              make_uint4(half[atom][0].x, half[atom][0].y, half[atom][1].x, half[atom][1].y);
-        tc::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
-        advance();
-      } else {
-        for (int i = 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows); i > 0; --i) {
-          tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);
-          if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
-          __syncwarp();
-          advance();
-        }
-      }
-    }
-  }
+  for (int atom = 0; atom < 2; ++atom)
+    *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) = make_uint4(part[atom][0].x, part[atom][0].y, part[atom][1].x, part[atom][1].y);
+  tc::fence_proxy_async_smem();
+  __syncwarp();
 }
 
 // Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane. The caller's
@@ -590,6 +561,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
     tc::mbar_wait(&sm.full_v[slot], turn, &sm.abort_flag);
     return sm.ring[slot];
   };
+  const bool interleaves = PT == 64 && (c >> 5) == 3;
   auto release = [&] {
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
@@ -608,6 +580,11 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
       uint64_t* operand_empty = &sm.va_empty[n & 1];
       const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
       if (kind == kStepPage) {
+        if (interleaves) {
+          tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);
+          interleave_scales(sm.ring[slot] + kKsOffset, lane);
+          if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
+        }
         const uint8_t* stage = arrived();
         const uint8_t* scales = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
         tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
@@ -692,7 +669,10 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
             }
             st16(operand + quarter * 16, v);
           }
-          for (int i = 0; i < stages; ++i) release();
+          for (int i = 0; i < stages; ++i) {
+            if (interleaves && lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);  // its phases follow the stage's uses
+            release();
+          }
           tc::tmem_wait_st();
           tc::fence_before_sync();
           __syncwarp();
@@ -717,6 +697,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
             }
             st8(operand + (place >> 4) * 8, v);
           }
+          if (interleaves && lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
           release();
         }
       }
@@ -1200,10 +1181,10 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       softmax<NT>(p, sm, walker, thread - 256);
     } else {
       trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
-      if (warp == 16) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
-      if (warp == 17) issue_scores<NT, PT>(sm, walker);
-      if (warp == 18) issue_output<NT>(sm, walker);
-      if (PT == 64 && warp == 19) interleave_scales<NT>(sm, walker, lane);
+      if (warp == 16) produce<NT, PT, 0>(p, sm, walker, &k_map, lane);
+      if (warp == 17) produce<NT, PT, 1>(p, sm, walker, &v_map, lane);
+      if (warp == 18) issue_scores<NT, PT>(sm, walker);
+      if (warp == 19) issue_output<NT>(sm, walker);
     }
   }
   tc::fence_before_sync();
