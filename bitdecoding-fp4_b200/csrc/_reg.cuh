@@ -4,21 +4,27 @@
 // tokens at a time,
 //     S^T [token, query]   = K   [token, channel]  * Q^T
 //     O^T [channel, query] = V^T [channel, token] * P^T
-// both as tcgen05.mma.kind::f16 with the cache operand A in tensor memory and the query-side operand B in
-// shared memory. E2M1 x E4M3 has at most six significant bits and lies in [2^-10, 2688], so a page's values
-// are exact in FP16: a thread reads its own token's (K) or channel's (V) 64 code bytes, converts and scales
-// them in registers and stores them straight into its tensor-memory lane; the dequantized tile never passes
-// through shared memory. P is stored as the softmax threads hold it, one token per thread with its queries
-// contiguous, which is the MN-major form of B.
 //
-// Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: a step votes
-// whether any score exceeds its query's maximum by more than 2^8, and only then are the maxima taken anew
-// (across threads) and O^T rescaled. Sums stay per thread until the unit ends. Probabilities carry a factor
+// S^T over a page is the block-scaled FP4 product of the codes as they lie in the cache (kind::mxf4nvf4, no
+// dequantization) with the query written as a sum of four FP4 terms, each the rounding of what the ones
+// before left: a term leaves at most 0.177 of its group's largest value (half a step of 2/6, the E4M3
+// scale's rounding included), four leave 10^-3, less than the BF16 rounding the query came with. Four terms
+// of K = 64 take the tensor time of one FP16 product.
+//
+// O^T over a page is a kind::f16 product with V^T in tensor memory: E2M1 x E4M3 has at most six significant
+// bits and lies in [2^-10, 2688], so a page's values are exact in FP16. A thread reads its own channel's 64
+// code bytes, converts and scales them in registers and stores them straight into its tensor-memory lane; the
+// dequantized tile never passes through shared memory. P is stored as the softmax threads hold it, one token
+// per thread with its queries contiguous, which is the MN-major form of operand B.
+//
+// Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: probabilities are
+// formed against them at once, and only when one comes out more than 2^8 above its maximum (the barrier
+// that ends a step carries that vote) are the maxima taken anew, O^T rescaled and the step formed again. Sums stay per thread until the unit ends. Probabilities carry a factor
 // 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
 //
-// The rolling tail and the drafts with the sink are two more steps of the same form over BF16 values: K is
-// scaled per token by a power of two into FP16's range (the softmax thread of the token undoes it), V and
-// P are BF16. Queries are scaled per tile the same way.
+// The rolling tail and the drafts with the sink are two more steps over BF16 values, both products kind::f16
+// with the cache side in tensor memory: K is scaled per token by a power of two into FP16's range (the softmax
+// thread of the token undoes it), V and P are BF16. Queries are scaled per tile the same way.
 //
 // Work is the sequence of all steps of all (row, head, tile) units, cut into equal runs, one per CTA, so any
 // mix of lengths is balanced; a unit that straddles CTAs leaves unnormalised parts that a second kernel adds.
@@ -40,35 +46,32 @@ constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
 // A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
 // 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
 constexpr int kBf16Pitch = 272, kBf16Rows = 64;
+// Named barriers: the softmax threads, the two halves of the values' threads.
+constexpr int kSoftmaxBarrier = 1, kValuesBarrier = 2;
+constexpr int kTerms = 4;             // FP4 terms of a query
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
-constexpr float kGrowth = 8.0f;     // a maximum is renewed when a score exceeds it by more than this (log2)
+constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renewed when one exceeds this, 2^8 above
 
-// A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (128
-// threads for NT = 64, 256 for 128) the kernel spilled, into an L1 that shared memory has left 24 KB of.
+// Two warpgroups of softmax and two of values. With 64 queries the softmax halves take 32 queries each (sums
+// stay in registers for a whole unit; 64 spilled, into an L1 that shared memory has left 24 KB of); with 32 or
+// 16, where a step is all latency, they take the two steps of a block. The values' halves take even and odd steps.
 template <int NT>
 struct Shape {
-  static constexpr int kColumns = NT < 32 ? NT : 32;        // queries per softmax thread
-  static constexpr int kGroups = NT / kColumns;             // softmax groups of 128 threads
-  static constexpr int kBlocks = (NT + 63) / 64;            // 128-byte rows of P per token
-  static constexpr int kKBuffers = NT > 96 ? 1 : 2;         // operand buffers in tensor memory, as many as it holds
-  static constexpr int kVBuffers = NT > 64 ? 1 : 2;
-  static constexpr int kStages = NT > 96 ? 5 : NT > 64 ? 6 : 8;
-  static constexpr int kSoftmaxThreads = 128 * kGroups;
-  static constexpr int kThreads = 256 + kSoftmaxThreads + 128;  // keys, values, softmax, control (two of its warps idle)
+  static constexpr bool kByStep = NT <= 32;
+  static constexpr int kColumns = kByStep ? NT : NT / 2;  // queries per softmax thread
+  static constexpr int kOut = NT / 2;                     // queries whose output a half rescales and writes
+  static constexpr int kStages = NT > 32 ? 6 : 7;
+  static constexpr int kThreads = 256 + 256 + 128;  // values, softmax, control
   // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
   // must not exceed what the launch was given.
-  static constexpr int kLaunchRegs = kGroups == 4 ? 72 : kGroups == 3 ? 80 : kGroups == 2 ? 96 : 128;
-  static constexpr int kSoftmaxRegs = kGroups == 4 ? 80 : kGroups == 3 ? 96 : kGroups == 2 ? 112 : 144;
-  static constexpr int kKeyRegs = kGroups == 4 ? 80 : kGroups == 3 ? 88 : kGroups == 2 ? 112 : 152;
-  static constexpr int kValueRegs = kGroups == 4 ? 64 : kGroups == 3 ? 64 : kGroups == 2 ? 88 : 128;
-  static constexpr int kControlRegs = kGroups == 4 ? 40 : kGroups == 3 ? 40 : kGroups == 2 ? 56 : 88;
-  static_assert(kSoftmaxRegs * kGroups + kKeyRegs + kValueRegs + kControlRegs <= kLaunchRegs * (3 + kGroups), "registers");
+  static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 136, kValueRegs = 72, kControlRegs = 64;
+  static_assert(2 * kSoftmaxRegs + 2 * kValueRegs + kControlRegs <= 5 * kLaunchRegs, "registers");
   static_assert(kLaunchRegs * kThreads <= 65536, "registers");
-  static constexpr bool kHold = kGroups <= 2;  // a thread's scores stay in registers between the vote and the exponentials
-  // tensor memory columns
-  static constexpr int kS = 0, kO = 2 * NT, kK = 3 * NT, kV = kK + 64 * kKBuffers;
-  static_assert(kV + 64 * kVBuffers <= 512, "tensor memory");
+  // tensor memory columns: scores (two blocks of two steps), output, values (two steps; a BF16 step's keys before
+  // its values), scales of the keys (two steps) and of the query terms
+  static constexpr int kS = 0, kO = 4 * NT, kV = kO + NT, kKs = kV + 128, kQs = kKs + 16;
+  static_assert(kQs + 8 * kTerms <= 512, "tensor memory");
 };
 
 template <int FROM, int TO>
@@ -81,27 +84,30 @@ template <int NT>
 struct Smem {
   using Sh = Shape<NT>;
   alignas(1024) uint8_t ring[Sh::kStages][kStage];
-  alignas(1024) uint8_t q[2][NT * 128];  // two halves of 64 channels, K-major, 128-byte swizzle
-  alignas(1024) uint8_t p[2][Sh::kBlocks * 16384];  // MN-major: 128-byte rows of 64 queries per token, swizzled
+  alignas(1024) uint8_t q[2][NT * 128];          // FP16: two halves of 64 channels, K-major, 128-byte swizzle
+  alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
+  alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
+  alignas(1024) uint8_t p[2][2][16384];            // [block][step] MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
   float factor[NT];
   float total[NT];
-  float col_max[4][NT];
-  float col_sum[4][NT];
+  float col_max[8][NT];
+  float col_sum[8][NT];
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
-  float q_max[16];
+  float q_max[8];
   int parents[BDFP4_MAX_TREE_NODES];
   uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
-  uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];
-  uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
+  uint64_t k_ready[Sh::kStages];  // 64-token pages: the stage's key scales are whole atoms
+  uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];  // by step
+  uint64_t s_full[2][2], s_empty[2], p_full[2], p_empty[2];  // [block][step] and [block]
   uint64_t q_full, o_full, o_empty, drained;
   long long sums[Sh::kThreads / 32];
   int start_row;
   long long start_offset, first, last, per_cta;
   uint32_t tmem;
-  int abort_flag;
+  int abort_flag, ignored_flag;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -120,12 +126,14 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-__device__ __forceinline__ bool bar_any(int id, bool pred) {
+__device__ __forceinline__ void softmax_sync() { bar_sync(kSoftmaxBarrier, 256); }
+
+__device__ __forceinline__ bool softmax_any(bool pred) {
   uint32_t out;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(out)
-      : "r"((uint32_t)pred), "r"(id)
+      : "r"((uint32_t)pred), "n"(kSoftmaxBarrier)
       : "memory");
   return out != 0;
 }
@@ -173,27 +181,24 @@ __device__ __forceinline__ void dequantize8(uint32_t codes, __half2 scale, uint3
   for (int i = 0; i < 4; ++i) out[i] = h2(__hmul2(*reinterpret_cast<__half2*>(&v[i]), scale));
 }
 
-// Four E4M3 bytes -> four FP16 pairs (scale, scale).
+// Two E4M3 bytes -> two FP16 pairs (scale, scale).
 __device__ __forceinline__ void scale_pairs(uint32_t bytes, __half2* out) {
-  uint32_t lo, hi;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(bytes));
-  const __half2 a = *reinterpret_cast<__half2*>(&lo), b = *reinterpret_cast<__half2*>(&hi);
-  out[0] = __low2half2(a);
-  out[1] = __high2half2(a);
-  out[2] = __low2half2(b);
-  out[3] = __high2half2(b);
+  uint32_t both;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(both) : "r"(bytes));
+  const __half2 pair = *reinterpret_cast<__half2*>(&both);
+  out[0] = __low2half2(pair);
+  out[1] = __high2half2(pair);
 }
 
-// The power of two that brings `amax` into [2^14, 2^15), and its inverse. Zero, infinite or NaN: 1.
+// The power of two that brings `amax` into [2^10, 2^11), where FP16 has 25 binades below and the FP4 terms'
+// E4M3 scales (up to 448 = 2688 / 6) reach their fourth, and its inverse. Zero, infinite or NaN: 1.
 __device__ __forceinline__ float fp16_scale(float amax, float* inverse) {
   const int e = (int)((__float_as_uint(amax) >> 23) & 0xffu);
   if (e == 0 || e == 255) {
     *inverse = 1.0f;
     return 1.0f;
   }
-  const int field = min(127 + 14 + 127 - e, 253);
+  const int field = min(127 + 10 + 127 - e, 253);
   *inverse = __uint_as_float((uint32_t)(254 - field) << 23);
   return __uint_as_float((uint32_t)field << 23);
 }
@@ -275,12 +280,50 @@ struct Walker {
 
 // ---- roles -----------------------------------------------------------------------------------------
 
-template <int NT, int PT>
-__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* k_map,
-                                        const CUtensorMap* v_map, int lane) {
+// The roles' loops run side by side on every scheduler and share its instruction cache, so waiting is a dozen
+// instructions, one when the phase is already over. After about two seconds, or once another thread has given
+// up, a wait ends without its phase; the roles go through the rest of their motions and the kernel reports it.
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 begin, now;\n\t.reg .b32 given_up;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+      "@p bra OVER;\n\t"
+      "mov.u64 begin, %%globaltimer;\n"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+      "@p bra OVER;\n\t"
+      "ld.volatile.shared.b32 given_up, [%2];\n\t"
+      "setp.ne.b32 p, given_up, 0;\n\t"
+      "@p bra OVER;\n\t"
+      "mov.u64 now, %%globaltimer;\n\t"
+      "sub.u64 now, now, begin;\n\t"
+      "setp.lt.u64 p, now, %3;\n\t"
+      "@p bra AGAIN;\n\t"
+      "st.volatile.shared.b32 [%2], 1;\n"
+      "OVER:\n\t}" ::"r"(tc::smem_u32(bar)),
+      "r"(parity), "r"(tc::smem_u32(abort_flag)), "n"(tc::kWaitLimitNs)
+      : "memory");
+}
+
+// One thread of a converged warp. tcgen05.mma and the bulk copies take their operands from uniform registers:
+// behind an elected predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32
+// (N = 64) to 64 cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its
+// size, and the copies of a step were longer than its HBM time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(elected));
+  return elected != 0;
+}
+
+// One side's copies: SIDE 0 brings a page's key codes and scales, SIDE 1 its values' and the rows of the BF16
+// steps. Two warps, because a copy keeps its issuer for 80 cycles and a step of 64-token pages has eight.
+template <int NT, int PT, int SIDE>
+__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* map, int lane) {
   using Sh = Shape<NT>;
   constexpr int kEntries = kPage / PT;
   const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
+  const int64_t codes_pitch = p.codes_pitch[SIDE], scales_pitch = p.scales_pitch[SIDE];
+  uint64_t* full = SIDE ? sm.full_v : sm.full_k;
   int slot = 0, issued = 0;
   uint32_t turn = 0;
   auto advance = [&] {
@@ -291,6 +334,8 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
   bool known = false;
   for (; walker.next(u, known); known = true) {
     const int32_t* table = p.table + u.row * p.table_stride;
+    const uint8_t* codes = p.codes[SIDE] + u.head * (PT == 128 ? 8192 : 4096);
+    const uint8_t* scales = p.scales[SIDE] + u.head * (PT == 128 ? 1024 : 512);
     const int stop = min(u.end, u.info.pages);
     for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
       const int entry = batch * kEntries + lane;
@@ -307,26 +352,19 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
         int page[kEntries];
 #pragma unroll
         for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
-        if (lane == 0) {
-          tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+        wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+        if (elect_one()) {
           uint8_t* stage = sm.ring[slot];
-          tc::mbar_expect_tx(&sm.full_k[slot], 9216);
-          tc::mbar_expect_tx(&sm.full_v[slot], 9216);
+          tc::mbar_expect_tx(&full[slot], 9216);
           if constexpr (PT == 128) {
-            tc::tma_load_4d(stage, k_map, &sm.full_k[slot], 0, u.head, 0, page[0]);
-            tc::bulk_load(stage + kKsOffset, p.scales[0] + page[0] * p.scales_pitch[0] + u.head * 1024, 1024, &sm.full_k[slot]);
-            tc::tma_load_3d(stage + kVOffset, v_map, &sm.full_v[slot], 0, u.head * kHeadDim, page[0]);
-            tc::bulk_load(stage + kVsOffset, p.scales[1] + page[0] * p.scales_pitch[1] + u.head * 1024, 1024, &sm.full_v[slot]);
+            if constexpr (SIDE == 0) tc::tma_load_4d(stage, map, &full[slot], 0, u.head, 0, page[0]);
+            else tc::tma_load_3d(stage + kVOffset, map, &full[slot], 0, u.head * kHeadDim, page[0]);
+            tc::bulk_load(stage + (SIDE ? kVsOffset : kKsOffset), scales + page[0] * scales_pitch, 1024, &full[slot]);
           } else {
 #pragma unroll
             for (int e = 0; e < kEntries; ++e) {
-              tc::bulk_load(stage + e * 4096, p.codes[0] + page[e] * p.codes_pitch[0] + u.head * 4096, 4096, &sm.full_k[slot]);
-              tc::bulk_load(stage + kKsOffset + e * 512, p.scales[0] + page[e] * p.scales_pitch[0] + u.head * 512, 512,
-                            &sm.full_k[slot]);
-              tc::bulk_load(stage + kVOffset + e * 4096, p.codes[1] + page[e] * p.codes_pitch[1] + u.head * 4096, 4096,
-                            &sm.full_v[slot]);
-              tc::bulk_load(stage + kVsOffset + e * 512, p.scales[1] + page[e] * p.scales_pitch[1] + u.head * 512, 512,
-                            &sm.full_v[slot]);
+              tc::bulk_load(stage + (SIDE ? kVOffset : 0) + e * 4096, codes + page[e] * codes_pitch, 4096, &full[slot]);
+              tc::bulk_load(stage + (SIDE ? kVsOffset : kKsOffset) + e * 512, scales + page[e] * scales_pitch, 512, &full[slot]);
             }
           }
         }
@@ -343,22 +381,22 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
                                           : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
         const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
         for (int first = 0; first < places; first += kBf16Rows) {
-          const int end = min(first + kBf16Rows, places);
-          uint64_t* full = side ? &sm.full_v[slot] : &sm.full_k[slot];
-          if (lane == 0) {
-            tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+          wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+          if (SIDE == 0) {
+            if (lane == 0) tc::mbar_arrive(&full[slot]);  // nothing for the FP4 product here
+          } else {
+            const int end = min(first + kBf16Rows, places);
             // the sink's places behind its length stay empty
             const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
-            tc::mbar_expect_tx(full, (end - first - absent) * 256);
-            tc::mbar_arrive(side ? &sm.full_k[slot] : &sm.full_v[slot]);  // the other side only passes the stage on
-          }
-          __syncwarp();
-          for (int i = first + lane; i < end; i += 32) {
-            const __nv_bfloat16* source = nullptr;
-            if (kind == kStepTail) source = tail + i * tail_row;
-            else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
-            else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
-            if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, full);
+            if (lane == 0) tc::mbar_expect_tx(&full[slot], (end - first - absent) * 256);
+            __syncwarp();
+            for (int i = first + lane; i < end; i += 32) {
+              const __nv_bfloat16* source = nullptr;
+              if (kind == kStepTail) source = tail + i * tail_row;
+              else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
+              else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
+              if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, &full[slot]);
+            }
           }
           __syncwarp();
           advance();
@@ -367,258 +405,307 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
     }
   }
   // After an abort nobody else waits for the copies still in flight: no CTA may end under them.
-  if (lane == 0 && sm.abort_flag) {
-    int ignore = 0;
+  if (lane == 0 && *static_cast<volatile int*>(&sm.abort_flag)) {
     for (int back = min(issued, Sh::kStages); back > 0; --back) {
       const int at = issued - back;
-      tc::mbar_wait(&sm.full_k[at % Sh::kStages], (at / Sh::kStages) & 1, &ignore);
-      tc::mbar_wait(&sm.full_v[at % Sh::kStages], (at / Sh::kStages) & 1, &ignore);
+      wait(&full[at % Sh::kStages], (at / Sh::kStages) & 1, &sm.ignored_flag);
     }
   }
   __syncwarp();
 }
 
-template <int NT>
-__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
+// The products are issued by two warps, one for the scores and one for the output: an MMA keeps its issuer
+// for 40 to 60 cycles, and the sixteen of a step one after another were longer than the step's HBM time. The
+// whole warp walks and waits; one thread of it issues.
+template <int NT, int PT>
+__device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
   using Sh = Shape<NT>;
-  constexpr uint32_t kScores = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
-  const uint32_t tmem = sm.tmem;
-  const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p);
-  int n = 0, unit = 0;
+  constexpr uint32_t kFp4 = tc::nvf4_idesc(128, NT), kF16 = f16_idesc(NT, 0, false);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  const uint32_t q = tc::smem_u32(sm.q), ring = tc::smem_u32(sm.ring);
+  const uint64_t q_codes = tc::fp4_tile_desc(tc::smem_u32(sm.q_codes), 0);
+  const uint64_t q_scales = tc::sf_atom_desc(tc::smem_u32(sm.q_scales));
+  int n = 0, block = 0, unit = 0, slot = 0;
+  uint32_t turn = 0, bf16_turn = 0;  // bf16_turn: one bit per half of the values' threads
   Unit u;
   bool known = false;
   for (; walker.next(u, known); known = true) {
-    auto output = [&](int step, int j) {  // O^T += V^T P^T of step `step` of the unit, the CTA's j-th
-      const StepKind kind = step_kind(u.info, step);
-      const int slices = step_slices(u.info, kind);
-      const int a = j % Sh::kVBuffers;
-      tc::mbar_wait(&sm.va_full[a], (j / Sh::kVBuffers) & 1, &sm.abort_flag);
-      tc::mbar_wait(&sm.p_full[j & 1], (j >> 1) & 1, &sm.abort_flag);
-      const bool first = step == u.begin;
-      if (first) tc::mbar_wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      const uint32_t tile = prob + (j & 1) * Sh::kBlocks * 16384;
-      for (int s = 0; s < slices; ++s)
-        mma_ts(tmem + Sh::kO, tmem + Sh::kV + a * 64 + s * 8, tc::smem_desc(tile + s * 2048, tc::kSwizzle128B, 1024, 16384),
-               kind == kStepPage ? kPages : kBf16, !(first && s == 0));
-      tc::commit(&sm.va_empty[a]);
-      tc::commit(&sm.p_empty[j & 1]);
-    };
-    tc::mbar_wait(&sm.q_full, unit & 1, &sm.abort_flag);
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const int a = n % Sh::kKBuffers;
-      tc::mbar_wait(&sm.ka_full[a], (n / Sh::kKBuffers) & 1, &sm.abort_flag);
-      tc::mbar_wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
-      tc::fence_after_sync();
+    wait(&sm.q_full, unit & 1, &sm.abort_flag);
+    tc::fence_after_sync();
+    if (elect_one()) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
-        mma_ts(tmem + Sh::kS + (n & 1) * NT, tmem + Sh::kK + a * 64 + s * 8,
-               tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
-      tc::commit(&sm.s_full[n & 1]);
-      tc::commit(&sm.ka_empty[a]);
-      if (step > u.begin) output(step - 1, n - 1);
+      for (int i = 0; i < 2 * kTerms; ++i) tc::cp_sf_atom(tmem + Sh::kQs + i * 4, q_scales + i * 32);
     }
-    output(u.end - 1, n - 1);
-    tc::commit(&sm.o_full);
+    __syncwarp();
+    for (int step = u.begin; step < u.end; ++step, ++n) {
+      const StepKind kind = step_kind(u.info, step);
+      const int within = (step - u.begin) & 1, set = block & 1;
+      const uint32_t scores = tmem + Sh::kS + (2 * set + within) * NT;
+      if (within == 0) wait(&sm.s_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
+      if (kind == kStepPage) {
+        wait(PT == 64 ? &sm.k_ready[slot] : &sm.full_k[slot], turn, &sm.abort_flag);
+        tc::fence_after_sync();
+        const uint32_t stage = ring + slot * kStage;
+        const uint64_t codes = tc::fp4_tile_desc(stage, 0), atoms = tc::sf_atom_desc(stage + kKsOffset);
+        const uint32_t scales = tmem + Sh::kKs + (n & 1) * 8;
+        if (elect_one()) {
+          tc::cp_sf_atom(scales, atoms);
+          tc::cp_sf_atom(scales + 4, atoms + 32);
+#pragma unroll 1
+          for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term)
+              tc::mma_nvf4(scores, codes + 2 * s, q_codes + term * NT * 4 + 2 * s, kFp4, scales + 4 * s,
+                           tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
+          }
+          tc::commit(&sm.s_full[set][within]);
+          tc::commit(&sm.empty[slot]);
+        }
+        __syncwarp();
+        if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+      } else {
+        for (int i = 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows); i > 0; --i) {
+          wait(&sm.full_k[slot], turn, &sm.abort_flag);  // the stage is not this product's
+          if (elect_one()) tc::mbar_arrive(&sm.empty[slot]);
+          __syncwarp();
+          if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+        }
+        wait(&sm.ka_full[n & 1], (bf16_turn >> (n & 1)) & 1, &sm.abort_flag);
+        bf16_turn ^= 1u << (n & 1);
+        tc::fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+            mma_ts(scores, tmem + Sh::kV + (n & 1) * 64 + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kF16, s > 0);
+          tc::commit(&sm.s_full[set][within]);
+          tc::commit(&sm.ka_empty[n & 1]);
+        }
+        __syncwarp();
+      }
+      if (within == 1 || step + 1 == u.end) {
+        if (within == 0 && elect_one()) tc::mbar_arrive(&sm.s_full[set][1]);  // a block of one step
+        __syncwarp();
+        ++block;
+      }
+    }
     ++unit;
   }
-  int ignore = 0;  // also after an abort: tensor memory is freed behind the last product
-  tc::commit(&sm.drained);
-  tc::mbar_wait(&sm.drained, 0, &ignore);
+  // also after an abort: tensor memory is freed behind the last product
+  if (elect_one()) tc::commit(&sm.drained);
+  __syncwarp();
+  wait(&sm.drained, 0, &sm.ignored_flag);
 }
 
-// Sixteen code words (128 values) and the scales of their eight groups.
-__device__ __forceinline__ void store_dequantized(uint32_t a, const uint4* chunk, uint32_t scales0, uint32_t scales1) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    __half2 scale[4];
-    scale_pairs(j < 2 ? scales0 : scales1, scale);
-    uint32_t v[16];
-    dequantize8(chunk[j].x, scale[2 * (j & 1)], v);
-    dequantize8(chunk[j].y, scale[2 * (j & 1)], v + 4);
-    dequantize8(chunk[j].z, scale[2 * (j & 1) + 1], v + 8);
-    dequantize8(chunk[j].w, scale[2 * (j & 1) + 1], v + 12);
-    st16(a + 16 * j, v);
-  }
-}
-
-// One side of the ring as its consumers (four warps) see it.
 template <int NT>
-struct Ring {
-  Smem<NT>& sm;
-  uint64_t* full;
-  int lane, slot;
-  uint32_t turn;
-  __device__ Ring(Smem<NT>& s, uint64_t* f, int l) : sm(s), full(f), lane(l), slot(0), turn(0) {}
-  __device__ __forceinline__ const uint8_t* wait() {
-    tc::mbar_wait(&full[slot], turn, &sm.abort_flag);
-    return sm.ring[slot];
+__device__ __forceinline__ void issue_output(Smem<NT>& sm, Walker walker) {
+  using Sh = Shape<NT>;
+  constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  const uint64_t prob = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
+  int n = 0, block = 0, unit = 0;
+  Unit u;
+  bool known = false;
+  for (; walker.next(u, known); known = true) {
+    wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
+    for (int step = u.begin; step < u.end; ++step, ++n) {
+      const StepKind kind = step_kind(u.info, step);
+      const int within = (step - u.begin) & 1, set = block & 1;
+      wait(&sm.va_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
+      if (within == 0) wait(&sm.p_full[set], (block >> 1) & 1, &sm.abort_flag);
+      tc::fence_after_sync();
+      const bool first = step == u.begin, closes = within == 1 || step + 1 == u.end;
+      const uint64_t tile = prob + (2 * set + within) * 1024;
+      const uint32_t operand = tmem + Sh::kV + (n & 1) * 64;
+      if (elect_one()) {
+        if (kind == kStepPage) {
+#pragma unroll 2
+          for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
+            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kPages, !(first && s == 0));
+        } else {
+          const int slices = step_slices(u.info, kind);
+          for (int s = 0; s < slices; ++s)
+            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kBf16, !(first && s == 0));
+        }
+        tc::commit(&sm.va_empty[n & 1]);
+        if (closes) tc::commit(&sm.p_empty[set]);
+        if (step + 1 == u.end) tc::commit(&sm.o_full);
+      }
+      __syncwarp();
+      if (closes) ++block;
+    }
+    ++unit;
   }
-  __device__ __forceinline__ void release() {
+  if (elect_one()) tc::commit(&sm.drained);
+  __syncwarp();
+  wait(&sm.drained, 0, &sm.ignored_flag);
+}
+
+// 64-token pages: the key scales of a step's two pages come as half atoms (32 rows of 8 bytes); one warp
+// interleaves them, in place, into the two whole atoms the MMA reads.
+__device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
+  uint2 part[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[i & 1][i >> 1] = *reinterpret_cast<const uint2*>(scales + (i >> 1) * 512 + (i & 1) * 256 + lane * 8);
+  __syncwarp();
+#pragma unroll
+  for (int atom = 0; atom < 2; ++atom)
+    *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) = make_uint4(part[atom][0].x, part[atom][0].y, part[atom][1].x, part[atom][1].y);
+  tc::fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane. The caller's
+// loop over a channel's four chunks stays rolled: three roles run side by side on every scheduler, and with
+// the 300 instructions of the unrolled form the warps waited for instructions a third of the time.
+__device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint32_t scales) {
+  __half2 scale[2];
+  scale_pairs(scales, scale);
+  uint32_t v[16];
+  dequantize8(chunk.x, scale[0], v);
+  dequantize8(chunk.y, scale[0], v + 4);
+  dequantize8(chunk.z, scale[1], v + 8);
+  dequantize8(chunk.w, scale[1], v + 12);
+  st16(a, v);
+}
+
+// The values' warps: thread c of a half holds channel c of its steps' V^T, and token c of a BF16 step's K.
+template <int NT, int PT>
+__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
+  const int c = thread & 127, lane = c & 31, half = thread >> 7;
+  using Sh = Shape<NT>;
+  const uint32_t lanes = (uint32_t)(c & ~31) << 16;
+  int slot = 0, n = 0;
+  uint32_t turn = 0, bf16_turn = 0;
+  auto pass = [&](int stages) {  // the other half's
+    slot += stages;
+    if (slot >= Sh::kStages) slot -= Sh::kStages, turn ^= 1;
+  };
+  auto arrived = [&]() -> uint8_t* {
+    wait(&sm.full_v[slot], turn, &sm.abort_flag);
+    return sm.ring[slot];
+  };
+  const bool interleaves = PT == 64 && (c >> 5) == 3;
+  auto release = [&] {
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
-    if (++slot == Shape<NT>::kStages) slot = 0, turn ^= 1;
-  }
-  __device__ __forceinline__ void pass(int stages) {
-    for (int i = 0; i < stages; ++i) {
-      wait();
-      release();
-    }
-  }
-};
-
-// Keys: thread t holds token t of every step.
-template <int NT, int PT>
-__device__ __forceinline__ void keys(const TreeParams& p, Smem<NT>& sm, Walker walker, int t) {
-  using Sh = Shape<NT>;
-  const int lane = t & 31;
-  const uint32_t tmem = sm.tmem + Sh::kK + ((uint32_t)(t & ~31) << 16);
-  Ring<NT> ring(sm, sm.full_k, lane);
-  int n = 0;
+    pass(1);
+  };
   Unit u;
   bool known = false;
   for (; walker.next(u, known); known = true) {
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const uint32_t operand = tmem + (n % Sh::kKBuffers) * 64;
-      uint64_t* operand_empty = &sm.ka_empty[n % Sh::kKBuffers];
-      const uint32_t empty_parity = ((n / Sh::kKBuffers) & 1) ^ 1;
+      if ((n & 1) != half) {
+        pass(kind == kStepPage ? 1 : 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows));
+        continue;
+      }
+      const uint32_t operand = sm.tmem + Sh::kV + (n & 1) * 64 + lanes;
+      uint64_t* operand_empty = &sm.va_empty[n & 1];
+      const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
       if (kind == kStepPage) {
-        const uint8_t* stage = ring.wait();
-        uint4 chunk[4];
-        const uint8_t* row = stage + t * 64;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) chunk[j] = *reinterpret_cast<const uint4*>(row + ((j ^ ((t >> 1) & 3)) * 16));
-        const uint8_t* at = PT == 128 ? stage + kKsOffset + (t & 31) * 16 + (t >> 5) * 4
-                                      : stage + kKsOffset + (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4;
-        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(at);
-        const uint32_t s1 = *reinterpret_cast<const uint32_t*>(at + (PT == 128 ? 512 : 256));
-        ring.release();
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-        store_dequantized(operand, chunk, s0, s1);
-      } else {
-        const int places = bf16_places(u.info, kind);
-        const int stages = (places + kBf16Rows - 1) / kBf16Rows;
-        // a step's stages are held together; both have arrived when each has been waited for
-        ring.wait();
-        uint8_t* const stage0 = sm.ring[ring.slot];
-        uint8_t* stage1 = stage0;
-        if (stages > 1) {
-          const bool wraps = ring.slot + 1 == Sh::kStages;
-          const int next = wraps ? 0 : ring.slot + 1;
-          tc::mbar_wait(&sm.full_k[next], ring.turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
-          stage1 = sm.ring[next];
+        if (interleaves) {
+          wait(&sm.full_k[slot], turn, &sm.abort_flag);
+          interleave_scales(sm.ring[slot] + kKsOffset, lane);
+          if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
         }
-        auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
-        bool there = t < places;
-        if (kind == kStepDraft) {
-          if (t < BDFP4_MAX_SINK) there = t < u.info.sink;
-          if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
-            const int group = t & 7;
-            const int64_t shift_at = u.head * kHeadDim + group * kGroup;
-            for (int first = 0; first < u.info.count; first += 16) {
-              // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
-              const int node = min(first + (t >> 3), u.info.count - 1);
-              uint4* at = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + node) + group * 32);
-              const uint4 raw[2] = {at[0], at[1]};
-              const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-              float v[16];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-              }
-              if (p.rotate && p.key_shift) cache_basis16<BDFP4_SHIFT_F32, true>(v, group, p.key_shift, shift_at);
-              else if (p.rotate) cache_basis16<BDFP4_SHIFT_NONE, true>(v, group, nullptr, 0);
-              else cache_basis16<BDFP4_SHIFT_F32, false>(v, group, p.key_shift, shift_at);
-              if (first + (t >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
-            }
-            tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
-            bar_sync(4, 128);
-          }
-        }
-        const uint4* row = reinterpret_cast<const uint4*>(row_of(min(t, places - 1)));
-        float amax = 0.0f;
-        if (there) {
-#pragma unroll 4
-          for (int j = 0; j < 16; ++j) {
-            const uint4 r = row[j];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-          }
-        }
-        float inverse;
-        const float scale = fp16_scale(amax, &inverse);
-        sm.key_factor[n & 7][t] = inverse;
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
+        const uint8_t* stage = arrived();
+        const uint8_t* scales = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
+        wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
 #pragma unroll 1
-        for (int quarter = 0; quarter < 4; ++quarter) {
-          uint32_t v[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 r = make_uint4(0, 0, 0, 0);
-            if (there) r = row[quarter * 4 + j];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
-          }
-          st16(operand + quarter * 16, v);
-        }
-        for (int i = 0; i < stages; ++i) ring.release();
-        ring.pass(stages);  // the values'
-      }
-      tc::tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.ka_full[n % Sh::kKBuffers]);
-    }
-  }
-}
-
-// Values: thread c holds channel c of every step.
-template <int NT, int PT>
-__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker walker, int c) {
-  using Sh = Shape<NT>;
-  const int lane = c & 31;
-  const uint32_t tmem = sm.tmem + Sh::kV + ((uint32_t)(c & ~31) << 16);
-  Ring<NT> ring(sm, sm.full_v, lane);
-  int n = 0;
-  Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const StepKind kind = step_kind(u.info, step);
-      const uint32_t operand = tmem + (n % Sh::kVBuffers) * 64;
-      uint64_t* operand_empty = &sm.va_empty[n % Sh::kVBuffers];
-      const uint32_t empty_parity = ((n / Sh::kVBuffers) & 1) ^ 1;
-      if (kind == kStepPage) {
-        const uint8_t* stage = ring.wait();
-        uint4 chunk[4];
-#pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint8_t* at = PT == 128 ? stage + kVOffset + c * 64 + ((j ^ ((c >> 1) & 3)) * 16)
                                         : stage + kVOffset + (j >> 1) * 4096 + c * 32 + (((j & 1) ^ ((c >> 2) & 1)) * 16);
-          chunk[j] = *reinterpret_cast<const uint4*>(at);
+          store_dequantized(operand + 16 * j, *reinterpret_cast<const uint4*>(at),
+                            *reinterpret_cast<const uint16_t*>(scales + (j >> 1) * 512 + (j & 1) * 2));
         }
-        const uint8_t* at = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
-        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(at);
-        const uint32_t s1 = *reinterpret_cast<const uint32_t*>(at + 512);
-        ring.release();
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-        store_dequantized(operand, chunk, s0, s1);
+        release();
       } else {
         const int places = bf16_places(u.info, kind);
-        ring.pass((places + kBf16Rows - 1) / kBf16Rows);  // the keys'
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
+        const int stages = (places + kBf16Rows - 1) / kBf16Rows;
+        // keys first, through the buffer that takes the values after the score product
+        wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
+        {  // a step's stages are held together
+          uint8_t* const stage0 = arrived();
+          uint8_t* stage1 = stage0;
+          if (stages > 1) {
+            const bool wraps = slot + 1 == Sh::kStages;
+            const int next = wraps ? 0 : slot + 1;
+            wait(&sm.full_v[next], turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
+            stage1 = sm.ring[next];
+          }
+          auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
+          bool there = c < places;
+          if (kind == kStepDraft) {
+            if (c < BDFP4_MAX_SINK) there = c < u.info.sink;
+            if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
+              const int group = c & 7;
+              const int64_t shift_at = u.head * kHeadDim + group * kGroup;
+              for (int first = 0; first < u.info.count; first += 16) {
+                // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
+                const int node = min(first + (c >> 3), u.info.count - 1);
+                uint4* at = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + node) + group * 32);
+                const uint4 raw[2] = {at[0], at[1]};
+                const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  v[2 * i] = __uint_as_float(w[i] << 16);
+                  v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                }
+                if (p.rotate && p.key_shift) cache_basis16<BDFP4_SHIFT_F32, true>(v, group, p.key_shift, shift_at);
+                else if (p.rotate) cache_basis16<BDFP4_SHIFT_NONE, true>(v, group, nullptr, 0);
+                else cache_basis16<BDFP4_SHIFT_F32, false>(v, group, p.key_shift, shift_at);
+                if (first + (c >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
+              }
+              tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
+              bar_sync(kValuesBarrier + half, 128);
+            }
+          }
+          const uint4* row = reinterpret_cast<const uint4*>(row_of(min(c, places - 1)));
+          float amax = 0.0f;
+          if (there) {
+#pragma unroll 4
+            for (int j = 0; j < 16; ++j) {
+              const uint4 r = row[j];
+              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+            }
+          }
+          float inverse;
+          const float scale = fp16_scale(amax, &inverse);
+          sm.key_factor[n & 7][c] = inverse;
+#pragma unroll 1
+          for (int quarter = 0; quarter < 4; ++quarter) {
+            uint32_t v[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint4 r = make_uint4(0, 0, 0, 0);
+              if (there) r = row[quarter * 4 + j];
+              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
+            }
+            st16(operand + quarter * 16, v);
+          }
+          for (int i = 0; i < stages; ++i) {
+            if (interleaves && lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);  // its phases follow the stage's uses
+            release();
+          }
+          tc::tmem_wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sm.ka_full[half]);
+          wait(&sm.ka_empty[half], bf16_turn, &sm.abort_flag);
+          tc::fence_after_sync();
+          bf16_turn ^= 1;
+        }
         for (int first = 0; first < places; first += kBf16Rows) {
-          const uint8_t* stage = ring.wait() + 2 * c;
+          const uint8_t* stage = arrived() + 2 * c;
           const int slices = (min(places - first, kBf16Rows) + 15) / 16;
           for (int s = 0; s < slices; ++s) {
             const int place = first + s * 16;
@@ -633,23 +720,24 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
             }
             st8(operand + (place >> 4) * 8, v);
           }
-          ring.release();
+          if (interleaves && lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
+          release();
         }
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.va_full[n % Sh::kVBuffers]);
+      if (lane == 0) tc::mbar_arrive(&sm.va_full[n & 1]);
     }
   }
 }
 
-// The tile's queries into shared memory: rotated if asked, scaled by one power of two into FP16's range
-// (rows of the tile whose largest value is 2^-29 of the tile's keep full precision). Returns what undoes it.
+// The tile's queries into shared memory: rotated if asked, scaled by one power of two, as FP16 for the BF16 steps
+// and as FP4 terms for the pages. One scale for the tile: a query whose largest value is 2^-8 of the tile's
+// still has all four terms above E4M3's smallest scale. Returns what undoes the scaling.
 template <int NT>
 __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
-  using Sh = Shape<NT>;
-  constexpr int kPerPass = Sh::kSoftmaxThreads / 8, kPasses = NT / kPerPass;
+  constexpr int kPerPass = 32, kPasses = (NT + kPerPass - 1) / kPerPass;
   const int group = thread & 7;
   const int queries = u.info.count * p.ratio;
   float v[kPasses][16];
@@ -659,7 +747,7 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
     const int query = u.tile * NT + i * kPerPass + (thread >> 3);
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[i][j] = 0.0f;
-    if (query < queries)
+    if (query < queries && i * kPerPass + (thread >> 3) < NT)
       load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
                        (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
   }
@@ -677,14 +765,15 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
   }
   amax = warp_max(amax);
   if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
-  bar_sync(3, Sh::kSoftmaxThreads);
+  softmax_sync();
 #pragma unroll
-  for (int w = 0; w < Sh::kSoftmaxThreads / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
+  for (int w = 0; w < 8; ++w) amax = fmaxf(amax, sm.q_max[w]);
   float inverse;
   const float scale = fp16_scale(amax, &inverse);
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = i * kPerPass + (thread >> 3);
+    if (NT < kPerPass && r >= NT) break;
     uint8_t* row = sm.q[group >> 2] + r * 128;
     uint32_t w[8];
 #pragma unroll
@@ -692,9 +781,29 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
     const int chunk = (group & 3) * 2;
     *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+    float left[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) left[j] = v[i][j] * scale;
+    const int at = r * 64 + group * 8;
+#pragma unroll 1
+    for (int term = 0; term < kTerms; ++term) {
+      float largest = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(left[j]));
+      const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
+      GroupCodes codes;
+      codes.scale = e4m3_to_float(byte);
+      encode16(left, codes.scale, codes.lo, codes.hi);
+      *reinterpret_cast<uint2*>(sm.q_codes[term] + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
+      sm.q_scales[term][scale_tile_offset(r, group)] = (uint8_t)byte;
+      float rest[16];
+      group_residual16(left, codes, rest);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) left[j] = rest[j];
+    }
   }
   tc::fence_proxy_async_smem();
-  bar_sync(3, Sh::kSoftmaxThreads);
+  softmax_sync();
   if (thread == 0) tc::mbar_arrive(&sm.q_full);
   return inverse;
 }
@@ -725,178 +834,220 @@ template <int NT>
 __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
   using Sh = Shape<NT>;
   constexpr int C = Sh::kColumns;
-  const int t = thread & 127, lane = thread & 31, warp = t >> 5, group = thread >> 7;
-  const int first_column = group * C;
-  const int barrier = 1 + group;
+  const int t = thread & 127, lane = thread & 31, warp = thread >> 5, half = thread >> 7;
+  const int first_column = Sh::kByStep ? 0 : half * C;
   const uint32_t lanes = (uint32_t)(t & ~31) << 16;
-  float* base = sm.base + first_column;
-  float* top = sm.top + first_column;
-  int n = 0, unit = 0;
+  const float* base = sm.base + first_column;
+  int n = 0, block = 0, unit = 0;
   Unit u;
   if (!walker.next(u, false)) return;
   bool more = true;
   float q_inverse = load_queries<NT>(p, sm, u, thread);
   while (more) {
-    for (int j = t; j < C; j += 128) {
-      top[j] = kNoMax;
-      base[j] = kShift - kNoMax;
-      // the draft nodes the query of column j sees
-      const int query = u.tile * NT + first_column + j;
+    if (thread < NT) {
+      sm.top[thread] = kNoMax;
+      sm.base[thread] = kShift - kNoMax;
+      // the draft nodes that this query sees
+      const int query = u.tile * NT + thread;
       uint64_t seen = 0;
       for (int node = min(query / p.ratio, u.info.count - 1); node >= 0;) {
         seen |= 1ull << node;
         const int parent = sm.parents[node];
         node = parent < node ? parent : -1;
       }
-      sm.family[first_column + j] = seen;
+      sm.family[thread] = seen;
     }
     float2 sum[C / 2];
 #pragma unroll
     for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
-    bar_sync(barrier, 128);
+    softmax_sync();
     const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const StepKind kind = step_kind(u.info, step);
-      bool dead;  // no query sees this thread's token
-      if (kind == kStepPage) dead = step == 0 && t < u.info.sink;
-      else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
-      else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-      const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
-      const int node = t - BDFP4_MAX_SINK;
-      tc::mbar_wait(&sm.s_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      float f = page_factor;
-      if (kind != kStepPage) f = p.scale_log2 * q_inverse * sm.key_factor[n & 7][t];
-      const float2 f2 = make_float2(f, f);
-      const uint32_t scores = sm.tmem + Sh::kS + (n & 1) * NT + first_column + lanes;
-      auto load16 = [&](int j, float* s) {
-        tc::tmem_ld16(scores + j, s);
-        tc::tmem_wait_ld();
-        if (masked) {
+    for (int block_begin = u.begin; block_begin < u.end; block_begin += 2, ++block) {
+      const int steps = min(2, u.end - block_begin), set = block & 1;
+      // this half's steps of the block
+      const int from = Sh::kByStep ? half : 0, to = Sh::kByStep ? min(half + 1, steps) : steps;
+      float s[C];  // the block's probabilities, both steps' added
+      bool high = false;
+      // A step in which every query sees every token. True when a probability of this thread exceeds kHighest: its
+      // query's maximum has to be renewed, and the block formed again.
+      auto form_plain = [&](int i) {
+        const float2 f2 = make_float2(page_factor, page_factor);
+        const uint32_t scores = sm.tmem + Sh::kS + (2 * set + i) * NT + first_column + lanes;
+        uint8_t* const row = sm.p[set][i] + t * 128;
+        float v[Sh::kByStep ? 1 : 16];
+        if constexpr (Sh::kByStep) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!((sm.family[first_column + j + i] >> node) & 1)) s[i] = -INFINITY;
+          for (int j = 0; j < C; j += 16) tc::tmem_ld16(scores + j, s + j);
+          tc::tmem_wait_ld();
         }
-      };
-      // scores -> log2 units above the maxima, plus kShift
-      auto above16 = [&](int j, float* s) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(base + j + i);
-          const float2 y0 = __ffma2_rn(make_float2(s[i], s[i + 1]), f2, make_float2(b.x, b.y));
-          const float2 y1 = __ffma2_rn(make_float2(s[i + 2], s[i + 3]), f2, make_float2(b.z, b.w));
-          s[i] = y0.x, s[i + 1] = y0.y, s[i + 2] = y1.x, s[i + 3] = y1.y;
-        }
-      };
-      float held[Sh::kHold ? C : 16];
-      float highest = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < C; j += 16) {
-        float* s = Sh::kHold ? held + j : held;
-        load16(j, s);
-        above16(j, s);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) highest = fmaxf(highest, s[i]);
-      }
-      if (bar_any(barrier, highest > kGrowth + kShift && !dead)) {
+        __half2 most = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < C; j += 16) {
-          float s[16];
-          load16(j, s);
-          float mine = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float m = warp_max(dead ? -INFINITY : s[i] * f);
-            if (lane == i) mine = m;
+          float* x = Sh::kByStep ? s + j : v;
+          if constexpr (!Sh::kByStep) {
+            tc::tmem_ld16(scores + j, x);
+            tc::tmem_wait_ld();
           }
-          if (lane < 16) sm.col_max[warp][first_column + j + lane] = mine;
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(base + j + c);
+            const float2 y0 = __ffma2_rn(make_float2(x[c], x[c + 1]), f2, make_float2(b.x, b.y));
+            const float2 y1 = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), f2, make_float2(b.z, b.w));
+            x[c] = ex2(y0.x), x[c + 1] = ex2(y0.y), x[c + 2] = ex2(y1.x), x[c + 3] = ex2(y1.y);
+          }
+          uint32_t w[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const __half2 pair = __floats2half2_rn(x[2 * c], x[2 * c + 1]);
+            most = __hmax2(most, pair);
+            w[c] = h2(pair);
+          }
+          const int chunk = (first_column + j) >> 3;
+          *reinterpret_cast<uint4*>(row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+          if constexpr (!Sh::kByStep) {
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              const float2 both = __fadd2_rn(make_float2(s[j + c], s[j + c + 1]), make_float2(x[c], x[c + 1]));
+              s[j + c] = both.x, s[j + c + 1] = both.y;
+            }
+          }
         }
-        bar_sync(barrier, 128);
-        for (int j = t; j < C; j += 128) {
-          const int col = first_column + j;
-          const float before = top[j];
-          const float now = fmaxf(fmaxf(fmaxf(sm.col_max[0][col], sm.col_max[1][col]),
-                                        fmaxf(sm.col_max[2][col], sm.col_max[3][col])), before);
-          top[j] = now;
-          base[j] = kShift - now;
-          sm.factor[col] = ex2(before - now);
+        high |= __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
+      };
+      // Any step: tokens that no query sees, drafts that some do not see, BF16 operands.
+      struct Step {
+        StepKind kind;
+        bool dead, masked;
+        float f;  // scores in log2 units above the maxima (plus kShift) are f * score + base
+        uint32_t scores;
+        uint8_t* row;
+      };
+      auto open = [&](int i) {
+        Step k;
+        k.kind = step_kind(u.info, block_begin + i);
+        if (k.kind == kStepPage) k.dead = block_begin + i == 0 && t < u.info.sink;  // no query sees this thread's token
+        else if (k.kind == kStepTail) k.dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
+        else k.dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
+        k.masked = k.kind == kStepDraft && t >= BDFP4_MAX_SINK && !k.dead;
+        k.f = k.kind == kStepPage ? page_factor : p.scale_log2 * q_inverse * sm.key_factor[(n + i) & 7][t];
+        k.scores = sm.tmem + Sh::kS + (2 * set + i) * NT + first_column + lanes;
+        k.row = sm.p[set][i] + t * 128;
+        return k;
+      };
+      auto load16 = [&](const Step& k, int j, float* v) {
+        tc::tmem_ld16(k.scores + j, v);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k.dead || (k.masked && !((sm.family[first_column + j + i] >> (t - BDFP4_MAX_SINK)) & 1))) v[i] = -INFINITY;
+      };
+      auto form_any = [&](int i) {
+        const Step k = open(i);
+#pragma unroll
+        for (int j = 0; j < C; j += 16) {
+          float v[16], most = 0.0f;
+          load16(k, j, v);
+          uint32_t w[8];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            v[c] = ex2(fmaf(v[c], k.f, base[j + c]));
+            most = fmaxf(most, v[c]);
+            s[j + c] += v[c];
+          }
+          high |= most > kHighest;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            w[c] = k.kind == kStepPage ? h2(__floats2half2_rn(v[2 * c], v[2 * c + 1]))
+                                       : pack_bf16x2(v[2 * c] * p.inverse_value_scale, v[2 * c + 1] * p.inverse_value_scale);
+          const int chunk = (first_column + j) >> 3;
+          *reinterpret_cast<uint4*>(k.row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(k.row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
         }
-        bar_sync(barrier, 128);
+      };
+      const bool plain = block_begin + steps <= u.info.pages && (block_begin > 0 || u.info.sink == 0);
+      // P of this block goes where the one before the last was
+      wait(&sm.p_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
+      bool renewed = false;
+      while (true) {
+        if (!Sh::kByStep || !plain || from >= to) {
+#pragma unroll
+          for (int j = 0; j < C; ++j) s[j] = 0.0f;
+        }
+        high = false;
+#pragma unroll 1
+        for (int i = from; i < to; ++i) {
+          wait(&sm.s_full[set][i], (block >> 1) & 1, &sm.abort_flag);
+          tc::fence_after_sync();
+          if (plain) form_plain(i);
+          else form_any(i);
+        }
+        tc::fence_before_sync();
+        tc::fence_proxy_async_smem();
+        // against renewed maxima nothing is high: the second vote only ends the step
+        if (!softmax_any(high) || renewed) break;
+        renewed = true;
+        float mine = -INFINITY;
+#pragma unroll 1
+        for (int i = from; i < to; ++i) {
+          const Step k = open(i);
+#pragma unroll
+          for (int j = 0; j < C; j += 16) {
+            float v[16];
+            load16(k, j, v);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float m = warp_max(v[c] * k.f);
+              if (lane == j + c) mine = fmaxf(mine, m);
+            }
+          }
+        }
+        if (lane < C) sm.col_max[warp][first_column + lane] = mine;
+        softmax_sync();
+        if (thread < NT) {
+          const float before = sm.top[thread];
+          float now = before;
+          const int w0 = Sh::kByStep ? 0 : thread / C * 4;
+#pragma unroll
+          for (int w = 0; w < (Sh::kByStep ? 8 : 4); ++w) now = fmaxf(now, sm.col_max[w0 + w][thread]);
+          sm.top[thread] = now;
+          sm.base[thread] = kShift - now;
+          sm.factor[thread] = ex2(before - now);
+        }
+        softmax_sync();
 #pragma unroll
         for (int j = 0; j < C / 2; ++j) {
           sum[j].x *= sm.factor[first_column + 2 * j];
           sum[j].y *= sm.factor[first_column + 2 * j + 1];
         }
-        if (step > u.begin) {  // what O^T holds is of the old maxima
-          tc::mbar_wait(&sm.p_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, &sm.abort_flag);
+        if (block_begin > u.begin) {  // what O^T holds is of the old maxima
+          wait(&sm.p_empty[set ^ 1], ((block - 1) >> 1) & 1, &sm.abort_flag);
           tc::fence_after_sync();
 #pragma unroll 1
-          for (int j = 0; j < C; j += 16) {
-            float o[16];
-            const uint32_t at = sm.tmem + Sh::kO + first_column + j + lanes;
-            tc::tmem_ld16(at, o);
+          for (int j = half * Sh::kOut; j < (half + 1) * Sh::kOut; j += 8) {
+            float o[8];
+            uint32_t r[8];
+            const uint32_t at = sm.tmem + Sh::kO + j + lanes;
+            tc::tmem_ld8(at, o);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= sm.factor[first_column + j + i];
-            tc::tmem_st16(at, o);
+            for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(o[i] * sm.factor[j + i]);
+            st8(at, r);
           }
           tc::tmem_wait_st();
         }
-        if constexpr (Sh::kHold) {
-#pragma unroll
-          for (int j = 0; j < C; j += 16) {
-            load16(j, held + j);
-            above16(j, held + j);
-          }
-        }
       }
-      if constexpr (Sh::kHold) {  // the scores are in registers: the next but one may come
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.s_empty[n & 1]);
+      // the barrier stands behind every thread's scores read and probabilities written
+      if (thread == 0) {
+        tc::mbar_arrive(&sm.p_full[set]);
+        tc::mbar_arrive(&sm.s_empty[set]);
       }
-      // P of this step goes where the one before the last was
-      tc::mbar_wait(&sm.p_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
 #pragma unroll
-      for (int j = 0; j < C; j += 16) {
-        float* s = Sh::kHold ? held + j : held;
-        if constexpr (!Sh::kHold) {
-          load16(j, s);
-          above16(j, s);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = ex2(s[i]);
-        if (dead) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-        }
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[j / 2 + i] = __fadd2_rn(sum[j / 2 + i], make_float2(s[2 * i], s[2 * i + 1]));
-        if (kind == kStepPage) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = h2(__floats2half2_rn(s[2 * i], s[2 * i + 1]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = pack_bf16x2(s[2 * i] * p.inverse_value_scale, s[2 * i + 1] * p.inverse_value_scale);
-        }
-        const int column = first_column + j;
-        uint8_t* row = sm.p[n & 1] + (column >> 6) * 16384 + t * 128;
-        const int chunk = (column & 63) >> 3;
-        *reinterpret_cast<uint4*>(row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-      tc::fence_before_sync();
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (!Sh::kHold) tc::mbar_arrive(&sm.s_empty[n & 1]);
-        tc::mbar_arrive(&sm.p_full[n & 1]);
-      }
+      for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
+      n += steps;
     }
 
-    {  // each query's weight: first over a warp's 32 tokens, then (below) over the four warps
+    {  // each query's weight: first over a warp's 32 tokens, then (below) over the warps
       float v[C];
 #pragma unroll
       for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
@@ -906,40 +1057,42 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     Unit following = u;
     more = walker.next(following, true);
     float next_inverse = 1.0f;
-    bar_sync(3, Sh::kSoftmaxThreads);  // both groups have seen their last scores; the parents are free
-    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
-    bar_sync(barrier, 128);
+    softmax_sync();  // the column sums are there; the parents are free
     const bool whole = u.begin == 0 && u.end == u.info.steps;
     // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
     const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
-    for (int j = t; j < C; j += 128) {
-      const int col = first_column + j;
-      const float total = (sm.col_sum[0][col] + sm.col_sum[1][col]) + (sm.col_sum[2][col] + sm.col_sum[3][col]);
+    if (thread < NT) {
+      const int w0 = Sh::kByStep ? 0 : thread / C * 4;
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < (Sh::kByStep ? 8 : 4); ++w) total += sm.col_sum[w0 + w][thread];
       if (whole) {
-        sm.total[col] = total > 0.0f ? p.value_scale / total : 0.0f;
+        sm.total[thread] = total > 0.0f ? p.value_scale / total : 0.0f;
       } else {
-        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[j];
-        p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
+        p.partial_stat[(int64_t)(2 * part) * NT + thread] = sm.top[thread];
+        p.partial_stat[(int64_t)(2 * part + 1) * NT + thread] = total;
       }
     }
-    bar_sync(barrier, 128);
-    tc::mbar_wait(&sm.o_full, unit & 1, &sm.abort_flag);
+    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
+    softmax_sync();
+    wait(&sm.o_full, unit & 1, &sm.abort_flag);
     tc::fence_after_sync();
-    const int queries = min(u.info.count * p.ratio - u.tile * NT - first_column, C);
-    int query = u.tile * NT + first_column;
+    const int out_first = half * Sh::kOut;
+    const int queries = min(u.info.count * p.ratio - u.tile * NT - out_first, Sh::kOut);
+    const int query = u.tile * NT + out_first;
     int out_node = query / p.ratio, out_head = query % p.ratio;
     __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
-    float* partial = p.partial + ((int64_t)part * NT + first_column) * kHeadDim + t;
-#pragma unroll
-    for (int j = 0; j < C; j += 16) {
-      float o[16];
-      tc::tmem_ld16(sm.tmem + Sh::kO + first_column + j + lanes, o);
+    float* partial = p.partial + ((int64_t)part * NT + out_first) * kHeadDim + t;
+#pragma unroll 1
+    for (int j = 0; j < Sh::kOut; j += 8) {
+      float o[8];
+      tc::tmem_ld8(sm.tmem + Sh::kO + out_first + j + lanes, o);
       tc::tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         if (j + i < queries) {
           if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[first_column + j + i]);
+            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[out_first + j + i]);
             if (++out_head == p.ratio) out_head = 0, ++out_node;
           } else {
             partial[(int64_t)(j + i) * kHeadDim] = o[i];
@@ -948,9 +1101,8 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       }
     }
     tc::fence_before_sync();
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.o_empty);
-    bar_sync(barrier, 128);  // base, top and total are written anew
+    softmax_sync();  // the output has been read; base, top and total are written anew
+    if (thread == 0) tc::mbar_arrive(&sm.o_empty);
     if (!whole && u.begin == 0 && thread == 0) {
       TreeSplit split;
       split.row = u.row;
@@ -987,24 +1139,26 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     for (int i = 0; i < Sh::kStages; ++i) {
       tc::mbar_init(&sm.full_k[i], 1);
       tc::mbar_init(&sm.full_v[i], 1);
-      tc::mbar_init(&sm.empty[i], 8);
+      tc::mbar_init(&sm.empty[i], 5);  // the values' four warps and the score product
+      tc::mbar_init(&sm.k_ready[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sm.ka_full[i], 4);
-      tc::mbar_init(&sm.va_full[i], 4);
       tc::mbar_init(&sm.ka_empty[i], 1);
+      tc::mbar_init(&sm.va_full[i], 4);
       tc::mbar_init(&sm.va_empty[i], 1);
-      tc::mbar_init(&sm.s_full[i], 1);
-      tc::mbar_init(&sm.s_empty[i], 4 * Sh::kGroups);
-      tc::mbar_init(&sm.p_full[i], 4 * Sh::kGroups);
+      tc::mbar_init(&sm.s_full[i][0], 1);
+      tc::mbar_init(&sm.s_full[i][1], 1);
+      tc::mbar_init(&sm.s_empty[i], 1);
+      tc::mbar_init(&sm.p_full[i], 1);
       tc::mbar_init(&sm.p_empty[i], 1);
     }
     tc::mbar_init(&sm.q_full, 1);
     tc::mbar_init(&sm.o_full, 1);
-    tc::mbar_init(&sm.o_empty, 4 * Sh::kGroups);
-    tc::mbar_init(&sm.drained, 1);
+    tc::mbar_init(&sm.o_empty, 1);
+    tc::mbar_init(&sm.drained, 2);
     tc::fence_barrier_init();
-    sm.abort_flag = 0;
+    sm.abort_flag = sm.ignored_flag = 0;
     TreeSplit none;
     none.row = -1;
     none.head = none.tile = none.last = 0;
@@ -1052,16 +1206,13 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   tc::fence_after_sync();
   if (sm.first < sm.last) {
     const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
-    if (warp < 4) {
-      trade_registers<Sh::kLaunchRegs, Sh::kKeyRegs>();
-    } else if (warp < 8) {
+    if (warp < 8) {
       trade_registers<Sh::kLaunchRegs, Sh::kValueRegs>();
-    } else if (warp < 8 + 4 * Sh::kGroups) {
+    } else if (warp < 16) {
       trade_registers<Sh::kLaunchRegs, Sh::kSoftmaxRegs>();
     } else {
       trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
-      if (warp == 9 + 4 * Sh::kGroups && lane == 0) issue<NT>(sm, walker);
-      __syncwarp();
+      if (warp == 17) produce<NT, PT, 1>(p, sm, walker, &v_map, lane);
     }
   }
   tc::fence_before_sync();
@@ -1090,9 +1241,7 @@ static cudaError_t launch_tile(const CUtensorMap& k_map, const CUtensorMap& v_ma
   switch (p.tile) {
     case 16: return launch<16, PT>(k_map, v_map, p, stream);
     case 32: return launch<32, PT>(k_map, v_map, p, stream);
-    case 64: return launch<64, PT>(k_map, v_map, p, stream);
-    case 96: return launch<96, PT>(k_map, v_map, p, stream);
-    default: return launch<128, PT>(k_map, v_map, p, stream);
+    default: return launch<64, PT>(k_map, v_map, p, stream);
   }
 }
 

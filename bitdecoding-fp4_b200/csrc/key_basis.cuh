@@ -44,4 +44,21 @@ __device__ __forceinline__ void cache_basis16(float* v, int group, const void* s
   if (ROTATE || SHIFT_TYPE != BDFP4_SHIFT_NONE) round_to_bf16(v);
 }
 
+// The same with the rotation and an FP32 shift chosen at run time, in one copy of the code. `shift` points at
+// this group's sixteen values, or is null.
+__device__ __forceinline__ void cache_basis16_any(float* v, int group, bool rotate, const float* shift) {
+  if (rotate) {
+    hadamard_butterflies(v, group);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __fmul_rn(v[j], (float)0.08838834764831845);
+  }
+  if (shift) {
+    float centre[16];
+    load_shift16<BDFP4_SHIFT_F32>(shift, 0, centre);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __fsub_rn(v[j], centre[j]);
+  }
+  round_to_bf16(v);
+}
+
 }  // namespace bdfp4

@@ -17,10 +17,14 @@
 // dequantized tile never passes through shared memory. P is stored as the softmax threads hold it, one token
 // per thread with its queries contiguous, which is the MN-major form of operand B.
 //
-// Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: probabilities are
-// formed against them at once, and only when one comes out more than 2^8 above its maximum (the barrier
-// that ends a step carries that vote) are the maxima taken anew, O^T rescaled and the step formed again. Sums stay per thread until the unit ends. Probabilities carry a factor
+// Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: after a unit's first
+// block (of two steps) probabilities are formed against them at once, and only when one comes out more than
+// 2^8 above its maximum (the barrier that ends a block carries that vote) are the maxima taken anew, O^T
+// rescaled and the block formed again. Sums stay per thread until the unit ends. Probabilities carry a factor
 // 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
+//
+// What bounds it: five roles run side by side on every scheduler, and the sum of their code is larger than its
+// instruction cache. Code that runs once per unit is kept in rolled loops, and the common path short.
 //
 // The rolling tail and the drafts with the sink are two more steps over BF16 values, both products kind::f16
 // with the cache side in tensor memory: K is scaled per token by a power of two into FP16's range (the softmax
@@ -80,6 +84,20 @@ __device__ __forceinline__ void trade_registers() {
   if constexpr (TO < FROM) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
 }
 
+struct RowInfo {
+  int count, pages, residual, sink, slot;  // pages: 128-token steps in the FP4 cache
+  int steps;                               // of one unit: pages, tail, drafts with sink
+  int tiles;
+};
+
+// A run of steps of one (row, head, tile).
+struct Unit {
+  RowInfo info;
+  int row, head, tile, begin, end;  // steps [begin, end) are this CTA's; begin < 0: no more units
+};
+constexpr int kUnits = 4;  // of the ring through which the key producer hands them to the other roles
+constexpr int kUnitReaders = 8 + 8 + 3;  // warps: values, softmax, value producer, score issuer, output issuer
+
 template <int NT>
 struct Smem {
   using Sh = Shape<NT>;
@@ -93,11 +111,15 @@ struct Smem {
   float top[NT];        // maximum, log2 units
   float factor[NT];
   float total[NT];
+  float extra[NT];      // weights of the steps that were not plain
   float col_max[8][NT];
   float col_sum[8][NT];
+  float step_sum[2][8][NT];  // [block] a not plain block's weights, by warp
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
   float q_max[8];
   int parents[BDFP4_MAX_TREE_NODES];
+  Unit units[kUnits];
+  uint64_t unit_full[kUnits], unit_empty[kUnits];
   uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
   uint64_t k_ready[Sh::kStages];  // 64-token pages: the stage's key scales are whole atoms
   uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];  // by step
@@ -107,7 +129,7 @@ struct Smem {
   int start_row;
   long long start_offset, first, last, per_cta;
   uint32_t tmem;
-  int abort_flag;
+  int abort_flag, ignored_flag;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -128,15 +150,16 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 
 __device__ __forceinline__ void softmax_sync() { bar_sync(kSoftmaxBarrier, 256); }
 
-__device__ __forceinline__ bool softmax_any(bool pred) {
+__device__ __forceinline__ bool bar_any(int id, int threads, bool pred) {
   uint32_t out;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(out)
-      : "r"((uint32_t)pred), "n"(kSoftmaxBarrier)
+      : "r"((uint32_t)pred), "r"(id), "r"(threads)
       : "memory");
   return out != 0;
 }
+__device__ __forceinline__ bool softmax_any(bool pred) { return bar_any(kSoftmaxBarrier, 256, pred); }
 
 // kind::f16 with A in tensor memory (lane = row, a 32-bit column = two neighbouring K values).
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
@@ -203,12 +226,6 @@ __device__ __forceinline__ float fp16_scale(float amax, float* inverse) {
   return __uint_as_float((uint32_t)field << 23);
 }
 
-struct RowInfo {
-  int count, pages, residual, sink, slot;  // pages: 128-token steps in the FP4 cache
-  int steps;                               // of one unit: pages, tail, drafts with sink
-  int tiles;
-};
-
 __device__ __forceinline__ RowInfo row_info(const TreeParams& p, int row, int page_tokens) {
   RowInfo r;
   r.count = p.node_counts ? min(max(p.node_counts[row], 0), p.nodes) : p.nodes;
@@ -229,11 +246,6 @@ __device__ __forceinline__ RowInfo row_info(const TreeParams& p, int row, int pa
   return r;
 }
 
-struct Unit {
-  RowInfo info;
-  int row, head, tile, begin, end;  // steps [begin, end) of the unit are this CTA's
-};
-
 enum StepKind { kStepPage, kStepTail, kStepDraft };
 
 __device__ __forceinline__ StepKind step_kind(const RowInfo& r, int step) {
@@ -248,8 +260,7 @@ __device__ __forceinline__ int step_slices(const RowInfo& r, StepKind kind) {
   return kind == kStepPage ? 8 : (bf16_places(r, kind) + 15) / 16;
 }
 
-// The units of this CTA in order; every role walks them on its own. Steps are counted in 32 bits within a
-// row (the host refuses larger rows).
+// The units of this CTA in order. Steps are counted in 32 bits within a row (the host refuses larger rows).
 struct Walker {
   const TreeParams& p;
   int row, page_tokens, offset, left;
@@ -280,6 +291,31 @@ struct Walker {
 
 // ---- roles -----------------------------------------------------------------------------------------
 
+// The roles' loops run side by side on every scheduler and share its instruction cache, so waiting is a dozen
+// instructions, one when the phase is already over. After about two seconds, or once another thread has given
+// up, a wait ends without its phase; the roles go through the rest of their motions and the kernel reports it.
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 begin, now;\n\t.reg .b32 given_up;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+      "@p bra OVER;\n\t"
+      "mov.u64 begin, %%globaltimer;\n"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+      "@p bra OVER;\n\t"
+      "ld.volatile.shared.b32 given_up, [%2];\n\t"
+      "setp.ne.b32 p, given_up, 0;\n\t"
+      "@p bra OVER;\n\t"
+      "mov.u64 now, %%globaltimer;\n\t"
+      "sub.u64 now, now, begin;\n\t"
+      "setp.lt.u64 p, now, %3;\n\t"
+      "@p bra AGAIN;\n\t"
+      "st.volatile.shared.b32 [%2], 1;\n"
+      "OVER:\n\t}" ::"r"(tc::smem_u32(bar)),
+      "r"(parity), "r"(tc::smem_u32(abort_flag)), "n"(tc::kWaitLimitNs)
+      : "memory");
+}
+
 // One thread of a converged warp. tcgen05.mma and the bulk copies take their operands from uniform registers:
 // behind an elected predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32
 // (N = 64) to 64 cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its
@@ -290,10 +326,29 @@ __device__ __forceinline__ bool elect_one() {
   return elected != 0;
 }
 
+// A role's view of the ring of units.
+template <int NT>
+struct Units {
+  Smem<NT>& sm;
+  int next_unit;
+  __device__ explicit Units(Smem<NT>& s) : sm(s), next_unit(0) {}
+  // The whole warp: the next unit into `u`; false when there is none, or when a wait has been given up (then `u`
+  // may hold anything). Roles whose warps meet at barriers have to agree on the answer.
+  __device__ __forceinline__ bool next(Unit& u) {
+    const int at = next_unit % kUnits;
+    wait(&sm.unit_full[at], (next_unit / kUnits) & 1, &sm.abort_flag);
+    u = sm.units[at];
+    ++next_unit;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&sm.unit_empty[at]);
+    return __all_sync(0xffffffffu, u.begin >= 0 && *static_cast<volatile int*>(&sm.abort_flag) == 0);
+  }
+};
+
 // One side's copies: SIDE 0 brings a page's key codes and scales, SIDE 1 its values' and the rows of the BF16
 // steps. Two warps, because a copy keeps its issuer for 80 cycles and a step of 64-token pages has eight.
 template <int NT, int PT, int SIDE>
-__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* map, int lane) {
+__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const CUtensorMap* map, int lane) {
   using Sh = Shape<NT>;
   constexpr int kEntries = kPage / PT;
   const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
@@ -305,12 +360,37 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
     ++issued;
     if (++slot == Sh::kStages) slot = 0, turn ^= 1;
   };
-  Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
+  // the key producer walks the units and publishes each before the one in front of it is produced
+  Units<NT> units(sm);
+  Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
+  Unit u, following;
+  bool known = false, more = true;
+  int published = 0;
+  auto publish = [&] {
+    more = more && walker.next(following, known);
+    known = true;
+    wait(&sm.unit_empty[published % kUnits], ((published / kUnits) & 1) ^ 1, &sm.abort_flag);
+    if (lane == 0) {
+      if (!more) following.begin = -1;
+      sm.units[published % kUnits] = following;
+      tc::mbar_arrive(&sm.unit_full[published % kUnits]);
+    }
+    __syncwarp();
+    ++published;
+  };
+  if (SIDE == 0) publish();
+  while (true) {
+    if (SIDE == 0) {
+      if (!more) break;
+      u = following;
+      publish();
+    } else if (!units.next(u)) {
+      break;
+    }
     const int32_t* table = p.table + u.row * p.table_stride;
     const uint8_t* codes = p.codes[SIDE] + u.head * (PT == 128 ? 8192 : 4096);
     const uint8_t* scales = p.scales[SIDE] + u.head * (PT == 128 ? 1024 : 512);
+    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&sm.abort_flag) != 0)) break;
     const int stop = min(u.end, u.info.pages);
     for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
       const int entry = batch * kEntries + lane;
@@ -327,7 +407,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
         int page[kEntries];
 #pragma unroll
         for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
-        tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+        wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
         if (elect_one()) {
           uint8_t* stage = sm.ring[slot];
           tc::mbar_expect_tx(&full[slot], 9216);
@@ -356,7 +436,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
                                           : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
         const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
         for (int first = 0; first < places; first += kBf16Rows) {
-          tc::mbar_wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+          wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
           if (SIDE == 0) {
             if (lane == 0) tc::mbar_arrive(&full[slot]);  // nothing for the FP4 product here
           } else {
@@ -380,11 +460,10 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
     }
   }
   // After an abort nobody else waits for the copies still in flight: no CTA may end under them.
-  if (lane == 0 && sm.abort_flag) {
-    int ignore = 0;
+  if (lane == 0 && *static_cast<volatile int*>(&sm.abort_flag)) {
     for (int back = min(issued, Sh::kStages); back > 0; --back) {
       const int at = issued - back;
-      tc::mbar_wait(&full[at % Sh::kStages], (at / Sh::kStages) & 1, &ignore);
+      wait(&full[at % Sh::kStages], (at / Sh::kStages) & 1, &sm.ignored_flag);
     }
   }
   __syncwarp();
@@ -394,7 +473,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
 // for 40 to 60 cycles, and the sixteen of a step one after another were longer than the step's HBM time. The
 // whole warp walks and waits; one thread of it issues.
 template <int NT, int PT>
-__device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
+__device__ __forceinline__ void issue_scores(Smem<NT>& sm) {
   using Sh = Shape<NT>;
   constexpr uint32_t kFp4 = tc::nvf4_idesc(128, NT), kF16 = f16_idesc(NT, 0, false);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
@@ -403,10 +482,10 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
   const uint64_t q_scales = tc::sf_atom_desc(tc::smem_u32(sm.q_scales));
   int n = 0, block = 0, unit = 0, slot = 0;
   uint32_t turn = 0, bf16_turn = 0;  // bf16_turn: one bit per half of the values' threads
+  Units<NT> units(sm);
   Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
-    tc::mbar_wait(&sm.q_full, unit & 1, &sm.abort_flag);
+  while (units.next(u)) {
+    wait(&sm.q_full, unit & 1, &sm.abort_flag);
     tc::fence_after_sync();
     if (elect_one()) {
 #pragma unroll
@@ -417,9 +496,9 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
       const StepKind kind = step_kind(u.info, step);
       const int within = (step - u.begin) & 1, set = block & 1;
       const uint32_t scores = tmem + Sh::kS + (2 * set + within) * NT;
-      if (within == 0) tc::mbar_wait(&sm.s_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
+      if (within == 0) wait(&sm.s_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
       if (kind == kStepPage) {
-        tc::mbar_wait(PT == 64 ? &sm.k_ready[slot] : &sm.full_k[slot], turn, &sm.abort_flag);
+        wait(PT == 64 ? &sm.k_ready[slot] : &sm.full_k[slot], turn, &sm.abort_flag);
         tc::fence_after_sync();
         const uint32_t stage = ring + slot * kStage;
         const uint64_t codes = tc::fp4_tile_desc(stage, 0), atoms = tc::sf_atom_desc(stage + kKsOffset);
@@ -427,7 +506,7 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
         if (elect_one()) {
           tc::cp_sf_atom(scales, atoms);
           tc::cp_sf_atom(scales + 4, atoms + 32);
-#pragma unroll
+#pragma unroll 1
           for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
 #pragma unroll
             for (int term = 0; term < kTerms; ++term)
@@ -441,12 +520,12 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
         if (++slot == Sh::kStages) slot = 0, turn ^= 1;
       } else {
         for (int i = 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows); i > 0; --i) {
-          tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);  // the stage is not this product's
+          wait(&sm.full_k[slot], turn, &sm.abort_flag);  // the stage is not this product's
           if (elect_one()) tc::mbar_arrive(&sm.empty[slot]);
           __syncwarp();
           if (++slot == Sh::kStages) slot = 0, turn ^= 1;
         }
-        tc::mbar_wait(&sm.ka_full[n & 1], (bf16_turn >> (n & 1)) & 1, &sm.abort_flag);
+        wait(&sm.ka_full[n & 1], (bf16_turn >> (n & 1)) & 1, &sm.abort_flag);
         bf16_turn ^= 1u << (n & 1);
         tc::fence_after_sync();
         if (elect_one()) {
@@ -466,35 +545,35 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm, Walker walker) {
     }
     ++unit;
   }
-  int ignore = 0;  // also after an abort: tensor memory is freed behind the last product
+  // also after an abort: tensor memory is freed behind the last product
   if (elect_one()) tc::commit(&sm.drained);
   __syncwarp();
-  tc::mbar_wait(&sm.drained, 0, &ignore);
+  wait(&sm.drained, 0, &sm.ignored_flag);
 }
 
 template <int NT>
-__device__ __forceinline__ void issue_output(Smem<NT>& sm, Walker walker) {
+__device__ __forceinline__ void issue_output(Smem<NT>& sm) {
   using Sh = Shape<NT>;
   constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const uint64_t prob = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
   int n = 0, block = 0, unit = 0;
+  Units<NT> units(sm);
   Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
-    tc::mbar_wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
+  while (units.next(u)) {
+    wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
       const int within = (step - u.begin) & 1, set = block & 1;
-      tc::mbar_wait(&sm.va_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
-      if (within == 0) tc::mbar_wait(&sm.p_full[set], (block >> 1) & 1, &sm.abort_flag);
+      wait(&sm.va_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
+      if (within == 0) wait(&sm.p_full[set], (block >> 1) & 1, &sm.abort_flag);
       tc::fence_after_sync();
       const bool first = step == u.begin, closes = within == 1 || step + 1 == u.end;
       const uint64_t tile = prob + (2 * set + within) * 1024;
       const uint32_t operand = tmem + Sh::kV + (n & 1) * 64;
       if (elect_one()) {
         if (kind == kStepPage) {
-#pragma unroll
+#pragma unroll 2
           for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
             mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kPages, !(first && s == 0));
         } else {
@@ -511,10 +590,9 @@ __device__ __forceinline__ void issue_output(Smem<NT>& sm, Walker walker) {
     }
     ++unit;
   }
-  int ignore = 0;
   if (elect_one()) tc::commit(&sm.drained);
   __syncwarp();
-  tc::mbar_wait(&sm.drained, 0, &ignore);
+  wait(&sm.drained, 0, &sm.ignored_flag);
 }
 
 // 64-token pages: the key scales of a step's two pages come as half atoms (32 rows of 8 bytes); one warp
@@ -547,7 +625,7 @@ __device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint3
 
 // The values' warps: thread c of a half holds channel c of its steps' V^T, and token c of a BF16 step's K.
 template <int NT, int PT>
-__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
+__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, int thread) {
   const int c = thread & 127, lane = c & 31, half = thread >> 7;
   using Sh = Shape<NT>;
   const uint32_t lanes = (uint32_t)(c & ~31) << 16;
@@ -558,7 +636,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
     if (slot >= Sh::kStages) slot -= Sh::kStages, turn ^= 1;
   };
   auto arrived = [&]() -> uint8_t* {
-    tc::mbar_wait(&sm.full_v[slot], turn, &sm.abort_flag);
+    wait(&sm.full_v[slot], turn, &sm.abort_flag);
     return sm.ring[slot];
   };
   const bool interleaves = PT == 64 && (c >> 5) == 3;
@@ -567,9 +645,9 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
     if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
     pass(1);
   };
+  Units<NT> units(sm);
   Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
+  while (!bar_any(kValuesBarrier + half, 128, !units.next(u))) {
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
       if ((n & 1) != half) {
@@ -581,15 +659,15 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
       const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
       if (kind == kStepPage) {
         if (interleaves) {
-          tc::mbar_wait(&sm.full_k[slot], turn, &sm.abort_flag);
+          wait(&sm.full_k[slot], turn, &sm.abort_flag);
           interleave_scales(sm.ring[slot] + kKsOffset, lane);
           if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
         }
         const uint8_t* stage = arrived();
         const uint8_t* scales = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
+        wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-#pragma unroll 2
+#pragma unroll 1
         for (int j = 0; j < 4; ++j) {
           const uint8_t* at = PT == 128 ? stage + kVOffset + c * 64 + ((j ^ ((c >> 1) & 3)) * 16)
                                         : stage + kVOffset + (j >> 1) * 4096 + c * 32 + (((j & 1) ^ ((c >> 2) & 1)) * 16);
@@ -601,7 +679,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
         const int places = bf16_places(u.info, kind);
         const int stages = (places + kBf16Rows - 1) / kBf16Rows;
         // keys first, through the buffer that takes the values after the score product
-        tc::mbar_wait(operand_empty, empty_parity, &sm.abort_flag);
+        wait(operand_empty, empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
         {  // a step's stages are held together
           uint8_t* const stage0 = arrived();
@@ -609,7 +687,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
           if (stages > 1) {
             const bool wraps = slot + 1 == Sh::kStages;
             const int next = wraps ? 0 : slot + 1;
-            tc::mbar_wait(&sm.full_v[next], turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
+            wait(&sm.full_v[next], turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
             stage1 = sm.ring[next];
           }
           auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
@@ -618,7 +696,8 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
             if (c < BDFP4_MAX_SINK) there = c < u.info.sink;
             if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
               const int group = c & 7;
-              const int64_t shift_at = u.head * kHeadDim + group * kGroup;
+              const float* shift = p.key_shift ? p.key_shift + u.head * kHeadDim + group * kGroup : nullptr;
+#pragma unroll 1
               for (int first = 0; first < u.info.count; first += 16) {
                 // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
                 const int node = min(first + (c >> 3), u.info.count - 1);
@@ -631,9 +710,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
                   v[2 * i] = __uint_as_float(w[i] << 16);
                   v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
                 }
-                if (p.rotate && p.key_shift) cache_basis16<BDFP4_SHIFT_F32, true>(v, group, p.key_shift, shift_at);
-                else if (p.rotate) cache_basis16<BDFP4_SHIFT_NONE, true>(v, group, nullptr, 0);
-                else cache_basis16<BDFP4_SHIFT_F32, false>(v, group, p.key_shift, shift_at);
+                cache_basis16_any(v, group, p.rotate != 0, shift);
                 if (first + (c >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
               }
               tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
@@ -643,7 +720,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
           const uint4* row = reinterpret_cast<const uint4*>(row_of(min(c, places - 1)));
           float amax = 0.0f;
           if (there) {
-#pragma unroll 4
+#pragma unroll 2
             for (int j = 0; j < 16; ++j) {
               const uint4 r = row[j];
               const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -677,13 +754,14 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
           tc::fence_before_sync();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&sm.ka_full[half]);
-          tc::mbar_wait(&sm.ka_empty[half], bf16_turn, &sm.abort_flag);
+          wait(&sm.ka_empty[half], bf16_turn, &sm.abort_flag);
           tc::fence_after_sync();
           bf16_turn ^= 1;
         }
         for (int first = 0; first < places; first += kBf16Rows) {
           const uint8_t* stage = arrived() + 2 * c;
           const int slices = (min(places - first, kBf16Rows) + 15) / 16;
+#pragma unroll 1
           for (int s = 0; s < slices; ++s) {
             const int place = first + s * 16;
             const int stop = kind == kStepDraft && place == 0 ? u.info.sink : places;
@@ -714,69 +792,67 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker
 // still has all four terms above E4M3's smallest scale. Returns what undoes the scaling.
 template <int NT>
 __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
-  constexpr int kPerPass = 32, kPasses = (NT + kPerPass - 1) / kPerPass;
-  const int group = thread & 7;
+  const int group = thread & 7;  // eight threads hold one query
   const int queries = u.info.count * p.ratio;
-  float v[kPasses][16];
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int query = u.tile * NT + i * kPerPass + (thread >> 3);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[i][j] = 0.0f;
-    if (query < queries && i * kPerPass + (thread >> 3) < NT)
-      load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
-                       (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
-  }
   if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    if (p.rotate) {
-      hadamard_butterflies(v[i], group);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[i][j] *= kInvSqrt128;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (fabsf(v[i][j]) < INFINITY) amax = fmaxf(amax, fabsf(v[i][j]));
-  }
-  amax = warp_max(amax);
-  if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
-  softmax_sync();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) amax = fmaxf(amax, sm.q_max[w]);
-  float inverse;
-  const float scale = fp16_scale(amax, &inverse);
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int r = i * kPerPass + (thread >> 3);
-    if (NT < kPerPass && r >= NT) break;
-    uint8_t* row = sm.q[group >> 2] + r * 128;
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[i][2 * j] * scale, v[i][2 * j + 1] * scale));
-    const int chunk = (group & 3) * 2;
-    *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
-    float left[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) left[j] = v[i][j] * scale;
-    const int at = r * 64 + group * 8;
+  float scale = 1.0f, inverse = 1.0f;
 #pragma unroll 1
-    for (int term = 0; term < kTerms; ++term) {
-      float largest = 0.0f;
+  for (int phase = 0; phase < 2; ++phase) {  // the tile's largest value, then the operands
+    float amax = 0.0f;
+#pragma unroll 1
+    for (int r = thread >> 3; r < (NT < 32 ? 32 : NT); r += 32) {
+      const int query = u.tile * NT + r;
+      float v[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(left[j]));
-      const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
-      GroupCodes codes;
-      codes.scale = e4m3_to_float(byte);
-      encode16(left, codes.scale, codes.lo, codes.hi);
-      *reinterpret_cast<uint2*>(sm.q_codes[term] + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
-      sm.q_scales[term][scale_tile_offset(r, group)] = (uint8_t)byte;
-      float rest[16];
-      group_residual16(left, codes, rest);
+      for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+      if (query < queries && r < NT)
+        load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
+                         (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v);
+      if (p.rotate) {
+        hadamard_butterflies(v, group);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) left[j] = rest[j];
+        for (int j = 0; j < 16; ++j) v[j] *= kInvSqrt128;
+      }
+      if (phase == 0) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
+      } else if (r < NT) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] *= scale;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
+        uint8_t* row = sm.q[group >> 2] + r * 128;
+        const int chunk = (group & 3) * 2;
+        *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+        const int at = r * 64 + group * 8;
+#pragma unroll 1
+        for (int term = 0; term < kTerms; ++term) {
+          float largest = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(v[j]));
+          const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
+          GroupCodes codes;
+          codes.scale = e4m3_to_float(byte);
+          encode16(v, codes.scale, codes.lo, codes.hi);
+          *reinterpret_cast<uint2*>(sm.q_codes[term] + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
+          sm.q_scales[term][scale_tile_offset(r, group)] = (uint8_t)byte;
+          float rest[16];
+          group_residual16(v, codes, rest);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = rest[j];
+        }
+      }
+    }
+    if (phase == 0) {
+      amax = warp_max(amax);
+      if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
+      softmax_sync();
+#pragma unroll
+      for (int w = 0; w < 8; ++w) amax = fmaxf(amax, sm.q_max[w]);
+      scale = fp16_scale(amax, &inverse);
     }
   }
   tc::fence_proxy_async_smem();
@@ -808,22 +884,24 @@ __device__ __forceinline__ void reduce_columns(float* v, int lane, int column, S
 }
 
 template <int NT>
-__device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
+__device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, int thread) {
   using Sh = Shape<NT>;
   constexpr int C = Sh::kColumns;
   const int t = thread & 127, lane = thread & 31, warp = thread >> 5, half = thread >> 7;
   const int first_column = Sh::kByStep ? 0 : half * C;
   const uint32_t lanes = (uint32_t)(t & ~31) << 16;
   const float* base = sm.base + first_column;
+  // the warps that hold the columns of query `thread`
+  const int column_warps = Sh::kByStep ? 8 : 4, column_warp0 = Sh::kByStep ? 0 : (thread & (NT - 1)) / C * 4;
   int n = 0, block = 0, unit = 0;
+  Units<NT> units(sm);
   Unit u;
-  if (!walker.next(u, false)) return;
-  bool more = true;
-  float q_inverse = load_queries<NT>(p, sm, u, thread);
+  bool more = !softmax_any(!units.next(u));
+  float q_inverse = more ? load_queries<NT>(p, sm, u, thread) : 1.0f;
   while (more) {
     if (thread < NT) {
       sm.top[thread] = kNoMax;
-      sm.base[thread] = kShift - kNoMax;
+      sm.extra[thread] = 0.0f;
       // the draft nodes that this query sees
       const int query = u.tile * NT + thread;
       uint64_t seen = 0;
@@ -843,174 +921,199 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       const int steps = min(2, u.end - block_begin), set = block & 1;
       // this half's steps of the block
       const int from = Sh::kByStep ? half : 0, to = Sh::kByStep ? min(half + 1, steps) : steps;
-      // One step of the block: its scores in log2 units above the maxima (plus kShift) are f * score + base.
+      // a block in which every query sees every token, and all of it FP4
+      const bool plain = block_begin + steps <= u.info.pages && (block_begin > 0 || u.info.sink == 0);
+      auto scores_ready = [&](int i) {
+        wait(&sm.s_full[set][i], (block >> 1) & 1, &sm.abort_flag);
+        tc::fence_after_sync();
+      };
+      // Any step: scores in log2 units above the maxima (plus kShift) are f * score + base; a token may be seen by
+      // no query or, a draft, by some.
       struct Step {
         StepKind kind;
-        bool dead, special, masked;  // special is the same for all tokens
+        bool dead, masked;
         float f;
         uint32_t scores;
-        uint8_t* row;
       };
       auto open = [&](int i) {
         Step k;
         k.kind = step_kind(u.info, block_begin + i);
-        if (k.kind == kStepPage) k.dead = block_begin + i == 0 && t < u.info.sink;  // no query sees this thread's token
+        if (k.kind == kStepPage) k.dead = block_begin + i == 0 && t < u.info.sink;
         else if (k.kind == kStepTail) k.dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
         else k.dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-        k.special = k.kind != kStepPage || (block_begin + i == 0 && u.info.sink > 0);
         k.masked = k.kind == kStepDraft && t >= BDFP4_MAX_SINK && !k.dead;
         k.f = k.kind == kStepPage ? page_factor : p.scale_log2 * q_inverse * sm.key_factor[(n + i) & 7][t];
         k.scores = sm.tmem + Sh::kS + (2 * set + i) * NT + first_column + lanes;
-        k.row = sm.p[set][i] + t * 128;
         return k;
       };
-      auto mask16 = [&](const Step& k, int j, float* v) {
-        if (k.special) {
+      auto load8 = [&](const Step& k, int j, float* v) {
+        tc::tmem_ld8(k.scores + j, v);
+        tc::tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (k.dead || (k.masked && !((sm.family[first_column + j + i] >> (t - BDFP4_MAX_SINK)) & 1))) v[i] = -INFINITY;
-        }
+        for (int c = 0; c < 8; ++c)
+          if (k.dead || (k.masked && !((sm.family[first_column + j + c] >> (t - BDFP4_MAX_SINK)) & 1))) v[c] = -INFINITY;
       };
-      // The step's probabilities, added to s in FP32 and stored rounded. True when one of this thread's exceeds
-      // kHighest: its query's maximum has to be renewed, and the block formed again.
-      float s[C];
-      auto form = [&](int i) -> bool {
-        const Step k = open(i);
-        const float2 f2 = make_float2(k.f, k.f);
-        bool high = false;
-        float all[Sh::kByStep ? C : 16];
-        if constexpr (Sh::kByStep) {
+      float s[C];  // a plain block's probabilities, both steps' added
+      bool high, fresh = block_begin == u.begin;
+      // P of this block goes where the one before the last was
+      wait(&sm.p_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
+      while (true) {
+        if (fresh) {  // take the maxima anew; what was summed so far is brought down to them
+          float mine = -INFINITY;
+#pragma unroll 1
+          for (int i = from; i < to; ++i) {
+            scores_ready(i);
+            const Step k = open(i);
+#pragma unroll 1
+            for (int j = 0; j < C; j += 8) {
+              float v[8];
+              load8(k, j, v);
 #pragma unroll
-          for (int j = 0; j < C; j += 16) tc::tmem_ld16(k.scores + j, all + j);
-          tc::tmem_wait_ld();
-        }
-#pragma unroll
-        for (int j = 0; j < C; j += 16) {
-          float* v = Sh::kByStep ? all + j : all;
-          if constexpr (!Sh::kByStep) {
-            tc::tmem_ld16(k.scores + j, v);
-            tc::tmem_wait_ld();
-          }
-          mask16(k, j, v);
-#pragma unroll
-          for (int c = 0; c < 16; c += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(base + j + c);
-            const float2 y0 = __ffma2_rn(make_float2(v[c], v[c + 1]), f2, make_float2(b.x, b.y));
-            const float2 y1 = __ffma2_rn(make_float2(v[c + 2], v[c + 3]), f2, make_float2(b.z, b.w));
-            v[c] = ex2(y0.x), v[c + 1] = ex2(y0.y), v[c + 2] = ex2(y1.x), v[c + 3] = ex2(y1.y);
-          }
-          uint32_t w[8];
-          if (k.kind == kStepPage) {
-            __half2 most = __floats2half2_rn(0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const __half2 pair = __floats2half2_rn(v[2 * c], v[2 * c + 1]);
-              most = __hmax2(most, pair);
-              w[c] = h2(pair);
+              for (int c = 0; c < 8; ++c) {
+                const float m = warp_max(v[c] * k.f);
+                if (lane == j + c) mine = fmaxf(mine, m);
+              }
             }
-            high |= __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
-          } else {
-            float most = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              most = fmaxf(most, fmaxf(v[2 * c], v[2 * c + 1]));
-              w[c] = pack_bf16x2(v[2 * c] * p.inverse_value_scale, v[2 * c + 1] * p.inverse_value_scale);
-            }
-            high |= most > kHighest;
           }
-          const int chunk = (first_column + j) >> 3;
-          *reinterpret_cast<uint4*>(k.row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4*>(k.row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+          if (lane < C) sm.col_max[warp][first_column + lane] = mine;
+          softmax_sync();
+          if (thread < NT) {
+            const float before = sm.top[thread];
+            float now = before;
+            for (int w = 0; w < column_warps; ++w) now = fmaxf(now, sm.col_max[column_warp0 + w][thread]);
+            const float factor = ex2(before - now);
+            sm.top[thread] = now;
+            sm.base[thread] = kShift - now;
+            sm.factor[thread] = factor;
+            sm.extra[thread] *= factor;
+          }
+          softmax_sync();
+          if (block_begin > u.begin) {
 #pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            const float2 both = __fadd2_rn(make_float2(s[j + c], s[j + c + 1]), make_float2(v[c], v[c + 1]));
-            s[j + c] = both.x, s[j + c + 1] = both.y;
+            for (int j = 0; j < C / 2; ++j) {
+              sum[j].x *= sm.factor[first_column + 2 * j];
+              sum[j].y *= sm.factor[first_column + 2 * j + 1];
+            }
+            wait(&sm.p_empty[set ^ 1], ((block - 1) >> 1) & 1, &sm.abort_flag);
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int j = half * Sh::kOut; j < (half + 1) * Sh::kOut; j += 8) {
+              float o[8];
+              uint32_t r[8];
+              const uint32_t at = sm.tmem + Sh::kO + j + lanes;
+              tc::tmem_ld8(at, o);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(o[i] * sm.factor[j + i]);
+              st8(at, r);
+            }
+            tc::tmem_wait_st();
           }
         }
-        return high;
-      };
-      auto fence = [&] {
+        high = false;
+        if (plain) {
+          if (!Sh::kByStep) {
+#pragma unroll
+            for (int j = 0; j < C; ++j) s[j] = 0.0f;
+          }
+          const float2 f2 = make_float2(page_factor, page_factor);
+          __half2 most = __floats2half2_rn(0.0f, 0.0f);
+#pragma unroll 1
+          for (int i = from; i < to; ++i) {
+            scores_ready(i);
+            const uint32_t scores = sm.tmem + Sh::kS + (2 * set + i) * NT + first_column + lanes;
+            uint8_t* const row = sm.p[set][i] + t * 128;
+            float v[Sh::kByStep ? 1 : 16];
+            if constexpr (Sh::kByStep) {
+#pragma unroll
+              for (int j = 0; j < C; j += 16) tc::tmem_ld16(scores + j, s + j);
+              tc::tmem_wait_ld();
+            }
+#pragma unroll
+            for (int j = 0; j < C; j += 16) {
+              float* x = Sh::kByStep ? s + j : v;
+              if constexpr (!Sh::kByStep) {
+                tc::tmem_ld16(scores + j, x);
+                tc::tmem_wait_ld();
+              }
+#pragma unroll
+              for (int c = 0; c < 16; c += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(base + j + c);
+                const float2 y0 = __ffma2_rn(make_float2(x[c], x[c + 1]), f2, make_float2(b.x, b.y));
+                const float2 y1 = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), f2, make_float2(b.z, b.w));
+                x[c] = ex2(y0.x), x[c + 1] = ex2(y0.y), x[c + 2] = ex2(y1.x), x[c + 3] = ex2(y1.y);
+              }
+              uint32_t w[8];
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const __half2 pair = __floats2half2_rn(x[2 * c], x[2 * c + 1]);
+                most = __hmax2(most, pair);
+                w[c] = h2(pair);
+              }
+              const int chunk = (first_column + j) >> 3;
+              *reinterpret_cast<uint4*>(row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+              if constexpr (!Sh::kByStep) {
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) {
+                  const float2 both = __fadd2_rn(make_float2(s[j + c], s[j + c + 1]), make_float2(x[c], x[c + 1]));
+                  s[j + c] = both.x, s[j + c + 1] = both.y;
+                }
+              }
+            }
+          }
+          high = __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
+        } else {
+          float* const sums = sm.step_sum[set][warp] + first_column;
+          if (from >= to && lane < C) sums[lane] = 0.0f;
+#pragma unroll 1
+          for (int i = from; i < to; ++i) {
+            scores_ready(i);
+            const Step k = open(i);
+            uint8_t* const row = sm.p[set][i] + t * 128;
+#pragma unroll 1
+            for (int j = 0; j < C; j += 8) {
+              float v[8];
+              load8(k, j, v);
+              uint32_t w[4];
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                v[c] = ex2(fmaf(v[c], k.f, base[j + c]));
+                high |= v[c] > kHighest;
+              }
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                w[c] = k.kind == kStepPage ? h2(__floats2half2_rn(v[2 * c], v[2 * c + 1]))
+                                           : pack_bf16x2(v[2 * c] * p.inverse_value_scale, v[2 * c + 1] * p.inverse_value_scale);
+              *reinterpret_cast<uint4*>(row + ((((first_column + j) >> 3) ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+              // four lanes end up with each column's sum
+              reduce_columns<8, 16>(v, lane, j, [&](int column, float total) {
+                if ((lane & 3) == 0) sums[column] = i > from ? sums[column] + total : total;
+              });
+            }
+          }
+        }
         tc::fence_before_sync();
         tc::fence_proxy_async_smem();
-      };
-#pragma unroll
-      for (int j = 0; j < C; ++j) s[j] = 0.0f;
-      // P of this block goes where the one before the last was
-      tc::mbar_wait(&sm.p_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
-      bool high = false;
-#pragma unroll 1
-      for (int i = from; i < to; ++i) {
-        tc::mbar_wait(&sm.s_full[set][i], (block >> 1) & 1, &sm.abort_flag);
-        tc::fence_after_sync();
-        high |= form(i);
-      }
-      fence();
-      if (softmax_any(high)) {
-        float mine = -INFINITY;
-#pragma unroll 1
-        for (int i = from; i < to; ++i) {
-          const Step k = open(i);
-#pragma unroll
-          for (int j = 0; j < C; j += 16) {
-            float v[16];
-            tc::tmem_ld16(k.scores + j, v);
-            tc::tmem_wait_ld();
-            mask16(k, j, v);
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float m = warp_max(v[c] * k.f);
-              if (lane == j + c) mine = fmaxf(mine, m);
-            }
-          }
-        }
-        if (lane < C) sm.col_max[warp][first_column + lane] = mine;
-        softmax_sync();
-        if (thread < NT) {
-          const float before = sm.top[thread];
-          float now = before;
-          const int w0 = Sh::kByStep ? 0 : thread / C * 4;
-#pragma unroll
-          for (int w = 0; w < (Sh::kByStep ? 8 : 4); ++w) now = fmaxf(now, sm.col_max[w0 + w][thread]);
-          sm.top[thread] = now;
-          sm.base[thread] = kShift - now;
-          sm.factor[thread] = ex2(before - now);
-        }
-        softmax_sync();
-#pragma unroll
-        for (int j = 0; j < C / 2; ++j) {
-          sum[j].x *= sm.factor[first_column + 2 * j];
-          sum[j].y *= sm.factor[first_column + 2 * j + 1];
-        }
-#pragma unroll
-        for (int j = 0; j < C; ++j) s[j] = 0.0f;
-#pragma unroll 1
-        for (int i = from; i < to; ++i) form(i);
-        if (block_begin > u.begin) {  // what O^T holds is of the old maxima
-          tc::mbar_wait(&sm.p_empty[set ^ 1], ((block - 1) >> 1) & 1, &sm.abort_flag);
-          tc::fence_after_sync();
-#pragma unroll 1
-          for (int j = half * Sh::kOut; j < (half + 1) * Sh::kOut; j += 8) {
-            float o[8];
-            uint32_t r[8];
-            const uint32_t at = sm.tmem + Sh::kO + j + lanes;
-            tc::tmem_ld8(at, o);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(o[i] * sm.factor[j + i]);
-            st8(at, r);
-          }
-          tc::tmem_wait_st();
-        }
-        fence();
-        softmax_sync();
+        // against maxima just taken nothing is high: the vote then only ends the block
+        if (!softmax_any(high) || fresh) break;
+        fresh = true;
       }
       // the barrier stands behind every thread's scores read and probabilities written
       if (thread == 0) {
         tc::mbar_arrive(&sm.p_full[set]);
         tc::mbar_arrive(&sm.s_empty[set]);
       }
+      if (plain) {
+        if (from < to) {
 #pragma unroll
-      for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
+          for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
+        }
+      } else if (thread < NT) {
+        float total = sm.extra[thread];
+        for (int w = 0; w < column_warps; ++w) total += sm.step_sum[set][column_warp0 + w][thread];
+        sm.extra[thread] = total;
+      }
       n += steps;
     }
 
@@ -1020,19 +1123,16 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
       reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col_sum[warp][first_column + j] = total; });
     }
-    // the next unit's queries go in while this one's last product runs: all its scores are done
-    Unit following = u;
-    more = walker.next(following, true);
+    Unit following;
+    // (the barrier also stands behind the column sums, and frees the parents)
+    more = !softmax_any(!units.next(following));
     float next_inverse = 1.0f;
-    softmax_sync();  // the column sums are there; the parents are free
     const bool whole = u.begin == 0 && u.end == u.info.steps;
     // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
     const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
     if (thread < NT) {
-      const int w0 = Sh::kByStep ? 0 : thread / C * 4;
-      float total = 0.0f;
-#pragma unroll
-      for (int w = 0; w < (Sh::kByStep ? 8 : 4); ++w) total += sm.col_sum[w0 + w][thread];
+      float total = sm.extra[thread];
+      for (int w = 0; w < column_warps; ++w) total += sm.col_sum[column_warp0 + w][thread];
       if (whole) {
         sm.total[thread] = total > 0.0f ? p.value_scale / total : 0.0f;
       } else {
@@ -1040,9 +1140,10 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
         p.partial_stat[(int64_t)(2 * part + 1) * NT + thread] = total;
       }
     }
+    // the next unit's queries go in while this one's last product runs: all its scores are done
     if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
     softmax_sync();
-    tc::mbar_wait(&sm.o_full, unit & 1, &sm.abort_flag);
+    wait(&sm.o_full, unit & 1, &sm.abort_flag);
     tc::fence_after_sync();
     const int out_first = half * Sh::kOut;
     const int queries = min(u.info.count * p.ratio - u.tile * NT - out_first, Sh::kOut);
@@ -1068,7 +1169,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       }
     }
     tc::fence_before_sync();
-    softmax_sync();  // the output has been read; base, top and total are written anew
+    softmax_sync();  // the output has been read; what is kept per query is written anew
     if (thread == 0) tc::mbar_arrive(&sm.o_empty);
     if (!whole && u.begin == 0 && thread == 0) {
       TreeSplit split;
@@ -1120,12 +1221,16 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       tc::mbar_init(&sm.p_full[i], 1);
       tc::mbar_init(&sm.p_empty[i], 1);
     }
+    for (int i = 0; i < kUnits; ++i) {
+      tc::mbar_init(&sm.unit_full[i], 1);
+      tc::mbar_init(&sm.unit_empty[i], kUnitReaders);
+    }
     tc::mbar_init(&sm.q_full, 1);
     tc::mbar_init(&sm.o_full, 1);
     tc::mbar_init(&sm.o_empty, 1);
     tc::mbar_init(&sm.drained, 2);
     tc::fence_barrier_init();
-    sm.abort_flag = 0;
+    sm.abort_flag = sm.ignored_flag = 0;
     TreeSplit none;
     none.row = -1;
     none.head = none.tile = none.last = 0;
@@ -1172,19 +1277,18 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   __syncthreads();
   tc::fence_after_sync();
   if (sm.first < sm.last) {
-    const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
     if (warp < 8) {
       trade_registers<Sh::kLaunchRegs, Sh::kValueRegs>();
-      values<NT, PT>(p, sm, walker, thread);
+      values<NT, PT>(p, sm, thread);
     } else if (warp < 16) {
       trade_registers<Sh::kLaunchRegs, Sh::kSoftmaxRegs>();
-      softmax<NT>(p, sm, walker, thread - 256);
+      softmax<NT>(p, sm, thread - 256);
     } else {
       trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
-      if (warp == 16) produce<NT, PT, 0>(p, sm, walker, &k_map, lane);
-      if (warp == 17) produce<NT, PT, 1>(p, sm, walker, &v_map, lane);
-      if (warp == 18) issue_scores<NT, PT>(sm, walker);
-      if (warp == 19) issue_output<NT>(sm, walker);
+      if (warp == 16) produce<NT, PT, 0>(p, sm, &k_map, lane);
+      if (warp == 17) produce<NT, PT, 1>(p, sm, &v_map, lane);
+      if (warp == 18) issue_scores<NT, PT>(sm);
+      if (warp == 19) issue_output<NT>(sm);
     }
   }
   tc::fence_before_sync();
