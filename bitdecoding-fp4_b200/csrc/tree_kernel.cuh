@@ -50,31 +50,33 @@ constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
 // A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
 // 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
 constexpr int kBf16Pitch = 272, kBf16Rows = 64;
-// Named barriers: the softmax threads, the two halves of the values' threads.
-constexpr int kSoftmaxBarrier = 1, kValuesBarrier = 2;
+// Named barriers: the softmax threads, each stream of them, each half of the values' threads.
+constexpr int kSoftmaxBarrier = 1, kStreamBarrier = 2, kValuesBarrier = 4;
 constexpr int kTerms = 4;             // FP4 terms of a query
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
 constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renewed when one exceeds this, 2^8 above
 
-// Two warpgroups of softmax and two of values. With 64 queries the softmax halves take 32 queries each (sums
-// stay in registers for a whole unit; 64 spilled, into an L1 that shared memory has left 24 KB of); with 32 or
-// 16, where a step is all latency, they take the two steps of a block. The values' halves take even and odd steps.
+// A unit's blocks of two steps go alternately to two streams, each a softmax of its own (maxima, sums, output)
+// in a warpgroup of its own, joined when the unit ends: one stream's block is a chain of latencies (scores out
+// of tensor memory, exponentials, stores, fences, a barrier) that the other fills. The values' two warpgroups
+// take even and odd steps. Tiles of 64 queries were built too and lost: their sums and scores leave no registers
+// for a second stream, and a step cost 2000 cycles against 2 x 600.
 template <int NT>
 struct Shape {
-  static constexpr bool kByStep = NT <= 32;
-  static constexpr int kColumns = kByStep ? NT : NT / 2;  // queries per softmax thread
-  static constexpr int kOut = NT / 2;                     // queries whose output a half rescales and writes
-  static constexpr int kStages = NT > 32 ? 6 : 7;
+  static constexpr int kOut = NT / 2;  // queries whose output a warpgroup writes
+  static constexpr int kStages = 7;
   static constexpr int kThreads = 256 + 256 + 128;  // values, softmax, control
   // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
   // must not exceed what the launch was given.
   static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 136, kValueRegs = 72, kControlRegs = 64;
   static_assert(2 * kSoftmaxRegs + 2 * kValueRegs + kControlRegs <= 5 * kLaunchRegs, "registers");
   static_assert(kLaunchRegs * kThreads <= 65536, "registers");
-  // tensor memory columns: scores (two blocks of two steps), output, values (two steps; a BF16 step's keys before
-  // its values), scales of the keys (two steps) and of the query terms
-  static constexpr int kS = 0, kO = 4 * NT, kV = kO + NT, kKs = kV + 128, kQs = kKs + 16;
+  static constexpr int kRow = NT * 2;  // bytes of a token's probabilities: the swizzle span of P
+  static constexpr uint64_t kSwizzle = NT == 32 ? tc::kSwizzle64B : tc::kSwizzle32B;
+  // tensor memory columns: scores [stream][set][step], output [stream], values (two steps; a BF16 step's keys
+  // before its values), scales of the keys (two steps) and of the query terms
+  static constexpr int kS = 0, kO = 8 * NT, kV = 10 * NT, kKs = kV + 128, kQs = kKs + 16;
   static_assert(kQs + 8 * kTerms <= 512, "tensor memory");
 };
 
@@ -82,6 +84,13 @@ template <int FROM, int TO>
 __device__ __forceinline__ void trade_registers() {
   if constexpr (TO > FROM) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TO));
   if constexpr (TO < FROM) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
+}
+
+// A value the compiler may not reason about: in a rolled loop a condition on it is not hoisted out (which would
+// make one copy of the loop per outcome).
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+r"(x));
+  return x;
 }
 
 struct RowInfo {
@@ -105,16 +114,13 @@ struct Smem {
   alignas(1024) uint8_t q[2][NT * 128];          // FP16: two halves of 64 channels, K-major, 128-byte swizzle
   alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
   alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
-  alignas(1024) uint8_t p[2][2][16384];            // [block][step] MN-major: 128-byte rows of 64 queries per token, swizzled
+  alignas(1024) uint8_t p[2][2][2][128 * Sh::kRow];  // [stream][set][step] MN-major: a row of queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
-  float base[NT];       // kShift - maximum
-  float top[NT];        // maximum, log2 units
-  float factor[NT];
-  float total[NT];
-  float extra[NT];      // weights of the steps that were not plain
-  float col_max[8][NT];
-  float col_sum[8][NT];
-  float step_sum[2][8][NT];  // [block] a not plain block's weights, by warp
+  // by stream: kShift - maximum; maximum, log2 units; what a renewal scales by; weights of not plain blocks
+  float base[2][NT], top[2][NT], factor[2][NT], extra[2][NT];
+  float share[2][NT];   // what a stream's output is multiplied by
+  float warp_value[2][4][NT];   // a block's maxima, a unit's sums, by warp
+  float step_sum[2][2][4][NT];  // [stream][set] a not plain block's weights, by warp
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
   float q_max[8];
   int parents[BDFP4_MAX_TREE_NODES];
@@ -123,11 +129,12 @@ struct Smem {
   uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
   uint64_t k_ready[Sh::kStages];  // 64-token pages: the stage's key scales are whole atoms
   uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];  // by step
-  uint64_t s_full[2][2], s_empty[2], p_full[2], p_empty[2];  // [block][step] and [block]
+  uint64_t s_full[2][2][2], s_empty[2][2], p_full[2][2], p_empty[2][2];  // [stream][set], s_full by step too
   uint64_t q_full, o_full, o_empty, drained;
   long long sums[Sh::kThreads / 32];
   int start_row;
-  long long start_offset, first, last, per_cta;
+  long long start_offset, first, last;
+  int per_cta;
   uint32_t tmem;
   int abort_flag, ignored_flag;
 };
@@ -269,6 +276,7 @@ struct Walker {
   // `known`: u is a unit of this walk, so its row's lengths need not be read again.
   __device__ __forceinline__ bool next(Unit& u, bool known) {
     if (left <= 0) return false;
+#pragma unroll 1
     while (true) {
       if (!known || u.row != row) u.info = row_info(p, row, page_tokens);
       const int whole = u.info.steps * u.info.tiles * p.heads_kv;
@@ -379,6 +387,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
     ++published;
   };
   if (SIDE == 0) publish();
+#pragma unroll 1
   while (true) {
     if (SIDE == 0) {
       if (!more) break;
@@ -392,6 +401,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
     const uint8_t* scales = p.scales[SIDE] + u.head * (PT == 128 ? 1024 : 512);
     if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&sm.abort_flag) != 0)) break;
     const int stop = min(u.end, u.info.pages);
+#pragma unroll 1
     for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
       const int entry = batch * kEntries + lane;
       int mine = 0;
@@ -403,6 +413,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
         }
       }
       const int steps = min(32 / kEntries, stop - batch);
+#pragma unroll 1
       for (int i = 0; i < steps; ++i) {
         int page[kEntries];
 #pragma unroll
@@ -427,14 +438,17 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
         advance();
       }
     }
+#pragma unroll 1
     for (int step = max(u.begin, u.info.pages); step < u.end; ++step) {
       const StepKind kind = step_kind(u.info, step);
       const int places = bf16_places(u.info, kind);
+#pragma unroll 1
       for (int side = 0; side < 2; ++side) {
         const __nv_bfloat16* tail = (side ? p.tail_value : p.tail_key) + u.info.slot * p.tail_slot + u.head * kHeadDim;
         const __nv_bfloat16* draft = side ? p.draft_value + u.row * p.draft_value_row + u.head * kHeadDim
                                           : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
         const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
+#pragma unroll 1
         for (int first = 0; first < places; first += kBf16Rows) {
           wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
           if (SIDE == 0) {
@@ -445,6 +459,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
             const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
             if (lane == 0) tc::mbar_expect_tx(&full[slot], (end - first - absent) * 256);
             __syncwarp();
+#pragma unroll 1
             for (int i = first + lane; i < end; i += 32) {
               const __nv_bfloat16* source = nullptr;
               if (kind == kStepTail) source = tail + i * tail_row;
@@ -461,6 +476,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
   }
   // After an abort nobody else waits for the copies still in flight: no CTA may end under them.
   if (lane == 0 && *static_cast<volatile int*>(&sm.abort_flag)) {
+#pragma unroll 1
     for (int back = min(issued, Sh::kStages); back > 0; --back) {
       const int at = issued - back;
       wait(&full[at % Sh::kStages], (at / Sh::kStages) & 1, &sm.ignored_flag);
@@ -484,6 +500,7 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm) {
   uint32_t turn = 0, bf16_turn = 0;  // bf16_turn: one bit per half of the values' threads
   Units<NT> units(sm);
   Unit u;
+#pragma unroll 1
   while (units.next(u)) {
     wait(&sm.q_full, unit & 1, &sm.abort_flag);
     tc::fence_after_sync();
@@ -492,11 +509,13 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm) {
       for (int i = 0; i < 2 * kTerms; ++i) tc::cp_sf_atom(tmem + Sh::kQs + i * 4, q_scales + i * 32);
     }
     __syncwarp();
+#pragma unroll 1
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const int within = (step - u.begin) & 1, set = block & 1;
-      const uint32_t scores = tmem + Sh::kS + (2 * set + within) * NT;
-      if (within == 0) wait(&sm.s_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
+      const int within = (step - u.begin) & 1, stream = block & 1, set = (block >> 1) & 1;
+      const uint32_t scores = tmem + Sh::kS + (4 * stream + 2 * set + within) * NT;
+      uint64_t* full = &sm.s_full[stream][set][within];
+      if (within == 0) wait(&sm.s_empty[stream][set], ((block >> 2) & 1) ^ 1, &sm.abort_flag);
       if (kind == kStepPage) {
         wait(PT == 64 ? &sm.k_ready[slot] : &sm.full_k[slot], turn, &sm.abort_flag);
         tc::fence_after_sync();
@@ -513,12 +532,13 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm) {
               tc::mma_nvf4(scores, codes + 2 * s, q_codes + term * NT * 4 + 2 * s, kFp4, scales + 4 * s,
                            tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
           }
-          tc::commit(&sm.s_full[set][within]);
+          tc::commit(full);
           tc::commit(&sm.empty[slot]);
         }
         __syncwarp();
         if (++slot == Sh::kStages) slot = 0, turn ^= 1;
       } else {
+#pragma unroll 1
         for (int i = 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows); i > 0; --i) {
           wait(&sm.full_k[slot], turn, &sm.abort_flag);  // the stage is not this product's
           if (elect_one()) tc::mbar_arrive(&sm.empty[slot]);
@@ -532,13 +552,13 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm) {
 #pragma unroll
           for (int s = 0; s < 8; ++s)
             mma_ts(scores, tmem + Sh::kV + (n & 1) * 64 + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kF16, s > 0);
-          tc::commit(&sm.s_full[set][within]);
+          tc::commit(full);
           tc::commit(&sm.ka_empty[n & 1]);
         }
         __syncwarp();
       }
       if (within == 1 || step + 1 == u.end) {
-        if (within == 0 && elect_one()) tc::mbar_arrive(&sm.s_full[set][1]);  // a block of one step
+        if (within == 0 && elect_one()) tc::mbar_arrive(&sm.s_full[stream][set][1]);  // a block of one step
         __syncwarp();
         ++block;
       }
@@ -556,33 +576,33 @@ __device__ __forceinline__ void issue_output(Smem<NT>& sm) {
   using Sh = Shape<NT>;
   constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-  const uint64_t prob = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
+  // eight tokens' rows are one swizzle atom, a tile is one atom wide
+  const uint64_t prob = tc::smem_desc(tc::smem_u32(sm.p), Sh::kSwizzle, 8 * Sh::kRow, 8 * Sh::kRow);
   int n = 0, block = 0, unit = 0;
   Units<NT> units(sm);
   Unit u;
+#pragma unroll 1
   while (units.next(u)) {
     wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
+#pragma unroll 1
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const int within = (step - u.begin) & 1, set = block & 1;
+      const int within = (step - u.begin) & 1, stream = block & 1, set = (block >> 1) & 1;
       wait(&sm.va_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
-      if (within == 0) wait(&sm.p_full[set], (block >> 1) & 1, &sm.abort_flag);
+      if (within == 0) wait(&sm.p_full[stream][set], (block >> 2) & 1, &sm.abort_flag);
       tc::fence_after_sync();
-      const bool first = step == u.begin, closes = within == 1 || step + 1 == u.end;
-      const uint64_t tile = prob + (2 * set + within) * 1024;
-      const uint32_t operand = tmem + Sh::kV + (n & 1) * 64;
+      const bool first = within == 0 && step - u.begin < 4;  // of its stream in this unit
+      const bool closes = within == 1 || step + 1 == u.end;
+      const uint64_t tile = prob + (4 * stream + 2 * set + within) * (128 * Sh::kRow / 16);
+      const uint32_t operand = tmem + Sh::kV + (n & 1) * 64, output = tmem + Sh::kO + stream * NT;
       if (elect_one()) {
-        if (kind == kStepPage) {
-#pragma unroll 2
-          for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
-            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kPages, !(first && s == 0));
-        } else {
-          const int slices = step_slices(u.info, kind);
-          for (int s = 0; s < slices; ++s)
-            mma_ts(tmem + Sh::kO, operand + s * 8, tile + s * 128, kBf16, !(first && s == 0));
-        }
+        const uint32_t idesc = kind == kStepPage ? kPages : kBf16;
+        const int slices = step_slices(u.info, kind);
+#pragma unroll 1
+        for (int s = 0; s < slices; ++s)  // 16 tokens further: 16 rows of P, 8 columns of V
+          mma_ts(output, operand + s * 8, tile + s * Sh::kRow, idesc, !(first && s == 0));
         tc::commit(&sm.va_empty[n & 1]);
-        if (closes) tc::commit(&sm.p_empty[set]);
+        if (closes) tc::commit(&sm.p_empty[stream][set]);
         if (step + 1 == u.end) tc::commit(&sm.o_full);
       }
       __syncwarp();
@@ -647,7 +667,9 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, int th
   };
   Units<NT> units(sm);
   Unit u;
+#pragma unroll 1
   while (!bar_any(kValuesBarrier + half, 128, !units.next(u))) {
+#pragma unroll 1
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
       if ((n & 1) != half) {
@@ -746,6 +768,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, int th
             }
             st16(operand + quarter * 16, v);
           }
+#pragma unroll 1
           for (int i = 0; i < stages; ++i) {
             if (interleaves && lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);  // its phases follow the stage's uses
             release();
@@ -758,6 +781,7 @@ __device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, int th
           tc::fence_after_sync();
           bf16_turn ^= 1;
         }
+#pragma unroll 1
         for (int first = 0; first < places; first += kBf16Rows) {
           const uint8_t* stage = arrived() + 2 * c;
           const int slices = (min(places - first, kBf16Rows) + 15) / 16;
@@ -808,12 +832,12 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
       if (query < queries && r < NT)
         load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
                          (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v);
-      if (p.rotate) {
+      if (opaque(p.rotate)) {
         hadamard_butterflies(v, group);
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] *= kInvSqrt128;
       }
-      if (phase == 0) {
+      if (opaque(phase) == 0) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
@@ -836,7 +860,14 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm,
           const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
           GroupCodes codes;
           codes.scale = e4m3_to_float(byte);
-          encode16(v, codes.scale, codes.lo, codes.hi);
+          // (an approximate reciprocal: what it rounds otherwise is left to the next term)
+          float inverse_scale;
+          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse_scale) : "f"(fmaxf(codes.scale, 1.0e-30f)));
+          float scaled[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) scaled[j] = v[j] * inverse_scale;
+          codes.lo = pack_e2m1x8(scaled);
+          codes.hi = pack_e2m1x8(scaled + 8);
           *reinterpret_cast<uint2*>(sm.q_codes[term] + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
           sm.q_scales[term][scale_tile_offset(r, group)] = (uint8_t)byte;
           float rest[16];
@@ -886,88 +917,188 @@ __device__ __forceinline__ void reduce_columns(float* v, int lane, int column, S
 template <int NT>
 __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, int thread) {
   using Sh = Shape<NT>;
-  constexpr int C = Sh::kColumns;
-  const int t = thread & 127, lane = thread & 31, warp = thread >> 5, half = thread >> 7;
-  const int first_column = Sh::kByStep ? 0 : half * C;
+  const int t = thread & 127, lane = thread & 31, warp = t >> 5, stream = thread >> 7;
   const uint32_t lanes = (uint32_t)(t & ~31) << 16;
-  const float* base = sm.base + first_column;
-  // the warps that hold the columns of query `thread`
-  const int column_warps = Sh::kByStep ? 8 : 4, column_warp0 = Sh::kByStep ? 0 : (thread & (NT - 1)) / C * 4;
-  int n = 0, block = 0, unit = 0;
+  const float* base = sm.base[stream];
+  const int barrier = kStreamBarrier + stream;
+  const uint32_t output = sm.tmem + Sh::kO + stream * NT + lanes;
+  int blocks = 0, unit = 0;  // of the CTA so far
+  int n = 0;
+  float q_inverse = 1.0f;
+  float2 sum[NT / 2];
   Units<NT> units(sm);
-  Unit u;
-  bool more = !softmax_any(!units.next(u));
-  float q_inverse = more ? load_queries<NT>(p, sm, u, thread) : 1.0f;
-  while (more) {
-    if (thread < NT) {
-      sm.top[thread] = kNoMax;
-      sm.extra[thread] = 0.0f;
-      // the draft nodes that this query sees
-      const int query = u.tile * NT + thread;
-      uint64_t seen = 0;
-      for (int node = min(query / p.ratio, u.info.count - 1); node >= 0;) {
-        seen |= 1ull << node;
-        const int parent = sm.parents[node];
-        node = parent < node ? parent : -1;
-      }
-      sm.family[thread] = seen;
-    }
-    float2 sum[C / 2];
+  Unit u, following;
+  bool running = false;
+#pragma unroll 1
+  while (true) {
+    // the next unit's queries go in while this one's last products run: all its scores are done
+    const bool more = !softmax_any(!units.next(following));
+    float next_inverse = 1.0f;
+    if (running) {  // each query's weight in this stream, by warp
+      float v[NT];
 #pragma unroll
-    for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
+      for (int j = 0; j < NT / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
+      reduce_columns<NT, 16>(v, lane, 0, [&](int j, float total) { sm.warp_value[stream][warp][j] = total; });
+    }
+    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
+    if (running) {
+      softmax_sync();
+      const bool whole = u.begin == 0 && u.end == u.info.steps, both = u.end - u.begin > 2;
+      // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
+      const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
+      if (thread < NT) {  // join the streams
+        float total[2], top = fmaxf(sm.top[0][thread], sm.top[1][thread]), sum_of_both = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          total[h] = sm.extra[h][thread];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) total[h] += sm.warp_value[h][w][thread];
+          sm.share[h][thread] = ex2(sm.top[h][thread] - top);
+          sum_of_both += total[h] * sm.share[h][thread];
+        }
+        if (whole) {
+          const float scale = sum_of_both > 0.0f ? p.value_scale / sum_of_both : 0.0f;
+          sm.share[0][thread] *= scale;
+          sm.share[1][thread] *= scale;
+        } else {
+          p.partial_stat[(int64_t)(2 * part) * NT + thread] = top;
+          p.partial_stat[(int64_t)(2 * part + 1) * NT + thread] = sum_of_both;
+        }
+      }
+      softmax_sync();
+      wait(&sm.o_full, unit & 1, &sm.abort_flag);
+      tc::fence_after_sync();
+      const int out_first = stream * Sh::kOut;
+      const int queries = min(u.info.count * p.ratio - u.tile * NT - out_first, Sh::kOut);
+      const int query = u.tile * NT + out_first;
+      int out_node = query / p.ratio, out_head = query % p.ratio;
+      __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
+      float* partial = p.partial + ((int64_t)part * NT + out_first) * kHeadDim + t;
+      const uint32_t first_output = sm.tmem + Sh::kO + ((blocks - (u.end - u.begin + 1) / 2) & 1) * NT + out_first + lanes;
+      const uint32_t second_output = sm.tmem + Sh::kO + ((blocks - (u.end - u.begin + 1) / 2 + 1) & 1) * NT + out_first + lanes;
+      const float* first_share = sm.share[(blocks - (u.end - u.begin + 1) / 2) & 1] + out_first;
+      const float* second_share = sm.share[(blocks - (u.end - u.begin + 1) / 2 + 1) & 1] + out_first;
+#pragma unroll 1
+      for (int j = 0; j < queries; j += 8) {
+        float o[8], o2[8];
+        tc::tmem_ld8(first_output + j, o);
+        tc::tmem_ld8(second_output + j, o2);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[i] *= first_share[j + i];
+          if (both) o[i] = fmaf(o2[i], second_share[j + i], o[i]);  // (a stream without blocks holds anything)
+          if (j + i < queries) {
+            if (whole) out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i]);
+            else partial[(j + i) * kHeadDim] = o[i];
+          }
+          if (++out_head == p.ratio) out_head = 0, ++out_node;
+        }
+      }
+      tc::fence_before_sync();
+      softmax_sync();  // the output has been read; what is kept per query is written anew
+      if (thread == 0) {
+        tc::mbar_arrive(&sm.o_empty);
+        if (!whole && u.begin == 0) {
+          TreeSplit split;
+          split.row = u.row;
+          split.head = u.head;
+          split.tile = u.tile;
+          // this CTA's run ends inside the unit; the runs behind it are as long
+          split.last = blockIdx.x + (u.info.steps - u.end + sm.per_cta - 1) / sm.per_cta;
+          p.splits[blockIdx.x] = split;
+        }
+      }
+      ++unit;
+    }
+    if (!more) break;
+    running = true;
+    u = following;
+    q_inverse = next_inverse;
+
+    if (t < NT) {
+      sm.top[stream][t] = kNoMax;
+      sm.extra[stream][t] = 0.0f;
+      if (stream == 0) {  // the draft nodes that this query sees
+        uint64_t seen = 0;
+#pragma unroll 1
+        for (int node = min((u.tile * NT + t) / p.ratio, u.info.count - 1); node >= 0;) {
+          seen |= 1ull << node;
+          const int parent = sm.parents[node];
+          node = parent < node ? parent : -1;
+        }
+        sm.family[t] = seen;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
     softmax_sync();
     const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
-    for (int block_begin = u.begin; block_begin < u.end; block_begin += 2, ++block) {
-      const int steps = min(2, u.end - block_begin), set = block & 1;
-      // this half's steps of the block
-      const int from = Sh::kByStep ? half : 0, to = Sh::kByStep ? min(half + 1, steps) : steps;
+    const int all_blocks = (u.end - u.begin + 1) / 2;
+#pragma unroll 1
+    for (int k = (stream ^ blocks) & 1; k < all_blocks; k += 2) {
+      const int block = blocks + k, block_begin = u.begin + 2 * k;
+      const int steps = min(2, u.end - block_begin), set = (block >> 1) & 1;
+      const uint32_t parity = (block >> 2) & 1;
       // a block in which every query sees every token, and all of it FP4
       const bool plain = block_begin + steps <= u.info.pages && (block_begin > 0 || u.info.sink == 0);
+      const uint32_t scores0 = sm.tmem + Sh::kS + (4 * stream + 2 * set) * NT + lanes;
       auto scores_ready = [&](int i) {
-        wait(&sm.s_full[set][i], (block >> 1) & 1, &sm.abort_flag);
+        wait(&sm.s_full[stream][set][i], parity, &sm.abort_flag);
         tc::fence_after_sync();
+      };
+      // Where 16 bytes of P go: chunk index XORed as the swizzle does.
+      uint8_t* const p_rows = sm.p[stream][set][0] + t * Sh::kRow;
+      auto p_chunk = [&](int i, int chunk) {
+        return reinterpret_cast<uint4*>(p_rows + i * (128 * Sh::kRow) + ((chunk ^ (NT == 32 ? (t >> 1) & 3 : (t >> 2) & 1)) * 16));
       };
       // Any step: scores in log2 units above the maxima (plus kShift) are f * score + base; a token may be seen by
       // no query or, a draft, by some.
       struct Step {
         StepKind kind;
-        bool dead, masked;
+        int node;             // of this thread's token, if a draft
+        uint32_t all, alive;  // 1: every query sees the token; 1: some may
         float f;
-        uint32_t scores;
       };
       auto open = [&](int i) {
         Step k;
         k.kind = step_kind(u.info, block_begin + i);
-        if (k.kind == kStepPage) k.dead = block_begin + i == 0 && t < u.info.sink;
-        else if (k.kind == kStepTail) k.dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
-        else k.dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-        k.masked = k.kind == kStepDraft && t >= BDFP4_MAX_SINK && !k.dead;
-        k.f = k.kind == kStepPage ? page_factor : p.scale_log2 * q_inverse * sm.key_factor[(n + i) & 7][t];
-        k.scores = sm.tmem + Sh::kS + (2 * set + i) * NT + first_column + lanes;
+        bool dead;
+        if (k.kind == kStepPage) dead = block_begin + i == 0 && t < u.info.sink;
+        else if (k.kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
+        else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
+        const bool draft = k.kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
+        k.node = draft ? t - BDFP4_MAX_SINK : 0;
+        k.all = draft ? 0 : 1;
+        k.alive = dead ? 0 : 1;
+        k.f = k.kind == kStepPage ? page_factor : p.scale_log2 * q_inverse * sm.key_factor[(n + 2 * (block - blocks) + i) & 7][t];
         return k;
       };
-      auto load8 = [&](const Step& k, int j, float* v) {
-        tc::tmem_ld8(k.scores + j, v);
+      auto load8 = [&](const Step& k, int i, int j, float* v) {
+        tc::tmem_ld8(scores0 + i * NT + j, v);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (k.dead || (k.masked && !((sm.family[first_column + j + c] >> (t - BDFP4_MAX_SINK)) & 1))) v[c] = -INFINITY;
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t seen = (uint32_t)(sm.family[j + c] >> k.node) | k.all;
+          if (!(seen & k.alive)) v[c] = -INFINITY;
+        }
       };
-      float s[C];  // a plain block's probabilities, both steps' added
-      bool high, fresh = block_begin == u.begin;
-      // P of this block goes where the one before the last was
-      wait(&sm.p_empty[set], ((block >> 1) & 1) ^ 1, &sm.abort_flag);
+      float s[NT];  // a plain block's probabilities, both steps' added
+      bool high, fresh = k < 2;
+      // P of this block goes where the stream's one before the last was
+      wait(&sm.p_empty[stream][set], parity ^ 1, &sm.abort_flag);
+#pragma unroll 1
       while (true) {
         if (fresh) {  // take the maxima anew; what was summed so far is brought down to them
           float mine = -INFINITY;
 #pragma unroll 1
-          for (int i = from; i < to; ++i) {
+          for (int i = 0; i < steps; ++i) {
             scores_ready(i);
             const Step k = open(i);
 #pragma unroll 1
-            for (int j = 0; j < C; j += 8) {
+            for (int j = 0; j < NT; j += 8) {
               float v[8];
-              load8(k, j, v);
+              load8(k, i, j, v);
 #pragma unroll
               for (int c = 0; c < 8; ++c) {
                 const float m = warp_max(v[c] * k.f);
@@ -975,106 +1106,91 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, int t
               }
             }
           }
-          if (lane < C) sm.col_max[warp][first_column + lane] = mine;
-          softmax_sync();
-          if (thread < NT) {
-            const float before = sm.top[thread];
+          if (lane < NT) sm.warp_value[stream][warp][lane] = mine;
+          bar_sync(barrier, 128);
+          if (t < NT) {
+            const float before = sm.top[stream][t];
             float now = before;
-            for (int w = 0; w < column_warps; ++w) now = fmaxf(now, sm.col_max[column_warp0 + w][thread]);
-            const float factor = ex2(before - now);
-            sm.top[thread] = now;
-            sm.base[thread] = kShift - now;
-            sm.factor[thread] = factor;
-            sm.extra[thread] *= factor;
-          }
-          softmax_sync();
-          if (block_begin > u.begin) {
 #pragma unroll
-            for (int j = 0; j < C / 2; ++j) {
-              sum[j].x *= sm.factor[first_column + 2 * j];
-              sum[j].y *= sm.factor[first_column + 2 * j + 1];
+            for (int w = 0; w < 4; ++w) now = fmaxf(now, sm.warp_value[stream][w][t]);
+            const float factor = ex2(before - now);
+            sm.top[stream][t] = now;
+            sm.base[stream][t] = kShift - now;
+            sm.factor[stream][t] = factor;
+            sm.extra[stream][t] *= factor;
+          }
+          bar_sync(barrier, 128);
+          if (k >= 2) {
+#pragma unroll
+            for (int j = 0; j < NT / 2; ++j) {
+              sum[j].x *= sm.factor[stream][2 * j];
+              sum[j].y *= sm.factor[stream][2 * j + 1];
             }
-            wait(&sm.p_empty[set ^ 1], ((block - 1) >> 1) & 1, &sm.abort_flag);
+            const int last = block - 2;  // the stream's
+            wait(&sm.p_empty[stream][(last >> 1) & 1], (last >> 2) & 1, &sm.abort_flag);
             tc::fence_after_sync();
 #pragma unroll 1
-            for (int j = half * Sh::kOut; j < (half + 1) * Sh::kOut; j += 8) {
+            for (int j = 0; j < NT; j += 8) {
               float o[8];
               uint32_t r[8];
-              const uint32_t at = sm.tmem + Sh::kO + j + lanes;
-              tc::tmem_ld8(at, o);
+              tc::tmem_ld8(output + j, o);
               tc::tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(o[i] * sm.factor[j + i]);
-              st8(at, r);
+              for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(o[i] * sm.factor[stream][j + i]);
+              st8(output + j, r);
             }
             tc::tmem_wait_st();
           }
         }
         high = false;
         if (plain) {
-          if (!Sh::kByStep) {
 #pragma unroll
-            for (int j = 0; j < C; ++j) s[j] = 0.0f;
-          }
+          for (int j = 0; j < NT; ++j) s[j] = 0.0f;
           const float2 f2 = make_float2(page_factor, page_factor);
           __half2 most = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll 1
-          for (int i = from; i < to; ++i) {
+          for (int i = 0; i < steps; ++i) {
             scores_ready(i);
-            const uint32_t scores = sm.tmem + Sh::kS + (2 * set + i) * NT + first_column + lanes;
-            uint8_t* const row = sm.p[set][i] + t * 128;
-            float v[Sh::kByStep ? 1 : 16];
-            if constexpr (Sh::kByStep) {
+            float x[NT];
 #pragma unroll
-              for (int j = 0; j < C; j += 16) tc::tmem_ld16(scores + j, s + j);
-              tc::tmem_wait_ld();
-            }
+            for (int j = 0; j < NT; j += 16) tc::tmem_ld16(scores0 + i * NT + j, x + j);
+            tc::tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < C; j += 16) {
-              float* x = Sh::kByStep ? s + j : v;
-              if constexpr (!Sh::kByStep) {
-                tc::tmem_ld16(scores + j, x);
-                tc::tmem_wait_ld();
-              }
+            for (int j = 0; j < NT; j += 8) {
+              uint32_t w[4];
 #pragma unroll
-              for (int c = 0; c < 16; c += 4) {
-                const float4 b = *reinterpret_cast<const float4*>(base + j + c);
+              for (int c = j; c < j + 8; c += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(base + c);
                 const float2 y0 = __ffma2_rn(make_float2(x[c], x[c + 1]), f2, make_float2(b.x, b.y));
                 const float2 y1 = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), f2, make_float2(b.z, b.w));
                 x[c] = ex2(y0.x), x[c + 1] = ex2(y0.y), x[c + 2] = ex2(y1.x), x[c + 3] = ex2(y1.y);
               }
-              uint32_t w[8];
 #pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                const __half2 pair = __floats2half2_rn(x[2 * c], x[2 * c + 1]);
+              for (int c = 0; c < 4; ++c) {
+                const __half2 pair = __floats2half2_rn(x[j + 2 * c], x[j + 2 * c + 1]);
                 most = __hmax2(most, pair);
                 w[c] = h2(pair);
               }
-              const int chunk = (first_column + j) >> 3;
-              *reinterpret_cast<uint4*>(row + ((chunk ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-              *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (t & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
-              if constexpr (!Sh::kByStep) {
+              *p_chunk(i, j >> 3) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
 #pragma unroll
-                for (int c = 0; c < 16; c += 2) {
-                  const float2 both = __fadd2_rn(make_float2(s[j + c], s[j + c + 1]), make_float2(x[c], x[c + 1]));
-                  s[j + c] = both.x, s[j + c + 1] = both.y;
-                }
-              }
+            for (int c = 0; c < NT; c += 2) {
+              const float2 two = __fadd2_rn(make_float2(s[c], s[c + 1]), make_float2(x[c], x[c + 1]));
+              s[c] = two.x, s[c + 1] = two.y;
             }
           }
           high = __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
         } else {
-          float* const sums = sm.step_sum[set][warp] + first_column;
-          if (from >= to && lane < C) sums[lane] = 0.0f;
+          float* const sums = sm.step_sum[stream][set][warp];
 #pragma unroll 1
-          for (int i = from; i < to; ++i) {
+          for (int i = 0; i < steps; ++i) {
             scores_ready(i);
             const Step k = open(i);
-            uint8_t* const row = sm.p[set][i] + t * 128;
 #pragma unroll 1
-            for (int j = 0; j < C; j += 8) {
+            for (int j = 0; j < NT; j += 8) {
               float v[8];
-              load8(k, j, v);
+              load8(k, i, j, v);
+              const bool page = opaque(k.kind) == kStepPage;
               uint32_t w[4];
 #pragma unroll
               for (int c = 0; c < 8; ++c) {
@@ -1083,12 +1199,12 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, int t
               }
 #pragma unroll
               for (int c = 0; c < 4; ++c)
-                w[c] = k.kind == kStepPage ? h2(__floats2half2_rn(v[2 * c], v[2 * c + 1]))
-                                           : pack_bf16x2(v[2 * c] * p.inverse_value_scale, v[2 * c + 1] * p.inverse_value_scale);
-              *reinterpret_cast<uint4*>(row + ((((first_column + j) >> 3) ^ (t & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+                w[c] = page ? h2(__floats2half2_rn(v[2 * c], v[2 * c + 1]))
+                            : pack_bf16x2(v[2 * c] * p.inverse_value_scale, v[2 * c + 1] * p.inverse_value_scale);
+              *p_chunk(i, j >> 3) = make_uint4(w[0], w[1], w[2], w[3]);
               // four lanes end up with each column's sum
               reduce_columns<8, 16>(v, lane, j, [&](int column, float total) {
-                if ((lane & 3) == 0) sums[column] = i > from ? sums[column] + total : total;
+                if ((lane & 3) == 0) sums[column] = opaque(i) > 0 ? sums[column] + total : total;
               });
             }
           }
@@ -1096,93 +1212,26 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, int t
         tc::fence_before_sync();
         tc::fence_proxy_async_smem();
         // against maxima just taken nothing is high: the vote then only ends the block
-        if (!softmax_any(high) || fresh) break;
+        if (!bar_any(barrier, 128, high) || fresh) break;
         fresh = true;
       }
       // the barrier stands behind every thread's scores read and probabilities written
-      if (thread == 0) {
-        tc::mbar_arrive(&sm.p_full[set]);
-        tc::mbar_arrive(&sm.s_empty[set]);
+      if (t == 0) {
+        tc::mbar_arrive(&sm.p_full[stream][set]);
+        tc::mbar_arrive(&sm.s_empty[stream][set]);
       }
       if (plain) {
-        if (from < to) {
 #pragma unroll
-          for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
-        }
-      } else if (thread < NT) {
-        float total = sm.extra[thread];
-        for (int w = 0; w < column_warps; ++w) total += sm.step_sum[set][column_warp0 + w][thread];
-        sm.extra[thread] = total;
-      }
-      n += steps;
-    }
-
-    {  // each query's weight: first over a warp's 32 tokens, then (below) over the warps
-      float v[C];
+        for (int j = 0; j < NT / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
+      } else if (t < NT) {
+        float total = sm.extra[stream][t];
 #pragma unroll
-      for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
-      reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col_sum[warp][first_column + j] = total; });
-    }
-    Unit following;
-    // (the barrier also stands behind the column sums, and frees the parents)
-    more = !softmax_any(!units.next(following));
-    float next_inverse = 1.0f;
-    const bool whole = u.begin == 0 && u.end == u.info.steps;
-    // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
-    const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
-    if (thread < NT) {
-      float total = sm.extra[thread];
-      for (int w = 0; w < column_warps; ++w) total += sm.col_sum[column_warp0 + w][thread];
-      if (whole) {
-        sm.total[thread] = total > 0.0f ? p.value_scale / total : 0.0f;
-      } else {
-        p.partial_stat[(int64_t)(2 * part) * NT + thread] = sm.top[thread];
-        p.partial_stat[(int64_t)(2 * part + 1) * NT + thread] = total;
+        for (int w = 0; w < 4; ++w) total += sm.step_sum[stream][set][w][t];
+        sm.extra[stream][t] = total;
       }
     }
-    // the next unit's queries go in while this one's last product runs: all its scores are done
-    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
-    softmax_sync();
-    wait(&sm.o_full, unit & 1, &sm.abort_flag);
-    tc::fence_after_sync();
-    const int out_first = half * Sh::kOut;
-    const int queries = min(u.info.count * p.ratio - u.tile * NT - out_first, Sh::kOut);
-    const int query = u.tile * NT + out_first;
-    int out_node = query / p.ratio, out_head = query % p.ratio;
-    __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
-    float* partial = p.partial + ((int64_t)part * NT + out_first) * kHeadDim + t;
-#pragma unroll 1
-    for (int j = 0; j < Sh::kOut; j += 8) {
-      float o[8];
-      tc::tmem_ld8(sm.tmem + Sh::kO + out_first + j + lanes, o);
-      tc::tmem_wait_ld();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (j + i < queries) {
-          if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[out_first + j + i]);
-            if (++out_head == p.ratio) out_head = 0, ++out_node;
-          } else {
-            partial[(int64_t)(j + i) * kHeadDim] = o[i];
-          }
-        }
-      }
-    }
-    tc::fence_before_sync();
-    softmax_sync();  // the output has been read; what is kept per query is written anew
-    if (thread == 0) tc::mbar_arrive(&sm.o_empty);
-    if (!whole && u.begin == 0 && thread == 0) {
-      TreeSplit split;
-      split.row = u.row;
-      split.head = u.head;
-      split.tile = u.tile;
-      // the unit's last step, counted over the whole launch, names the CTA it ends in
-      split.last = (int)((sm.last + (u.info.steps - u.end) - 1) / sm.per_cta);
-      p.splits[blockIdx.x] = split;
-    }
-    q_inverse = next_inverse;
-    u = following;
-    ++unit;
+    blocks += all_blocks;
+    n += u.end - u.begin;
   }
 }
 
@@ -1197,30 +1246,37 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 
   // all steps of the launch, and where this CTA's run begins
   long long mine = 0;
+#pragma unroll 1
   for (int row = thread; row < p.rows; row += Sh::kThreads) {
     const RowInfo r = row_info(p, row, PT);
     mine += (long long)r.steps * r.tiles * p.heads_kv;
   }
+#pragma unroll 1
   for (int step = 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
   if (lane == 0) sm.sums[warp] = mine;
   if (thread == 0) {
+#pragma unroll 1
     for (int i = 0; i < Sh::kStages; ++i) {
       tc::mbar_init(&sm.full_k[i], 1);
       tc::mbar_init(&sm.full_v[i], 1);
       tc::mbar_init(&sm.empty[i], 5);  // the values' four warps and the score product
       tc::mbar_init(&sm.k_ready[i], 1);
     }
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sm.ka_full[i], 4);
       tc::mbar_init(&sm.ka_empty[i], 1);
       tc::mbar_init(&sm.va_full[i], 4);
       tc::mbar_init(&sm.va_empty[i], 1);
-      tc::mbar_init(&sm.s_full[i][0], 1);
-      tc::mbar_init(&sm.s_full[i][1], 1);
-      tc::mbar_init(&sm.s_empty[i], 1);
-      tc::mbar_init(&sm.p_full[i], 1);
-      tc::mbar_init(&sm.p_empty[i], 1);
+      for (int set = 0; set < 2; ++set) {
+        tc::mbar_init(&sm.s_full[i][set][0], 1);
+        tc::mbar_init(&sm.s_full[i][set][1], 1);
+        tc::mbar_init(&sm.s_empty[i][set], 1);
+        tc::mbar_init(&sm.p_full[i][set], 1);
+        tc::mbar_init(&sm.p_empty[i][set], 1);
+      }
     }
+#pragma unroll 1
     for (int i = 0; i < kUnits; ++i) {
       tc::mbar_init(&sm.unit_full[i], 1);
       tc::mbar_init(&sm.unit_empty[i], kUnitReaders);
@@ -1239,15 +1295,17 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   __syncthreads();
   if (warp == 0) {
     long long all = 0;
+#pragma unroll 1
     for (int w = 0; w < Sh::kThreads / 32; ++w) all += sm.sums[w];
     const long long per = max((all + gridDim.x - 1) / gridDim.x, 1ll);
     const long long first = per * blockIdx.x, last = min(first + per, all);
     if (lane == 0) {
-      sm.per_cta = per;
+      sm.per_cta = (int)min(per, (long long)INT32_MAX / 2);  // a unit that straddles is shorter
       sm.first = first;
       sm.last = last;
     }
     long long before = 0;
+#pragma unroll 1
     for (int row0 = 0; row0 < p.rows && first < last; row0 += 32) {
       long long steps = 0;
       if (row0 + lane < p.rows) {
@@ -1255,6 +1313,7 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         steps = (long long)r.steps * r.tiles * p.heads_kv;
       }
       long long upto = steps;
+#pragma unroll 1
       for (int step = 1; step < 32; step <<= 1) {
         const long long left = __shfl_up_sync(0xffffffffu, upto, step);
         if (lane >= step) upto += left;
@@ -1316,8 +1375,7 @@ template <int PT>
 static cudaError_t launch_tile(const CUtensorMap& k_map, const CUtensorMap& v_map, const TreeParams& p, cudaStream_t stream) {
   switch (p.tile) {
     case 16: return launch<16, PT>(k_map, v_map, p, stream);
-    case 32: return launch<32, PT>(k_map, v_map, p, stream);
-    default: return launch<64, PT>(k_map, v_map, p, stream);
+    default: return launch<32, PT>(k_map, v_map, p, stream);
   }
 }
 
