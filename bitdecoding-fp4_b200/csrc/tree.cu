@@ -15,7 +15,9 @@ namespace bdfp4 {
 static int tree_tile(int queries) {
   const int tiles = (queries + kTreeMaxTile - 1) / kTreeMaxTile;
   const int each = (queries + tiles - 1) / tiles;
-  return each <= 16 ? 16 : kTreeMaxTile;
+  for (int tile : {16, 32})
+    if (each <= tile) return tile;
+  return kTreeMaxTile;
 }
 
 // One block per (CTA that a straddling unit begins in, eight query rows): thread c adds channel c of the

@@ -4,31 +4,28 @@
 // tokens at a time,
 //     S^T [token, query]   = K   [token, channel]  * Q^T
 //     O^T [channel, query] = V^T [channel, token] * P^T
+// both as tcgen05.mma.kind::f16 with the cache operand A in tensor memory and the query-side operand B in
+// shared memory. E2M1 x E4M3 has at most six significant bits and lies in [2^-10, 2688], so a page's values
+// are exact in FP16: a thread reads its own token's (K) or channel's (V) code bytes, converts and scales
+// them in registers and stores them straight into its tensor-memory lane; the dequantized tile never passes
+// through shared memory. P is stored as the softmax threads hold it, one token per thread with its queries
+// contiguous, which is the MN-major form of B.
 //
-// S^T over a page is the block-scaled FP4 product of the codes as they lie in the cache (kind::mxf4nvf4, no
-// dequantization) with the query written as a sum of four FP4 terms, each the rounding of what the ones
-// before left: a term leaves at most 0.177 of its group's largest value (half a step of 2/6, the E4M3
-// scale's rounding included), four leave 10^-3, less than the BF16 rounding the query came with. Four terms
-// of K = 64 take the tensor time of one FP16 product.
+// Two CTAs share an SM, and within a CTA the same eight warps convert K, convert V and take the softmax, one
+// after the other; only the copies and the products have warps of their own. What one CTA waits for (a product,
+// a barrier, tensor memory) the other fills. Warps of one role each (keys, values, softmax, side by side on
+// every scheduler) were built first: they waited for instructions a third of the time, since the sum of their
+// loops is larger than a scheduler's instruction cache.
 //
-// O^T over a page is a kind::f16 product with V^T in tensor memory: E2M1 x E4M3 has at most six significant
-// bits and lies in [2^-10, 2688], so a page's values are exact in FP16. A thread reads its own channel's 64
-// code bytes, converts and scales them in registers and stores them straight into its tensor-memory lane; the
-// dequantized tile never passes through shared memory. P is stored as the softmax threads hold it, one token
-// per thread with its queries contiguous, which is the MN-major form of operand B.
+// Thread r (of 128, twice: each half has half of the channels, tokens or queries) owns token r of S^T. Maxima
+// are per query, in shared memory, and lazy: probabilities are formed against them at once, and only when one
+// comes out more than 2^8 above its maximum (the barrier that ends a step carries that vote) are the maxima
+// taken anew, O^T rescaled and the step formed again. Sums stay per thread until the unit ends. Probabilities
+// carry a factor 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
 //
-// Softmax thread t owns token t of S^T. Maxima are per query, in shared memory, and lazy: after a unit's first
-// block (of two steps) probabilities are formed against them at once, and only when one comes out more than
-// 2^8 above its maximum (the barrier that ends a block carries that vote) are the maxima taken anew, O^T
-// rescaled and the block formed again. Sums stay per thread until the unit ends. Probabilities carry a factor
-// 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
-//
-// What bounds it: five roles run side by side on every scheduler, and the sum of their code is larger than its
-// instruction cache. Code that runs once per unit is kept in rolled loops, and the common path short.
-//
-// The rolling tail and the drafts with the sink are two more steps over BF16 values, both products kind::f16
-// with the cache side in tensor memory: K is scaled per token by a power of two into FP16's range (the softmax
-// thread of the token undoes it), V and P are BF16. Queries are scaled per tile the same way.
+// The rolling tail and the drafts with the sink are two more steps of the same form over BF16 values: K is
+// scaled per token by a power of two into FP16's range (the softmax thread of the token undoes it), V and
+// P are BF16. Queries are scaled per tile the same way.
 //
 // Work is the sequence of all steps of all (row, head, tile) units, cut into equal runs, one per CTA, so any
 // mix of lengths is balanced; a unit that straddles CTAs leaves unnormalised parts that a second kernel adds.
@@ -50,91 +47,45 @@ constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
 // A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
 // 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
 constexpr int kBf16Pitch = 272, kBf16Rows = 64;
-// Named barriers: the softmax threads, each stream of them, each half of the values' threads.
-constexpr int kSoftmaxBarrier = 1, kStreamBarrier = 2, kValuesBarrier = 4;
-constexpr int kTerms = 4;             // FP4 terms of a query
+// Named barriers: one per half, and all eight working warps.
+constexpr int kHalfBarrier = 1, kWorkBarrier = 3;
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
 constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renewed when one exceeds this, 2^8 above
 
-// A unit's blocks of two steps go alternately to two streams, each a softmax of its own (maxima, sums, output)
-// in a warpgroup of its own, joined when the unit ends: one stream's block is a chain of latencies (scores out
-// of tensor memory, exponentials, stores, fences, a barrier) that the other fills. The values' two warpgroups
-// take even and odd steps. Tiles of 64 queries were built too and lost: their sums and scores leave no registers
-// for a second stream, and a step cost 2000 cycles against 2 x 600.
+constexpr int kWorkers = 256;              // two halves of 128
+constexpr int kThreads = kWorkers + 64;    // and a warp each for copies and products
+constexpr int kStages = 4;                 // as many as two CTAs' shared memory holds
+constexpr int kTmemColumns = 256;          // half of what an SM has
+
 template <int NT>
 struct Shape {
-  static constexpr int kOut = NT / 2;  // queries whose output a warpgroup writes
-  static constexpr int kStages = 7;
-  static constexpr int kThreads = 256 + 256 + 128;  // values, softmax, control
-  // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
-  // must not exceed what the launch was given.
-  static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 136, kValueRegs = 72, kControlRegs = 64;
-  static_assert(2 * kSoftmaxRegs + 2 * kValueRegs + kControlRegs <= 5 * kLaunchRegs, "registers");
-  static_assert(kLaunchRegs * kThreads <= 65536, "registers");
-  static constexpr int kRow = NT * 2;  // bytes of a token's probabilities: the swizzle span of P
-  static constexpr uint64_t kSwizzle = NT == 32 ? tc::kSwizzle64B : tc::kSwizzle32B;
-  // tensor memory columns: scores [stream][set][step], output [stream], values (two steps; a BF16 step's keys
-  // before its values), scales of the keys (two steps) and of the query terms
-  static constexpr int kS = 0, kO = 8 * NT, kV = 10 * NT, kKs = kV + 128, kQs = kKs + 16;
-  static_assert(kQs + 8 * kTerms <= 512, "tensor memory");
+  static constexpr int kColumns = NT / 2;  // queries per thread
+  // tensor memory columns
+  static constexpr int kS = 0, kO = NT, kK = 2 * NT, kV = kK + 64;
+  static_assert(kV + 64 <= kTmemColumns, "tensor memory");
 };
-
-template <int FROM, int TO>
-__device__ __forceinline__ void trade_registers() {
-  if constexpr (TO > FROM) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TO));
-  if constexpr (TO < FROM) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
-}
-
-// A value the compiler may not reason about: in a rolled loop a condition on it is not hoisted out (which would
-// make one copy of the loop per outcome).
-__device__ __forceinline__ int opaque(int x) {
-  asm volatile("" : "+r"(x));
-  return x;
-}
-
-struct RowInfo {
-  int count, pages, residual, sink, slot;  // pages: 128-token steps in the FP4 cache
-  int steps;                               // of one unit: pages, tail, drafts with sink
-  int tiles;
-};
-
-// A run of steps of one (row, head, tile).
-struct Unit {
-  RowInfo info;
-  int row, head, tile, begin, end;  // steps [begin, end) are this CTA's; begin < 0: no more units
-};
-constexpr int kUnits = 4;  // of the ring through which the key producer hands them to the other roles
-constexpr int kUnitReaders = 8 + 8 + 3;  // warps: values, softmax, value producer, score issuer, output issuer
 
 template <int NT>
 struct Smem {
   using Sh = Shape<NT>;
-  alignas(1024) uint8_t ring[Sh::kStages][kStage];
-  alignas(1024) uint8_t q[2][NT * 128];          // FP16: two halves of 64 channels, K-major, 128-byte swizzle
-  alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
-  alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
-  alignas(1024) uint8_t p[2][2][2][128 * Sh::kRow];  // [stream][set][step] MN-major: a row of queries per token, swizzled
+  alignas(1024) uint8_t ring[kStages][kStage];
+  alignas(1024) uint8_t q[2][NT * 128];  // two halves of 64 channels, K-major, 128-byte swizzle
+  alignas(1024) uint8_t p[16384];        // MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
-  // by stream: kShift - maximum; maximum, log2 units; what a renewal scales by; weights of not plain blocks
-  float base[2][NT], top[2][NT], factor[2][NT], extra[2][NT];
-  float share[2][NT];   // what a stream's output is multiplied by
-  float warp_value[2][4][NT];   // a block's maxima, a unit's sums, by warp
-  float step_sum[2][2][4][NT];  // [stream][set] a not plain block's weights, by warp
-  float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
+  float base[NT];       // kShift - maximum
+  float top[NT];        // maximum, log2 units
+  float factor[NT];
+  float total[NT];
+  float col_max[4][NT];
+  float col_sum[4][NT];
   float q_max[8];
   int parents[BDFP4_MAX_TREE_NODES];
-  Unit units[kUnits];
-  uint64_t unit_full[kUnits], unit_empty[kUnits];
-  uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
-  uint64_t k_ready[Sh::kStages];  // 64-token pages: the stage's key scales are whole atoms
-  uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];  // by step
-  uint64_t s_full[2][2][2], s_empty[2][2], p_full[2][2], p_empty[2][2];  // [stream][set], s_full by step too
-  uint64_t q_full, o_full, o_empty, drained;
-  long long sums[Sh::kThreads / 32];
+  uint64_t full[kStages], empty[kStages];
+  uint64_t k_full, s_full, p_full, o_full, drained;
+  long long sums[kThreads / 32];
   int start_row;
-  long long start_offset, first, last;
-  int per_cta;
+  long long start_offset, first, last, per_cta;
   uint32_t tmem;
   int abort_flag, ignored_flag;
 };
@@ -155,18 +106,15 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-__device__ __forceinline__ void softmax_sync() { bar_sync(kSoftmaxBarrier, 256); }
-
-__device__ __forceinline__ bool bar_any(int id, int threads, bool pred) {
+__device__ __forceinline__ bool bar_any(int id, bool pred) {
   uint32_t out;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(out)
-      : "r"((uint32_t)pred), "r"(id), "r"(threads)
+      : "r"((uint32_t)pred), "r"(id)
       : "memory");
   return out != 0;
 }
-__device__ __forceinline__ bool softmax_any(bool pred) { return bar_any(kSoftmaxBarrier, 256, pred); }
 
 // kind::f16 with A in tensor memory (lane = row, a 32-bit column = two neighbouring K values).
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
@@ -198,6 +146,13 @@ __device__ __forceinline__ void st8(uint32_t address, const uint32_t* v) {
                : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t address, float* v) {
+  if constexpr (N == 8) tc::tmem_ld8(address, v);
+#pragma unroll
+  for (int j = 0; j + 16 <= N; j += 16) tc::tmem_ld16(address + j, v + j);
+}
+
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
 // Eight E2M1 codes times one FP16 scale -> eight FP16 values in four words, in code order. Exact.
@@ -220,18 +175,23 @@ __device__ __forceinline__ void scale_pairs(uint32_t bytes, __half2* out) {
   out[1] = __high2half2(pair);
 }
 
-// The power of two that brings `amax` into [2^10, 2^11), where FP16 has 25 binades below and the FP4 terms'
-// E4M3 scales (up to 448 = 2688 / 6) reach their fourth, and its inverse. Zero, infinite or NaN: 1.
+// The power of two that brings `amax` into [2^14, 2^15), and its inverse. Zero, infinite or NaN: 1.
 __device__ __forceinline__ float fp16_scale(float amax, float* inverse) {
   const int e = (int)((__float_as_uint(amax) >> 23) & 0xffu);
   if (e == 0 || e == 255) {
     *inverse = 1.0f;
     return 1.0f;
   }
-  const int field = min(127 + 10 + 127 - e, 253);
+  const int field = min(127 + 14 + 127 - e, 253);
   *inverse = __uint_as_float((uint32_t)(254 - field) << 23);
   return __uint_as_float((uint32_t)field << 23);
 }
+
+struct RowInfo {
+  int count, pages, residual, sink, slot;  // pages: 128-token steps in the FP4 cache
+  int steps;                               // of one unit: pages, tail, drafts with sink
+  int tiles;
+};
 
 __device__ __forceinline__ RowInfo row_info(const TreeParams& p, int row, int page_tokens) {
   RowInfo r;
@@ -253,6 +213,11 @@ __device__ __forceinline__ RowInfo row_info(const TreeParams& p, int row, int pa
   return r;
 }
 
+struct Unit {
+  RowInfo info;
+  int row, head, tile, begin, end;  // steps [begin, end) of the unit are this CTA's
+};
+
 enum StepKind { kStepPage, kStepTail, kStepDraft };
 
 __device__ __forceinline__ StepKind step_kind(const RowInfo& r, int step) {
@@ -267,7 +232,8 @@ __device__ __forceinline__ int step_slices(const RowInfo& r, StepKind kind) {
   return kind == kStepPage ? 8 : (bf16_places(r, kind) + 15) / 16;
 }
 
-// The units of this CTA in order. Steps are counted in 32 bits within a row (the host refuses larger rows).
+// The units of this CTA in order; every role walks them on its own. Steps are counted in 32 bits within a
+// row (the host refuses larger rows).
 struct Walker {
   const TreeParams& p;
   int row, page_tokens, offset, left;
@@ -276,7 +242,6 @@ struct Walker {
   // `known`: u is a unit of this walk, so its row's lengths need not be read again.
   __device__ __forceinline__ bool next(Unit& u, bool known) {
     if (left <= 0) return false;
-#pragma unroll 1
     while (true) {
       if (!known || u.row != row) u.info = row_info(p, row, page_tokens);
       const int whole = u.info.steps * u.info.tiles * p.heads_kv;
@@ -299,8 +264,7 @@ struct Walker {
 
 // ---- roles -----------------------------------------------------------------------------------------
 
-// The roles' loops run side by side on every scheduler and share its instruction cache, so waiting is a dozen
-// instructions, one when the phase is already over. After about two seconds, or once another thread has given
+// Waiting is a dozen instructions, one when the phase is already over. After about two seconds, or once another thread has given
 // up, a wait ends without its phase; the roles go through the rest of their motions and the kernel reports it.
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
   asm volatile(
@@ -324,82 +288,35 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* abort_
       : "memory");
 }
 
-// One thread of a converged warp. tcgen05.mma and the bulk copies take their operands from uniform registers:
-// behind an elected predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32
-// (N = 64) to 64 cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its
-// size, and the copies of a step were longer than its HBM time.
+// One thread of a converged warp. tcgen05.mma takes its descriptors from uniform registers: behind an elected
+// predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32 (N = 64) to 64
+// cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its size.
 __device__ __forceinline__ bool elect_one() {
   uint32_t elected;
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(elected));
   return elected != 0;
 }
 
-// A role's view of the ring of units.
-template <int NT>
-struct Units {
-  Smem<NT>& sm;
-  int next_unit;
-  __device__ explicit Units(Smem<NT>& s) : sm(s), next_unit(0) {}
-  // The whole warp: the next unit into `u`; false when there is none, or when a wait has been given up (then `u`
-  // may hold anything). Roles whose warps meet at barriers have to agree on the answer.
-  __device__ __forceinline__ bool next(Unit& u) {
-    const int at = next_unit % kUnits;
-    wait(&sm.unit_full[at], (next_unit / kUnits) & 1, &sm.abort_flag);
-    u = sm.units[at];
-    ++next_unit;
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&sm.unit_empty[at]);
-    return __all_sync(0xffffffffu, u.begin >= 0 && *static_cast<volatile int*>(&sm.abort_flag) == 0);
+// A place in the ring of stages; everyone who keeps one visits every stage in order.
+struct Place {
+  int slot = 0;
+  uint32_t turn = 0;
+  __device__ __forceinline__ void advance() {
+    if (++slot == kStages) slot = 0, turn ^= 1;
   }
 };
 
-// One side's copies: SIDE 0 brings a page's key codes and scales, SIDE 1 its values' and the rows of the BF16
-// steps. Two warps, because a copy keeps its issuer for 80 cycles and a step of 64-token pages has eight.
-template <int NT, int PT, int SIDE>
-__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const CUtensorMap* map, int lane) {
-  using Sh = Shape<NT>;
+template <int NT, int PT>
+__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* k_map,
+                                        const CUtensorMap* v_map, int lane) {
   constexpr int kEntries = kPage / PT;
   const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
-  const int64_t codes_pitch = p.codes_pitch[SIDE], scales_pitch = p.scales_pitch[SIDE];
-  uint64_t* full = SIDE ? sm.full_v : sm.full_k;
-  int slot = 0, issued = 0;
-  uint32_t turn = 0;
-  auto advance = [&] {
-    ++issued;
-    if (++slot == Sh::kStages) slot = 0, turn ^= 1;
-  };
-  // the key producer walks the units and publishes each before the one in front of it is produced
-  Units<NT> units(sm);
-  Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
-  Unit u, following;
-  bool known = false, more = true;
-  int published = 0;
-  auto publish = [&] {
-    more = more && walker.next(following, known);
-    known = true;
-    wait(&sm.unit_empty[published % kUnits], ((published / kUnits) & 1) ^ 1, &sm.abort_flag);
-    if (lane == 0) {
-      if (!more) following.begin = -1;
-      sm.units[published % kUnits] = following;
-      tc::mbar_arrive(&sm.unit_full[published % kUnits]);
-    }
-    __syncwarp();
-    ++published;
-  };
-  if (SIDE == 0) publish();
+  Place at;
+  Unit u;
+  bool known = false;
 #pragma unroll 1
-  while (true) {
-    if (SIDE == 0) {
-      if (!more) break;
-      u = following;
-      publish();
-    } else if (!units.next(u)) {
-      break;
-    }
+  for (; walker.next(u, known); known = true) {
     const int32_t* table = p.table + u.row * p.table_stride;
-    const uint8_t* codes = p.codes[SIDE] + u.head * (PT == 128 ? 8192 : 4096);
-    const uint8_t* scales = p.scales[SIDE] + u.head * (PT == 128 ? 1024 : 512);
-    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&sm.abort_flag) != 0)) break;
     const int stop = min(u.end, u.info.pages);
 #pragma unroll 1
     for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
@@ -418,24 +335,28 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
         int page[kEntries];
 #pragma unroll
         for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
-        wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
+        wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
+        uint64_t* const full = &sm.full[at.slot];
         if (elect_one()) {
-          uint8_t* stage = sm.ring[slot];
-          tc::mbar_expect_tx(&full[slot], 9216);
+          uint8_t* stage = sm.ring[at.slot];
+          tc::mbar_expect_tx(full, 18432);
           if constexpr (PT == 128) {
-            if constexpr (SIDE == 0) tc::tma_load_4d(stage, map, &full[slot], 0, u.head, 0, page[0]);
-            else tc::tma_load_3d(stage + kVOffset, map, &full[slot], 0, u.head * kHeadDim, page[0]);
-            tc::bulk_load(stage + (SIDE ? kVsOffset : kKsOffset), scales + page[0] * scales_pitch, 1024, &full[slot]);
+            tc::tma_load_4d(stage, k_map, full, 0, u.head, 0, page[0]);
+            tc::bulk_load(stage + kKsOffset, p.scales[0] + page[0] * p.scales_pitch[0] + u.head * 1024, 1024, full);
+            tc::tma_load_3d(stage + kVOffset, v_map, full, 0, u.head * kHeadDim, page[0]);
+            tc::bulk_load(stage + kVsOffset, p.scales[1] + page[0] * p.scales_pitch[1] + u.head * 1024, 1024, full);
           } else {
 #pragma unroll
             for (int e = 0; e < kEntries; ++e) {
-              tc::bulk_load(stage + (SIDE ? kVOffset : 0) + e * 4096, codes + page[e] * codes_pitch, 4096, &full[slot]);
-              tc::bulk_load(stage + (SIDE ? kVsOffset : kKsOffset) + e * 512, scales + page[e] * scales_pitch, 512, &full[slot]);
+              tc::bulk_load(stage + e * 4096, p.codes[0] + page[e] * p.codes_pitch[0] + u.head * 4096, 4096, full);
+              tc::bulk_load(stage + kKsOffset + e * 512, p.scales[0] + page[e] * p.scales_pitch[0] + u.head * 512, 512, full);
+              tc::bulk_load(stage + kVOffset + e * 4096, p.codes[1] + page[e] * p.codes_pitch[1] + u.head * 4096, 4096, full);
+              tc::bulk_load(stage + kVsOffset + e * 512, p.scales[1] + page[e] * p.scales_pitch[1] + u.head * 512, 512, full);
             }
           }
         }
         __syncwarp();
-        advance();
+        at.advance();
       }
     }
 #pragma unroll 1
@@ -450,120 +371,82 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, const
         const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
 #pragma unroll 1
         for (int first = 0; first < places; first += kBf16Rows) {
-          wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
-          if (SIDE == 0) {
-            if (lane == 0) tc::mbar_arrive(&full[slot]);  // nothing for the FP4 product here
-          } else {
-            const int end = min(first + kBf16Rows, places);
-            // the sink's places behind its length stay empty
-            const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
-            if (lane == 0) tc::mbar_expect_tx(&full[slot], (end - first - absent) * 256);
-            __syncwarp();
+          const int end = min(first + kBf16Rows, places);
+          wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
+          uint64_t* const full = &sm.full[at.slot];
+          // the sink's places behind its length stay empty
+          const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
+          if (elect_one()) tc::mbar_expect_tx(full, (end - first - absent) * 256);
+          __syncwarp();
 #pragma unroll 1
-            for (int i = first + lane; i < end; i += 32) {
-              const __nv_bfloat16* source = nullptr;
-              if (kind == kStepTail) source = tail + i * tail_row;
-              else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
-              else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
-              if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, &full[slot]);
-            }
+          for (int i = first + lane; i < end; i += 32) {
+            const __nv_bfloat16* source = nullptr;
+            if (kind == kStepTail) source = tail + i * tail_row;
+            else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
+            else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
+            if (source) tc::bulk_load(sm.ring[at.slot] + (i - first) * kBf16Pitch, source, 256, full);
           }
           __syncwarp();
-          advance();
+          at.advance();
         }
       }
     }
   }
-  // After an abort nobody else waits for the copies still in flight: no CTA may end under them.
-  if (lane == 0 && *static_cast<volatile int*>(&sm.abort_flag)) {
+  // After an abort nobody else waits for the copies still in flight: no CTA may end under them. (A stage that was
+  // never filled, or whose last use is over, is in a phase whose predecessor has ended.)
+  if (*static_cast<volatile int*>(&sm.abort_flag)) {
 #pragma unroll 1
-    for (int back = min(issued, Sh::kStages); back > 0; --back) {
-      const int at = issued - back;
-      wait(&full[at % Sh::kStages], (at / Sh::kStages) & 1, &sm.ignored_flag);
+    for (int i = 0; i < kStages; ++i) {
+      wait(&sm.full[at.slot], at.turn ^ 1, &sm.ignored_flag);
+      at.advance();
     }
   }
   __syncwarp();
 }
 
-// The products are issued by two warps, one for the scores and one for the output: an MMA keeps its issuer
-// for 40 to 60 cycles, and the sixteen of a step one after another were longer than the step's HBM time. The
-// whole warp walks and waits; one thread of it issues.
-template <int NT, int PT>
-__device__ __forceinline__ void issue_scores(Smem<NT>& sm) {
+// The whole warp walks and waits; one thread of it issues.
+template <int NT>
+__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   using Sh = Shape<NT>;
-  constexpr uint32_t kFp4 = tc::nvf4_idesc(128, NT), kF16 = f16_idesc(NT, 0, false);
+  constexpr uint32_t kScores = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-  const uint32_t q = tc::smem_u32(sm.q), ring = tc::smem_u32(sm.ring);
-  const uint64_t q_codes = tc::fp4_tile_desc(tc::smem_u32(sm.q_codes), 0);
-  const uint64_t q_scales = tc::sf_atom_desc(tc::smem_u32(sm.q_scales));
-  int n = 0, block = 0, unit = 0, slot = 0;
-  uint32_t turn = 0, bf16_turn = 0;  // bf16_turn: one bit per half of the values' threads
-  Units<NT> units(sm);
+  const uint32_t q = tc::smem_u32(sm.q);
+  const uint64_t tile = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
+  uint32_t parity = 0;
   Unit u;
+  bool known = false;
 #pragma unroll 1
-  while (units.next(u)) {
-    wait(&sm.q_full, unit & 1, &sm.abort_flag);
-    tc::fence_after_sync();
-    if (elect_one()) {
+  for (; walker.next(u, known); known = true) {
+#pragma unroll 1
+    for (int step = u.begin; step < u.end; ++step, parity ^= 1) {
+      wait(&sm.k_full, parity, &sm.abort_flag);
+      tc::fence_after_sync();
+      if (elect_one()) {
 #pragma unroll
-      for (int i = 0; i < 2 * kTerms; ++i) tc::cp_sf_atom(tmem + Sh::kQs + i * 4, q_scales + i * 32);
-    }
-    __syncwarp();
-#pragma unroll 1
-    for (int step = u.begin; step < u.end; ++step, ++n) {
+        for (int s = 0; s < 8; ++s)
+          mma_ts(tmem + Sh::kS, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
+        tc::commit(&sm.s_full);
+      }
+      __syncwarp();
+      wait(&sm.p_full, parity, &sm.abort_flag);  // P, and before it V
+      tc::fence_after_sync();
       const StepKind kind = step_kind(u.info, step);
-      const int within = (step - u.begin) & 1, stream = block & 1, set = (block >> 1) & 1;
-      const uint32_t scores = tmem + Sh::kS + (4 * stream + 2 * set + within) * NT;
-      uint64_t* full = &sm.s_full[stream][set][within];
-      if (within == 0) wait(&sm.s_empty[stream][set], ((block >> 2) & 1) ^ 1, &sm.abort_flag);
-      if (kind == kStepPage) {
-        wait(PT == 64 ? &sm.k_ready[slot] : &sm.full_k[slot], turn, &sm.abort_flag);
-        tc::fence_after_sync();
-        const uint32_t stage = ring + slot * kStage;
-        const uint64_t codes = tc::fp4_tile_desc(stage, 0), atoms = tc::sf_atom_desc(stage + kKsOffset);
-        const uint32_t scales = tmem + Sh::kKs + (n & 1) * 8;
-        if (elect_one()) {
-          tc::cp_sf_atom(scales, atoms);
-          tc::cp_sf_atom(scales + 4, atoms + 32);
-#pragma unroll 1
-          for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
+      const bool first = step == u.begin;
+      if (elect_one()) {
+        if (kind == kStepPage) {
 #pragma unroll
-            for (int term = 0; term < kTerms; ++term)
-              tc::mma_nvf4(scores, codes + 2 * s, q_codes + term * NT * 4 + 2 * s, kFp4, scales + 4 * s,
-                           tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
-          }
-          tc::commit(full);
-          tc::commit(&sm.empty[slot]);
-        }
-        __syncwarp();
-        if (++slot == Sh::kStages) slot = 0, turn ^= 1;
-      } else {
+          for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
+            mma_ts(tmem + Sh::kO, tmem + Sh::kV + s * 8, tile + s * 128, kPages, !(first && s == 0));
+        } else {
+          const int slices = step_slices(u.info, kind);
 #pragma unroll 1
-        for (int i = 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows); i > 0; --i) {
-          wait(&sm.full_k[slot], turn, &sm.abort_flag);  // the stage is not this product's
-          if (elect_one()) tc::mbar_arrive(&sm.empty[slot]);
-          __syncwarp();
-          if (++slot == Sh::kStages) slot = 0, turn ^= 1;
+          for (int s = 0; s < slices; ++s)
+            mma_ts(tmem + Sh::kO, tmem + Sh::kV + s * 8, tile + s * 128, kBf16, !(first && s == 0));
         }
-        wait(&sm.ka_full[n & 1], (bf16_turn >> (n & 1)) & 1, &sm.abort_flag);
-        bf16_turn ^= 1u << (n & 1);
-        tc::fence_after_sync();
-        if (elect_one()) {
-#pragma unroll
-          for (int s = 0; s < 8; ++s)
-            mma_ts(scores, tmem + Sh::kV + (n & 1) * 64 + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kF16, s > 0);
-          tc::commit(full);
-          tc::commit(&sm.ka_empty[n & 1]);
-        }
-        __syncwarp();
+        tc::commit(&sm.o_full);
       }
-      if (within == 1 || step + 1 == u.end) {
-        if (within == 0 && elect_one()) tc::mbar_arrive(&sm.s_full[stream][set][1]);  // a block of one step
-        __syncwarp();
-        ++block;
-      }
+      __syncwarp();
     }
-    ++unit;
   }
   // also after an abort: tensor memory is freed behind the last product
   if (elect_one()) tc::commit(&sm.drained);
@@ -571,67 +454,7 @@ __device__ __forceinline__ void issue_scores(Smem<NT>& sm) {
   wait(&sm.drained, 0, &sm.ignored_flag);
 }
 
-template <int NT>
-__device__ __forceinline__ void issue_output(Smem<NT>& sm) {
-  using Sh = Shape<NT>;
-  constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
-  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-  // eight tokens' rows are one swizzle atom, a tile is one atom wide
-  const uint64_t prob = tc::smem_desc(tc::smem_u32(sm.p), Sh::kSwizzle, 8 * Sh::kRow, 8 * Sh::kRow);
-  int n = 0, block = 0, unit = 0;
-  Units<NT> units(sm);
-  Unit u;
-#pragma unroll 1
-  while (units.next(u)) {
-    wait(&sm.o_empty, (unit & 1) ^ 1, &sm.abort_flag);
-#pragma unroll 1
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const StepKind kind = step_kind(u.info, step);
-      const int within = (step - u.begin) & 1, stream = block & 1, set = (block >> 1) & 1;
-      wait(&sm.va_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
-      if (within == 0) wait(&sm.p_full[stream][set], (block >> 2) & 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      const bool first = within == 0 && step - u.begin < 4;  // of its stream in this unit
-      const bool closes = within == 1 || step + 1 == u.end;
-      const uint64_t tile = prob + (4 * stream + 2 * set + within) * (128 * Sh::kRow / 16);
-      const uint32_t operand = tmem + Sh::kV + (n & 1) * 64, output = tmem + Sh::kO + stream * NT;
-      if (elect_one()) {
-        const uint32_t idesc = kind == kStepPage ? kPages : kBf16;
-        const int slices = step_slices(u.info, kind);
-#pragma unroll 1
-        for (int s = 0; s < slices; ++s)  // 16 tokens further: 16 rows of P, 8 columns of V
-          mma_ts(output, operand + s * 8, tile + s * Sh::kRow, idesc, !(first && s == 0));
-        tc::commit(&sm.va_empty[n & 1]);
-        if (closes) tc::commit(&sm.p_empty[stream][set]);
-        if (step + 1 == u.end) tc::commit(&sm.o_full);
-      }
-      __syncwarp();
-      if (closes) ++block;
-    }
-    ++unit;
-  }
-  if (elect_one()) tc::commit(&sm.drained);
-  __syncwarp();
-  wait(&sm.drained, 0, &sm.ignored_flag);
-}
-
-// 64-token pages: the key scales of a step's two pages come as half atoms (32 rows of 8 bytes); one warp
-// interleaves them, in place, into the two whole atoms the MMA reads.
-__device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
-  uint2 part[2][2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[i & 1][i >> 1] = *reinterpret_cast<const uint2*>(scales + (i >> 1) * 512 + (i & 1) * 256 + lane * 8);
-  __syncwarp();
-#pragma unroll
-  for (int atom = 0; atom < 2; ++atom)
-    *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) = make_uint4(part[atom][0].x, part[atom][0].y, part[atom][1].x, part[atom][1].y);
-  tc::fence_proxy_async_smem();
-  __syncwarp();
-}
-
-// Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane. The caller's
-// loop over a channel's four chunks stays rolled: three roles run side by side on every scheduler, and with
-// the 300 instructions of the unrolled form the warps waited for instructions a third of the time.
+// Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane.
 __device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint32_t scales) {
   __half2 scale[2];
   scale_pairs(scales, scale);
@@ -643,252 +466,56 @@ __device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint3
   st16(a, v);
 }
 
-// The values' warps: thread c of a half holds channel c of its steps' V^T, and token c of a BF16 step's K.
-template <int NT, int PT>
-__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, int thread) {
-  const int c = thread & 127, lane = c & 31, half = thread >> 7;
-  using Sh = Shape<NT>;
-  const uint32_t lanes = (uint32_t)(c & ~31) << 16;
-  int slot = 0, n = 0;
-  uint32_t turn = 0, bf16_turn = 0;
-  auto pass = [&](int stages) {  // the other half's
-    slot += stages;
-    if (slot >= Sh::kStages) slot -= Sh::kStages, turn ^= 1;
-  };
-  auto arrived = [&]() -> uint8_t* {
-    wait(&sm.full_v[slot], turn, &sm.abort_flag);
-    return sm.ring[slot];
-  };
-  const bool interleaves = PT == 64 && (c >> 5) == 3;
-  auto release = [&] {
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
-    pass(1);
-  };
-  Units<NT> units(sm);
-  Unit u;
-#pragma unroll 1
-  while (!bar_any(kValuesBarrier + half, 128, !units.next(u))) {
-#pragma unroll 1
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const StepKind kind = step_kind(u.info, step);
-      if ((n & 1) != half) {
-        pass(kind == kStepPage ? 1 : 2 * ((bf16_places(u.info, kind) + kBf16Rows - 1) / kBf16Rows));
-        continue;
-      }
-      const uint32_t operand = sm.tmem + Sh::kV + (n & 1) * 64 + lanes;
-      uint64_t* operand_empty = &sm.va_empty[n & 1];
-      const uint32_t empty_parity = ((n >> 1) & 1) ^ 1;
-      if (kind == kStepPage) {
-        if (interleaves) {
-          wait(&sm.full_k[slot], turn, &sm.abort_flag);
-          interleave_scales(sm.ring[slot] + kKsOffset, lane);
-          if (lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
-        }
-        const uint8_t* stage = arrived();
-        const uint8_t* scales = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
-        wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-#pragma unroll 1
-        for (int j = 0; j < 4; ++j) {
-          const uint8_t* at = PT == 128 ? stage + kVOffset + c * 64 + ((j ^ ((c >> 1) & 3)) * 16)
-                                        : stage + kVOffset + (j >> 1) * 4096 + c * 32 + (((j & 1) ^ ((c >> 2) & 1)) * 16);
-          store_dequantized(operand + 16 * j, *reinterpret_cast<const uint4*>(at),
-                            *reinterpret_cast<const uint16_t*>(scales + (j >> 1) * 512 + (j & 1) * 2));
-        }
-        release();
-      } else {
-        const int places = bf16_places(u.info, kind);
-        const int stages = (places + kBf16Rows - 1) / kBf16Rows;
-        // keys first, through the buffer that takes the values after the score product
-        wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-        {  // a step's stages are held together
-          uint8_t* const stage0 = arrived();
-          uint8_t* stage1 = stage0;
-          if (stages > 1) {
-            const bool wraps = slot + 1 == Sh::kStages;
-            const int next = wraps ? 0 : slot + 1;
-            wait(&sm.full_v[next], turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
-            stage1 = sm.ring[next];
-          }
-          auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
-          bool there = c < places;
-          if (kind == kStepDraft) {
-            if (c < BDFP4_MAX_SINK) there = c < u.info.sink;
-            if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
-              const int group = c & 7;
-              const float* shift = p.key_shift ? p.key_shift + u.head * kHeadDim + group * kGroup : nullptr;
-#pragma unroll 1
-              for (int first = 0; first < u.info.count; first += 16) {
-                // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
-                const int node = min(first + (c >> 3), u.info.count - 1);
-                uint4* at = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + node) + group * 32);
-                const uint4 raw[2] = {at[0], at[1]};
-                const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-                float v[16];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  v[2 * i] = __uint_as_float(w[i] << 16);
-                  v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-                }
-                cache_basis16_any(v, group, p.rotate != 0, shift);
-                if (first + (c >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
-              }
-              tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
-              bar_sync(kValuesBarrier + half, 128);
-            }
-          }
-          const uint4* row = reinterpret_cast<const uint4*>(row_of(min(c, places - 1)));
-          float amax = 0.0f;
-          if (there) {
-#pragma unroll 2
-            for (int j = 0; j < 16; ++j) {
-              const uint4 r = row[j];
-              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-            }
-          }
-          float inverse;
-          const float scale = fp16_scale(amax, &inverse);
-          sm.key_factor[n & 7][c] = inverse;
-#pragma unroll 1
-          for (int quarter = 0; quarter < 4; ++quarter) {
-            uint32_t v[16];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint4 r = make_uint4(0, 0, 0, 0);
-              if (there) r = row[quarter * 4 + j];
-              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
-            }
-            st16(operand + quarter * 16, v);
-          }
-#pragma unroll 1
-          for (int i = 0; i < stages; ++i) {
-            if (interleaves && lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);  // its phases follow the stage's uses
-            release();
-          }
-          tc::tmem_wait_st();
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&sm.ka_full[half]);
-          wait(&sm.ka_empty[half], bf16_turn, &sm.abort_flag);
-          tc::fence_after_sync();
-          bf16_turn ^= 1;
-        }
-#pragma unroll 1
-        for (int first = 0; first < places; first += kBf16Rows) {
-          const uint8_t* stage = arrived() + 2 * c;
-          const int slices = (min(places - first, kBf16Rows) + 15) / 16;
-#pragma unroll 1
-          for (int s = 0; s < slices; ++s) {
-            const int place = first + s * 16;
-            const int stop = kind == kStepDraft && place == 0 ? u.info.sink : places;
-            uint32_t v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint32_t lo = 0, hi = 0;
-              if (place + 2 * i < stop) lo = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i) * kBf16Pitch);
-              if (place + 2 * i + 1 < stop) hi = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i + 1) * kBf16Pitch);
-              v[i] = lo | (hi << 16);
-            }
-            st8(operand + (place >> 4) * 8, v);
-          }
-          if (interleaves && lane == 0) tc::mbar_arrive(&sm.k_ready[slot]);
-          release();
-        }
-      }
-      tc::tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.va_full[n & 1]);
-    }
-  }
-}
-
-// The tile's queries into shared memory: rotated if asked, scaled by one power of two, as FP16 for the BF16 steps
-// and as FP4 terms for the pages. One scale for the tile: a query whose largest value is 2^-8 of the tile's
-// still has all four terms above E4M3's smallest scale. Returns what undoes the scaling.
+// The tile's queries into shared memory: rotated if asked, scaled by one power of two into FP16's range
+// (rows of the tile whose largest value is 2^-29 of the tile's keep full precision). Returns what undoes it.
 template <int NT>
 __device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
-  const int group = thread & 7;  // eight threads hold one query
-  const int queries = u.info.count * p.ratio;
+  constexpr int kPerPass = kWorkers / 8, kPasses = (NT + kPerPass - 1) / kPerPass;
+  const int group = thread & 7;
+  const int queries = min(u.info.count * p.ratio - u.tile * NT, NT);
+  float v[kPasses][16];
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = i * kPerPass + (thread >> 3), query = u.tile * NT + r;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[i][j] = 0.0f;
+    if (r < queries)
+      load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
+                       (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
+  }
   if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
-  float scale = 1.0f, inverse = 1.0f;
-#pragma unroll 1
-  for (int phase = 0; phase < 2; ++phase) {  // the tile's largest value, then the operands
-    float amax = 0.0f;
-#pragma unroll 1
-    for (int r = thread >> 3; r < (NT < 32 ? 32 : NT); r += 32) {
-      const int query = u.tile * NT + r;
-      float v[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-      if (query < queries && r < NT)
-        load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
-                         (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v);
-      if (opaque(p.rotate)) {
-        hadamard_butterflies(v, group);
+  for (int i = 0; i < kPasses; ++i) {
+    if (p.rotate) {
+      hadamard_butterflies(v[i], group);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] *= kInvSqrt128;
-      }
-      if (opaque(phase) == 0) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
-      } else if (r < NT) {
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] *= scale;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
-        uint8_t* row = sm.q[group >> 2] + r * 128;
-        const int chunk = (group & 3) * 2;
-        *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
-        const int at = r * 64 + group * 8;
-#pragma unroll 1
-        for (int term = 0; term < kTerms; ++term) {
-          float largest = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(v[j]));
-          const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
-          GroupCodes codes;
-          codes.scale = e4m3_to_float(byte);
-          // (an approximate reciprocal: what it rounds otherwise is left to the next term)
-          float inverse_scale;
-          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse_scale) : "f"(fmaxf(codes.scale, 1.0e-30f)));
-          float scaled[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) scaled[j] = v[j] * inverse_scale;
-          codes.lo = pack_e2m1x8(scaled);
-          codes.hi = pack_e2m1x8(scaled + 8);
-          *reinterpret_cast<uint2*>(sm.q_codes[term] + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
-          sm.q_scales[term][scale_tile_offset(r, group)] = (uint8_t)byte;
-          float rest[16];
-          group_residual16(v, codes, rest);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = rest[j];
-        }
-      }
+      for (int j = 0; j < 16; ++j) v[i][j] *= kInvSqrt128;
     }
-    if (phase == 0) {
-      amax = warp_max(amax);
-      if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
-      softmax_sync();
 #pragma unroll
-      for (int w = 0; w < 8; ++w) amax = fmaxf(amax, sm.q_max[w]);
-      scale = fp16_scale(amax, &inverse);
-    }
+    for (int j = 0; j < 16; ++j)
+      if (fabsf(v[i][j]) < INFINITY) amax = fmaxf(amax, fabsf(v[i][j]));
+  }
+  amax = warp_max(amax);
+  if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
+  bar_sync(kWorkBarrier, kWorkers);
+#pragma unroll
+  for (int w = 0; w < kWorkers / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
+  float inverse;
+  const float scale = fp16_scale(amax, &inverse);
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = i * kPerPass + (thread >> 3);
+    if (kPasses * kPerPass > NT && r >= NT) break;
+    uint8_t* row = sm.q[group >> 2] + r * 128;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[i][2 * j] * scale, v[i][2 * j + 1] * scale));
+    const int chunk = (group & 3) * 2;
+    *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
   }
   tc::fence_proxy_async_smem();
-  softmax_sync();
-  if (thread == 0) tc::mbar_arrive(&sm.q_full);
   return inverse;
 }
 
@@ -914,331 +541,375 @@ __device__ __forceinline__ void reduce_columns(float* v, int lane, int column, S
   }
 }
 
+// One stage's release, by a whole warp.
 template <int NT>
-__device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, int thread) {
-  using Sh = Shape<NT>;
-  const int t = thread & 127, lane = thread & 31, warp = t >> 5, stream = thread >> 7;
-  const uint32_t lanes = (uint32_t)(t & ~31) << 16;
-  const float* base = sm.base[stream];
-  const int barrier = kStreamBarrier + stream;
-  const uint32_t output = sm.tmem + Sh::kO + stream * NT + lanes;
-  int blocks = 0, unit = 0;  // of the CTA so far
-  int n = 0;
-  float q_inverse = 1.0f;
-  float2 sum[NT / 2];
-  Units<NT> units(sm);
-  Unit u, following;
-  bool running = false;
+__device__ __forceinline__ void release(Smem<NT>& sm, Place& at, int lane) {
+  __syncwarp();
+  if (lane == 0) tc::mbar_arrive(&sm.empty[at.slot]);
+  at.advance();
+}
+
+// The keys of a BF16 step: thread r of either half brings its half of token r's channels. Returns what undoes
+// the token's scaling.
+template <int NT>
+__device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem<NT>& sm, const Unit& u, StepKind kind, Place& at,
+                                        uint32_t operand, int thread) {
+  const int r = thread & 127, half = thread >> 7, lane = thread & 31;
+  const int places = bf16_places(u.info, kind);
+  const bool two = places > kBf16Rows;
+  // a step's stages are held together
+  Place second = at;
+  wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+  if (two) {
+    second.advance();
+    wait(&sm.full[second.slot], second.turn, &sm.abort_flag);
+  }
+  uint8_t* const stage0 = sm.ring[at.slot];
+  uint8_t* const stage1 = sm.ring[second.slot];
+  auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
+  bool there = r < places;
+  if (kind == kStepDraft) {
+    if (r < BDFP4_MAX_SINK) there = r < u.info.sink;
+    if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
+      const int group = thread & 7;
+      const float* shift = p.key_shift ? p.key_shift + u.head * kHeadDim + group * kGroup : nullptr;
 #pragma unroll 1
-  while (true) {
-    // the next unit's queries go in while this one's last products run: all its scores are done
-    const bool more = !softmax_any(!units.next(following));
-    float next_inverse = 1.0f;
-    if (running) {  // each query's weight in this stream, by warp
-      float v[NT];
-#pragma unroll
-      for (int j = 0; j < NT / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
-      reduce_columns<NT, 16>(v, lane, 0, [&](int j, float total) { sm.warp_value[stream][warp][j] = total; });
-    }
-    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
-    if (running) {
-      softmax_sync();
-      const bool whole = u.begin == 0 && u.end == u.info.steps, both = u.end - u.begin > 2;
-      // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
-      const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
-      if (thread < NT) {  // join the streams
-        float total[2], top = fmaxf(sm.top[0][thread], sm.top[1][thread]), sum_of_both = 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          total[h] = sm.extra[h][thread];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) total[h] += sm.warp_value[h][w][thread];
-          sm.share[h][thread] = ex2(sm.top[h][thread] - top);
-          sum_of_both += total[h] * sm.share[h][thread];
-        }
-        if (whole) {
-          const float scale = sum_of_both > 0.0f ? p.value_scale / sum_of_both : 0.0f;
-          sm.share[0][thread] *= scale;
-          sm.share[1][thread] *= scale;
-        } else {
-          p.partial_stat[(int64_t)(2 * part) * NT + thread] = top;
-          p.partial_stat[(int64_t)(2 * part + 1) * NT + thread] = sum_of_both;
-        }
-      }
-      softmax_sync();
-      wait(&sm.o_full, unit & 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      const int out_first = stream * Sh::kOut;
-      const int queries = min(u.info.count * p.ratio - u.tile * NT - out_first, Sh::kOut);
-      const int query = u.tile * NT + out_first;
-      int out_node = query / p.ratio, out_head = query % p.ratio;
-      __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
-      float* partial = p.partial + ((int64_t)part * NT + out_first) * kHeadDim + t;
-      const uint32_t first_output = sm.tmem + Sh::kO + ((blocks - (u.end - u.begin + 1) / 2) & 1) * NT + out_first + lanes;
-      const uint32_t second_output = sm.tmem + Sh::kO + ((blocks - (u.end - u.begin + 1) / 2 + 1) & 1) * NT + out_first + lanes;
-      const float* first_share = sm.share[(blocks - (u.end - u.begin + 1) / 2) & 1] + out_first;
-      const float* second_share = sm.share[(blocks - (u.end - u.begin + 1) / 2 + 1) & 1] + out_first;
-#pragma unroll 1
-      for (int j = 0; j < queries; j += 8) {
-        float o[8], o2[8];
-        tc::tmem_ld8(first_output + j, o);
-        tc::tmem_ld8(second_output + j, o2);
-        tc::tmem_wait_ld();
+      for (int first = 0; first < u.info.count; first += kWorkers / 8) {
+        // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
+        const int node = first + (thread >> 3);
+        uint4* at16 = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + min(node, u.info.count - 1)) + group * 32);
+        const uint4 raw[2] = {at16[0], at16[1]};
+        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+        float v[16];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          o[i] *= first_share[j + i];
-          if (both) o[i] = fmaf(o2[i], second_share[j + i], o[i]);  // (a stream without blocks holds anything)
-          if (j + i < queries) {
-            if (whole) out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i]);
-            else partial[(j + i) * kHeadDim] = o[i];
-          }
-          if (++out_head == p.ratio) out_head = 0, ++out_node;
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
+        __syncwarp();  // a thread that follows along may read the row that another of its warp writes
+        cache_basis16_any(v, group, p.rotate != 0, shift);
+        if (node < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at16), v);
       }
-      tc::fence_before_sync();
-      softmax_sync();  // the output has been read; what is kept per query is written anew
-      if (thread == 0) {
-        tc::mbar_arrive(&sm.o_empty);
-        if (!whole && u.begin == 0) {
-          TreeSplit split;
-          split.row = u.row;
-          split.head = u.head;
-          split.tile = u.tile;
-          // this CTA's run ends inside the unit; the runs behind it are as long
-          split.last = blockIdx.x + (u.info.steps - u.end + sm.per_cta - 1) / sm.per_cta;
-          p.splits[blockIdx.x] = split;
-        }
-      }
-      ++unit;
+      tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
+      bar_sync(kWorkBarrier, kWorkers);
     }
-    if (!more) break;
-    running = true;
-    u = following;
-    q_inverse = next_inverse;
+  }
+  const uint4* row = reinterpret_cast<const uint4*>(row_of(min(r, places - 1)));
+  float amax = 0.0f;
+  if (there) {
+#pragma unroll 4
+    for (int j = 0; j < 16; ++j) {
+      const uint4 q = row[j];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+    }
+  }
+  float inverse;
+  const float scale = fp16_scale(amax, &inverse);
+#pragma unroll 1
+  for (int quarter = 2 * half; quarter < 2 * half + 2; ++quarter) {
+    uint32_t v[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (there) q = row[quarter * 4 + j];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
+    }
+    st16(operand + quarter * 16, v);
+  }
+  release(sm, at, lane);
+  if (two) release(sm, at, lane);
+  return inverse;
+}
 
-    if (t < NT) {
-      sm.top[stream][t] = kNoMax;
-      sm.extra[stream][t] = 0.0f;
-      if (stream == 0) {  // the draft nodes that this query sees
-        uint64_t seen = 0;
+// The values of a BF16 step: half h brings the tokens of the step's stage h into channel r's lane.
+template <int NT>
+__device__ __forceinline__ void bf16_values(Smem<NT>& sm, const Unit& u, StepKind kind, Place& at, uint32_t operand, int thread) {
+  const int c = thread & 127, half = thread >> 7, lane = thread & 31;
+  const int places = bf16_places(u.info, kind);
 #pragma unroll 1
-        for (int node = min((u.tile * NT + t) / p.ratio, u.info.count - 1); node >= 0;) {
-          seen |= 1ull << node;
-          const int parent = sm.parents[node];
-          node = parent < node ? parent : -1;
+  for (int first = 0; first < places; first += kBf16Rows) {
+    wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+    if ((first > 0) == (half > 0)) {
+      const uint8_t* stage = sm.ring[at.slot] + 2 * c;
+      const int slices = (min(places - first, kBf16Rows) + 15) / 16;
+#pragma unroll 1
+      for (int s = 0; s < slices; ++s) {
+        const int place = first + s * 16;
+        const int stop = kind == kStepDraft && place == 0 ? u.info.sink : places;
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t lo = 0, hi = 0;
+          if (place + 2 * i < stop) lo = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i) * kBf16Pitch);
+          if (place + 2 * i + 1 < stop) hi = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i + 1) * kBf16Pitch);
+          v[i] = lo | (hi << 16);
         }
-        sm.family[t] = seen;
+        st8(operand + (place >> 4) * 8, v);
       }
     }
-#pragma unroll
-    for (int j = 0; j < NT / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
-    softmax_sync();
-    const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
-    const int all_blocks = (u.end - u.begin + 1) / 2;
-#pragma unroll 1
-    for (int k = (stream ^ blocks) & 1; k < all_blocks; k += 2) {
-      const int block = blocks + k, block_begin = u.begin + 2 * k;
-      const int steps = min(2, u.end - block_begin), set = (block >> 1) & 1;
-      const uint32_t parity = (block >> 2) & 1;
-      // a block in which every query sees every token, and all of it FP4
-      const bool plain = block_begin + steps <= u.info.pages && (block_begin > 0 || u.info.sink == 0);
-      const uint32_t scores0 = sm.tmem + Sh::kS + (4 * stream + 2 * set) * NT + lanes;
-      auto scores_ready = [&](int i) {
-        wait(&sm.s_full[stream][set][i], parity, &sm.abort_flag);
-        tc::fence_after_sync();
-      };
-      // Where 16 bytes of P go: chunk index XORed as the swizzle does.
-      uint8_t* const p_rows = sm.p[stream][set][0] + t * Sh::kRow;
-      auto p_chunk = [&](int i, int chunk) {
-        return reinterpret_cast<uint4*>(p_rows + i * (128 * Sh::kRow) + ((chunk ^ (NT == 32 ? (t >> 1) & 3 : (t >> 2) & 1)) * 16));
-      };
-      // Any step: scores in log2 units above the maxima (plus kShift) are f * score + base; a token may be seen by
-      // no query or, a draft, by some.
-      struct Step {
-        StepKind kind;
-        int node;             // of this thread's token, if a draft
-        uint32_t all, alive;  // 1: every query sees the token; 1: some may
-        float f;
-      };
-      auto open = [&](int i) {
-        Step k;
-        k.kind = step_kind(u.info, block_begin + i);
-        bool dead;
-        if (k.kind == kStepPage) dead = block_begin + i == 0 && t < u.info.sink;
-        else if (k.kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
-        else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-        const bool draft = k.kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
-        k.node = draft ? t - BDFP4_MAX_SINK : 0;
-        k.all = draft ? 0 : 1;
-        k.alive = dead ? 0 : 1;
-        k.f = k.kind == kStepPage ? page_factor : p.scale_log2 * q_inverse * sm.key_factor[(n + 2 * (block - blocks) + i) & 7][t];
-        return k;
-      };
-      auto load8 = [&](const Step& k, int i, int j, float* v) {
-        tc::tmem_ld8(scores0 + i * NT + j, v);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t seen = (uint32_t)(sm.family[j + c] >> k.node) | k.all;
-          if (!(seen & k.alive)) v[c] = -INFINITY;
-        }
-      };
-      float s[NT];  // a plain block's probabilities, both steps' added
-      bool high, fresh = k < 2;
-      // P of this block goes where the stream's one before the last was
-      wait(&sm.p_empty[stream][set], parity ^ 1, &sm.abort_flag);
-#pragma unroll 1
-      while (true) {
-        if (fresh) {  // take the maxima anew; what was summed so far is brought down to them
-          float mine = -INFINITY;
-#pragma unroll 1
-          for (int i = 0; i < steps; ++i) {
-            scores_ready(i);
-            const Step k = open(i);
-#pragma unroll 1
-            for (int j = 0; j < NT; j += 8) {
-              float v[8];
-              load8(k, i, j, v);
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                const float m = warp_max(v[c] * k.f);
-                if (lane == j + c) mine = fmaxf(mine, m);
-              }
-            }
-          }
-          if (lane < NT) sm.warp_value[stream][warp][lane] = mine;
-          bar_sync(barrier, 128);
-          if (t < NT) {
-            const float before = sm.top[stream][t];
-            float now = before;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) now = fmaxf(now, sm.warp_value[stream][w][t]);
-            const float factor = ex2(before - now);
-            sm.top[stream][t] = now;
-            sm.base[stream][t] = kShift - now;
-            sm.factor[stream][t] = factor;
-            sm.extra[stream][t] *= factor;
-          }
-          bar_sync(barrier, 128);
-          if (k >= 2) {
-#pragma unroll
-            for (int j = 0; j < NT / 2; ++j) {
-              sum[j].x *= sm.factor[stream][2 * j];
-              sum[j].y *= sm.factor[stream][2 * j + 1];
-            }
-            const int last = block - 2;  // the stream's
-            wait(&sm.p_empty[stream][(last >> 1) & 1], (last >> 2) & 1, &sm.abort_flag);
-            tc::fence_after_sync();
-#pragma unroll 1
-            for (int j = 0; j < NT; j += 8) {
-              float o[8];
-              uint32_t r[8];
-              tc::tmem_ld8(output + j, o);
-              tc::tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(o[i] * sm.factor[stream][j + i]);
-              st8(output + j, r);
-            }
-            tc::tmem_wait_st();
-          }
-        }
-        high = false;
-        if (plain) {
-#pragma unroll
-          for (int j = 0; j < NT; ++j) s[j] = 0.0f;
-          const float2 f2 = make_float2(page_factor, page_factor);
-          __half2 most = __floats2half2_rn(0.0f, 0.0f);
-#pragma unroll 1
-          for (int i = 0; i < steps; ++i) {
-            scores_ready(i);
-            float x[NT];
-#pragma unroll
-            for (int j = 0; j < NT; j += 16) tc::tmem_ld16(scores0 + i * NT + j, x + j);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < NT; j += 8) {
-              uint32_t w[4];
-#pragma unroll
-              for (int c = j; c < j + 8; c += 4) {
-                const float4 b = *reinterpret_cast<const float4*>(base + c);
-                const float2 y0 = __ffma2_rn(make_float2(x[c], x[c + 1]), f2, make_float2(b.x, b.y));
-                const float2 y1 = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), f2, make_float2(b.z, b.w));
-                x[c] = ex2(y0.x), x[c + 1] = ex2(y0.y), x[c + 2] = ex2(y1.x), x[c + 3] = ex2(y1.y);
-              }
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const __half2 pair = __floats2half2_rn(x[j + 2 * c], x[j + 2 * c + 1]);
-                most = __hmax2(most, pair);
-                w[c] = h2(pair);
-              }
-              *p_chunk(i, j >> 3) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-#pragma unroll
-            for (int c = 0; c < NT; c += 2) {
-              const float2 two = __fadd2_rn(make_float2(s[c], s[c + 1]), make_float2(x[c], x[c + 1]));
-              s[c] = two.x, s[c + 1] = two.y;
-            }
-          }
-          high = __half2float(__hmax(__low2half(most), __high2half(most))) > kHighest;
-        } else {
-          float* const sums = sm.step_sum[stream][set][warp];
-#pragma unroll 1
-          for (int i = 0; i < steps; ++i) {
-            scores_ready(i);
-            const Step k = open(i);
-#pragma unroll 1
-            for (int j = 0; j < NT; j += 8) {
-              float v[8];
-              load8(k, i, j, v);
-              const bool page = opaque(k.kind) == kStepPage;
-              uint32_t w[4];
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                v[c] = ex2(fmaf(v[c], k.f, base[j + c]));
-                high |= v[c] > kHighest;
-              }
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                w[c] = page ? h2(__floats2half2_rn(v[2 * c], v[2 * c + 1]))
-                            : pack_bf16x2(v[2 * c] * p.inverse_value_scale, v[2 * c + 1] * p.inverse_value_scale);
-              *p_chunk(i, j >> 3) = make_uint4(w[0], w[1], w[2], w[3]);
-              // four lanes end up with each column's sum
-              reduce_columns<8, 16>(v, lane, j, [&](int column, float total) {
-                if ((lane & 3) == 0) sums[column] = opaque(i) > 0 ? sums[column] + total : total;
-              });
-            }
-          }
-        }
-        tc::fence_before_sync();
-        tc::fence_proxy_async_smem();
-        // against maxima just taken nothing is high: the vote then only ends the block
-        if (!bar_any(barrier, 128, high) || fresh) break;
-        fresh = true;
-      }
-      // the barrier stands behind every thread's scores read and probabilities written
-      if (t == 0) {
-        tc::mbar_arrive(&sm.p_full[stream][set]);
-        tc::mbar_arrive(&sm.s_empty[stream][set]);
-      }
-      if (plain) {
-#pragma unroll
-        for (int j = 0; j < NT / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
-      } else if (t < NT) {
-        float total = sm.extra[stream][t];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) total += sm.step_sum[stream][set][w][t];
-        sm.extra[stream][t] = total;
-      }
-    }
-    blocks += all_blocks;
-    n += u.end - u.begin;
+    release(sm, at, lane);
   }
 }
 
 template <int NT, int PT>
-__global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
-tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const TreeParams p) {
+__device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
   using Sh = Shape<NT>;
+  constexpr int C = Sh::kColumns;
+  const int t = thread & 127, lane = thread & 31, warp = t >> 5, half = thread >> 7;
+  const int first_column = half * C;
+  const int barrier = kHalfBarrier + half;
+  const uint32_t lanes = sm.tmem + ((uint32_t)(t & ~31) << 16);
+  const uint32_t scores = lanes + Sh::kS + first_column, k_operand = lanes + Sh::kK, v_operand = lanes + Sh::kV;
+  float* base = sm.base + first_column;
+  float* top = sm.top + first_column;
+  // where this thread's codes and scales lie in a stage: half of token t's channels, half of channel t's tokens
+  const int k_codes = t * 64, k_swizzle = (t >> 1) & 3;
+  const int k_scales = kKsOffset + half * (PT == 128 ? 512 : 256) +
+                       (PT == 128 ? (t & 31) * 16 + (t >> 5) * 4 : (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4);
+  const int v_codes = kVOffset + (PT == 128 ? t * 64 : half * 4096 + t * 32);
+  const int v_scales = kVsOffset + half * 512 + (t & 31) * 16 + (t >> 5) * 4;
+  uint8_t* const p_row = sm.p + t * 128;
+  const int p_chunk = first_column >> 3, p_swizzle = t & 7;
+  Place at;
+  uint32_t parity = 0;
+  bool any = false;  // a step has been taken
+  Unit u;
+  bool known = false;
+#pragma unroll 1
+  for (; walker.next(u, known); known = true) {
+    const float q_inverse = load_queries<NT>(p, sm, u, thread);
+    if (t < C) {
+      top[t] = kNoMax;
+      base[t] = kShift - kNoMax;
+      // the draft nodes the query of column t sees
+      const int query = u.tile * NT + first_column + t;
+      uint64_t seen = 0;
+#pragma unroll 1
+      for (int node = min(query / p.ratio, u.info.count - 1); node >= 0;) {
+        seen |= 1ull << node;
+        const int parent = sm.parents[node];
+        node = parent < node ? parent : -1;
+      }
+      sm.family[first_column + t] = seen;
+    }
+    float2 sum[C / 2];
+#pragma unroll
+    for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
+    bar_sync(barrier, 128);
+    const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
+#pragma unroll 1
+    for (int step = u.begin; step < u.end; ++step) {
+      const StepKind kind = step_kind(u.info, step);
+      const int stage_slot = at.slot;
+      float f = page_factor;
+      // K: the scores of the step before have been waited for, so its operand is free
+      if (kind == kStepPage) {
+        wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+        const uint8_t* stage = sm.ring[stage_slot];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          store_dequantized(k_operand + 32 * half + 16 * j,
+                            *reinterpret_cast<const uint4*>(stage + k_codes + (((2 * half + j) ^ k_swizzle) * 16)),
+                            *reinterpret_cast<const uint16_t*>(stage + k_scales + 2 * j));
+      } else {
+        f = p.scale_log2 * q_inverse * bf16_keys<NT>(p, sm, u, kind, at, k_operand, thread);
+      }
+      tc::tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sm.k_full);
+      // V, once the product of the step before is done with its operand, P and (for a rescaling) the output
+      if (any) wait(&sm.o_full, parity ^ 1, &sm.abort_flag);
+      tc::fence_after_sync();
+      if (kind == kStepPage) {
+        const uint8_t* stage = sm.ring[stage_slot];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          store_dequantized(v_operand + 32 * half + 16 * j,
+                            *reinterpret_cast<const uint4*>(
+                                stage + v_codes + (PT == 128 ? ((2 * half + j) ^ k_swizzle) * 16 : (j ^ ((t >> 2) & 1)) * 16)),
+                            *reinterpret_cast<const uint16_t*>(stage + v_scales + 2 * j));
+        release(sm, at, lane);
+      } else {
+        bf16_values<NT>(sm, u, kind, at, v_operand, thread);
+      }
+
+      bool dead;  // no query sees this thread's token
+      if (kind == kStepPage) dead = step == 0 && t < u.info.sink;
+      else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
+      else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
+      const bool special = kind != kStepPage || (step == 0 && u.info.sink > 0);  // the same in the whole half
+      const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
+      const int node = t - BDFP4_MAX_SINK;
+      const float2 f2 = make_float2(f, f);
+      tc::tmem_wait_st();
+      wait(&sm.s_full, parity, &sm.abort_flag);
+      tc::fence_after_sync();
+
+      float s[C];
+      auto load = [&] {
+        tmem_load<C>(scores, s);
+        tc::tmem_wait_ld();
+        if (special) {
+#pragma unroll
+          for (int j = 0; j < C; ++j)
+            if (dead || (masked && !((sm.family[first_column + j] >> node) & 1))) s[j] = -INFINITY;
+        }
+      };
+      // The step's probabilities into s and, rounded, into shared memory. True when one of this thread's
+      // exceeds kHighest: its query's maximum has to be renewed, and the step formed again.
+      auto form = [&]() -> bool {
+        __half2 most = __floats2half2_rn(0.0f, 0.0f);
+        float most32 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < C; j += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(base + j + i);
+            const float2 y0 = __ffma2_rn(make_float2(s[j + i], s[j + i + 1]), f2, make_float2(b.x, b.y));
+            const float2 y1 = __ffma2_rn(make_float2(s[j + i + 2], s[j + i + 3]), f2, make_float2(b.z, b.w));
+            s[j + i] = ex2(y0.x), s[j + i + 1] = ex2(y0.y), s[j + i + 2] = ex2(y1.x), s[j + i + 3] = ex2(y1.y);
+          }
+          if (kind == kStepPage) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const __half2 pair = __floats2half2_rn(s[j + 2 * i], s[j + 2 * i + 1]);
+              most = __hmax2(most, pair);
+              w[i] = h2(pair);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              most32 = fmaxf(most32, fmaxf(s[j + 2 * i], s[j + 2 * i + 1]));
+              w[i] = pack_bf16x2(s[j + 2 * i] * p.inverse_value_scale, s[j + 2 * i + 1] * p.inverse_value_scale);
+            }
+          }
+          *reinterpret_cast<uint4*>(p_row + (((p_chunk + (j >> 3)) ^ p_swizzle) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        tc::fence_before_sync();
+        tc::fence_proxy_async_smem();
+        return fmaxf(most32, __half2float(__hmax(__low2half(most), __high2half(most)))) > kHighest;
+      };
+      load();
+      if (bar_any(barrier, form())) {
+        load();
+        float mine = 0.0f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          const float m = warp_max(s[j] * f);
+          if (lane == j) mine = m;
+        }
+        if (lane < C) sm.col_max[warp][first_column + lane] = mine;
+        bar_sync(barrier, 128);
+        if (t < C) {
+          const int col = first_column + t;
+          const float before = top[t];
+          const float now = fmaxf(fmaxf(fmaxf(sm.col_max[0][col], sm.col_max[1][col]),
+                                        fmaxf(sm.col_max[2][col], sm.col_max[3][col])), before);
+          top[t] = now;
+          base[t] = kShift - now;
+          sm.factor[col] = ex2(before - now);
+        }
+        bar_sync(barrier, 128);
+#pragma unroll
+        for (int j = 0; j < C / 2; ++j) {
+          sum[j].x *= sm.factor[first_column + 2 * j];
+          sum[j].y *= sm.factor[first_column + 2 * j + 1];
+        }
+        form();
+        if (step > u.begin) {  // what O^T holds is of the old maxima
+#pragma unroll 1
+          for (int j = 0; j < C; j += 8) {
+            float o[8];
+            const uint32_t column = lanes + Sh::kO + first_column + j;
+            tc::tmem_ld8(column, o);
+            tc::tmem_wait_ld();
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(o[i] * sm.factor[first_column + j + i]);
+            st8(column, w);
+          }
+          tc::tmem_wait_st();
+          tc::fence_before_sync();
+        }
+        bar_sync(barrier, 128);
+      }
+      // the half's barrier stands behind every thread's scores read, values and probabilities written
+      if (t == 0) tc::mbar_arrive(&sm.p_full);
+#pragma unroll
+      for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
+      parity ^= 1;
+      any = true;
+    }
+
+    {  // each query's weight: first over a warp's 32 tokens, then (below) over the four warps
+      float v[C];
+#pragma unroll
+      for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
+      reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col_sum[warp][first_column + j] = total; });
+    }
+    bar_sync(barrier, 128);
+    const bool whole = u.begin == 0 && u.end == u.info.steps;
+    // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
+    const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
+    if (t < C) {
+      const int col = first_column + t;
+      const float total = (sm.col_sum[0][col] + sm.col_sum[1][col]) + (sm.col_sum[2][col] + sm.col_sum[3][col]);
+      if (whole) {
+        sm.total[col] = total > 0.0f ? p.value_scale / total : 0.0f;
+      } else {
+        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[t];
+        p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
+      }
+    }
+    bar_sync(barrier, 128);
+    wait(&sm.o_full, parity ^ 1, &sm.abort_flag);
+    tc::fence_after_sync();
+    const int queries = min(u.info.count * p.ratio - u.tile * NT - first_column, C);
+    const int query = u.tile * NT + first_column;
+    int out_node = query / p.ratio, out_head = query % p.ratio;
+    __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
+    float* partial = p.partial + ((int64_t)part * NT + first_column) * kHeadDim + t;
+#pragma unroll 1
+    for (int j = 0; j < C; j += 8) {
+      float o[8];
+      tc::tmem_ld8(lanes + Sh::kO + first_column + j, o);
+      tc::tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (j + i < queries) {
+          if (whole) {
+            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[first_column + j + i]);
+            if (++out_head == p.ratio) out_head = 0, ++out_node;
+          } else {
+            partial[(int64_t)(j + i) * kHeadDim] = o[i];
+          }
+        }
+      }
+    }
+    tc::fence_before_sync();
+    if (!whole && u.begin == 0 && thread == 0) {
+      TreeSplit split;
+      split.row = u.row;
+      split.head = u.head;
+      split.tile = u.tile;
+      // the unit's last step, counted over the whole launch, names the CTA it ends in
+      split.last = (int)((sm.last + (u.info.steps - u.end) - 1) / sm.per_cta);
+      p.splits[blockIdx.x] = split;
+    }
+  }
+}
+
+template <int NT, int PT>
+__global__ void __launch_bounds__(kThreads, 2)
+tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const TreeParams p) {
   extern __shared__ uint8_t raw_smem[];
   Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
@@ -1247,44 +918,23 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   // all steps of the launch, and where this CTA's run begins
   long long mine = 0;
 #pragma unroll 1
-  for (int row = thread; row < p.rows; row += Sh::kThreads) {
+  for (int row = thread; row < p.rows; row += kThreads) {
     const RowInfo r = row_info(p, row, PT);
     mine += (long long)r.steps * r.tiles * p.heads_kv;
   }
-#pragma unroll 1
   for (int step = 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
   if (lane == 0) sm.sums[warp] = mine;
   if (thread == 0) {
 #pragma unroll 1
-    for (int i = 0; i < Sh::kStages; ++i) {
-      tc::mbar_init(&sm.full_k[i], 1);
-      tc::mbar_init(&sm.full_v[i], 1);
-      tc::mbar_init(&sm.empty[i], 5);  // the values' four warps and the score product
-      tc::mbar_init(&sm.k_ready[i], 1);
+    for (int i = 0; i < kStages; ++i) {
+      tc::mbar_init(&sm.full[i], 1);
+      tc::mbar_init(&sm.empty[i], 8);
     }
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&sm.ka_full[i], 4);
-      tc::mbar_init(&sm.ka_empty[i], 1);
-      tc::mbar_init(&sm.va_full[i], 4);
-      tc::mbar_init(&sm.va_empty[i], 1);
-      for (int set = 0; set < 2; ++set) {
-        tc::mbar_init(&sm.s_full[i][set][0], 1);
-        tc::mbar_init(&sm.s_full[i][set][1], 1);
-        tc::mbar_init(&sm.s_empty[i][set], 1);
-        tc::mbar_init(&sm.p_full[i][set], 1);
-        tc::mbar_init(&sm.p_empty[i][set], 1);
-      }
-    }
-#pragma unroll 1
-    for (int i = 0; i < kUnits; ++i) {
-      tc::mbar_init(&sm.unit_full[i], 1);
-      tc::mbar_init(&sm.unit_empty[i], kUnitReaders);
-    }
-    tc::mbar_init(&sm.q_full, 1);
+    tc::mbar_init(&sm.k_full, 8);
+    tc::mbar_init(&sm.s_full, 1);
+    tc::mbar_init(&sm.p_full, 2);
     tc::mbar_init(&sm.o_full, 1);
-    tc::mbar_init(&sm.o_empty, 1);
-    tc::mbar_init(&sm.drained, 2);
+    tc::mbar_init(&sm.drained, 1);
     tc::fence_barrier_init();
     sm.abort_flag = sm.ignored_flag = 0;
     TreeSplit none;
@@ -1295,12 +945,11 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   __syncthreads();
   if (warp == 0) {
     long long all = 0;
-#pragma unroll 1
-    for (int w = 0; w < Sh::kThreads / 32; ++w) all += sm.sums[w];
+    for (int w = 0; w < kThreads / 32; ++w) all += sm.sums[w];
     const long long per = max((all + gridDim.x - 1) / gridDim.x, 1ll);
     const long long first = per * blockIdx.x, last = min(first + per, all);
     if (lane == 0) {
-      sm.per_cta = (int)min(per, (long long)INT32_MAX / 2);  // a unit that straddles is shorter
+      sm.per_cta = per;
       sm.first = first;
       sm.last = last;
     }
@@ -1313,7 +962,6 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         steps = (long long)r.steps * r.tiles * p.heads_kv;
       }
       long long upto = steps;
-#pragma unroll 1
       for (int step = 1; step < 32; step <<= 1) {
         const long long left = __shfl_up_sync(0xffffffffu, upto, step);
         if (lane >= step) upto += left;
@@ -1329,32 +977,23 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
     __syncwarp();
-    tc::tmem_alloc(&sm.tmem, 512);
+    tc::tmem_alloc(&sm.tmem, kTmemColumns);
     tc::tmem_relinquish();
     tc::fence_before_sync();
   }
   __syncthreads();
   tc::fence_after_sync();
   if (sm.first < sm.last) {
-    if (warp < 8) {
-      trade_registers<Sh::kLaunchRegs, Sh::kValueRegs>();
-      values<NT, PT>(p, sm, thread);
-    } else if (warp < 16) {
-      trade_registers<Sh::kLaunchRegs, Sh::kSoftmaxRegs>();
-      softmax<NT>(p, sm, thread - 256);
-    } else {
-      trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
-      if (warp == 16) produce<NT, PT, 0>(p, sm, &k_map, lane);
-      if (warp == 17) produce<NT, PT, 1>(p, sm, &v_map, lane);
-      if (warp == 18) issue_scores<NT, PT>(sm);
-      if (warp == 19) issue_output<NT>(sm);
-    }
+    const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
+    if (warp < kWorkers / 32) work<NT, PT>(p, sm, walker, thread);
+    else if (warp == kWorkers / 32) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
+    else issue<NT>(sm, walker);
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   if (thread == 0 && sm.abort_flag && p.error_word) atomicOr(p.error_word, (int)BDFP4_DEV_WAIT_TIMEOUT);
-  if (warp == 0) tc::tmem_dealloc(sm.tmem, 512);
+  if (warp == 0) tc::tmem_dealloc(sm.tmem, kTmemColumns);
 }
 
 template <int NT, int PT>
@@ -1367,7 +1006,7 @@ static cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, co
     if (e != cudaSuccess) return e;
     if (slot >= 0) configured.done[slot] = true;
   }
-  tree_kernel<NT, PT><<<kTreeCtas, Shape<NT>::kThreads, smem, stream>>>(k_map, v_map, p);
+  tree_kernel<NT, PT><<<kTreeCtas, kThreads, smem, stream>>>(k_map, v_map, p);
   return cudaGetLastError();
 }
 
@@ -1375,7 +1014,8 @@ template <int PT>
 static cudaError_t launch_tile(const CUtensorMap& k_map, const CUtensorMap& v_map, const TreeParams& p, cudaStream_t stream) {
   switch (p.tile) {
     case 16: return launch<16, PT>(k_map, v_map, p, stream);
-    default: return launch<32, PT>(k_map, v_map, p, stream);
+    case 32: return launch<32, PT>(k_map, v_map, p, stream);
+    default: return launch<64, PT>(k_map, v_map, p, stream);
   }
 }
 

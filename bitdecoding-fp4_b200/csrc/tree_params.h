@@ -10,9 +10,9 @@
 
 namespace bdfp4 {
 
-// CTAs of a launch: one per SM of a B200. They share nothing but the workspace, so any number is correct.
-constexpr int kTreeCtas = 148;
-constexpr int kTreeMaxTile = 32;  // query rows (node x query head of one KV head) of a CTA's tile at most
+// CTAs of a launch: two per SM of a B200. They share nothing but the workspace, so any number is correct.
+constexpr int kTreeCtas = 296;
+constexpr int kTreeMaxTile = 64;  // query rows (node x query head of one KV head) of a CTA's tile at most
 
 // A unit that begins in CTA c and does not end there: its parts lie in slot 2c + 1 and in slots 2c' of the
 // CTAs c < c' <= last.
