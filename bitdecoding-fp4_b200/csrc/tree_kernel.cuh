@@ -51,7 +51,7 @@ constexpr int kBf16Pitch = 272, kBf16Rows = 64;
 constexpr int kHalfBarrier = 1, kWorkBarrier = 3;
 constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
 constexpr float kShift = 7.0f;      // probabilities carry 2^7
-constexpr float kHighest = 32768.0f;  // ... and their queries' maxima are renewed when one exceeds this, 2^8 above
+constexpr float kGrowth = 8.0f;     // a maximum is renewed when a score exceeds it by more than this (log2)
 
 constexpr int kWorkers = 256;              // two halves of 128
 constexpr int kThreads = kWorkers + 64;    // and a warp each for copies and products
@@ -73,9 +73,9 @@ struct Smem {
   alignas(1024) uint8_t q[2][NT * 128];  // two halves of 64 channels, K-major, 128-byte swizzle
   alignas(1024) uint8_t p[16384];        // MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
-  float base[NT];       // kShift - maximum
+  float base[NT];       // kShift - maximum, 0 while there is none
   float top[NT];        // maximum, log2 units
-  float factor[NT];
+  float factor[NT], shift[NT];  // what a renewal does to sums and scores
   float total[NT];
   float col_max[4][NT];
   float col_sum[4][NT];
@@ -412,26 +412,32 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const uint32_t q = tc::smem_u32(sm.q);
   const uint64_t tile = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
-  uint32_t parity = 0;
+  uint32_t k_parity = 0, p_parity = 0;
   Unit u;
   bool known = false;
 #pragma unroll 1
   for (; walker.next(u, known); known = true) {
+    // a step's scores go before the output of the one before
 #pragma unroll 1
-    for (int step = u.begin; step < u.end; ++step, parity ^= 1) {
-      wait(&sm.k_full, parity, &sm.abort_flag);
-      tc::fence_after_sync();
-      if (elect_one()) {
+    for (int step = u.begin; step <= u.end; ++step) {
+      if (step < u.end) {
+        wait(&sm.k_full, k_parity, &sm.abort_flag);
+        k_parity ^= 1;
+        tc::fence_after_sync();
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          mma_ts(tmem + Sh::kS, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
-        tc::commit(&sm.s_full);
+          for (int s = 0; s < 8; ++s)
+            mma_ts(tmem + Sh::kS, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
+          tc::commit(&sm.s_full);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      wait(&sm.p_full, parity, &sm.abort_flag);  // P, and before it V
+      if (step == u.begin) continue;
+      wait(&sm.p_full, p_parity, &sm.abort_flag);  // P, and before it V
+      p_parity ^= 1;
       tc::fence_after_sync();
-      const StepKind kind = step_kind(u.info, step);
-      const bool first = step == u.begin;
+      const StepKind kind = step_kind(u.info, step - 1);
+      const bool first = step - 1 == u.begin;
       if (elect_one()) {
         if (kind == kStepPage) {
 #pragma unroll
@@ -624,6 +630,8 @@ __device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem<NT>& sm, co
   }
   release(sm, at, lane);
   if (two) release(sm, at, lane);
+  at.advance();  // the values'
+  if (two) at.advance();
   return inverse;
 }
 
@@ -632,6 +640,8 @@ template <int NT>
 __device__ __forceinline__ void bf16_values(Smem<NT>& sm, const Unit& u, StepKind kind, Place& at, uint32_t operand, int thread) {
   const int c = thread & 127, half = thread >> 7, lane = thread & 31;
   const int places = bf16_places(u.info, kind);
+  at.advance();  // the keys'
+  if (places > kBf16Rows) at.advance();
 #pragma unroll 1
   for (int first = 0; first < places; first += kBf16Rows) {
     wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
@@ -676,7 +686,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
   const int v_scales = kVsOffset + half * 512 + (t & 31) * 16 + (t >> 5) * 4;
   uint8_t* const p_row = sm.p + t * 128;
   const int p_chunk = first_column >> 3, p_swizzle = t & 7;
-  Place at;
+  Place k_at, v_at;  // a page's stage serves both; of a BF16 step each passes over the other's
   uint32_t parity = 0;
   bool any = false;  // a step has been taken
   Unit u;
@@ -686,7 +696,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     const float q_inverse = load_queries<NT>(p, sm, u, thread);
     if (t < C) {
       top[t] = kNoMax;
-      base[t] = kShift - kNoMax;
+      base[t] = 0.0f;  // scores as they are
       // the draft nodes the query of column t sees
       const int query = u.tile * NT + first_column + t;
       uint64_t seen = 0;
@@ -703,127 +713,112 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
     bar_sync(barrier, 128);
     const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
-#pragma unroll 1
-    for (int step = u.begin; step < u.end; ++step) {
+    // Keys of a step into their operand, which the scores of the step before must have left. Returns what turns
+    // its scores into log2 units.
+    auto bring_keys = [&](int step) -> float {
       const StepKind kind = step_kind(u.info, step);
-      const int stage_slot = at.slot;
       float f = page_factor;
-      // K: the scores of the step before have been waited for, so its operand is free
       if (kind == kStepPage) {
-        wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
-        const uint8_t* stage = sm.ring[stage_slot];
+        wait(&sm.full[k_at.slot], k_at.turn, &sm.abort_flag);
+        const uint8_t* stage = sm.ring[k_at.slot];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           store_dequantized(k_operand + 32 * half + 16 * j,
                             *reinterpret_cast<const uint4*>(stage + k_codes + (((2 * half + j) ^ k_swizzle) * 16)),
                             *reinterpret_cast<const uint16_t*>(stage + k_scales + 2 * j));
+        k_at.advance();
       } else {
-        f = p.scale_log2 * q_inverse * bf16_keys<NT>(p, sm, u, kind, at, k_operand, thread);
+        f = p.scale_log2 * q_inverse * bf16_keys<NT>(p, sm, u, kind, k_at, k_operand, thread);
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sm.k_full);
+      return f;
+    };
+    float f = bring_keys(u.begin);
+#pragma unroll 1
+    for (int step = u.begin; step < u.end; ++step) {
+      const StepKind kind = step_kind(u.info, step);
+      const bool special = kind != kStepPage || (step == 0 && u.info.sink > 0);  // the same in the whole half
+      wait(&sm.s_full, parity, &sm.abort_flag);
+      tc::fence_after_sync();
+
+      float s[C];
+      tmem_load<C>(scores, s);
+      tc::tmem_wait_ld();
+      if (special) {
+        bool dead;  // no query sees this thread's token
+        if (kind == kStepPage) dead = t < u.info.sink;
+        else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
+        else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
+        const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
+        const int node = t - BDFP4_MAX_SINK;
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (dead || (masked && !((sm.family[first_column + j] >> node) & 1))) s[j] = -INFINITY;
+      }
+      // scores -> log2 units above the maxima, plus kShift
+      const float2 f2 = make_float2(f, f);
+      float highest = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < C; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(base + j);
+        const float2 y0 = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, make_float2(b.x, b.y));
+        const float2 y1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), f2, make_float2(b.z, b.w));
+        s[j] = y0.x, s[j + 1] = y0.y, s[j + 2] = y1.x, s[j + 3] = y1.y;
+        highest = fmaxf(fmaxf(highest, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
+      }
+      tc::fence_before_sync();
+      // the next step's scores are taken while this one's probabilities are formed
+      float next_f = f;
+      if (step + 1 < u.end) next_f = bring_keys(step + 1);
       // V, once the product of the step before is done with its operand, P and (for a rescaling) the output
       if (any) wait(&sm.o_full, parity ^ 1, &sm.abort_flag);
       tc::fence_after_sync();
       if (kind == kStepPage) {
-        const uint8_t* stage = sm.ring[stage_slot];
+        const uint8_t* stage = sm.ring[v_at.slot];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           store_dequantized(v_operand + 32 * half + 16 * j,
                             *reinterpret_cast<const uint4*>(
                                 stage + v_codes + (PT == 128 ? ((2 * half + j) ^ k_swizzle) * 16 : (j ^ ((t >> 2) & 1)) * 16)),
                             *reinterpret_cast<const uint16_t*>(stage + v_scales + 2 * j));
-        release(sm, at, lane);
+        release(sm, v_at, lane);
       } else {
-        bf16_values<NT>(sm, u, kind, at, v_operand, thread);
+        bf16_values<NT>(sm, u, kind, v_at, v_operand, thread);
       }
-
-      bool dead;  // no query sees this thread's token
-      if (kind == kStepPage) dead = step == 0 && t < u.info.sink;
-      else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
-      else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-      const bool special = kind != kStepPage || (step == 0 && u.info.sink > 0);  // the same in the whole half
-      const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
-      const int node = t - BDFP4_MAX_SINK;
-      const float2 f2 = make_float2(f, f);
-      tc::tmem_wait_st();
-      wait(&sm.s_full, parity, &sm.abort_flag);
-      tc::fence_after_sync();
-
-      float s[C];
-      auto load = [&] {
-        tmem_load<C>(scores, s);
-        tc::tmem_wait_ld();
-        if (special) {
-#pragma unroll
-          for (int j = 0; j < C; ++j)
-            if (dead || (masked && !((sm.family[first_column + j] >> node) & 1))) s[j] = -INFINITY;
-        }
-      };
-      // The step's probabilities into s and, rounded, into shared memory. True when one of this thread's
-      // exceeds kHighest: its query's maximum has to be renewed, and the step formed again.
-      auto form = [&]() -> bool {
-        __half2 most = __floats2half2_rn(0.0f, 0.0f);
-        float most32 = 0.0f;
-#pragma unroll
-        for (int j = 0; j < C; j += 8) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(base + j + i);
-            const float2 y0 = __ffma2_rn(make_float2(s[j + i], s[j + i + 1]), f2, make_float2(b.x, b.y));
-            const float2 y1 = __ffma2_rn(make_float2(s[j + i + 2], s[j + i + 3]), f2, make_float2(b.z, b.w));
-            s[j + i] = ex2(y0.x), s[j + i + 1] = ex2(y0.y), s[j + i + 2] = ex2(y1.x), s[j + i + 3] = ex2(y1.y);
-          }
-          if (kind == kStepPage) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const __half2 pair = __floats2half2_rn(s[j + 2 * i], s[j + 2 * i + 1]);
-              most = __hmax2(most, pair);
-              w[i] = h2(pair);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              most32 = fmaxf(most32, fmaxf(s[j + 2 * i], s[j + 2 * i + 1]));
-              w[i] = pack_bf16x2(s[j + 2 * i] * p.inverse_value_scale, s[j + 2 * i + 1] * p.inverse_value_scale);
-            }
-          }
-          *reinterpret_cast<uint4*>(p_row + (((p_chunk + (j >> 3)) ^ p_swizzle) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        tc::fence_before_sync();
-        tc::fence_proxy_async_smem();
-        return fmaxf(most32, __half2float(__hmax(__low2half(most), __high2half(most)))) > kHighest;
-      };
-      load();
-      if (bar_any(barrier, form())) {
-        load();
+      // Maxima are taken in a unit's first step, in one that could be the first with anything to see (a tail may
+      // hold nothing but sink), and when a score exceeds its query's by too much.
+      const bool forced = step == u.begin || (kind == kStepDraft && u.info.pages == 0);
+      if (bar_any(barrier, forced || highest > kShift + kGrowth)) {
         float mine = 0.0f;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-          const float m = warp_max(s[j] * f);
+          const float m = warp_max(s[j]);
           if (lane == j) mine = m;
         }
         if (lane < C) sm.col_max[warp][first_column + lane] = mine;
         bar_sync(barrier, 128);
         if (t < C) {
           const int col = first_column + t;
-          const float before = top[t];
+          const float before = top[t], was = base[t];
           const float now = fmaxf(fmaxf(fmaxf(sm.col_max[0][col], sm.col_max[1][col]),
-                                        fmaxf(sm.col_max[2][col], sm.col_max[3][col])), before);
+                                        fmaxf(sm.col_max[2][col], sm.col_max[3][col])) - was, before);
+          const float is = now == kNoMax ? 0.0f : kShift - now;
           top[t] = now;
-          base[t] = kShift - now;
+          base[t] = is;
+          sm.shift[col] = is - was;
           sm.factor[col] = ex2(before - now);
         }
         bar_sync(barrier, 128);
 #pragma unroll
         for (int j = 0; j < C / 2; ++j) {
+          s[2 * j] += sm.shift[first_column + 2 * j];
+          s[2 * j + 1] += sm.shift[first_column + 2 * j + 1];
           sum[j].x *= sm.factor[first_column + 2 * j];
           sum[j].y *= sm.factor[first_column + 2 * j + 1];
         }
-        form();
         if (step > u.begin) {  // what O^T holds is of the old maxima
 #pragma unroll 1
           for (int j = 0; j < C; j += 8) {
@@ -836,15 +831,31 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
             for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(o[i] * sm.factor[first_column + j + i]);
             st8(column, w);
           }
-          tc::tmem_wait_st();
-          tc::fence_before_sync();
         }
-        bar_sync(barrier, 128);
       }
-      // the half's barrier stands behind every thread's scores read, values and probabilities written
-      if (t == 0) tc::mbar_arrive(&sm.p_full);
+#pragma unroll
+      for (int j = 0; j < C; j += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[j + i] = ex2(s[j + i]);
+        if (kind == kStepPage) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = h2(__floats2half2_rn(s[j + 2 * i], s[j + 2 * i + 1]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = pack_bf16x2(s[j + 2 * i] * p.inverse_value_scale, s[j + 2 * i + 1] * p.inverse_value_scale);
+        }
+        *reinterpret_cast<uint4*>(p_row + (((p_chunk + (j >> 3)) ^ p_swizzle) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      tc::tmem_wait_st();
+      tc::fence_before_sync();
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sm.p_full);
 #pragma unroll
       for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
+      f = next_f;
       parity ^= 1;
       any = true;
     }
@@ -911,7 +922,8 @@ template <int NT, int PT>
 __global__ void __launch_bounds__(kThreads, 2)
 tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const TreeParams p) {
   extern __shared__ uint8_t raw_smem[];
-  Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  // (an offset, not a masked pointer: the compiler has to see that this is shared memory)
+  Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(raw_smem + (-tc::smem_u32(raw_smem) & 1023u));
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
   dependents_may_launch();
 
@@ -932,7 +944,7 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
     tc::mbar_init(&sm.k_full, 8);
     tc::mbar_init(&sm.s_full, 1);
-    tc::mbar_init(&sm.p_full, 2);
+    tc::mbar_init(&sm.p_full, 8);
     tc::mbar_init(&sm.o_full, 1);
     tc::mbar_init(&sm.drained, 1);
     tc::fence_barrier_init();
