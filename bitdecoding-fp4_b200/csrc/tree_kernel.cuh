@@ -684,6 +684,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
                        (PT == 128 ? (t & 31) * 16 + (t >> 5) * 4 : (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4);
   const int v_codes = kVOffset + (PT == 128 ? t * 64 : half * 4096 + t * 32);
   const int v_scales = kVsOffset + half * 512 + (t & 31) * 16 + (t >> 5) * 4;
+  const int v_chunk0 = PT == 128 ? ((2 * half) ^ k_swizzle) * 16 : ((t >> 2) & 1) * 16;  // the other one's is 16 off
   uint8_t* const p_row = sm.p + t * 128;
   const int p_chunk = first_column >> 3, p_swizzle = t & 7;
   Place k_at, v_at;  // a page's stage serves both; of a BF16 step each passes over the other's
@@ -721,11 +722,11 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
       if (kind == kStepPage) {
         wait(&sm.full[k_at.slot], k_at.turn, &sm.abort_flag);
         const uint8_t* stage = sm.ring[k_at.slot];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          store_dequantized(k_operand + 32 * half + 16 * j,
-                            *reinterpret_cast<const uint4*>(stage + k_codes + (((2 * half + j) ^ k_swizzle) * 16)),
-                            *reinterpret_cast<const uint16_t*>(stage + k_scales + 2 * j));
+        const uint32_t scale = *reinterpret_cast<const uint32_t*>(stage + k_scales);
+        const uint4 chunk0 = *reinterpret_cast<const uint4*>(stage + k_codes + (((2 * half) ^ k_swizzle) * 16));
+        const uint4 chunk1 = *reinterpret_cast<const uint4*>(stage + k_codes + (((2 * half + 1) ^ k_swizzle) * 16));
+        store_dequantized(k_operand + 32 * half, chunk0, scale);
+        store_dequantized(k_operand + 32 * half + 16, chunk1, scale >> 16);
         k_at.advance();
       } else {
         f = p.scale_log2 * q_inverse * bf16_keys<NT>(p, sm, u, kind, k_at, k_operand, thread);
@@ -778,12 +779,11 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
       tc::fence_after_sync();
       if (kind == kStepPage) {
         const uint8_t* stage = sm.ring[v_at.slot];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          store_dequantized(v_operand + 32 * half + 16 * j,
-                            *reinterpret_cast<const uint4*>(
-                                stage + v_codes + (PT == 128 ? ((2 * half + j) ^ k_swizzle) * 16 : (j ^ ((t >> 2) & 1)) * 16)),
-                            *reinterpret_cast<const uint16_t*>(stage + v_scales + 2 * j));
+        const uint32_t scale = *reinterpret_cast<const uint32_t*>(stage + v_scales);
+        const uint4 chunk0 = *reinterpret_cast<const uint4*>(stage + v_codes + v_chunk0);
+        const uint4 chunk1 = *reinterpret_cast<const uint4*>(stage + v_codes + (v_chunk0 ^ 16));
+        store_dequantized(v_operand + 32 * half, chunk0, scale);
+        store_dequantized(v_operand + 32 * half + 16, chunk1, scale >> 16);
         release(sm, v_at, lane);
       } else {
         bf16_values<NT>(sm, u, kind, v_at, v_operand, thread);
