@@ -57,32 +57,36 @@ constexpr int kWorkers = 256;              // two halves of 128
 constexpr int kThreads = kWorkers + 64;    // and a warp each for copies and products
 constexpr int kStages = 4;                 // as many as two CTAs' shared memory holds
 constexpr int kTmemColumns = 256;          // half of what an SM has
+constexpr int kTerms = 4;                  // FP4 terms of a query
 
 template <int NT>
 struct Shape {
   static constexpr int kColumns = NT / 2;  // queries per thread
   // tensor memory columns
-  static constexpr int kS = 0, kO = NT, kK = 2 * NT, kV = kK + 64;
-  static_assert(kV + 64 <= kTmemColumns, "tensor memory");
+  // (the keys of a BF16 step lie where a page's product had its scales: pages come first in a unit)
+  static constexpr int kS = 0, kO = NT, kV = 2 * NT, kK = kV + 64, kKs = kK, kQs = kKs + 8;
+  static_assert(kK + 64 <= kTmemColumns && kQs + 8 * kTerms <= kTmemColumns, "tensor memory");
+  // shared memory of the queries: FP4 terms (codes, then two scale atoms each) for the pages, then FP16
+  static constexpr int kTermCodes = NT * 64, kQueries = NT * 256 + kTerms * 1024;
 };
 
 template <int NT>
 struct Smem {
   using Sh = Shape<NT>;
   alignas(1024) uint8_t ring[kStages][kStage];
-  alignas(1024) uint8_t q[2][NT * 128];  // two halves of 64 channels, K-major, 128-byte swizzle
+  // The queries. Against pages, kTerms tiles of FP4 codes (K-major, 64-byte swizzle), then as many pairs of scale
+  // atoms; against BF16 steps, FP16 in two halves of 64 channels (K-major, 128-byte swizzle).
+  alignas(1024) uint8_t q[Sh::kQueries];
   alignas(1024) uint8_t p[16384];        // MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum, 0 while there is none
   float top[NT];        // maximum, log2 units
-  float factor[NT], shift[NT];  // what a renewal does to sums and scores
-  float total[NT];
-  float col_max[4][NT];
-  float col_sum[4][NT];
+  float factor[NT], shift[NT];  // what a renewal does to sums and scores (at a unit's end: 1 / weight)
+  float col[4][NT];             // a warp's maxima, then sums
   float q_max[8];
   int parents[BDFP4_MAX_TREE_NODES];
   uint64_t full[kStages], empty[kStages];
-  uint64_t k_full, s_full, p_full, o_full, drained;
+  uint64_t s_ready, s_full, p_full, o_full, drained;  // s_ready: the scores before are read, BF16 keys in their operand
   long long sums[kThreads / 32];
   int start_row;
   long long start_offset, first, last, per_cta;
@@ -175,14 +179,15 @@ __device__ __forceinline__ void scale_pairs(uint32_t bytes, __half2* out) {
   out[1] = __high2half2(pair);
 }
 
-// The power of two that brings `amax` into [2^14, 2^15), and its inverse. Zero, infinite or NaN: 1.
-__device__ __forceinline__ float fp16_scale(float amax, float* inverse) {
+// The power of two that brings `amax` into [2^TO, 2^(TO + 1)), and its inverse. Zero, infinite or NaN: 1.
+template <int TO>
+__device__ __forceinline__ float scale_to(float amax, float* inverse) {
   const int e = (int)((__float_as_uint(amax) >> 23) & 0xffu);
   if (e == 0 || e == 255) {
     *inverse = 1.0f;
     return 1.0f;
   }
-  const int field = min(127 + 14 + 127 - e, 253);
+  const int field = min(127 + TO + 127 - e, 253);
   *inverse = __uint_as_float((uint32_t)(254 - field) << 23);
   return __uint_as_float((uint32_t)field << 23);
 }
@@ -226,6 +231,9 @@ __device__ __forceinline__ StepKind step_kind(const RowInfo& r, int step) {
 // Token places of a BF16 step: the tail's tokens, or 16 places of the sink and the drafts behind them.
 __device__ __forceinline__ int bf16_places(const RowInfo& r, StepKind kind) {
   return kind == kStepTail ? r.residual : BDFP4_MAX_SINK + r.count;
+}
+__device__ __forceinline__ int bf16_stages(const RowInfo& r, StepKind kind) {  // of each side
+  return (bf16_places(r, kind) + kBf16Rows - 1) / kBf16Rows;
 }
 // 16-token slices of a step that hold anything.
 __device__ __forceinline__ int step_slices(const RowInfo& r, StepKind kind) {
@@ -404,15 +412,33 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walke
   __syncwarp();
 }
 
+// The key scales of two 64-token pages into whole atoms, in place, by one warp.
+__device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
+  uint2 part[2][2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    part[e & 1][e >> 1] = *reinterpret_cast<const uint2*>(scales + (e >> 1) * 512 + (e & 1) * 256 + lane * 8);
+  __syncwarp();
+#pragma unroll
+  for (int atom = 0; atom < 2; ++atom)
+    *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) =
+        make_uint4(part[atom][0].x, part[atom][0].y, part[atom][1].x, part[atom][1].y);
+  tc::fence_proxy_async_smem();
+  __syncwarp();
+}
+
 // The whole warp walks and waits; one thread of it issues.
-template <int NT>
-__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
+template <int NT, int PT>
+__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
   using Sh = Shape<NT>;
-  constexpr uint32_t kScores = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
+  constexpr uint32_t kFp4 = tc::nvf4_idesc(128, NT), kF16 = f16_idesc(NT, 0, false);
+  constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-  const uint32_t q = tc::smem_u32(sm.q);
+  const uint32_t q = tc::smem_u32(sm.q), ring = tc::smem_u32(sm.ring);
+  const uint64_t q_codes = tc::fp4_tile_desc(q, 0), q_scales = tc::sf_atom_desc(q + kTerms * Sh::kTermCodes);
   const uint64_t tile = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
   uint32_t k_parity = 0, p_parity = 0;
+  Place at;
   Unit u;
   bool known = false;
 #pragma unroll 1
@@ -421,16 +447,46 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
 #pragma unroll 1
     for (int step = u.begin; step <= u.end; ++step) {
       if (step < u.end) {
-        wait(&sm.k_full, k_parity, &sm.abort_flag);
+        const StepKind kind = step_kind(u.info, step);
+        wait(&sm.s_ready, k_parity, &sm.abort_flag);
         k_parity ^= 1;
-        tc::fence_after_sync();
-        if (elect_one()) {
+        if (kind == kStepPage) {
+          wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+          if constexpr (PT == 64) interleave_scales(sm.ring[at.slot] + kKsOffset, lane);
+          tc::fence_after_sync();
+          const uint32_t stage = ring + at.slot * kStage;
+          const uint64_t codes = tc::fp4_tile_desc(stage, 0), atoms = tc::sf_atom_desc(stage + kKsOffset);
+          if (elect_one()) {
+            if (step == u.begin) {
+#pragma unroll 1
+              for (int i = 0; i < 2 * kTerms; ++i) tc::cp_sf_atom(tmem + Sh::kQs + i * 4, q_scales + i * 32);
+            }
+            tc::cp_sf_atom(tmem + Sh::kKs, atoms);
+            tc::cp_sf_atom(tmem + Sh::kKs + 4, atoms + 32);
 #pragma unroll
-          for (int s = 0; s < 8; ++s)
-            mma_ts(tmem + Sh::kS, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
-          tc::commit(&sm.s_full);
+            for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
+#pragma unroll
+              for (int term = 0; term < kTerms; ++term)
+                tc::mma_nvf4(tmem + Sh::kS, codes + 2 * s, q_codes + term * (Sh::kTermCodes / 16) + 2 * s, kFp4,
+                             tmem + Sh::kKs + 4 * s, tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
+            }
+            tc::commit(&sm.s_full);
+            tc::commit(&sm.empty[at.slot]);
+          }
+          __syncwarp();
+          at.advance();
+        } else {
+#pragma unroll 1
+          for (int i = 2 * bf16_stages(u.info, kind); i > 0; --i) at.advance();
+          tc::fence_after_sync();
+          if (elect_one()) {
+#pragma unroll 1
+            for (int s = 0; s < 8; ++s)
+              mma_ts(tmem + Sh::kS, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kF16, s > 0);
+            tc::commit(&sm.s_full);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
       if (step == u.begin) continue;
       wait(&sm.p_full, p_parity, &sm.abort_flag);  // P, and before it V
@@ -472,57 +528,92 @@ __device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint3
   st16(a, v);
 }
 
-// The tile's queries into shared memory: rotated if asked, scaled by one power of two into FP16's range
-// (rows of the tile whose largest value is 2^-29 of the tile's keep full precision). Returns what undoes it.
+// A group of a query: zero outside the tile; rotated if asked.
 template <int NT>
-__device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
-  constexpr int kPerPass = kWorkers / 8, kPasses = (NT + kPerPass - 1) / kPerPass;
-  const int group = thread & 7;
-  const int queries = min(u.info.count * p.ratio - u.tile * NT, NT);
-  float v[kPasses][16];
+__device__ __forceinline__ void load_query16(const TreeParams& p, const Unit& u, int r, int group, float* v) {
+  const int queries = min(u.info.count * p.ratio - u.tile * NT, NT), query = u.tile * NT + r;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+  if (r < queries)
+    load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
+                     (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v);
+  if (p.rotate) {
+    hadamard_butterflies(v, group);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] *= kInvSqrt128;
+  }
+}
+
+// The power of two that the tile's queries are scaled with: a query whose largest value is 2^-8 of the tile's
+// still has all four terms above E4M3's smallest scale.
+template <int NT>
+__device__ __forceinline__ float query_scale(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread, float* inverse) {
   float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int r = i * kPerPass + (thread >> 3), query = u.tile * NT + r;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[i][j] = 0.0f;
-    if (r < queries)
-      load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
-                       (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
-  }
-  if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    if (p.rotate) {
-      hadamard_butterflies(v[i], group);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[i][j] *= kInvSqrt128;
-    }
+  for (int r = thread >> 3; r < (NT < kWorkers / 8 ? kWorkers / 8 : NT); r += kWorkers / 8) {
+    float v[16];
+    load_query16<NT>(p, u, r, thread & 7, v);
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (fabsf(v[i][j]) < INFINITY) amax = fmaxf(amax, fabsf(v[i][j]));
+      if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
   }
+  if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
   amax = warp_max(amax);
   if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
   bar_sync(kWorkBarrier, kWorkers);
 #pragma unroll
   for (int w = 0; w < kWorkers / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
-  float inverse;
-  const float scale = fp16_scale(amax, &inverse);
+  return scale_to<10>(amax, inverse);
+}
+
+// The tile's queries into shared memory, by eight threads each: as FP4 terms for pages, as FP16 for BF16 steps.
+template <int NT>
+__device__ __forceinline__ void load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread, float scale, bool terms) {
+  using Sh = Shape<NT>;
+  const int group = thread & 7;
+#pragma unroll 1
+  for (int r = thread >> 3; r < (NT < kWorkers / 8 ? kWorkers / 8 : NT); r += kWorkers / 8) {
+    float v[16];
+    load_query16<NT>(p, u, r, group, v);
+    if (r >= NT) continue;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int r = i * kPerPass + (thread >> 3);
-    if (kPasses * kPerPass > NT && r >= NT) break;
-    uint8_t* row = sm.q[group >> 2] + r * 128;
-    uint32_t w[8];
+    for (int j = 0; j < 16; ++j) v[j] *= scale;
+    if (terms) {
+      const int at = r * 64 + group * 8;
+#pragma unroll 1
+      for (int term = 0; term < kTerms; ++term) {
+        float largest = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[i][2 * j] * scale, v[i][2 * j + 1] * scale));
-    const int chunk = (group & 3) * 2;
-    *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+        for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(v[j]));
+        const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
+        GroupCodes codes;
+        codes.scale = e4m3_to_float(byte);
+        // (an approximate reciprocal: what it rounds otherwise is left to the next term)
+        float inverse_scale;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse_scale) : "f"(fmaxf(codes.scale, 1.0e-30f)));
+        float scaled[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) scaled[j] = v[j] * inverse_scale;
+        codes.lo = pack_e2m1x8(scaled);
+        codes.hi = pack_e2m1x8(scaled + 8);
+        *reinterpret_cast<uint2*>(sm.q + term * Sh::kTermCodes + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
+        sm.q[kTerms * Sh::kTermCodes + term * 1024 + scale_tile_offset(r, group)] = (uint8_t)byte;
+        float rest[16];
+        group_residual16(v, codes, rest);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = rest[j];
+      }
+    } else {
+      uint8_t* row = sm.q + (group >> 2) * NT * 128 + r * 128;
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
+      const int chunk = (group & 3) * 2;
+      *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
   }
   tc::fence_proxy_async_smem();
-  return inverse;
 }
 
 // Sums of N per-lane columns over the warp: every exchange halves what a lane holds, until it holds N / 32 (at
@@ -547,20 +638,22 @@ __device__ __forceinline__ void reduce_columns(float* v, int lane, int column, S
   }
 }
 
-// One stage's release, by a whole warp.
+// One stage's release, by a whole warp. A page's stage waits for its score product too; for a BF16 step's one
+// warp arrives in its place.
 template <int NT>
-__device__ __forceinline__ void release(Smem<NT>& sm, Place& at, int lane) {
+__device__ __forceinline__ void release(Smem<NT>& sm, Place& at, int thread, bool bf16) {
   __syncwarp();
-  if (lane == 0) tc::mbar_arrive(&sm.empty[at.slot]);
+  if ((thread & 31) == 0) tc::mbar_arrive(&sm.empty[at.slot]);
+  if (bf16 && thread == 0) tc::mbar_arrive(&sm.empty[at.slot]);
   at.advance();
 }
 
 // The keys of a BF16 step: thread r of either half brings its half of token r's channels. Returns what undoes
 // the token's scaling.
 template <int NT>
-__device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem<NT>& sm, const Unit& u, StepKind kind, Place& at,
+__device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem<NT>& sm, const Unit& u, StepKind kind, Place at,
                                         uint32_t operand, int thread) {
-  const int r = thread & 127, half = thread >> 7, lane = thread & 31;
+  const int r = thread & 127, half = thread >> 7;
   const int places = bf16_places(u.info, kind);
   const bool two = places > kBf16Rows;
   // a step's stages are held together
@@ -613,7 +706,7 @@ __device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem<NT>& sm, co
     }
   }
   float inverse;
-  const float scale = fp16_scale(amax, &inverse);
+  const float scale = scale_to<14>(amax, &inverse);
 #pragma unroll 1
   for (int quarter = 2 * half; quarter < 2 * half + 2; ++quarter) {
     uint32_t v[16];
@@ -628,17 +721,15 @@ __device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem<NT>& sm, co
     }
     st16(operand + quarter * 16, v);
   }
-  release(sm, at, lane);
-  if (two) release(sm, at, lane);
-  at.advance();  // the values'
-  if (two) at.advance();
+  release(sm, at, thread, true);
+  if (two) release(sm, at, thread, true);
   return inverse;
 }
 
 // The values of a BF16 step: half h brings the tokens of the step's stage h into channel r's lane.
 template <int NT>
 __device__ __forceinline__ void bf16_values(Smem<NT>& sm, const Unit& u, StepKind kind, Place& at, uint32_t operand, int thread) {
-  const int c = thread & 127, half = thread >> 7, lane = thread & 31;
+  const int c = thread & 127, half = thread >> 7;
   const int places = bf16_places(u.info, kind);
   at.advance();  // the keys'
   if (places > kBf16Rows) at.advance();
@@ -663,7 +754,7 @@ __device__ __forceinline__ void bf16_values(Smem<NT>& sm, const Unit& u, StepKin
         st8(operand + (place >> 4) * 8, v);
       }
     }
-    release(sm, at, lane);
+    release(sm, at, thread, true);
   }
 }
 
@@ -678,23 +769,23 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
   const uint32_t scores = lanes + Sh::kS + first_column, k_operand = lanes + Sh::kK, v_operand = lanes + Sh::kV;
   float* base = sm.base + first_column;
   float* top = sm.top + first_column;
-  // where this thread's codes and scales lie in a stage: half of token t's channels, half of channel t's tokens
-  const int k_codes = t * 64, k_swizzle = (t >> 1) & 3;
-  const int k_scales = kKsOffset + half * (PT == 128 ? 512 : 256) +
-                       (PT == 128 ? (t & 31) * 16 + (t >> 5) * 4 : (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4);
+  // where this thread's codes and scales lie in a stage: half of channel t's tokens
+  const int v_swizzle = (t >> 1) & 3;
   const int v_codes = kVOffset + (PT == 128 ? t * 64 : half * 4096 + t * 32);
   const int v_scales = kVsOffset + half * 512 + (t & 31) * 16 + (t >> 5) * 4;
-  const int v_chunk0 = PT == 128 ? ((2 * half) ^ k_swizzle) * 16 : ((t >> 2) & 1) * 16;  // the other one's is 16 off
+  const int v_chunk0 = PT == 128 ? ((2 * half) ^ v_swizzle) * 16 : ((t >> 2) & 1) * 16;  // the other one's is 16 off
   uint8_t* const p_row = sm.p + t * 128;
   const int p_chunk = first_column >> 3, p_swizzle = t & 7;
-  Place k_at, v_at;  // a page's stage serves both; of a BF16 step each passes over the other's
+  Place v_at;
   uint32_t parity = 0;
   bool any = false;  // a step has been taken
   Unit u;
   bool known = false;
 #pragma unroll 1
   for (; walker.next(u, known); known = true) {
-    const float q_inverse = load_queries<NT>(p, sm, u, thread);
+    float q_inverse;
+    const float q_scale = query_scale<NT>(p, sm, u, thread, &q_inverse);
+    if (u.begin < u.info.pages) load_queries<NT>(p, sm, u, thread, q_scale, true);
     if (t < C) {
       top[t] = kNoMax;
       base[t] = 0.0f;  // scores as they are
@@ -714,30 +805,23 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
     bar_sync(barrier, 128);
     const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
-    // Keys of a step into their operand, which the scores of the step before must have left. Returns what turns
-    // its scores into log2 units.
-    auto bring_keys = [&](int step) -> float {
+    // Lets the scores of a step be taken: those of the step before are in registers. `keys`: where a BF16 step's
+    // keys are; they go into their operand first, and before a unit's first such step the queries change their
+    // form. Returns what turns the step's scores into log2 units.
+    auto let_scores = [&](int step, Place keys) -> float {
       const StepKind kind = step_kind(u.info, step);
       float f = page_factor;
-      if (kind == kStepPage) {
-        wait(&sm.full[k_at.slot], k_at.turn, &sm.abort_flag);
-        const uint8_t* stage = sm.ring[k_at.slot];
-        const uint32_t scale = *reinterpret_cast<const uint32_t*>(stage + k_scales);
-        const uint4 chunk0 = *reinterpret_cast<const uint4*>(stage + k_codes + (((2 * half) ^ k_swizzle) * 16));
-        const uint4 chunk1 = *reinterpret_cast<const uint4*>(stage + k_codes + (((2 * half + 1) ^ k_swizzle) * 16));
-        store_dequantized(k_operand + 32 * half, chunk0, scale);
-        store_dequantized(k_operand + 32 * half + 16, chunk1, scale >> 16);
-        k_at.advance();
-      } else {
-        f = p.scale_log2 * q_inverse * bf16_keys<NT>(p, sm, u, kind, k_at, k_operand, thread);
+      if (kind != kStepPage) {
+        if (step == max(u.begin, u.info.pages)) load_queries<NT>(p, sm, u, thread, q_scale, false);
+        f = p.scale_log2 * q_inverse * bf16_keys<NT>(p, sm, u, kind, keys, k_operand, thread);
+        tc::tmem_wait_st();
       }
-      tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.k_full);
+      if (lane == 0) tc::mbar_arrive(&sm.s_ready);
       return f;
     };
-    float f = bring_keys(u.begin);
+    float f = let_scores(u.begin, v_at);
 #pragma unroll 1
     for (int step = u.begin; step < u.end; ++step) {
       const StepKind kind = step_kind(u.info, step);
@@ -770,21 +854,26 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
         s[j] = y0.x, s[j + 1] = y0.y, s[j + 2] = y1.x, s[j + 3] = y1.y;
         highest = fmaxf(fmaxf(highest, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
       }
-      tc::fence_before_sync();
       // the next step's scores are taken while this one's probabilities are formed
       float next_f = f;
-      if (step + 1 < u.end) next_f = bring_keys(step + 1);
+      if (step + 1 < u.end) {
+        Place keys = v_at;
+#pragma unroll 1
+        for (int i = kind == kStepPage ? 1 : 2 * bf16_stages(u.info, kind); i > 0; --i) keys.advance();
+        next_f = let_scores(step + 1, keys);
+      }
       // V, once the product of the step before is done with its operand, P and (for a rescaling) the output
       if (any) wait(&sm.o_full, parity ^ 1, &sm.abort_flag);
       tc::fence_after_sync();
       if (kind == kStepPage) {
+        wait(&sm.full[v_at.slot], v_at.turn, &sm.abort_flag);
         const uint8_t* stage = sm.ring[v_at.slot];
         const uint32_t scale = *reinterpret_cast<const uint32_t*>(stage + v_scales);
         const uint4 chunk0 = *reinterpret_cast<const uint4*>(stage + v_codes + v_chunk0);
         const uint4 chunk1 = *reinterpret_cast<const uint4*>(stage + v_codes + (v_chunk0 ^ 16));
         store_dequantized(v_operand + 32 * half, chunk0, scale);
         store_dequantized(v_operand + 32 * half + 16, chunk1, scale >> 16);
-        release(sm, v_at, lane);
+        release(sm, v_at, thread, false);
       } else {
         bf16_values<NT>(sm, u, kind, v_at, v_operand, thread);
       }
@@ -798,13 +887,13 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
           const float m = warp_max(s[j]);
           if (lane == j) mine = m;
         }
-        if (lane < C) sm.col_max[warp][first_column + lane] = mine;
+        if (lane < C) sm.col[warp][first_column + lane] = mine;
         bar_sync(barrier, 128);
         if (t < C) {
           const int col = first_column + t;
           const float before = top[t], was = base[t];
-          const float now = fmaxf(fmaxf(fmaxf(sm.col_max[0][col], sm.col_max[1][col]),
-                                        fmaxf(sm.col_max[2][col], sm.col_max[3][col])) - was, before);
+          const float now = fmaxf(fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]),
+                                        fmaxf(sm.col[2][col], sm.col[3][col])) - was, before);
           const float is = now == kNoMax ? 0.0f : kShift - now;
           top[t] = now;
           base[t] = is;
@@ -864,7 +953,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
       float v[C];
 #pragma unroll
       for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
-      reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col_sum[warp][first_column + j] = total; });
+      reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col[warp][first_column + j] = total; });
     }
     bar_sync(barrier, 128);
     const bool whole = u.begin == 0 && u.end == u.info.steps;
@@ -872,9 +961,9 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
     if (t < C) {
       const int col = first_column + t;
-      const float total = (sm.col_sum[0][col] + sm.col_sum[1][col]) + (sm.col_sum[2][col] + sm.col_sum[3][col]);
+      const float total = (sm.col[0][col] + sm.col[1][col]) + (sm.col[2][col] + sm.col[3][col]);
       if (whole) {
-        sm.total[col] = total > 0.0f ? p.value_scale / total : 0.0f;
+        sm.factor[col] = total > 0.0f ? p.value_scale / total : 0.0f;
       } else {
         p.partial_stat[(int64_t)(2 * part) * NT + col] = top[t];
         p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
@@ -897,7 +986,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
       for (int i = 0; i < 8; ++i) {
         if (j + i < queries) {
           if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[first_column + j + i]);
+            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.factor[first_column + j + i]);
             if (++out_head == p.ratio) out_head = 0, ++out_node;
           } else {
             partial[(int64_t)(j + i) * kHeadDim] = o[i];
@@ -940,9 +1029,9 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) {
       tc::mbar_init(&sm.full[i], 1);
-      tc::mbar_init(&sm.empty[i], 8);
+      tc::mbar_init(&sm.empty[i], 9);  // the workers' warps and the score product
     }
-    tc::mbar_init(&sm.k_full, 8);
+    tc::mbar_init(&sm.s_ready, 8);
     tc::mbar_init(&sm.s_full, 1);
     tc::mbar_init(&sm.p_full, 8);
     tc::mbar_init(&sm.o_full, 1);
@@ -999,7 +1088,7 @@ tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
     if (warp < kWorkers / 32) work<NT, PT>(p, sm, walker, thread);
     else if (warp == kWorkers / 32) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
-    else issue<NT>(sm, walker);
+    else issue<NT, PT>(sm, walker, lane);
   }
   tc::fence_before_sync();
   __syncthreads();
