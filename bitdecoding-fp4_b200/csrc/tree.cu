@@ -1,5 +1,6 @@
 // C ABI of the tree attention: argument checks, the tile and its instantiation (tree_p128.cu, tree_p64.cu),
-// and the kernel that adds the parts of units that straddle CTAs. The attention itself is tree_kernel.cuh.
+// and the kernel that adds the parts of units that straddle CTAs. The attention itself is
+// tree_narrow.cuh and tree_wide.cuh.
 #include <cmath>
 
 #include "common.cuh"
@@ -15,10 +16,12 @@ namespace bdfp4 {
 static int tree_tile(int queries) {
   const int tiles = (queries + kTreeMaxTile - 1) / kTreeMaxTile;
   const int each = (queries + tiles - 1) / tiles;
-  for (int tile : {16, 32})
+  for (int tile : {16, 32, 64, 96})
     if (each <= tile) return tile;
   return kTreeMaxTile;
 }
+
+static int tree_ctas(int tile) { return tile <= kTreeNarrowTile ? kTreeNarrowCtas : kTreeWideCtas; }
 
 // One block per (CTA that a straddling unit begins in, eight query rows): thread c adds channel c of the
 // unit's parts, each weighted by 2^(its maximum - the largest).
@@ -73,7 +76,7 @@ static cudaError_t launch_merge(const TreeParams& p, cudaStream_t stream) {
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(kTreeCtas, (p.tile + kMergeRows - 1) / kMergeRows);
+  config.gridDim = dim3(p.ctas, (p.tile + kMergeRows - 1) / kMergeRows);
   config.blockDim = dim3(128);
   config.stream = stream;
   config.attrs = &attribute;
@@ -88,7 +91,7 @@ using namespace bdfp4;
 extern "C" int64_t bdfp4_tree_workspace_bytes(int32_t rows, int32_t nodes, int32_t heads_q, int32_t heads_kv) {
   if (rows < 1 || nodes < 1 || nodes > BDFP4_MAX_TREE_NODES || heads_kv < 1 || heads_q < 1 || heads_q % heads_kv) return 0;
   const int64_t tile = tree_tile(nodes * (heads_q / heads_kv));
-  return (int64_t)kTreeCtas * (2 * tile * (kHeadDim + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(TreeSplit));
+  return (int64_t)tree_ctas((int)tile) * (2 * tile * (kHeadDim + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(TreeSplit));
 }
 
 extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) {
@@ -176,9 +179,10 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
   p.out_node = a->out_node_stride;
   p.error_word = a->error_word;
   p.tile = tree_tile(a->nodes * p.ratio);
+  p.ctas = tree_ctas(p.tile);
   p.partial = static_cast<float*>(a->workspace);
-  p.partial_stat = p.partial + (int64_t)2 * kTreeCtas * p.tile * kHeadDim;
-  p.splits = reinterpret_cast<TreeSplit*>(p.partial_stat + (int64_t)4 * kTreeCtas * p.tile);
+  p.partial_stat = p.partial + (int64_t)2 * p.ctas * p.tile * kHeadDim;
+  p.splits = reinterpret_cast<TreeSplit*>(p.partial_stat + (int64_t)4 * p.ctas * p.tile);
   CUtensorMap k_map{}, v_map{};
   if (page_tokens == 128 && !cache_tensor_maps(a->key_codes, a->value_codes, a->heads_kv, page_tokens, a->pages,
                                                a->key_codes_pitch, a->value_codes_pitch, &k_map, &v_map))

@@ -1,1122 +1,20 @@
-// Attention of a tree of drafted tokens over the paged NVFP4 cache, on the tensor cores.
-//
-// Per (row, KV head) the queries are one matrix of nodes x ratio rows, cut into tiles of NT. Against 128
-// tokens at a time,
-//     S^T [token, query]   = K   [token, channel]  * Q^T
-//     O^T [channel, query] = V^T [channel, token] * P^T
-// both as tcgen05.mma.kind::f16 with the cache operand A in tensor memory and the query-side operand B in
-// shared memory. E2M1 x E4M3 has at most six significant bits and lies in [2^-10, 2688], so a page's values
-// are exact in FP16: a thread reads its own token's (K) or channel's (V) code bytes, converts and scales
-// them in registers and stores them straight into its tensor-memory lane; the dequantized tile never passes
-// through shared memory. P is stored as the softmax threads hold it, one token per thread with its queries
-// contiguous, which is the MN-major form of B.
-//
-// Two CTAs share an SM, and within a CTA the same eight warps convert K, convert V and take the softmax, one
-// after the other; only the copies and the products have warps of their own. What one CTA waits for (a product,
-// a barrier, tensor memory) the other fills. Warps of one role each (keys, values, softmax, side by side on
-// every scheduler) were built first: they waited for instructions a third of the time, since the sum of their
-// loops is larger than a scheduler's instruction cache.
-//
-// Thread r (of 128, twice: each half has half of the channels, tokens or queries) owns token r of S^T. Maxima
-// are per query, in shared memory, and lazy: probabilities are formed against them at once, and only when one
-// comes out more than 2^8 above its maximum (the barrier that ends a step carries that vote) are the maxima
-// taken anew, O^T rescaled and the step formed again. Sums stay per thread until the unit ends. Probabilities
-// carry a factor 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
-//
-// The rolling tail and the drafts with the sink are two more steps of the same form over BF16 values: K is
-// scaled per token by a power of two into FP16's range (the softmax thread of the token undoes it), V and
-// P are BF16. Queries are scaled per tile the same way.
-//
-// Work is the sequence of all steps of all (row, head, tile) units, cut into equal runs, one per CTA, so any
-// mix of lengths is balanced; a unit that straddles CTAs leaves unnormalised parts that a second kernel adds.
+// Launch by tile: the instantiations of one page size.
 #pragma once
 
-#include <cuda_fp16.h>
-
-#include "common.cuh"
-#include "host.h"
-#include "key_basis.cuh"
-#include "tcgen05.cuh"
-#include "tree_params.h"
+#include "tree_narrow.cuh"
+#include "tree_wide.cuh"
 
 namespace bdfp4 {
 namespace tree {
 
-constexpr int kStage = 18432;  // K codes 8192, V codes 8192, K scales 1024, V scales 1024
-constexpr int kVOffset = 8192, kKsOffset = 16384, kVsOffset = 17408;
-// A BF16 step (tail, or sink and drafts) takes one stage per 64 tokens for K, then as many for V; a token's
-// 256 bytes lie 272 apart, so that eight rows' 16-byte chunks fall on distinct banks.
-constexpr int kBf16Pitch = 272, kBf16Rows = 64;
-// Named barriers: one per half, and all eight working warps.
-constexpr int kHalfBarrier = 1, kWorkBarrier = 3;
-constexpr float kNoMax = -3.0e38f;  // a query that has seen no token yet
-constexpr float kShift = 7.0f;      // probabilities carry 2^7
-constexpr float kGrowth = 8.0f;     // a maximum is renewed when a score exceeds it by more than this (log2)
-
-constexpr int kWorkers = 256;              // two halves of 128
-constexpr int kThreads = kWorkers + 64;    // and a warp each for copies and products
-constexpr int kStages = 4;                 // as many as two CTAs' shared memory holds
-constexpr int kTmemColumns = 256;          // half of what an SM has
-constexpr int kTerms = 4;                  // FP4 terms of a query
-
-template <int NT>
-struct Shape {
-  static constexpr int kColumns = NT / 2;  // queries per thread
-  // tensor memory columns
-  // (the keys of a BF16 step lie where a page's product had its scales: pages come first in a unit)
-  static constexpr int kS = 0, kO = NT, kV = 2 * NT, kK = kV + 64, kKs = kK, kQs = kKs + 8;
-  static_assert(kK + 64 <= kTmemColumns && kQs + 8 * kTerms <= kTmemColumns, "tensor memory");
-  // shared memory of the queries: FP4 terms (codes, then two scale atoms each) for the pages, then FP16
-  static constexpr int kTermCodes = NT * 64, kQueries = NT * 256 + kTerms * 1024;
-};
-
-template <int NT>
-struct Smem {
-  using Sh = Shape<NT>;
-  alignas(1024) uint8_t ring[kStages][kStage];
-  // The queries. Against pages, kTerms tiles of FP4 codes (K-major, 64-byte swizzle), then as many pairs of scale
-  // atoms; against BF16 steps, FP16 in two halves of 64 channels (K-major, 128-byte swizzle).
-  alignas(1024) uint8_t q[Sh::kQueries];
-  alignas(1024) uint8_t p[16384];        // MN-major: 128-byte rows of 64 queries per token, swizzled
-  uint64_t family[NT];  // draft nodes each query sees
-  float base[NT];       // kShift - maximum, 0 while there is none
-  float top[NT];        // maximum, log2 units
-  float factor[NT], shift[NT];  // what a renewal does to sums and scores (at a unit's end: 1 / weight)
-  float col[4][NT];             // a warp's maxima, then sums
-  float q_max[8];
-  int parents[BDFP4_MAX_TREE_NODES];
-  uint64_t full[kStages], empty[kStages];
-  uint64_t s_ready, s_full, p_full, o_full, drained;  // s_ready: the scores before are read, BF16 keys in their operand
-  long long sums[kThreads / 32];
-  int start_row;
-  long long start_offset, first, last, per_cta;
-  uint32_t tmem;
-  int abort_flag, ignored_flag;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float warp_max(float x) {
-  float y;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ void bar_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
-__device__ __forceinline__ bool bar_any(int id, bool pred) {
-  uint32_t out;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(out)
-      : "r"((uint32_t)pred), "r"(id)
-      : "memory");
-  return out != 0;
-}
-
-// kind::f16 with A in tensor memory (lane = row, a 32-bit column = two neighbouring K values).
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
-}
-
-// FP32 accumulate; A K-major; B K-major (queries) or MN-major (probabilities, bit 16); operand format 0 FP16, 1 BF16.
-__host__ __device__ constexpr uint32_t f16_idesc(int n, int format, bool b_mn_major) {
-  return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) | ((b_mn_major ? 1u : 0u) << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-
-__device__ __forceinline__ void st16(uint32_t address, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::
-          "r"(address),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
-}
-
-__device__ __forceinline__ void st8(uint32_t address, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(address), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
-template <int N>
-__device__ __forceinline__ void tmem_load(uint32_t address, float* v) {
-  if constexpr (N == 8) tc::tmem_ld8(address, v);
-#pragma unroll
-  for (int j = 0; j + 16 <= N; j += 16) tc::tmem_ld16(address + j, v + j);
-}
-
-__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-
-// Eight E2M1 codes times one FP16 scale -> eight FP16 values in four words, in code order. Exact.
-__device__ __forceinline__ void dequantize8(uint32_t codes, __half2 scale, uint32_t* out) {
-  uint32_t v[4];
-  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-      : "r"(codes));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = h2(__hmul2(*reinterpret_cast<__half2*>(&v[i]), scale));
-}
-
-// Two E4M3 bytes -> two FP16 pairs (scale, scale).
-__device__ __forceinline__ void scale_pairs(uint32_t bytes, __half2* out) {
-  uint32_t both;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(both) : "r"(bytes));
-  const __half2 pair = *reinterpret_cast<__half2*>(&both);
-  out[0] = __low2half2(pair);
-  out[1] = __high2half2(pair);
-}
-
-// The power of two that brings `amax` into [2^TO, 2^(TO + 1)), and its inverse. Zero, infinite or NaN: 1.
-template <int TO>
-__device__ __forceinline__ float scale_to(float amax, float* inverse) {
-  const int e = (int)((__float_as_uint(amax) >> 23) & 0xffu);
-  if (e == 0 || e == 255) {
-    *inverse = 1.0f;
-    return 1.0f;
-  }
-  const int field = min(127 + TO + 127 - e, 253);
-  *inverse = __uint_as_float((uint32_t)(254 - field) << 23);
-  return __uint_as_float((uint32_t)field << 23);
-}
-
-struct RowInfo {
-  int count, pages, residual, sink, slot;  // pages: 128-token steps in the FP4 cache
-  int steps;                               // of one unit: pages, tail, drafts with sink
-  int tiles;
-};
-
-__device__ __forceinline__ RowInfo row_info(const TreeParams& p, int row, int page_tokens) {
-  RowInfo r;
-  r.count = p.node_counts ? min(max(p.node_counts[row], 0), p.nodes) : p.nodes;
-  const int entries = kPage / page_tokens;
-  r.pages = min(max(p.seqused_fp4[row], 0) / kPage, p.max_pages / entries);
-  r.residual = r.sink = r.slot = 0;
-  if (p.tail_key) {
-    r.slot = p.slot_ids[row];
-    if (r.slot >= 0 && r.slot < p.tail_slots) {
-      r.residual = min(max(p.residual[row], 0), kPage);
-      if (p.sink) r.sink = min(max(p.sink[row], 0), BDFP4_MAX_SINK);
-    } else {
-      r.slot = 0;
-    }
-  }
-  r.steps = r.pages + (r.residual > 0 ? 1 : 0) + 1;
-  r.tiles = (r.count * p.ratio + p.tile - 1) / p.tile;
-  return r;
-}
-
-struct Unit {
-  RowInfo info;
-  int row, head, tile, begin, end;  // steps [begin, end) of the unit are this CTA's
-};
-
-enum StepKind { kStepPage, kStepTail, kStepDraft };
-
-__device__ __forceinline__ StepKind step_kind(const RowInfo& r, int step) {
-  return step < r.pages ? kStepPage : (step == r.pages && r.residual > 0) ? kStepTail : kStepDraft;
-}
-// Token places of a BF16 step: the tail's tokens, or 16 places of the sink and the drafts behind them.
-__device__ __forceinline__ int bf16_places(const RowInfo& r, StepKind kind) {
-  return kind == kStepTail ? r.residual : BDFP4_MAX_SINK + r.count;
-}
-__device__ __forceinline__ int bf16_stages(const RowInfo& r, StepKind kind) {  // of each side
-  return (bf16_places(r, kind) + kBf16Rows - 1) / kBf16Rows;
-}
-// 16-token slices of a step that hold anything.
-__device__ __forceinline__ int step_slices(const RowInfo& r, StepKind kind) {
-  return kind == kStepPage ? 8 : (bf16_places(r, kind) + 15) / 16;
-}
-
-// The units of this CTA in order; every role walks them on its own. Steps are counted in 32 bits within a
-// row (the host refuses larger rows).
-struct Walker {
-  const TreeParams& p;
-  int row, page_tokens, offset, left;
-  __device__ Walker(const TreeParams& params, int start_row, int start_offset, int steps, int pt)
-      : p(params), row(start_row), page_tokens(pt), offset(start_offset), left(steps) {}
-  // `known`: u is a unit of this walk, so its row's lengths need not be read again.
-  __device__ __forceinline__ bool next(Unit& u, bool known) {
-    if (left <= 0) return false;
-    while (true) {
-      if (!known || u.row != row) u.info = row_info(p, row, page_tokens);
-      const int whole = u.info.steps * u.info.tiles * p.heads_kv;
-      if (offset < whole) break;
-      offset -= whole;
-      known = false;
-      if (++row >= p.rows) return false;
-    }
-    const int unit = offset / u.info.steps;
-    u.row = row;
-    u.head = unit / u.info.tiles;
-    u.tile = unit - u.head * u.info.tiles;
-    u.begin = offset - unit * u.info.steps;
-    u.end = min(u.info.steps, u.begin + left);
-    left -= u.end - u.begin;
-    offset += u.end - u.begin;
-    return true;
-  }
-};
-
-// ---- roles -----------------------------------------------------------------------------------------
-
-// Waiting is a dozen instructions, one when the phase is already over. After about two seconds, or once another thread has given
-// up, a wait ends without its phase; the roles go through the rest of their motions and the kernel reports it.
-__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* abort_flag) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 begin, now;\n\t.reg .b32 given_up;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
-      "@p bra OVER;\n\t"
-      "mov.u64 begin, %%globaltimer;\n"
-      "AGAIN:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
-      "@p bra OVER;\n\t"
-      "ld.volatile.shared.b32 given_up, [%2];\n\t"
-      "setp.ne.b32 p, given_up, 0;\n\t"
-      "@p bra OVER;\n\t"
-      "mov.u64 now, %%globaltimer;\n\t"
-      "sub.u64 now, now, begin;\n\t"
-      "setp.lt.u64 p, now, %3;\n\t"
-      "@p bra AGAIN;\n\t"
-      "st.volatile.shared.b32 [%2], 1;\n"
-      "OVER:\n\t}" ::"r"(tc::smem_u32(bar)),
-      "r"(parity), "r"(tc::smem_u32(abort_flag)), "n"(tc::kWaitLimitNs)
-      : "memory");
-}
-
-// One thread of a converged warp. tcgen05.mma takes its descriptors from uniform registers: behind an elected
-// predicate the warp's control flow stays uniform for the compiler, and an MMA issues in 32 (N = 64) to 64
-// cycles (N = 128), its tensor time; behind a test of the lane number it took 140 whatever its size.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t elected;
-  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(elected));
-  return elected != 0;
-}
-
-// A place in the ring of stages; everyone who keeps one visits every stage in order.
-struct Place {
-  int slot = 0;
-  uint32_t turn = 0;
-  __device__ __forceinline__ void advance() {
-    if (++slot == kStages) slot = 0, turn ^= 1;
-  }
-};
-
-template <int NT, int PT>
-__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* k_map,
-                                        const CUtensorMap* v_map, int lane) {
-  constexpr int kEntries = kPage / PT;
-  const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
-  Place at;
-  Unit u;
-  bool known = false;
-#pragma unroll 1
-  for (; walker.next(u, known); known = true) {
-    const int32_t* table = p.table + u.row * p.table_stride;
-    const int stop = min(u.end, u.info.pages);
-#pragma unroll 1
-    for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
-      const int entry = batch * kEntries + lane;
-      int mine = 0;
-      if (entry < stop * kEntries) {
-        mine = table[entry];
-        if (mine < 0 || mine >= p.pages) {
-          if (p.error_word) atomicOr(p.error_word, (int)BDFP4_DEV_BAD_PAGE);
-          mine = 0;
-        }
-      }
-      const int steps = min(32 / kEntries, stop - batch);
-#pragma unroll 1
-      for (int i = 0; i < steps; ++i) {
-        int page[kEntries];
-#pragma unroll
-        for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
-        wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
-        uint64_t* const full = &sm.full[at.slot];
-        if (elect_one()) {
-          uint8_t* stage = sm.ring[at.slot];
-          tc::mbar_expect_tx(full, 18432);
-          if constexpr (PT == 128) {
-            tc::tma_load_4d(stage, k_map, full, 0, u.head, 0, page[0]);
-            tc::bulk_load(stage + kKsOffset, p.scales[0] + page[0] * p.scales_pitch[0] + u.head * 1024, 1024, full);
-            tc::tma_load_3d(stage + kVOffset, v_map, full, 0, u.head * kHeadDim, page[0]);
-            tc::bulk_load(stage + kVsOffset, p.scales[1] + page[0] * p.scales_pitch[1] + u.head * 1024, 1024, full);
-          } else {
-#pragma unroll
-            for (int e = 0; e < kEntries; ++e) {
-              tc::bulk_load(stage + e * 4096, p.codes[0] + page[e] * p.codes_pitch[0] + u.head * 4096, 4096, full);
-              tc::bulk_load(stage + kKsOffset + e * 512, p.scales[0] + page[e] * p.scales_pitch[0] + u.head * 512, 512, full);
-              tc::bulk_load(stage + kVOffset + e * 4096, p.codes[1] + page[e] * p.codes_pitch[1] + u.head * 4096, 4096, full);
-              tc::bulk_load(stage + kVsOffset + e * 512, p.scales[1] + page[e] * p.scales_pitch[1] + u.head * 512, 512, full);
-            }
-          }
-        }
-        __syncwarp();
-        at.advance();
-      }
-    }
-#pragma unroll 1
-    for (int step = max(u.begin, u.info.pages); step < u.end; ++step) {
-      const StepKind kind = step_kind(u.info, step);
-      const int places = bf16_places(u.info, kind);
-#pragma unroll 1
-      for (int side = 0; side < 2; ++side) {
-        const __nv_bfloat16* tail = (side ? p.tail_value : p.tail_key) + u.info.slot * p.tail_slot + u.head * kHeadDim;
-        const __nv_bfloat16* draft = side ? p.draft_value + u.row * p.draft_value_row + u.head * kHeadDim
-                                          : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
-        const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
-#pragma unroll 1
-        for (int first = 0; first < places; first += kBf16Rows) {
-          const int end = min(first + kBf16Rows, places);
-          wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
-          uint64_t* const full = &sm.full[at.slot];
-          // the sink's places behind its length stay empty
-          const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
-          if (elect_one()) tc::mbar_expect_tx(full, (end - first - absent) * 256);
-          __syncwarp();
-#pragma unroll 1
-          for (int i = first + lane; i < end; i += 32) {
-            const __nv_bfloat16* source = nullptr;
-            if (kind == kStepTail) source = tail + i * tail_row;
-            else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
-            else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
-            if (source) tc::bulk_load(sm.ring[at.slot] + (i - first) * kBf16Pitch, source, 256, full);
-          }
-          __syncwarp();
-          at.advance();
-        }
-      }
-    }
-  }
-  // After an abort nobody else waits for the copies still in flight: no CTA may end under them. (A stage that was
-  // never filled, or whose last use is over, is in a phase whose predecessor has ended.)
-  if (*static_cast<volatile int*>(&sm.abort_flag)) {
-#pragma unroll 1
-    for (int i = 0; i < kStages; ++i) {
-      wait(&sm.full[at.slot], at.turn ^ 1, &sm.ignored_flag);
-      at.advance();
-    }
-  }
-  __syncwarp();
-}
-
-// The key scales of two 64-token pages into whole atoms, in place, by one warp.
-__device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
-  uint2 part[2][2];
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    part[e & 1][e >> 1] = *reinterpret_cast<const uint2*>(scales + (e >> 1) * 512 + (e & 1) * 256 + lane * 8);
-  __syncwarp();
-#pragma unroll
-  for (int atom = 0; atom < 2; ++atom)
-    *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) =
-        make_uint4(part[atom][0].x, part[atom][0].y, part[atom][1].x, part[atom][1].y);
-  tc::fence_proxy_async_smem();
-  __syncwarp();
-}
-
-// The whole warp walks and waits; one thread of it issues.
-template <int NT, int PT>
-__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
-  using Sh = Shape<NT>;
-  constexpr uint32_t kFp4 = tc::nvf4_idesc(128, NT), kF16 = f16_idesc(NT, 0, false);
-  constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
-  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-  const uint32_t q = tc::smem_u32(sm.q), ring = tc::smem_u32(sm.ring);
-  const uint64_t q_codes = tc::fp4_tile_desc(q, 0), q_scales = tc::sf_atom_desc(q + kTerms * Sh::kTermCodes);
-  const uint64_t tile = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
-  uint32_t k_parity = 0, p_parity = 0;
-  Place at;
-  Unit u;
-  bool known = false;
-#pragma unroll 1
-  for (; walker.next(u, known); known = true) {
-    // a step's scores go before the output of the one before
-#pragma unroll 1
-    for (int step = u.begin; step <= u.end; ++step) {
-      if (step < u.end) {
-        const StepKind kind = step_kind(u.info, step);
-        wait(&sm.s_ready, k_parity, &sm.abort_flag);
-        k_parity ^= 1;
-        if (kind == kStepPage) {
-          wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
-          if constexpr (PT == 64) interleave_scales(sm.ring[at.slot] + kKsOffset, lane);
-          tc::fence_after_sync();
-          const uint32_t stage = ring + at.slot * kStage;
-          const uint64_t codes = tc::fp4_tile_desc(stage, 0), atoms = tc::sf_atom_desc(stage + kKsOffset);
-          if (elect_one()) {
-            if (step == u.begin) {
-#pragma unroll 1
-              for (int i = 0; i < 2 * kTerms; ++i) tc::cp_sf_atom(tmem + Sh::kQs + i * 4, q_scales + i * 32);
-            }
-            tc::cp_sf_atom(tmem + Sh::kKs, atoms);
-            tc::cp_sf_atom(tmem + Sh::kKs + 4, atoms + 32);
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
-#pragma unroll
-              for (int term = 0; term < kTerms; ++term)
-                tc::mma_nvf4(tmem + Sh::kS, codes + 2 * s, q_codes + term * (Sh::kTermCodes / 16) + 2 * s, kFp4,
-                             tmem + Sh::kKs + 4 * s, tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
-            }
-            tc::commit(&sm.s_full);
-            tc::commit(&sm.empty[at.slot]);
-          }
-          __syncwarp();
-          at.advance();
-        } else {
-#pragma unroll 1
-          for (int i = 2 * bf16_stages(u.info, kind); i > 0; --i) at.advance();
-          tc::fence_after_sync();
-          if (elect_one()) {
-#pragma unroll 1
-            for (int s = 0; s < 8; ++s)
-              mma_ts(tmem + Sh::kS, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kF16, s > 0);
-            tc::commit(&sm.s_full);
-          }
-          __syncwarp();
-        }
-      }
-      if (step == u.begin) continue;
-      wait(&sm.p_full, p_parity, &sm.abort_flag);  // P, and before it V
-      p_parity ^= 1;
-      tc::fence_after_sync();
-      const StepKind kind = step_kind(u.info, step - 1);
-      const bool first = step - 1 == u.begin;
-      if (elect_one()) {
-        if (kind == kStepPage) {
-#pragma unroll
-          for (int s = 0; s < 8; ++s)  // 16 tokens further: 2048 bytes of P, 8 columns of V
-            mma_ts(tmem + Sh::kO, tmem + Sh::kV + s * 8, tile + s * 128, kPages, !(first && s == 0));
-        } else {
-          const int slices = step_slices(u.info, kind);
-#pragma unroll 1
-          for (int s = 0; s < slices; ++s)
-            mma_ts(tmem + Sh::kO, tmem + Sh::kV + s * 8, tile + s * 128, kBf16, !(first && s == 0));
-        }
-        tc::commit(&sm.o_full);
-      }
-      __syncwarp();
-    }
-  }
-  // also after an abort: tensor memory is freed behind the last product
-  if (elect_one()) tc::commit(&sm.drained);
-  __syncwarp();
-  wait(&sm.drained, 0, &sm.ignored_flag);
-}
-
-// Thirty-two codes and the scales of their two groups into sixteen columns of this thread's lane.
-__device__ __forceinline__ void store_dequantized(uint32_t a, uint4 chunk, uint32_t scales) {
-  __half2 scale[2];
-  scale_pairs(scales, scale);
-  uint32_t v[16];
-  dequantize8(chunk.x, scale[0], v);
-  dequantize8(chunk.y, scale[0], v + 4);
-  dequantize8(chunk.z, scale[1], v + 8);
-  dequantize8(chunk.w, scale[1], v + 12);
-  st16(a, v);
-}
-
-// A group of a query: zero outside the tile; rotated if asked.
-template <int NT>
-__device__ __forceinline__ void load_query16(const TreeParams& p, const Unit& u, int r, int group, float* v) {
-  const int queries = min(u.info.count * p.ratio - u.tile * NT, NT), query = u.tile * NT + r;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-  if (r < queries)
-    load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
-                     (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v);
-  if (p.rotate) {
-    hadamard_butterflies(v, group);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] *= kInvSqrt128;
-  }
-}
-
-// The power of two that the tile's queries are scaled with: a query whose largest value is 2^-8 of the tile's
-// still has all four terms above E4M3's smallest scale.
-template <int NT>
-__device__ __forceinline__ float query_scale(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread, float* inverse) {
-  float amax = 0.0f;
-#pragma unroll
-  for (int r = thread >> 3; r < (NT < kWorkers / 8 ? kWorkers / 8 : NT); r += kWorkers / 8) {
-    float v[16];
-    load_query16<NT>(p, u, r, thread & 7, v);
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
-  }
-  if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
-  amax = warp_max(amax);
-  if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
-  bar_sync(kWorkBarrier, kWorkers);
-#pragma unroll
-  for (int w = 0; w < kWorkers / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
-  return scale_to<10>(amax, inverse);
-}
-
-// The tile's queries into shared memory, by eight threads each: as FP4 terms for pages, as FP16 for BF16 steps.
-template <int NT>
-__device__ __forceinline__ void load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread, float scale, bool terms) {
-  using Sh = Shape<NT>;
-  const int group = thread & 7;
-#pragma unroll 1
-  for (int r = thread >> 3; r < (NT < kWorkers / 8 ? kWorkers / 8 : NT); r += kWorkers / 8) {
-    float v[16];
-    load_query16<NT>(p, u, r, group, v);
-    if (r >= NT) continue;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] *= scale;
-    if (terms) {
-      const int at = r * 64 + group * 8;
-#pragma unroll 1
-      for (int term = 0; term < kTerms; ++term) {
-        float largest = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(v[j]));
-        const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
-        GroupCodes codes;
-        codes.scale = e4m3_to_float(byte);
-        // (an approximate reciprocal: what it rounds otherwise is left to the next term)
-        float inverse_scale;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse_scale) : "f"(fmaxf(codes.scale, 1.0e-30f)));
-        float scaled[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) scaled[j] = v[j] * inverse_scale;
-        codes.lo = pack_e2m1x8(scaled);
-        codes.hi = pack_e2m1x8(scaled + 8);
-        *reinterpret_cast<uint2*>(sm.q + term * Sh::kTermCodes + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
-        sm.q[kTerms * Sh::kTermCodes + term * 1024 + scale_tile_offset(r, group)] = (uint8_t)byte;
-        float rest[16];
-        group_residual16(v, codes, rest);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = rest[j];
-      }
-    } else {
-      uint8_t* row = sm.q + (group >> 2) * NT * 128 + r * 128;
-      uint32_t w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
-      const int chunk = (group & 3) * 2;
-      *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-      *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-  }
-  tc::fence_proxy_async_smem();
-}
-
-// Sums of N per-lane columns over the warp: every exchange halves what a lane holds, until it holds N / 32 (at
-// least one) columns, which go to `store(column, sum)`.
-template <int N, int MASK, typename Store>
-__device__ __forceinline__ void reduce_columns(float* v, int lane, int column, Store store) {
-  if constexpr (MASK == 0) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) store(column + j, v[j]);
-  } else if constexpr (N % 2 == 0) {
-    const bool upper = (lane & MASK) != 0;
-#pragma unroll
-    for (int j = 0; j < N / 2; ++j) {
-      const float keep = upper ? v[j + N / 2] : v[j], send = upper ? v[j] : v[j + N / 2];
-      v[j] = keep + __shfl_xor_sync(0xffffffffu, send, MASK);
-    }
-    reduce_columns<N / 2, MASK / 2>(v, lane, column + (upper ? N / 2 : 0), store);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], MASK);
-    reduce_columns<N, MASK / 2>(v, lane, column, store);
-  }
-}
-
-// One stage's release, by a whole warp. A page's stage waits for its score product too; for a BF16 step's one
-// warp arrives in its place.
-template <int NT>
-__device__ __forceinline__ void release(Smem<NT>& sm, Place& at, int thread, bool bf16) {
-  __syncwarp();
-  if ((thread & 31) == 0) tc::mbar_arrive(&sm.empty[at.slot]);
-  if (bf16 && thread == 0) tc::mbar_arrive(&sm.empty[at.slot]);
-  at.advance();
-}
-
-// The keys of a BF16 step: thread r of either half brings its half of token r's channels. Returns what undoes
-// the token's scaling.
-template <int NT>
-__device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem<NT>& sm, const Unit& u, StepKind kind, Place at,
-                                        uint32_t operand, int thread) {
-  const int r = thread & 127, half = thread >> 7;
-  const int places = bf16_places(u.info, kind);
-  const bool two = places > kBf16Rows;
-  // a step's stages are held together
-  Place second = at;
-  wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
-  if (two) {
-    second.advance();
-    wait(&sm.full[second.slot], second.turn, &sm.abort_flag);
-  }
-  uint8_t* const stage0 = sm.ring[at.slot];
-  uint8_t* const stage1 = sm.ring[second.slot];
-  auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
-  bool there = r < places;
-  if (kind == kStepDraft) {
-    if (r < BDFP4_MAX_SINK) there = r < u.info.sink;
-    if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
-      const int group = thread & 7;
-      const float* shift = p.key_shift ? p.key_shift + u.head * kHeadDim + group * kGroup : nullptr;
-#pragma unroll 1
-      for (int first = 0; first < u.info.count; first += kWorkers / 8) {
-        // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
-        const int node = first + (thread >> 3);
-        uint4* at16 = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + min(node, u.info.count - 1)) + group * 32);
-        const uint4 raw[2] = {at16[0], at16[1]};
-        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[2 * i] = __uint_as_float(w[i] << 16);
-          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-        __syncwarp();  // a thread that follows along may read the row that another of its warp writes
-        cache_basis16_any(v, group, p.rotate != 0, shift);
-        if (node < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at16), v);
-      }
-      tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
-      bar_sync(kWorkBarrier, kWorkers);
-    }
-  }
-  const uint4* row = reinterpret_cast<const uint4*>(row_of(min(r, places - 1)));
-  float amax = 0.0f;
-  if (there) {
-#pragma unroll 4
-    for (int j = 0; j < 16; ++j) {
-      const uint4 q = row[j];
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-    }
-  }
-  float inverse;
-  const float scale = scale_to<14>(amax, &inverse);
-#pragma unroll 1
-  for (int quarter = 2 * half; quarter < 2 * half + 2; ++quarter) {
-    uint32_t v[16];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if (there) q = row[quarter * 4 + j];
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
-    }
-    st16(operand + quarter * 16, v);
-  }
-  release(sm, at, thread, true);
-  if (two) release(sm, at, thread, true);
-  return inverse;
-}
-
-// The values of a BF16 step: half h brings the tokens of the step's stage h into channel r's lane.
-template <int NT>
-__device__ __forceinline__ void bf16_values(Smem<NT>& sm, const Unit& u, StepKind kind, Place& at, uint32_t operand, int thread) {
-  const int c = thread & 127, half = thread >> 7;
-  const int places = bf16_places(u.info, kind);
-  at.advance();  // the keys'
-  if (places > kBf16Rows) at.advance();
-#pragma unroll 1
-  for (int first = 0; first < places; first += kBf16Rows) {
-    wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
-    if ((first > 0) == (half > 0)) {
-      const uint8_t* stage = sm.ring[at.slot] + 2 * c;
-      const int slices = (min(places - first, kBf16Rows) + 15) / 16;
-#pragma unroll 1
-      for (int s = 0; s < slices; ++s) {
-        const int place = first + s * 16;
-        const int stop = kind == kStepDraft && place == 0 ? u.info.sink : places;
-        uint32_t v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t lo = 0, hi = 0;
-          if (place + 2 * i < stop) lo = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i) * kBf16Pitch);
-          if (place + 2 * i + 1 < stop) hi = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i + 1) * kBf16Pitch);
-          v[i] = lo | (hi << 16);
-        }
-        st8(operand + (place >> 4) * 8, v);
-      }
-    }
-    release(sm, at, thread, true);
-  }
-}
-
-template <int NT, int PT>
-__device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
-  using Sh = Shape<NT>;
-  constexpr int C = Sh::kColumns;
-  const int t = thread & 127, lane = thread & 31, warp = t >> 5, half = thread >> 7;
-  const int first_column = half * C;
-  const int barrier = kHalfBarrier + half;
-  const uint32_t lanes = sm.tmem + ((uint32_t)(t & ~31) << 16);
-  const uint32_t scores = lanes + Sh::kS + first_column, k_operand = lanes + Sh::kK, v_operand = lanes + Sh::kV;
-  float* base = sm.base + first_column;
-  float* top = sm.top + first_column;
-  // where this thread's codes and scales lie in a stage: half of channel t's tokens
-  const int v_swizzle = (t >> 1) & 3;
-  const int v_codes = kVOffset + (PT == 128 ? t * 64 : half * 4096 + t * 32);
-  const int v_scales = kVsOffset + half * 512 + (t & 31) * 16 + (t >> 5) * 4;
-  const int v_chunk0 = PT == 128 ? ((2 * half) ^ v_swizzle) * 16 : ((t >> 2) & 1) * 16;  // the other one's is 16 off
-  uint8_t* const p_row = sm.p + t * 128;
-  const int p_chunk = first_column >> 3, p_swizzle = t & 7;
-  Place v_at;
-  uint32_t parity = 0;
-  bool any = false;  // a step has been taken
-  Unit u;
-  bool known = false;
-#pragma unroll 1
-  for (; walker.next(u, known); known = true) {
-    float q_inverse;
-    const float q_scale = query_scale<NT>(p, sm, u, thread, &q_inverse);
-    if (u.begin < u.info.pages) load_queries<NT>(p, sm, u, thread, q_scale, true);
-    if (t < C) {
-      top[t] = kNoMax;
-      base[t] = 0.0f;  // scores as they are
-      // the draft nodes the query of column t sees
-      const int query = u.tile * NT + first_column + t;
-      uint64_t seen = 0;
-#pragma unroll 1
-      for (int node = min(query / p.ratio, u.info.count - 1); node >= 0;) {
-        seen |= 1ull << node;
-        const int parent = sm.parents[node];
-        node = parent < node ? parent : -1;
-      }
-      sm.family[first_column + t] = seen;
-    }
-    float2 sum[C / 2];
-#pragma unroll
-    for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
-    bar_sync(barrier, 128);
-    const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
-    // Lets the scores of a step be taken: those of the step before are in registers. `keys`: where a BF16 step's
-    // keys are; they go into their operand first, and before a unit's first such step the queries change their
-    // form. Returns what turns the step's scores into log2 units.
-    auto let_scores = [&](int step, Place keys) -> float {
-      const StepKind kind = step_kind(u.info, step);
-      float f = page_factor;
-      if (kind != kStepPage) {
-        if (step == max(u.begin, u.info.pages)) load_queries<NT>(p, sm, u, thread, q_scale, false);
-        f = p.scale_log2 * q_inverse * bf16_keys<NT>(p, sm, u, kind, keys, k_operand, thread);
-        tc::tmem_wait_st();
-      }
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.s_ready);
-      return f;
-    };
-    float f = let_scores(u.begin, v_at);
-#pragma unroll 1
-    for (int step = u.begin; step < u.end; ++step) {
-      const StepKind kind = step_kind(u.info, step);
-      const bool special = kind != kStepPage || (step == 0 && u.info.sink > 0);  // the same in the whole half
-      wait(&sm.s_full, parity, &sm.abort_flag);
-      tc::fence_after_sync();
-
-      float s[C];
-      tmem_load<C>(scores, s);
-      tc::tmem_wait_ld();
-      if (special) {
-        bool dead;  // no query sees this thread's token
-        if (kind == kStepPage) dead = t < u.info.sink;
-        else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
-        else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-        const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
-        const int node = t - BDFP4_MAX_SINK;
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-          if (dead || (masked && !((sm.family[first_column + j] >> node) & 1))) s[j] = -INFINITY;
-      }
-      // scores -> log2 units above the maxima, plus kShift
-      const float2 f2 = make_float2(f, f);
-      float highest = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < C; j += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(base + j);
-        const float2 y0 = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, make_float2(b.x, b.y));
-        const float2 y1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), f2, make_float2(b.z, b.w));
-        s[j] = y0.x, s[j + 1] = y0.y, s[j + 2] = y1.x, s[j + 3] = y1.y;
-        highest = fmaxf(fmaxf(highest, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
-      }
-      // the next step's scores are taken while this one's probabilities are formed
-      float next_f = f;
-      if (step + 1 < u.end) {
-        Place keys = v_at;
-#pragma unroll 1
-        for (int i = kind == kStepPage ? 1 : 2 * bf16_stages(u.info, kind); i > 0; --i) keys.advance();
-        next_f = let_scores(step + 1, keys);
-      }
-      // V, once the product of the step before is done with its operand, P and (for a rescaling) the output
-      if (any) wait(&sm.o_full, parity ^ 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      if (kind == kStepPage) {
-        wait(&sm.full[v_at.slot], v_at.turn, &sm.abort_flag);
-        const uint8_t* stage = sm.ring[v_at.slot];
-        const uint32_t scale = *reinterpret_cast<const uint32_t*>(stage + v_scales);
-        const uint4 chunk0 = *reinterpret_cast<const uint4*>(stage + v_codes + v_chunk0);
-        const uint4 chunk1 = *reinterpret_cast<const uint4*>(stage + v_codes + (v_chunk0 ^ 16));
-        store_dequantized(v_operand + 32 * half, chunk0, scale);
-        store_dequantized(v_operand + 32 * half + 16, chunk1, scale >> 16);
-        release(sm, v_at, thread, false);
-      } else {
-        bf16_values<NT>(sm, u, kind, v_at, v_operand, thread);
-      }
-      // Maxima are taken in a unit's first step, in one that could be the first with anything to see (a tail may
-      // hold nothing but sink), and when a score exceeds its query's by too much.
-      const bool forced = step == u.begin || (kind == kStepDraft && u.info.pages == 0);
-      if (bar_any(barrier, forced || highest > kShift + kGrowth)) {
-        float mine = 0.0f;
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-          const float m = warp_max(s[j]);
-          if (lane == j) mine = m;
-        }
-        if (lane < C) sm.col[warp][first_column + lane] = mine;
-        bar_sync(barrier, 128);
-        if (t < C) {
-          const int col = first_column + t;
-          const float before = top[t], was = base[t];
-          const float now = fmaxf(fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]),
-                                        fmaxf(sm.col[2][col], sm.col[3][col])) - was, before);
-          const float is = now == kNoMax ? 0.0f : kShift - now;
-          top[t] = now;
-          base[t] = is;
-          sm.shift[col] = is - was;
-          sm.factor[col] = ex2(before - now);
-        }
-        bar_sync(barrier, 128);
-#pragma unroll
-        for (int j = 0; j < C / 2; ++j) {
-          s[2 * j] += sm.shift[first_column + 2 * j];
-          s[2 * j + 1] += sm.shift[first_column + 2 * j + 1];
-          sum[j].x *= sm.factor[first_column + 2 * j];
-          sum[j].y *= sm.factor[first_column + 2 * j + 1];
-        }
-        if (step > u.begin) {  // what O^T holds is of the old maxima
-#pragma unroll 1
-          for (int j = 0; j < C; j += 8) {
-            float o[8];
-            const uint32_t column = lanes + Sh::kO + first_column + j;
-            tc::tmem_ld8(column, o);
-            tc::tmem_wait_ld();
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(o[i] * sm.factor[first_column + j + i]);
-            st8(column, w);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < C; j += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[j + i] = ex2(s[j + i]);
-        if (kind == kStepPage) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = h2(__floats2half2_rn(s[j + 2 * i], s[j + 2 * i + 1]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = pack_bf16x2(s[j + 2 * i] * p.inverse_value_scale, s[j + 2 * i + 1] * p.inverse_value_scale);
-        }
-        *reinterpret_cast<uint4*>(p_row + (((p_chunk + (j >> 3)) ^ p_swizzle) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      tc::tmem_wait_st();
-      tc::fence_before_sync();
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.p_full);
-#pragma unroll
-      for (int j = 0; j < C / 2; ++j) sum[j] = __fadd2_rn(sum[j], make_float2(s[2 * j], s[2 * j + 1]));
-      f = next_f;
-      parity ^= 1;
-      any = true;
-    }
-
-    {  // each query's weight: first over a warp's 32 tokens, then (below) over the four warps
-      float v[C];
-#pragma unroll
-      for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
-      reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col[warp][first_column + j] = total; });
-    }
-    bar_sync(barrier, 128);
-    const bool whole = u.begin == 0 && u.end == u.info.steps;
-    // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
-    const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
-    if (t < C) {
-      const int col = first_column + t;
-      const float total = (sm.col[0][col] + sm.col[1][col]) + (sm.col[2][col] + sm.col[3][col]);
-      if (whole) {
-        sm.factor[col] = total > 0.0f ? p.value_scale / total : 0.0f;
-      } else {
-        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[t];
-        p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
-      }
-    }
-    bar_sync(barrier, 128);
-    wait(&sm.o_full, parity ^ 1, &sm.abort_flag);
-    tc::fence_after_sync();
-    const int queries = min(u.info.count * p.ratio - u.tile * NT - first_column, C);
-    const int query = u.tile * NT + first_column;
-    int out_node = query / p.ratio, out_head = query % p.ratio;
-    __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
-    float* partial = p.partial + ((int64_t)part * NT + first_column) * kHeadDim + t;
-#pragma unroll 1
-    for (int j = 0; j < C; j += 8) {
-      float o[8];
-      tc::tmem_ld8(lanes + Sh::kO + first_column + j, o);
-      tc::tmem_wait_ld();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (j + i < queries) {
-          if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.factor[first_column + j + i]);
-            if (++out_head == p.ratio) out_head = 0, ++out_node;
-          } else {
-            partial[(int64_t)(j + i) * kHeadDim] = o[i];
-          }
-        }
-      }
-    }
-    tc::fence_before_sync();
-    if (!whole && u.begin == 0 && thread == 0) {
-      TreeSplit split;
-      split.row = u.row;
-      split.head = u.head;
-      split.tile = u.tile;
-      // the unit's last step, counted over the whole launch, names the CTA it ends in
-      split.last = (int)((sm.last + (u.info.steps - u.end) - 1) / sm.per_cta);
-      p.splits[blockIdx.x] = split;
-    }
-  }
-}
-
-template <int NT, int PT>
-__global__ void __launch_bounds__(kThreads, 2)
-tree_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const TreeParams p) {
-  extern __shared__ uint8_t raw_smem[];
-  // (an offset, not a masked pointer: the compiler has to see that this is shared memory)
-  Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(raw_smem + (-tc::smem_u32(raw_smem) & 1023u));
-  const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
-  dependents_may_launch();
-
-  // all steps of the launch, and where this CTA's run begins
-  long long mine = 0;
-#pragma unroll 1
-  for (int row = thread; row < p.rows; row += kThreads) {
-    const RowInfo r = row_info(p, row, PT);
-    mine += (long long)r.steps * r.tiles * p.heads_kv;
-  }
-  for (int step = 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
-  if (lane == 0) sm.sums[warp] = mine;
-  if (thread == 0) {
-#pragma unroll 1
-    for (int i = 0; i < kStages; ++i) {
-      tc::mbar_init(&sm.full[i], 1);
-      tc::mbar_init(&sm.empty[i], 9);  // the workers' warps and the score product
-    }
-    tc::mbar_init(&sm.s_ready, 8);
-    tc::mbar_init(&sm.s_full, 1);
-    tc::mbar_init(&sm.p_full, 8);
-    tc::mbar_init(&sm.o_full, 1);
-    tc::mbar_init(&sm.drained, 1);
-    tc::fence_barrier_init();
-    sm.abort_flag = sm.ignored_flag = 0;
-    TreeSplit none;
-    none.row = -1;
-    none.head = none.tile = none.last = 0;
-    p.splits[blockIdx.x] = none;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    long long all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) all += sm.sums[w];
-    const long long per = max((all + gridDim.x - 1) / gridDim.x, 1ll);
-    const long long first = per * blockIdx.x, last = min(first + per, all);
-    if (lane == 0) {
-      sm.per_cta = per;
-      sm.first = first;
-      sm.last = last;
-    }
-    long long before = 0;
-#pragma unroll 1
-    for (int row0 = 0; row0 < p.rows && first < last; row0 += 32) {
-      long long steps = 0;
-      if (row0 + lane < p.rows) {
-        const RowInfo r = row_info(p, row0 + lane, PT);
-        steps = (long long)r.steps * r.tiles * p.heads_kv;
-      }
-      long long upto = steps;
-      for (int step = 1; step < 32; step <<= 1) {
-        const long long left = __shfl_up_sync(0xffffffffu, upto, step);
-        if (lane >= step) upto += left;
-      }
-      const unsigned holds = __ballot_sync(0xffffffffu, before + upto > first);
-      if (holds) {
-        if (lane == __ffs(holds) - 1) {
-          sm.start_row = row0 + lane;
-          sm.start_offset = first - (before + upto - steps);
-        }
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    __syncwarp();
-    tc::tmem_alloc(&sm.tmem, kTmemColumns);
-    tc::tmem_relinquish();
-    tc::fence_before_sync();
-  }
-  __syncthreads();
-  tc::fence_after_sync();
-  if (sm.first < sm.last) {
-    const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
-    if (warp < kWorkers / 32) work<NT, PT>(p, sm, walker, thread);
-    else if (warp == kWorkers / 32) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
-    else issue<NT, PT>(sm, walker, lane);
-  }
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::fence_after_sync();
-  if (thread == 0 && sm.abort_flag && p.error_word) atomicOr(p.error_word, (int)BDFP4_DEV_WAIT_TIMEOUT);
-  if (warp == 0) tc::tmem_dealloc(sm.tmem, kTmemColumns);
-}
-
-template <int NT, int PT>
-static cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const TreeParams& p, cudaStream_t stream) {
-  const int smem = (int)sizeof(Smem<NT>) + 1024;
-  static PerDeviceOnce configured;
-  const int slot = current_device_slot();
-  if (slot < 0 || !configured.done[slot]) {
-    cudaError_t e = cudaFuncSetAttribute(tree_kernel<NT, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    if (slot >= 0) configured.done[slot] = true;
-  }
-  tree_kernel<NT, PT><<<kTreeCtas, kThreads, smem, stream>>>(k_map, v_map, p);
-  return cudaGetLastError();
-}
-
 template <int PT>
 static cudaError_t launch_tile(const CUtensorMap& k_map, const CUtensorMap& v_map, const TreeParams& p, cudaStream_t stream) {
   switch (p.tile) {
-    case 16: return launch<16, PT>(k_map, v_map, p, stream);
-    case 32: return launch<32, PT>(k_map, v_map, p, stream);
-    default: return launch<64, PT>(k_map, v_map, p, stream);
+    case 16: return narrow::launch<16, PT>(k_map, v_map, p, stream);
+    case 32: return narrow::launch<32, PT>(k_map, v_map, p, stream);
+    case 64: return wide::launch<64, PT>(k_map, v_map, p, stream);
+    case 96: return wide::launch<96, PT>(k_map, v_map, p, stream);
+    default: return wide::launch<128, PT>(k_map, v_map, p, stream);
   }
 }
 

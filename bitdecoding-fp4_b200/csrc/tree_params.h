@@ -1,5 +1,5 @@
-// Launch parameters of the tree attention kernel and the entry points of its instantiation units. The kernel
-// template lives in tree_kernel.cuh and is instantiated in two translation units (128- and 64-token pages);
+// Launch parameters of the tree attention kernel and the entry points of its instantiation units. The kernels.
+// Their templates (tree_narrow.cuh, tree_wide.cuh) are instantiated in two translation units (128- and 64-token pages);
 // tree.cu holds the C ABI and the merge kernel.
 #pragma once
 
@@ -10,9 +10,11 @@
 
 namespace bdfp4 {
 
-// CTAs of a launch: two per SM of a B200. They share nothing but the workspace, so any number is correct.
-constexpr int kTreeCtas = 296;
-constexpr int kTreeMaxTile = 64;  // query rows (node x query head of one KV head) of a CTA's tile at most
+// CTAs of a launch: two per SM of a B200 for tiles of at most kTreeNarrowTile queries, else one. They share
+// nothing but the workspace, so any number is correct.
+constexpr int kTreeNarrowCtas = 296, kTreeWideCtas = 148;
+constexpr int kTreeNarrowTile = 32;
+constexpr int kTreeMaxTile = 128;  // query rows (node x query head of one KV head) of a CTA's tile at most
 
 // A unit that begins in CTA c and does not end there: its parts lie in slot 2c + 1 and in slots 2c' of the
 // CTAs c < c' <= last.
@@ -23,6 +25,7 @@ struct TreeSplit {
 struct TreeParams {
   int rows, nodes, heads_q, heads_kv, ratio;
   int tile;  // query rows per tile
+  int ctas;
   const __nv_bfloat16* query;
   int64_t query_row, query_node;
   const __nv_bfloat16* draft_key;
@@ -53,9 +56,9 @@ struct TreeParams {
   float value_scale, inverse_value_scale;
   __nv_bfloat16* out;
   int64_t out_row, out_node;
-  float* partial;  // [2 * kTreeCtas][tile][128] sums, then [2 * kTreeCtas][2][tile] maxima and weights
+  float* partial;  // [2 * ctas][tile][128] sums, then [2 * ctas][2][tile] maxima and weights
   float* partial_stat;
-  TreeSplit* splits;  // [kTreeCtas]
+  TreeSplit* splits;  // [ctas]
   int32_t* error_word;
 };
 
