@@ -18,6 +18,7 @@ others are drafts. ``parents[r, i] < i`` is the parent of node ``i``. A row may 
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -34,14 +35,17 @@ ROTATIONS = ("none", "hadamard")
 
 
 class _on_device:
-    """Launches go to the current device's context; the tensors' device is made current if it is not."""
+    """Launches go to the current device's context; the tensors' device is made current if it is not. Entering
+    gives the device's current stream (its handle alone: making a stream object costs 4 us)."""
 
     def __init__(self, device: torch.device) -> None:
+        self._index = device.index
         self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
+    def __enter__(self) -> int:
         if self._guard is not None:
             self._guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     def __exit__(self, *error):
         if self._guard is not None:
@@ -51,18 +55,22 @@ class _on_device:
 def _int32(tensor, name: str, shape: tuple, device) -> None:
     if (
         not isinstance(tensor, torch.Tensor) or tensor.dtype is not torch.int32 or tensor.device != device
-        or tuple(tensor.shape) != shape or (len(shape) and shape[-1] > 1 and tensor.stride(-1) != 1)
+        or tensor.shape != shape or (shape[-1] > 1 and tensor.stride(-1) != 1)
     ):
         raise ValueError(f"{name} must be INT32 {list(shape)} on {device}, dense along its last axis")
 
 
 def _tree_tensor(tensor, name: str, shape: tuple, device) -> None:
     """BF16 ``[..., nodes, heads, 128]`` with free leading strides."""
-    if (
-        not isinstance(tensor, torch.Tensor) or tensor.dtype is not torch.bfloat16 or tensor.device != device
-        or tuple(tensor.shape) != shape or tensor.stride(-1) != 1 or (shape[-2] > 1 and tensor.stride(-2) != HEAD_DIM)
-        or tensor.data_ptr() % 16 or any(s % 8 for s, n in zip(tensor.stride()[:-2], shape) if n > 1)
-    ):
+    ok = (isinstance(tensor, torch.Tensor) and tensor.dtype is torch.bfloat16 and tensor.device == device
+          and tensor.shape == shape and tensor.data_ptr() % 16 == 0)
+    if ok:
+        *outer, head, inner = tensor.stride()
+        ok = inner == 1 and (head == HEAD_DIM or shape[-2] == 1)
+        for stride, size in zip(outer, shape):
+            if stride % 8 and size > 1:
+                ok = False
+    if not ok:
         raise ValueError(f"{name} must be BF16 {list(shape)} on {device}, dense within a node and 16-byte aligned")
 
 
@@ -87,11 +95,9 @@ def _check_values(bad: torch.Tensor, message: str) -> None:
 
 def _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, device) -> tuple[int, int, int]:
     """(pages, page tokens, KV heads) of the four regions of an NVFP4 cache."""
-    for tensor, name in ((key_pages_fp4, "key_pages_fp4"), (key_scales, "key_scales"),
-                         (value_pages_fp4, "value_pages_fp4"), (value_scales, "value_scales")):
-        if not isinstance(tensor, torch.Tensor) or tensor.device != device:
-            raise ValueError(f"{name} must be a CUDA tensor on {device}")
-    packed = (torch.uint8, torch.float4_e2m1fn_x2)
+    packed, scales = (torch.uint8, torch.float4_e2m1fn_x2), (torch.uint8, torch.float8_e4m3fn)
+    if not isinstance(key_pages_fp4, torch.Tensor) or key_pages_fp4.device != device:
+        raise ValueError(f"key_pages_fp4 must be a CUDA tensor on {device}")
     if key_pages_fp4.dtype not in packed or key_pages_fp4.ndim != 4 or key_pages_fp4.shape[3] * 2 != HEAD_DIM:
         raise ValueError("key_pages_fp4 must be packed FP4 with shape [pages, 128, heads_kv, 64]")
     pages, page, heads, _ = key_pages_fp4.shape
@@ -105,21 +111,25 @@ def _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, dev
         value_scale_shape = (pages, 32, 4, 1, 4, 1, heads)
     else:
         raise ValueError("key_pages_fp4 must be packed FP4 with shape [pages, 128, heads_kv, 64]")
-    if value_pages_fp4.dtype not in packed or tuple(value_pages_fp4.shape) != (pages, heads, HEAD_DIM, page // 2):
-        raise ValueError(f"value_pages_fp4 must be packed FP4 with shape [pages, heads_kv, 128, {page // 2}]")
-    for tensor, name, inner in ((key_pages_fp4, "key_pages_fp4", key_inner),
-                                (value_pages_fp4, "value_pages_fp4", (HEAD_DIM * page // 2, page // 2, 1))):
-        if tensor.stride()[1:] != inner or tensor.stride(0) % 16 or tensor.data_ptr() % 16:
-            raise ValueError(f"{name} must be dense within a page with a 16-byte page pitch")
-    for tensor, name, shape, inner in ((key_scales, "key_scales", scale_shape, key_sf),
-                                       (value_scales, "value_scales", value_scale_shape, value_sf)):
-        if tuple(tensor.shape) != shape or tensor.dtype not in (torch.uint8, torch.float8_e4m3fn):
-            raise ValueError(f"{name} must hold E4M3 scale bytes with shape {shape}")
-        if tensor.stride()[1:] != inner or tensor.stride(0) % 16 or tensor.data_ptr() % 16:
-            raise ValueError(f"{name} must use the quantizer's scale layout with a 16-byte page pitch")
+    half = page // 2
+    for tensor, name, kinds, shape, inner in (
+        (key_pages_fp4, "key_pages_fp4", packed, (pages, page, heads, 64), key_inner),
+        (key_scales, "key_scales", scales, scale_shape, key_sf),
+        (value_pages_fp4, "value_pages_fp4", packed, (pages, heads, HEAD_DIM, half), (HEAD_DIM * half, half, 1)),
+        (value_scales, "value_scales", scales, value_scale_shape, value_sf),
+    ):
+        if not isinstance(tensor, torch.Tensor) or tensor.device != device:
+            raise ValueError(f"{name} must be a CUDA tensor on {device}")
+        if tensor.shape != shape or tensor.dtype not in kinds:
+            held = "packed FP4" if kinds is packed else "E4M3 scale bytes"
+            raise ValueError(f"{name} must hold {held} with shape {shape}")
+        pitch, *within = tensor.stride()
+        if tuple(within) != inner or pitch % 16 or tensor.data_ptr() % 16:
+            raise ValueError(f"{name} must be in the quantizer's layout, dense within a page, with a 16-byte page pitch")
     return pages, page, heads
 
 
+@functools.lru_cache(maxsize=1024)
 def tree_workspace_bytes(rows: int, nodes: int, heads_q: int, heads_kv: int) -> int:
     """Bytes of the workspace :func:`tree_decode` needs for these sizes (any contents)."""
     size = int(bdfp4.library().bdfp4_tree_workspace_bytes(rows, nodes, heads_q, heads_kv))
@@ -299,8 +309,8 @@ def tree_decode(
     a.out_row_stride, a.out_node_stride = out.stride()[:2]
     a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
     a.error_word = bdfp4.ptr(error_word)
-    with _on_device(device):
-        bdfp4.tree_decode(a, bdfp4.current_stream(device))
+    with _on_device(device) as stream:
+        bdfp4.tree_decode(a, stream)
     return out
 
 
@@ -378,8 +388,8 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, parents: tor
     a.uniforms, a.uniforms_row_stride = uniforms.data_ptr(), uniforms.stride(0)
     a.node_counts = bdfp4.ptr(node_counts)
     a.accepted, a.accepted_counts, a.next_tokens = (t.data_ptr() for t in out)
-    with _on_device(device):
-        bdfp4.verify_drafts(a, bdfp4.current_stream(device))
+    with _on_device(device) as stream:
+        bdfp4.verify_drafts(a, stream)
     return out
 
 
@@ -492,8 +502,7 @@ class DraftCommitter:
         a.key_shift = bdfp4.ptr(self._shift)
         a.new_seq_lens, a.seqused_fp4, a.seqused_residual, a.seqused_sink = (t.data_ptr() for t in lengths)
         a.error_word = bdfp4.ptr(self._error_word)
-        with _on_device(device):
-            stream = bdfp4.current_stream(device)
+        with _on_device(device) as stream:
             if self._seal is None:
                 a.part = bdfp4.COMMIT_ALL
                 bdfp4.commit_drafts(a, stream)
