@@ -23,8 +23,11 @@ static int tree_tile(int queries) {
 
 static int tree_ctas(int tile) { return tile <= kTreeNarrowTile ? kTreeNarrowCtas : kTreeWideCtas; }
 
-// One block per (CTA that a straddling unit begins in, eight query rows): thread c adds channel c of the
-// unit's parts, each weighted by 2^(its maximum - the largest).
+// One block per (CTA that a straddling unit begins in, eight query rows). First the parts' weights 2^(their
+// maximum - the largest) for each row, by 16 x GROUPS threads; then GROUPS threads per channel add every
+// GROUPS-th part each. It is latency that counts: for a single row's 66 parts (one token over 8192) the launch
+// took 0.8 us a part with one thread per channel that weighed each part against the ones before, 0.6 us with the
+// weights known before, 0.25 us with four. Wide tiles, of fewer parts and more blocks, take two.
 constexpr int kMergeRows = 8;
 
 __device__ __forceinline__ float merge_ex2(float x) {
@@ -33,7 +36,12 @@ __device__ __forceinline__ float merge_ex2(float x) {
   return y;
 }
 
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
+template <int GROUPS>
+__global__ void __launch_bounds__(128 * GROUPS) tree_merge_kernel(const TreeParams p) {
+  __shared__ float weight[kTreeNarrowCtas][kMergeRows];
+  constexpr int kRowThreads = 16 * GROUPS, kRowWarps = GROUPS / 2;
+  __shared__ float stat_of[kRowWarps][kMergeRows];  // by warp: maxima, then weights
+  __shared__ float sums[GROUPS - 1][kMergeRows][kHeadDim];
   wait_for_prior_kernels();
   const int cta = blockIdx.x;
   const TreeSplit split = p.splits[cta];
@@ -41,47 +49,79 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeParams p) {
   const int count = p.node_counts ? min(max(p.node_counts[split.row], 0), p.nodes) : p.nodes;
   const int first = blockIdx.y * kMergeRows;
   const int rows = min(min(count * p.ratio - split.tile * p.tile, p.tile) - first, kMergeRows);
-  float top[kMergeRows], total[kMergeRows], acc[kMergeRows];
-#pragma unroll
-  for (int r = 0; r < kMergeRows; ++r) top[r] = -3.0e38f, total[r] = 0.0f, acc[r] = 0.0f;
-  for (int c = cta; c <= split.last; ++c) {
-    const int part = 2 * c + (c == cta ? 1 : 0);
-    const float* value = p.partial + ((int64_t)part * p.tile + first) * kHeadDim + threadIdx.x;
-    const float* tops = p.partial_stat + (int64_t)(2 * part) * p.tile + first;
-#pragma unroll
-    for (int r = 0; r < kMergeRows; ++r) {
-      if (r < rows) {
-        const float v = __ldcg(value + r * kHeadDim), m = __ldcg(tops + r), w = __ldcg(tops + p.tile + r);
-        const float now = fmaxf(top[r], m);
-        const float before = merge_ex2(top[r] - now), mine = merge_ex2(m - now);
-        acc[r] = acc[r] * before + v * mine;
-        total[r] = total[r] * before + w * mine;
-        top[r] = now;
-      }
+  if (rows <= 0) return;
+  const int parts = split.last - cta + 1;
+  auto part = [&](int i) { return 2 * (cta + i) + (i == 0 ? 1 : 0); };
+  float total = 0.0f;
+  const int row = threadIdx.x / kRowThreads, lane = threadIdx.x % kRowThreads;  // (rows behind the tile's last repeat it)
+  {
+    const float* const stat = p.partial_stat + first + min(row, rows - 1);
+    float top = -3.0e38f;
+    for (int i = lane; i < parts; i += kRowThreads) {
+      const float m = __ldcg(stat + (int64_t)(2 * part(i)) * p.tile);
+      weight[i][row] = m;
+      top = fmaxf(top, m);
     }
+    for (int step = 16; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+    if ((lane & 31) == 0) stat_of[lane >> 5][row] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, stat_of[w][row]);
+    __syncthreads();
+    for (int i = lane; i < parts; i += kRowThreads) {
+      const float w = merge_ex2(weight[i][row] - top);
+      weight[i][row] = w;
+      total += w * __ldcg(stat + (int64_t)(2 * part(i) + 1) * p.tile);
+    }
+    for (int step = 16; step > 0; step >>= 1) total += __shfl_xor_sync(0xffffffffu, total, step);
+    if ((lane & 31) == 0) stat_of[lane >> 5][row] = total;
   }
+  __syncthreads();
+  const int channel = threadIdx.x & 127, group = threadIdx.x >> 7;
+  float acc[kMergeRows];
+#pragma unroll
+  for (int r = 0; r < kMergeRows; ++r) acc[r] = 0.0f;
+#pragma unroll 4
+  for (int i = group; i < parts; i += GROUPS) {
+    const float* value = p.partial + ((int64_t)part(i) * p.tile + first) * kHeadDim + channel;
+#pragma unroll
+    for (int r = 0; r < kMergeRows; ++r) acc[r] += __ldcg(value + r * kHeadDim) * weight[i][r];
+  }
+  if (group > 0) {
+#pragma unroll
+    for (int r = 0; r < kMergeRows; ++r) sums[group - 1][r][channel] = acc[r];
+  }
+  __syncthreads();
+  if (group > 0) return;
 #pragma unroll
   for (int r = 0; r < kMergeRows; ++r) {
     if (r < rows) {
+      float weights = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) weights += stat_of[w][r];
+      float sum = acc[r];
+#pragma unroll
+      for (int g = 0; g < GROUPS - 1; ++g) sum += sums[g][r][channel];
       const int query = split.tile * p.tile + first + r;
       p.out[split.row * p.out_row + (query / p.ratio) * p.out_node +
-            (int64_t)(split.head * p.ratio + query % p.ratio) * kHeadDim + threadIdx.x] =
-          __float2bfloat16_rn(total[r] > 0.0f ? acc[r] * (p.value_scale / total[r]) : 0.0f);
+            (int64_t)(split.head * p.ratio + query % p.ratio) * kHeadDim + channel] =
+          __float2bfloat16_rn(sum * (weights > 0.0f ? p.value_scale / weights : 0.0f));
     }
   }
 }
 
+template <int GROUPS>
 static cudaError_t launch_merge(const TreeParams& p, cudaStream_t stream) {
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(p.ctas, (p.tile + kMergeRows - 1) / kMergeRows);
-  config.blockDim = dim3(128);
+  config.blockDim = dim3(128 * GROUPS);
   config.stream = stream;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, tree_merge_kernel, p);
+  return cudaLaunchKernelEx(&config, tree_merge_kernel<GROUPS>, p);
 }
 
 }  // namespace bdfp4
@@ -189,6 +229,6 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
     return BDFP4_E_CUDA;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   cudaError_t e = page_tokens == 128 ? launch_tree_p128(k_map, v_map, p, stream) : launch_tree_p64(k_map, v_map, p, stream);
-  if (e == cudaSuccess) e = launch_merge(p, stream);
+  if (e == cudaSuccess) e = p.tile <= kTreeNarrowTile ? launch_merge<4>(p, stream) : launch_merge<2>(p, stream);
   return bdfp4::cuda_status(e);
 }
