@@ -264,5 +264,342 @@ __device__ __forceinline__ void reduce_columns(float* v, int lane, int column, S
   }
 }
 
+constexpr int kTerms = 4;  // FP4 terms of a query
+constexpr int kCacheThreads = 256;  // that bring the cache side: two halves of 128
+
+// A place in the ring of stages; everyone who keeps one visits every stage in order.
+template <int STAGES>
+struct Place {
+  int slot = 0;
+  uint32_t turn = 0;
+  __device__ __forceinline__ void advance() {
+    if (++slot == STAGES) slot = 0, turn ^= 1;
+  }
+};
+
+// The copies into the ring, by one warp. A page's step takes one stage, a BF16 step one per 64 tokens for K and then
+// as many for V.
+template <int PT, typename Smem>
+__device__ __forceinline__ void produce(const TreeParams& p, Smem& sm, Walker walker, const CUtensorMap* k_map,
+                                        const CUtensorMap* v_map, int lane) {
+  constexpr int kEntries = kPage / PT;
+  const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
+  Place<Smem::kStages> at;
+  Unit u;
+  bool known = false;
+#pragma unroll 1
+  for (; walker.next(u, known); known = true) {
+    const int32_t* table = p.table + u.row * p.table_stride;
+    const int stop = min(u.end, u.info.pages);
+#pragma unroll 1
+    for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
+      const int entry = batch * kEntries + lane;
+      int mine = 0;
+      if (entry < stop * kEntries) {
+        mine = table[entry];
+        if (mine < 0 || mine >= p.pages) {
+          if (p.error_word) atomicOr(p.error_word, (int)BDFP4_DEV_BAD_PAGE);
+          mine = 0;
+        }
+      }
+      const int steps = min(32 / kEntries, stop - batch);
+#pragma unroll 1
+      for (int i = 0; i < steps; ++i) {
+        int page[kEntries];
+#pragma unroll
+        for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
+        wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
+        uint64_t* const full = &sm.full[at.slot];
+        if (elect_one()) {
+          uint8_t* stage = sm.ring[at.slot];
+          tc::mbar_expect_tx(full, 18432);
+          if constexpr (PT == 128) {
+            tc::tma_load_4d(stage, k_map, full, 0, u.head, 0, page[0]);
+            tc::bulk_load(stage + kKsOffset, p.scales[0] + page[0] * p.scales_pitch[0] + u.head * 1024, 1024, full);
+            tc::tma_load_3d(stage + kVOffset, v_map, full, 0, u.head * kHeadDim, page[0]);
+            tc::bulk_load(stage + kVsOffset, p.scales[1] + page[0] * p.scales_pitch[1] + u.head * 1024, 1024, full);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kEntries; ++e) {
+              tc::bulk_load(stage + e * 4096, p.codes[0] + page[e] * p.codes_pitch[0] + u.head * 4096, 4096, full);
+              tc::bulk_load(stage + kKsOffset + e * 512, p.scales[0] + page[e] * p.scales_pitch[0] + u.head * 512, 512, full);
+              tc::bulk_load(stage + kVOffset + e * 4096, p.codes[1] + page[e] * p.codes_pitch[1] + u.head * 4096, 4096, full);
+              tc::bulk_load(stage + kVsOffset + e * 512, p.scales[1] + page[e] * p.scales_pitch[1] + u.head * 512, 512, full);
+            }
+          }
+        }
+        __syncwarp();
+        at.advance();
+      }
+    }
+#pragma unroll 1
+    for (int step = max(u.begin, u.info.pages); step < u.end; ++step) {
+      const StepKind kind = step_kind(u.info, step);
+      const int places = bf16_places(u.info, kind);
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {
+        const __nv_bfloat16* tail = (side ? p.tail_value : p.tail_key) + u.info.slot * p.tail_slot + u.head * kHeadDim;
+        const __nv_bfloat16* draft = side ? p.draft_value + u.row * p.draft_value_row + u.head * kHeadDim
+                                          : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
+        const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
+#pragma unroll 1
+        for (int first = 0; first < places; first += kBf16Rows) {
+          const int end = min(first + kBf16Rows, places);
+          wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
+          uint64_t* const full = &sm.full[at.slot];
+          // the sink's places behind its length stay empty
+          const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
+          if (elect_one()) tc::mbar_expect_tx(full, (end - first - absent) * 256);
+          __syncwarp();
+#pragma unroll 1
+          for (int i = first + lane; i < end; i += 32) {
+            const __nv_bfloat16* source = nullptr;
+            if (kind == kStepTail) source = tail + i * tail_row;
+            else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
+            else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
+            if (source) tc::bulk_load(sm.ring[at.slot] + (i - first) * kBf16Pitch, source, 256, full);
+          }
+          __syncwarp();
+          at.advance();
+        }
+      }
+    }
+  }
+  // After an abort nobody else waits for the copies still in flight: no CTA may end under them. (A stage that was
+  // never filled, or whose last use is over, is in a phase whose predecessor has ended.)
+  if (*static_cast<volatile int*>(&sm.abort_flag)) {
+#pragma unroll 1
+    for (int i = 0; i < Smem::kStages; ++i) {
+      wait(&sm.full[at.slot], at.turn ^ 1, &sm.ignored_flag);
+      at.advance();
+    }
+  }
+  __syncwarp();
+}
+
+// The key scales of two 64-token pages into whole atoms, in place, by one warp.
+__device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
+  uint2 part[2][2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    part[e & 1][e >> 1] = *reinterpret_cast<const uint2*>(scales + (e >> 1) * 512 + (e & 1) * 256 + lane * 8);
+  __syncwarp();
+#pragma unroll
+  for (int atom = 0; atom < 2; ++atom)
+    *reinterpret_cast<uint4*>(scales + atom * 512 + lane * 16) =
+        make_uint4(part[atom][0].x, part[atom][0].y, part[atom][1].x, part[atom][1].y);
+  tc::fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// A group of a query: zero outside the tile; rotated if asked.
+template <int NT>
+__device__ __forceinline__ void load_query16(const TreeParams& p, const Unit& u, int r, int group, float* v) {
+  const int queries = min(u.info.count * p.ratio - u.tile * NT, NT), query = u.tile * NT + r;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+  if (r < queries)
+    load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
+                     (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v);
+  if (p.rotate) {
+    hadamard_butterflies(v, group);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] *= kInvSqrt128;
+  }
+}
+
+// The power of two that the tile's queries are scaled with: a query whose largest value is 2^-8 of the tile's
+// still has all four terms above E4M3's smallest scale.
+template <int NT, int THREADS, typename Smem>
+__device__ __forceinline__ float query_scale(const TreeParams& p, Smem& sm, int barrier, const Unit& u, int thread, float* inverse) {
+  float amax = 0.0f;
+#pragma unroll
+  for (int r = thread >> 3; r < (NT < THREADS / 8 ? THREADS / 8 : NT); r += THREADS / 8) {
+    float v[16];
+    load_query16<NT>(p, u, r, thread & 7, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
+  }
+  if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
+  amax = warp_max(amax);
+  if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
+  bar_sync(barrier, THREADS);
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
+  return scale_to<10>(amax, inverse);
+}
+
+// The tile's queries into shared memory, by eight threads each: as FP4 terms for pages, as FP16 for BF16 steps.
+template <int NT, int THREADS, typename Smem>
+__device__ __forceinline__ void load_queries(const TreeParams& p, Smem& sm, const Unit& u, int thread, float scale, bool terms) {
+  constexpr int kTermCodes = NT * 64;
+  const int group = thread & 7;
+#pragma unroll 1
+  for (int r = thread >> 3; r < (NT < THREADS / 8 ? THREADS / 8 : NT); r += THREADS / 8) {
+    float v[16];
+    load_query16<NT>(p, u, r, group, v);
+    if (r >= NT) continue;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] *= scale;
+    if (terms) {
+      const int at = r * 64 + group * 8;
+#pragma unroll 1
+      for (int term = 0; term < kTerms; ++term) {
+        float largest = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(v[j]));
+        const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
+        GroupCodes codes;
+        codes.scale = e4m3_to_float(byte);
+        // (an approximate reciprocal: what it rounds otherwise is left to the next term)
+        float inverse_scale;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse_scale) : "f"(fmaxf(codes.scale, 1.0e-30f)));
+        float scaled[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) scaled[j] = v[j] * inverse_scale;
+        codes.lo = pack_e2m1x8(scaled);
+        codes.hi = pack_e2m1x8(scaled + 8);
+        *reinterpret_cast<uint2*>(sm.q + term * kTermCodes + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
+        sm.q[kTerms * kTermCodes + term * 1024 + scale_tile_offset(r, group)] = (uint8_t)byte;
+        float rest[16];
+        group_residual16(v, codes, rest);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = rest[j];
+      }
+    } else {
+      uint8_t* row = sm.q + (group >> 2) * NT * 128 + r * 128;
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
+      const int chunk = (group & 3) * 2;
+      *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  tc::fence_proxy_async_smem();
+}
+
+// One stage's release, by a whole warp. A page's stage waits for its score product too; for a BF16 step's one
+// warp arrives in its place.
+template <typename Smem>
+__device__ __forceinline__ void release(Smem& sm, Place<Smem::kStages>& at, int thread, bool bf16) {
+  __syncwarp();
+  if ((thread & 31) == 0) tc::mbar_arrive(&sm.empty[at.slot]);
+  if (bf16 && thread == 0) tc::mbar_arrive(&sm.empty[at.slot]);
+  at.advance();
+}
+
+// The keys of a BF16 step: thread r of either half brings its half of token r's channels. Returns what undoes
+// the token's scaling.
+template <typename Smem>
+__device__ __forceinline__ float bf16_keys(const TreeParams& p, Smem& sm, int barrier, const Unit& u, StepKind kind,
+                                           Place<Smem::kStages> at, uint32_t operand, int thread) {
+  const int r = thread & 127, half = thread >> 7;
+  const int places = bf16_places(u.info, kind);
+  const bool two = places > kBf16Rows;
+  // a step's stages are held together
+  Place<Smem::kStages> second = at;
+  wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+  if (two) {
+    second.advance();
+    wait(&sm.full[second.slot], second.turn, &sm.abort_flag);
+  }
+  uint8_t* const stage0 = sm.ring[at.slot];
+  uint8_t* const stage1 = sm.ring[second.slot];
+  auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
+  bool there = r < places;
+  if (kind == kStepDraft) {
+    if (r < BDFP4_MAX_SINK) there = r < u.info.sink;
+    if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
+      const int group = thread & 7;
+      const float* shift = p.key_shift ? p.key_shift + u.head * kHeadDim + group * kGroup : nullptr;
+#pragma unroll 1
+      for (int first = 0; first < u.info.count; first += kCacheThreads / 8) {
+        // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
+        const int node = first + (thread >> 3);
+        uint4* at16 = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + min(node, u.info.count - 1)) + group * 32);
+        const uint4 raw[2] = {at16[0], at16[1]};
+        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+        __syncwarp();  // a thread that follows along may read the row that another of its warp writes
+        cache_basis16_any(v, group, p.rotate != 0, shift);
+        if (node < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at16), v);
+      }
+      tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
+      bar_sync(barrier, kCacheThreads);
+    }
+  }
+  const uint4* row = reinterpret_cast<const uint4*>(row_of(min(r, places - 1)));
+  float amax = 0.0f;
+  if (there) {
+#pragma unroll 4
+    for (int j = 0; j < 16; ++j) {
+      const uint4 q = row[j];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+    }
+  }
+  float inverse;
+  const float scale = scale_to<14>(amax, &inverse);
+#pragma unroll 1
+  for (int quarter = 2 * half; quarter < 2 * half + 2; ++quarter) {
+    uint32_t v[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (there) q = row[quarter * 4 + j];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
+    }
+    st16(operand + quarter * 16, v);
+  }
+  release(sm, at, thread, true);
+  if (two) release(sm, at, thread, true);
+  return inverse;
+}
+
+// The values of a BF16 step: half h brings the tokens of the step's stage h into channel r's lane.
+template <typename Smem>
+__device__ __forceinline__ void bf16_values(Smem& sm, const Unit& u, StepKind kind, Place<Smem::kStages>& at,
+                                            uint32_t operand, int thread) {
+  const int c = thread & 127, half = thread >> 7;
+  const int places = bf16_places(u.info, kind);
+  at.advance();  // the keys'
+  if (places > kBf16Rows) at.advance();
+#pragma unroll 1
+  for (int first = 0; first < places; first += kBf16Rows) {
+    wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+    if ((first > 0) == (half > 0)) {
+      const uint8_t* stage = sm.ring[at.slot] + 2 * c;
+      const int slices = (min(places - first, kBf16Rows) + 15) / 16;
+#pragma unroll 1
+      for (int s = 0; s < slices; ++s) {
+        const int place = first + s * 16;
+        const int stop = kind == kStepDraft && place == 0 ? u.info.sink : places;
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t lo = 0, hi = 0;
+          if (place + 2 * i < stop) lo = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i) * kBf16Pitch);
+          if (place + 2 * i + 1 < stop) hi = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i + 1) * kBf16Pitch);
+          v[i] = lo | (hi << 16);
+        }
+        st8(operand + (place >> 4) * 8, v);
+      }
+    }
+    release(sm, at, thread, true);
+  }
+}
+
 }  // namespace tree
 }  // namespace bdfp4

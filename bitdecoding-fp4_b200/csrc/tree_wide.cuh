@@ -1,7 +1,6 @@
 // The tree attention for tiles of 64 to 128 queries: the same products as tree_narrow.cuh's with warps of one role
-// each, one CTA per SM. A step's keys and values are converted once for up to 128 queries, so what bounds it is
-// the softmax: 128 x NT exponentials and their surroundings, four groups of 128 threads with at most 32 queries
-// per thread. Both products are kind::f16 with the converted cache side in tensor memory.
+// each, one CTA per SM. A step's values are converted once for up to 128 queries, so what bounds it is the softmax:
+// 128 x NT exponentials and their surroundings, up to four groups of 128 threads with at most 32 queries per thread.
 #pragma once
 
 #include "tree_common.cuh"
@@ -12,7 +11,7 @@ namespace wide {
 
 // Named barriers: one per softmax group (four at most), all softmax threads, the key threads.
 constexpr int kCtas = kTreeWideCtas;
-constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kKeysBarrier = 6;
+constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kCacheBarrier = 6;
 
 // A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (128
 // threads for NT = 64, 256 for 128) the kernel spilled, into an L1 that shared memory has left 24 KB of.
@@ -21,24 +20,25 @@ struct Shape {
   static constexpr int kColumns = NT < 32 ? NT : 32;        // queries per softmax thread
   static constexpr int kGroups = NT / kColumns;             // softmax groups of 128 threads
   static constexpr int kBlocks = (NT + 63) / 64;            // 128-byte rows of P per token
-  static constexpr int kKBuffers = NT > 96 ? 1 : 2;         // operand buffers in tensor memory, as many as it holds
-  static constexpr int kVBuffers = NT > 64 ? 1 : 2;
-  static constexpr int kStages = NT > 96 ? 5 : NT > 64 ? 6 : 8;
+  static constexpr int kVBuffers = NT > 96 ? 1 : 2;         // operand buffers in tensor memory, as many as it holds
+  static constexpr int kStages = NT > 64 ? 6 : 8;
   static constexpr int kSoftmaxThreads = 128 * kGroups;
-  static constexpr int kThreads = 256 + kSoftmaxThreads + 128;  // keys, values, softmax, control (two of its warps idle)
+  static constexpr int kThreads = kCacheThreads + kSoftmaxThreads + 128;  // cache side, softmax, control (two of its warps idle)
   // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
   // must not exceed what the launch was given.
   static constexpr int kLaunchRegs = kGroups == 4 ? 72 : kGroups == 3 ? 80 : kGroups == 2 ? 96 : 128;
   static constexpr int kSoftmaxRegs = kGroups == 4 ? 80 : kGroups == 3 ? 96 : kGroups == 2 ? 112 : 144;
-  static constexpr int kKeyRegs = kGroups == 4 ? 80 : kGroups == 3 ? 88 : kGroups == 2 ? 112 : 152;
-  static constexpr int kValueRegs = kGroups == 4 ? 64 : kGroups == 3 ? 64 : kGroups == 2 ? 88 : 128;
+  static constexpr int kCacheRegs = kGroups == 4 ? 72 : kGroups == 3 ? 72 : kGroups == 2 ? 96 : 128;
   static constexpr int kControlRegs = kGroups == 4 ? 40 : kGroups == 3 ? 40 : kGroups == 2 ? 56 : 88;
-  static_assert(kSoftmaxRegs * kGroups + kKeyRegs + kValueRegs + kControlRegs <= kLaunchRegs * (3 + kGroups), "registers");
+  static_assert(kSoftmaxRegs * kGroups + 2 * kCacheRegs + kControlRegs <= kLaunchRegs * (3 + kGroups), "registers");
   static_assert(kLaunchRegs * kThreads <= 65536, "registers");
   static constexpr bool kHold = kGroups <= 2;  // a thread's scores stay in registers between the vote and the exponentials
   // tensor memory columns
-  static constexpr int kS = 0, kO = 2 * NT, kK = 3 * NT, kV = kK + 64 * kKBuffers;
-  static_assert(kV + 64 * kVBuffers <= 512, "tensor memory");
+  // (the keys of a BF16 step lie where the pages' products had their scales: pages come first in a unit)
+  static constexpr int kS = 0, kO = 2 * NT, kV = 3 * NT, kK = kV + 64 * kVBuffers, kKs = kK, kQs = kKs + 16;
+  static_assert(kK + 64 <= 512 && kQs + 8 * kTerms <= kK + 64, "tensor memory");
+  // shared memory of the queries: FP4 terms (codes, then two scale atoms each) for the pages, then FP16
+  static constexpr int kTermCodes = NT * 64, kQueries = NT * 256 + kTerms * 1024;
 };
 
 template <int FROM, int TO>
@@ -50,21 +50,22 @@ __device__ __forceinline__ void trade_registers() {
 template <int NT>
 struct Smem {
   using Sh = Shape<NT>;
-  alignas(1024) uint8_t ring[Sh::kStages][kStage];
-  alignas(1024) uint8_t q[2][NT * 128];  // two halves of 64 channels, K-major, 128-byte swizzle
+  static constexpr int kStages = Sh::kStages;
+  alignas(1024) uint8_t ring[kStages][kStage];
+  // The queries. Against pages, kTerms tiles of FP4 codes (K-major, 64-byte swizzle), then as many pairs of scale
+  // atoms; against BF16 steps, FP16 in two halves of 64 channels (K-major, 128-byte swizzle).
+  alignas(1024) uint8_t q[Sh::kQueries];
   alignas(1024) uint8_t p[2][Sh::kBlocks * 16384];  // MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
-  float factor[NT];
-  float total[NT];
-  float col_max[4][NT];
-  float col_sum[4][NT];
+  float factor[NT];     // what a renewal does to sums (at a unit's end: 1 / weight)
+  float col[4][NT];     // a warp's maxima, then sums
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
   float q_max[16];
   int parents[BDFP4_MAX_TREE_NODES];
-  uint64_t full_k[Sh::kStages], full_v[Sh::kStages], empty[Sh::kStages];
-  uint64_t ka_full[2], ka_empty[2], va_full[2], va_empty[2];
+  uint64_t full[kStages], empty[kStages];
+  uint64_t ka_full, ka_empty, va_full[2], va_empty[2];  // operands: BF16 keys, values
   uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
   uint64_t q_full, o_full, o_empty, drained;
   long long sums[Sh::kThreads / 32];
@@ -74,118 +75,21 @@ struct Smem {
   int abort_flag, ignored_flag;
 };
 
-template <int NT, int PT>
-__device__ __forceinline__ void produce(const TreeParams& p, Smem<NT>& sm, Walker walker, const CUtensorMap* k_map,
-                                        const CUtensorMap* v_map, int lane) {
-  using Sh = Shape<NT>;
-  constexpr int kEntries = kPage / PT;
-  const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
-  int slot = 0, issued = 0;
-  uint32_t turn = 0;
-  auto advance = [&] {
-    ++issued;
-    if (++slot == Sh::kStages) slot = 0, turn ^= 1;
-  };
-  Unit u;
-  bool known = false;
-  for (; walker.next(u, known); known = true) {
-    const int32_t* table = p.table + u.row * p.table_stride;
-    const int stop = min(u.end, u.info.pages);
-    for (int batch = u.begin; batch < stop; batch += 32 / kEntries) {
-      const int entry = batch * kEntries + lane;
-      int mine = 0;
-      if (entry < stop * kEntries) {
-        mine = table[entry];
-        if (mine < 0 || mine >= p.pages) {
-          if (p.error_word) atomicOr(p.error_word, (int)BDFP4_DEV_BAD_PAGE);
-          mine = 0;
-        }
-      }
-      const int steps = min(32 / kEntries, stop - batch);
-      for (int i = 0; i < steps; ++i) {
-        int page[kEntries];
-#pragma unroll
-        for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
-        wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
-        if (elect_one()) {
-          uint8_t* stage = sm.ring[slot];
-          tc::mbar_expect_tx(&sm.full_k[slot], 9216);
-          tc::mbar_expect_tx(&sm.full_v[slot], 9216);
-          if constexpr (PT == 128) {
-            tc::tma_load_4d(stage, k_map, &sm.full_k[slot], 0, u.head, 0, page[0]);
-            tc::bulk_load(stage + kKsOffset, p.scales[0] + page[0] * p.scales_pitch[0] + u.head * 1024, 1024, &sm.full_k[slot]);
-            tc::tma_load_3d(stage + kVOffset, v_map, &sm.full_v[slot], 0, u.head * kHeadDim, page[0]);
-            tc::bulk_load(stage + kVsOffset, p.scales[1] + page[0] * p.scales_pitch[1] + u.head * 1024, 1024, &sm.full_v[slot]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < kEntries; ++e) {
-              tc::bulk_load(stage + e * 4096, p.codes[0] + page[e] * p.codes_pitch[0] + u.head * 4096, 4096, &sm.full_k[slot]);
-              tc::bulk_load(stage + kKsOffset + e * 512, p.scales[0] + page[e] * p.scales_pitch[0] + u.head * 512, 512,
-                            &sm.full_k[slot]);
-              tc::bulk_load(stage + kVOffset + e * 4096, p.codes[1] + page[e] * p.codes_pitch[1] + u.head * 4096, 4096,
-                            &sm.full_v[slot]);
-              tc::bulk_load(stage + kVsOffset + e * 512, p.scales[1] + page[e] * p.scales_pitch[1] + u.head * 512, 512,
-                            &sm.full_v[slot]);
-            }
-          }
-        }
-        __syncwarp();
-        advance();
-      }
-    }
-    for (int step = max(u.begin, u.info.pages); step < u.end; ++step) {
-      const StepKind kind = step_kind(u.info, step);
-      const int places = bf16_places(u.info, kind);
-      for (int side = 0; side < 2; ++side) {
-        const __nv_bfloat16* tail = (side ? p.tail_value : p.tail_key) + u.info.slot * p.tail_slot + u.head * kHeadDim;
-        const __nv_bfloat16* draft = side ? p.draft_value + u.row * p.draft_value_row + u.head * kHeadDim
-                                          : p.draft_key + u.row * p.draft_key_row + u.head * kHeadDim;
-        const int64_t draft_node = side ? p.draft_value_node : p.draft_key_node;
-        for (int first = 0; first < places; first += kBf16Rows) {
-          const int end = min(first + kBf16Rows, places);
-          uint64_t* full = side ? &sm.full_v[slot] : &sm.full_k[slot];
-          wait(&sm.empty[slot], turn ^ 1, &sm.abort_flag);
-          if (elect_one()) {
-            // the sink's places behind its length stay empty
-            const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
-            tc::mbar_expect_tx(full, (end - first - absent) * 256);
-            tc::mbar_arrive(side ? &sm.full_k[slot] : &sm.full_v[slot]);  // the other side only passes the stage on
-          }
-          __syncwarp();
-          for (int i = first + lane; i < end; i += 32) {
-            const __nv_bfloat16* source = nullptr;
-            if (kind == kStepTail) source = tail + i * tail_row;
-            else if (i >= BDFP4_MAX_SINK) source = draft + (i - BDFP4_MAX_SINK) * draft_node;
-            else if (i < u.info.sink) source = tail + (kPage + i) * tail_row;
-            if (source) tc::bulk_load(sm.ring[slot] + (i - first) * kBf16Pitch, source, 256, full);
-          }
-          __syncwarp();
-          advance();
-        }
-      }
-    }
-  }
-  // After an abort nobody else waits for the copies still in flight: no CTA may end under them.
-  if (lane == 0 && *static_cast<volatile int*>(&sm.abort_flag)) {
-    for (int back = min(issued, Sh::kStages); back > 0; --back) {
-      const int at = issued - back;
-      wait(&sm.full_k[at % Sh::kStages], (at / Sh::kStages) & 1, &sm.ignored_flag);
-      wait(&sm.full_v[at % Sh::kStages], (at / Sh::kStages) & 1, &sm.ignored_flag);
-    }
-  }
-  __syncwarp();
-}
-
 // The whole warp walks and waits; one thread of it issues.
-template <int NT>
-__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
+template <int NT, int PT>
+__device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
   using Sh = Shape<NT>;
-  constexpr uint32_t kScores = f16_idesc(NT, 0, false), kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
+  constexpr uint32_t kFp4 = tc::nvf4_idesc(128, NT), kF16 = f16_idesc(NT, 0, false);
+  constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
-  const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p);
+  const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p), ring = tc::smem_u32(sm.ring);
+  const uint64_t q_codes = tc::fp4_tile_desc(q, 0), q_scales = tc::sf_atom_desc(q + kTerms * Sh::kTermCodes);
   int n = 0, unit = 0;
+  uint32_t q_turn = 0, ka_turn = 0;
+  Place<Sh::kStages> at;
   Unit u;
   bool known = false;
+#pragma unroll 1
   for (; walker.next(u, known); known = true) {
     auto output = [&](int step, int j) {  // O^T += V^T P^T of step `step` of the unit, the CTA's j-th
       const StepKind kind = step_kind(u.info, step);
@@ -212,21 +116,57 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
       }
       __syncwarp();
     };
-    wait(&sm.q_full, unit & 1, &sm.abort_flag);
+#pragma unroll 1
     for (int step = u.begin; step < u.end; ++step, ++n) {
-      const int a = n % Sh::kKBuffers;
-      wait(&sm.ka_full[a], (n / Sh::kKBuffers) & 1, &sm.abort_flag);
-      wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
-      tc::fence_after_sync();
-      if (elect_one()) {
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          mma_ts(tmem + Sh::kS + (n & 1) * NT, tmem + Sh::kK + a * 64 + s * 8,
-                 tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kScores, s > 0);
-        tc::commit(&sm.s_full[n & 1]);
-        tc::commit(&sm.ka_empty[a]);
+      const StepKind kind = step_kind(u.info, step);
+      if (step == u.begin || step == u.info.pages) {  // the queries come in the form of the step, and once more for BF16
+        wait(&sm.q_full, q_turn, &sm.abort_flag);
+        q_turn ^= 1;
       }
-      __syncwarp();
+      const uint32_t scores = tmem + Sh::kS + (n & 1) * NT;
+      wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
+      if (kind == kStepPage) {
+        wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+        if constexpr (PT == 64) interleave_scales(sm.ring[at.slot] + kKsOffset, lane);
+        tc::fence_after_sync();
+        const uint32_t stage = ring + at.slot * kStage;
+        const uint64_t codes = tc::fp4_tile_desc(stage, 0), atoms = tc::sf_atom_desc(stage + kKsOffset);
+        const uint32_t scales = tmem + Sh::kKs + (n & 1) * 8;
+        if (elect_one()) {
+          if (step == u.begin) {
+#pragma unroll 1
+            for (int i = 0; i < 2 * kTerms; ++i) tc::cp_sf_atom(tmem + Sh::kQs + i * 4, q_scales + i * 32);
+          }
+          tc::cp_sf_atom(scales, atoms);
+          tc::cp_sf_atom(scales + 4, atoms + 32);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term)
+              tc::mma_nvf4(scores, codes + 2 * s, q_codes + term * (Sh::kTermCodes / 16) + 2 * s, kFp4, scales + 4 * s,
+                           tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
+          }
+          tc::commit(&sm.s_full[n & 1]);
+          tc::commit(&sm.empty[at.slot]);
+        }
+        __syncwarp();
+        at.advance();
+      } else {
+#pragma unroll 1
+        for (int i = 2 * bf16_stages(u.info, kind); i > 0; --i) at.advance();
+        if (elect_one()) tc::commit(&sm.ka_empty);  // behind every product that reads scales or keys there
+        __syncwarp();
+        wait(&sm.ka_full, ka_turn, &sm.abort_flag);
+        ka_turn ^= 1;
+        tc::fence_after_sync();
+        if (elect_one()) {
+#pragma unroll 1
+          for (int s = 0; s < 8; ++s)
+            mma_ts(scores, tmem + Sh::kK + s * 8, tc::bf16_tile_desc(q + (s >> 2) * NT * 128, s & 3), kF16, s > 0);
+          tc::commit(&sm.s_full[n & 1]);
+        }
+        __syncwarp();
+      }
       if (step > u.begin) output(step - 1, n - 1);
     }
     output(u.end - 1, n - 1);
@@ -240,259 +180,70 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker) {
   wait(&sm.drained, 0, &sm.ignored_flag);
 }
 
-// One side of the ring as its consumers (four warps) see it.
-template <int NT>
-struct Ring {
-  Smem<NT>& sm;
-  uint64_t* full;
-  int lane, slot;
-  uint32_t turn;
-  __device__ Ring(Smem<NT>& s, uint64_t* f, int l) : sm(s), full(f), lane(l), slot(0), turn(0) {}
-  __device__ __forceinline__ const uint8_t* arrived() {
-    wait(&full[slot], turn, &sm.abort_flag);
-    return sm.ring[slot];
-  }
-  __device__ __forceinline__ void release() {
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.empty[slot]);
-    if (++slot == Shape<NT>::kStages) slot = 0, turn ^= 1;
-  }
-  __device__ __forceinline__ void pass(int stages) {
-    for (int i = 0; i < stages; ++i) {
-      arrived();
-      release();
-    }
-  }
-};
-
-// Keys: thread t holds token t of every step.
+// The cache side: half h of the threads converts tokens 64 h to 64 h + 63 of channel c of every step.
 template <int NT, int PT>
-__device__ __forceinline__ void keys(const TreeParams& p, Smem<NT>& sm, Walker walker, int t) {
+__device__ __forceinline__ void cache(const TreeParams& p, Smem<NT>& sm, Walker walker, int thread) {
   using Sh = Shape<NT>;
-  const int lane = t & 31;
-  const uint32_t tmem = sm.tmem + Sh::kK + ((uint32_t)(t & ~31) << 16);
-  Ring<NT> ring(sm, sm.full_k, lane);
+  const int c = thread & 127, half = thread >> 7, lane = thread & 31;
+  const uint32_t lanes = sm.tmem + ((uint32_t)(c & ~31) << 16);
+  const int codes = kVOffset + (PT == 128 ? c * 64 : half * 4096 + c * 32);
+  const int chunk = PT == 128 ? ((2 * half) ^ ((c >> 1) & 3)) * 16 : ((c >> 2) & 1) * 16;  // the other one's is 16 off
+  const int scales = kVsOffset + half * 512 + (c & 31) * 16 + (c >> 5) * 4;
+  Place<Sh::kStages> at;
   int n = 0;
+  uint32_t ka_turn = 0;
   Unit u;
   bool known = false;
-  for (; walker.next(u, known); known = true) {
-    for (int step = u.begin; step < u.end; ++step, ++n) {
-      const StepKind kind = step_kind(u.info, step);
-      const uint32_t operand = tmem + (n % Sh::kKBuffers) * 64;
-      uint64_t* operand_empty = &sm.ka_empty[n % Sh::kKBuffers];
-      const uint32_t empty_parity = ((n / Sh::kKBuffers) & 1) ^ 1;
-      if (kind == kStepPage) {
-        const uint8_t* stage = ring.arrived();
-        uint4 chunk[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) chunk[j] = *reinterpret_cast<const uint4*>(stage + t * 64 + ((j ^ ((t >> 1) & 3)) * 16));
-        const uint8_t* at = PT == 128 ? stage + kKsOffset + (t & 31) * 16 + (t >> 5) * 4
-                                      : stage + kKsOffset + (t >> 6) * 512 + (t & 31) * 8 + ((t >> 5) & 1) * 4;
-        const uint32_t scales[2] = {*reinterpret_cast<const uint32_t*>(at),
-                                    *reinterpret_cast<const uint32_t*>(at + (PT == 128 ? 512 : 256))};
-        ring.release();
-        wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) store_dequantized(operand + 16 * j, chunk[j], scales[j >> 1] >> (16 * (j & 1)));
-      } else {
-        const int places = bf16_places(u.info, kind);
-        const int stages = (places + kBf16Rows - 1) / kBf16Rows;
-        // a step's stages are held together; both have arrived when each has been waited for
-        ring.arrived();
-        uint8_t* const stage0 = sm.ring[ring.slot];
-        uint8_t* stage1 = stage0;
-        if (stages > 1) {
-          const bool wraps = ring.slot + 1 == Sh::kStages;
-          const int next = wraps ? 0 : ring.slot + 1;
-          wait(&sm.full_k[next], ring.turn ^ (wraps ? 1u : 0u), &sm.abort_flag);
-          stage1 = sm.ring[next];
-        }
-        auto row_of = [&](int place) { return (place < kBf16Rows ? stage0 : stage1) + (place & (kBf16Rows - 1)) * kBf16Pitch; };
-        bool there = t < places;
-        if (kind == kStepDraft) {
-          if (t < BDFP4_MAX_SINK) there = t < u.info.sink;
-          if (p.rotate || p.key_shift) {  // eight threads bring one draft key into the cache's basis, in place
-            const int group = t & 7;
-            const float* shift = p.key_shift ? p.key_shift + u.head * kHeadDim + group * kGroup : nullptr;
-            for (int first = 0; first < u.info.count; first += 16) {
-              // (threads past the last draft follow along for the exchange; what they make of it goes nowhere)
-              const int node = min(first + (t >> 3), u.info.count - 1);
-              uint4* at = reinterpret_cast<uint4*>(row_of(BDFP4_MAX_SINK + node) + group * 32);
-              const uint4 raw[2] = {at[0], at[1]};
-              const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-              float v[16];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-              }
-              cache_basis16_any(v, group, p.rotate != 0, shift);
-              if (first + (t >> 3) < u.info.count) store_bf16x16(reinterpret_cast<__nv_bfloat16*>(at), v);
-            }
-            tc::fence_proxy_async_smem();  // the stage is overwritten by copies next
-            bar_sync(kKeysBarrier, 128);
-          }
-        }
-        const uint4* row = reinterpret_cast<const uint4*>(row_of(min(t, places - 1)));
-        float amax = 0.0f;
-        if (there) {
-#pragma unroll 4
-          for (int j = 0; j < 16; ++j) {
-            const uint4 r = row[j];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-          }
-        }
-        float inverse;
-        const float scale = scale_to<14>(amax, &inverse);
-        sm.key_factor[n & 7][t] = inverse;
-        wait(operand_empty, empty_parity, &sm.abort_flag);
-        tc::fence_after_sync();
 #pragma unroll 1
-        for (int quarter = 0; quarter < 4; ++quarter) {
-          uint32_t v[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 r = make_uint4(0, 0, 0, 0);
-            if (there) r = row[quarter * 4 + j];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[4 * j + i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale));
-          }
-          st16(operand + quarter * 16, v);
-        }
-        for (int i = 0; i < stages; ++i) ring.release();
-        ring.pass(stages);  // the values'
-      }
-      tc::tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.ka_full[n % Sh::kKBuffers]);
-    }
-  }
-}
-
-// Values: thread c holds channel c of every step.
-template <int NT, int PT>
-__device__ __forceinline__ void values(const TreeParams& p, Smem<NT>& sm, Walker walker, int c) {
-  using Sh = Shape<NT>;
-  const int lane = c & 31;
-  const uint32_t tmem = sm.tmem + Sh::kV + ((uint32_t)(c & ~31) << 16);
-  Ring<NT> ring(sm, sm.full_v, lane);
-  int n = 0;
-  Unit u;
-  bool known = false;
   for (; walker.next(u, known); known = true) {
+#pragma unroll 1
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      const uint32_t operand = tmem + (n % Sh::kVBuffers) * 64;
-      uint64_t* operand_empty = &sm.va_empty[n % Sh::kVBuffers];
+      const int buffer = n % Sh::kVBuffers;
+      const uint32_t operand = lanes + Sh::kV + buffer * 64;
       const uint32_t empty_parity = ((n / Sh::kVBuffers) & 1) ^ 1;
       if (kind == kStepPage) {
-        const uint8_t* stage = ring.arrived();
-        uint4 chunk[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint8_t* at = PT == 128 ? stage + kVOffset + c * 64 + ((j ^ ((c >> 1) & 3)) * 16)
-                                        : stage + kVOffset + (j >> 1) * 4096 + c * 32 + (((j & 1) ^ ((c >> 2) & 1)) * 16);
-          chunk[j] = *reinterpret_cast<const uint4*>(at);
-        }
-        const uint8_t* at = stage + kVsOffset + (c & 31) * 16 + (c >> 5) * 4;
-        const uint32_t scales[2] = {*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + 512)};
-        ring.release();
-        wait(operand_empty, empty_parity, &sm.abort_flag);
+        wait(&sm.full[at.slot], at.turn, &sm.abort_flag);
+        const uint8_t* stage = sm.ring[at.slot];
+        const uint32_t scale = *reinterpret_cast<const uint32_t*>(stage + scales);
+        const uint4 chunk0 = *reinterpret_cast<const uint4*>(stage + codes + chunk);
+        const uint4 chunk1 = *reinterpret_cast<const uint4*>(stage + codes + (chunk ^ 16));
+        release(sm, at, thread, false);
+        wait(&sm.va_empty[buffer], empty_parity, &sm.abort_flag);
         tc::fence_after_sync();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) store_dequantized(operand + 16 * j, chunk[j], scales[j >> 1] >> (16 * (j & 1)));
+        store_dequantized(operand + 32 * half, chunk0, scale);
+        store_dequantized(operand + 32 * half + 16, chunk1, scale >> 16);
       } else {
-        const int places = bf16_places(u.info, kind);
-        ring.pass((places + kBf16Rows - 1) / kBf16Rows);  // the keys'
-        wait(operand_empty, empty_parity, &sm.abort_flag);
+        wait(&sm.ka_empty, ka_turn, &sm.abort_flag);
+        ka_turn ^= 1;
         tc::fence_after_sync();
-        for (int first = 0; first < places; first += kBf16Rows) {
-          const uint8_t* stage = ring.arrived() + 2 * c;
-          const int slices = (min(places - first, kBf16Rows) + 15) / 16;
-          for (int s = 0; s < slices; ++s) {
-            const int place = first + s * 16;
-            const int stop = kind == kStepDraft && place == 0 ? u.info.sink : places;
-            uint32_t v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint32_t lo = 0, hi = 0;
-              if (place + 2 * i < stop) lo = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i) * kBf16Pitch);
-              if (place + 2 * i + 1 < stop) hi = *reinterpret_cast<const uint16_t*>(stage + (s * 16 + 2 * i + 1) * kBf16Pitch);
-              v[i] = lo | (hi << 16);
-            }
-            st8(operand + (place >> 4) * 8, v);
-          }
-          ring.release();
-        }
+        const float inverse = bf16_keys(p, sm, kCacheBarrier, u, kind, at, lanes + Sh::kK, thread);
+        if (half == 0) sm.key_factor[n & 7][c] = inverse;
+        tc::tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.ka_full);
+        wait(&sm.va_empty[buffer], empty_parity, &sm.abort_flag);
+        tc::fence_after_sync();
+        bf16_values(sm, u, kind, at, operand, thread);
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.va_full[n % Sh::kVBuffers]);
+      if (lane == 0) tc::mbar_arrive(&sm.va_full[buffer]);
     }
   }
 }
 
-// The tile's queries into shared memory: rotated if asked, scaled by one power of two into FP16's range
-// (rows of the tile whose largest value is 2^-29 of the tile's keep full precision). Returns what undoes it.
+// The queries of a unit's first step into shared memory. Returns their scale, and what undoes it.
 template <int NT>
-__device__ __forceinline__ float load_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
-  using Sh = Shape<NT>;
-  constexpr int kPerPass = Sh::kSoftmaxThreads / 8, kPasses = NT / kPerPass;
-  const int group = thread & 7;
-  const int queries = u.info.count * p.ratio;
-  float v[kPasses][16];
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int query = u.tile * NT + i * kPerPass + (thread >> 3);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[i][j] = 0.0f;
-    if (query < queries)
-      load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
-                       (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
-  }
-  if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    if (p.rotate) {
-      hadamard_butterflies(v[i], group);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[i][j] *= kInvSqrt128;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (fabsf(v[i][j]) < INFINITY) amax = fmaxf(amax, fabsf(v[i][j]));
-  }
-  amax = warp_max(amax);
-  if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
-  bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);
-#pragma unroll
-  for (int w = 0; w < Sh::kSoftmaxThreads / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
-  float inverse;
-  const float scale = scale_to<14>(amax, &inverse);
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int r = i * kPerPass + (thread >> 3);
-    uint8_t* row = sm.q[group >> 2] + r * 128;
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[i][2 * j] * scale, v[i][2 * j + 1] * scale));
-    const int chunk = (group & 3) * 2;
-    *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
-  }
-  tc::fence_proxy_async_smem();
-  bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);
-  if (thread == 0) tc::mbar_arrive(&sm.q_full);
-  return inverse;
+__device__ __forceinline__ float first_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread, float* inverse) {
+  constexpr int kThreads = Shape<NT>::kSoftmaxThreads;
+  const float scale = query_scale<NT, kThreads>(p, sm, kSoftmaxBarrier, u, thread, inverse);
+  load_queries<NT, kThreads>(p, sm, u, thread, scale, u.begin < u.info.pages);
+  __syncwarp();
+  if ((thread & 31) == 0) tc::mbar_arrive(&sm.q_full);
+  return scale;
 }
 
 template <int NT>
@@ -509,7 +260,8 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
   Unit u;
   if (!walker.next(u, false)) return;
   bool more = true;
-  float q_inverse = load_queries<NT>(p, sm, u, thread);
+  float q_inverse;
+  float q_scale = first_queries<NT>(p, sm, u, thread, &q_inverse);
   while (more) {
     for (int j = t; j < C; j += 128) {
       top[j] = kNoMax;
@@ -537,6 +289,11 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
       const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
       const int node = t - BDFP4_MAX_SINK;
+      if (step == u.info.pages && step > u.begin) {  // (the pages' last scores have been waited for)
+        load_queries<NT, Sh::kSoftmaxThreads>(p, sm, u, thread, q_scale, false);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.q_full);
+      }
       wait(&sm.s_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
       tc::fence_after_sync();
       float f = page_factor;
@@ -583,14 +340,14 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
             const float m = warp_max(dead ? -INFINITY : s[i] * f);
             if (lane == i) mine = m;
           }
-          if (lane < 16) sm.col_max[warp][first_column + j + lane] = mine;
+          if (lane < 16) sm.col[warp][first_column + j + lane] = mine;
         }
         bar_sync(barrier, 128);
         for (int j = t; j < C; j += 128) {
           const int col = first_column + j;
           const float before = top[j];
-          const float now = fmaxf(fmaxf(fmaxf(sm.col_max[0][col], sm.col_max[1][col]),
-                                        fmaxf(sm.col_max[2][col], sm.col_max[3][col])), before);
+          const float now = fmaxf(fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]),
+                                        fmaxf(sm.col[2][col], sm.col[3][col])), before);
           top[j] = now;
           base[j] = kShift - now;
           sm.factor[col] = ex2(before - now);
@@ -674,23 +431,23 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       float v[C];
 #pragma unroll
       for (int j = 0; j < C / 2; ++j) v[2 * j] = sum[j].x, v[2 * j + 1] = sum[j].y;
-      reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col_sum[warp][first_column + j] = total; });
+      reduce_columns<C, 16>(v, lane, 0, [&](int j, float total) { sm.col[warp][first_column + j] = total; });
     }
     // the next unit's queries go in while this one's last product runs: all its scores are done
     Unit following = u;
     more = walker.next(following, true);
-    float next_inverse = 1.0f;
+    float next_inverse = 1.0f, next_scale = 1.0f;
     bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);  // both groups have seen their last scores; the parents are free
-    if (more) next_inverse = load_queries<NT>(p, sm, following, thread);
+    if (more) next_scale = first_queries<NT>(p, sm, following, thread, &next_inverse);
     bar_sync(barrier, 128);
     const bool whole = u.begin == 0 && u.end == u.info.steps;
     // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
     const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
     for (int j = t; j < C; j += 128) {
       const int col = first_column + j;
-      const float total = (sm.col_sum[0][col] + sm.col_sum[1][col]) + (sm.col_sum[2][col] + sm.col_sum[3][col]);
+      const float total = (sm.col[0][col] + sm.col[1][col]) + (sm.col[2][col] + sm.col[3][col]);
       if (whole) {
-        sm.total[col] = total > 0.0f ? p.value_scale / total : 0.0f;
+        sm.factor[col] = total > 0.0f ? p.value_scale / total : 0.0f;
       } else {
         p.partial_stat[(int64_t)(2 * part) * NT + col] = top[j];
         p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
@@ -713,7 +470,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       for (int i = 0; i < 16; ++i) {
         if (j + i < queries) {
           if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.total[first_column + j + i]);
+            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.factor[first_column + j + i]);
             if (++out_head == p.ratio) out_head = 0, ++out_node;
           } else {
             partial[(int64_t)(j + i) * kHeadDim] = o[i];
@@ -735,6 +492,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       p.splits[blockIdx.x] = split;
     }
     q_inverse = next_inverse;
+    q_scale = next_scale;
     u = following;
     ++unit;
   }
@@ -758,22 +516,23 @@ tree_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   for (int step = 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
   if (lane == 0) sm.sums[warp] = mine;
   if (thread == 0) {
+#pragma unroll 1
     for (int i = 0; i < Sh::kStages; ++i) {
-      tc::mbar_init(&sm.full_k[i], 1);
-      tc::mbar_init(&sm.full_v[i], 1);
-      tc::mbar_init(&sm.empty[i], 8);
+      tc::mbar_init(&sm.full[i], 1);
+      tc::mbar_init(&sm.empty[i], 9);  // the cache side's warps and the score product
     }
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&sm.ka_full[i], 4);
-      tc::mbar_init(&sm.va_full[i], 4);
-      tc::mbar_init(&sm.ka_empty[i], 1);
+      tc::mbar_init(&sm.va_full[i], 8);
       tc::mbar_init(&sm.va_empty[i], 1);
       tc::mbar_init(&sm.s_full[i], 1);
       tc::mbar_init(&sm.s_empty[i], 4 * Sh::kGroups);
       tc::mbar_init(&sm.p_full[i], 4 * Sh::kGroups);
       tc::mbar_init(&sm.p_empty[i], 1);
     }
-    tc::mbar_init(&sm.q_full, 1);
+    tc::mbar_init(&sm.ka_full, 8);
+    tc::mbar_init(&sm.ka_empty, 1);
+    tc::mbar_init(&sm.q_full, 4 * Sh::kGroups);
     tc::mbar_init(&sm.o_full, 1);
     tc::mbar_init(&sm.o_empty, 4 * Sh::kGroups);
     tc::mbar_init(&sm.drained, 1);
@@ -826,19 +585,16 @@ tree_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   tc::fence_after_sync();
   if (sm.first < sm.last) {
     const Walker walker(p, sm.start_row, (int)sm.start_offset, (int)(sm.last - sm.first), PT);
-    if (warp < 4) {
-      trade_registers<Sh::kLaunchRegs, Sh::kKeyRegs>();
-      keys<NT, PT>(p, sm, walker, thread);
-    } else if (warp < 8) {
-      trade_registers<Sh::kLaunchRegs, Sh::kValueRegs>();
-      values<NT, PT>(p, sm, walker, thread - 128);
+    if (warp < 8) {
+      trade_registers<Sh::kLaunchRegs, Sh::kCacheRegs>();
+      cache<NT, PT>(p, sm, walker, thread);
     } else if (warp < 8 + 4 * Sh::kGroups) {
       trade_registers<Sh::kLaunchRegs, Sh::kSoftmaxRegs>();
       softmax<NT>(p, sm, walker, thread - 256);
     } else {
       trade_registers<Sh::kLaunchRegs, Sh::kControlRegs>();
-      if (warp == 8 + 4 * Sh::kGroups) produce<NT, PT>(p, sm, walker, &k_map, &v_map, lane);
-      if (warp == 9 + 4 * Sh::kGroups) issue<NT>(sm, walker);
+      if (warp == 8 + 4 * Sh::kGroups) produce<PT>(p, sm, walker, &k_map, &v_map, lane);
+      if (warp == 9 + 4 * Sh::kGroups) issue<NT, PT>(sm, walker, lane);
     }
   }
   tc::fence_before_sync();
