@@ -392,92 +392,86 @@ __device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
   __syncwarp();
 }
 
-// A group of a query: zero outside the tile; rotated if asked.
-template <int NT>
-__device__ __forceinline__ void load_query16(const TreeParams& p, const Unit& u, int r, int group, float* v) {
-  const int queries = min(u.info.count * p.ratio - u.tile * NT, NT), query = u.tile * NT + r;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-  if (r < queries)
-    load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
-                     (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v);
-  if (p.rotate) {
-    hadamard_butterflies(v, group);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] *= kInvSqrt128;
-  }
-}
-
-// The power of two that the tile's queries are scaled with: a query whose largest value is 2^-8 of the tile's
-// still has all four terms above E4M3's smallest scale.
+// The tile's queries into shared memory, a group of sixteen values per thread and pass: as kTerms FP4 terms for the
+// pages, and as FP16 for the BF16 steps. Rotated if asked, and scaled by one power of two: a query whose largest
+// value is 2^-8 of the tile's still has all four terms above E4M3's smallest scale. Returns what undoes the scale.
 template <int NT, int THREADS, typename Smem>
-__device__ __forceinline__ float query_scale(const TreeParams& p, Smem& sm, int barrier, const Unit& u, int thread, float* inverse) {
-  float amax = 0.0f;
+__device__ __forceinline__ float load_queries(const TreeParams& p, Smem& sm, int barrier, const Unit& u, int thread) {
+  constexpr int kPerPass = THREADS / 8, kPasses = (NT + kPerPass - 1) / kPerPass;
+  const int group = thread & 7;
+  const int queries = min(u.info.count * p.ratio - u.tile * NT, NT);
+  float v[kPasses][16];
 #pragma unroll
-  for (int r = thread >> 3; r < (NT < THREADS / 8 ? THREADS / 8 : NT); r += THREADS / 8) {
-    float v[16];
-    load_query16<NT>(p, u, r, thread & 7, v);
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = i * kPerPass + (thread >> 3), query = u.tile * NT + r;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
+    for (int j = 0; j < 16; ++j) v[i][j] = 0.0f;
+    if (r < queries)
+      load_bf16x16(p.query + u.row * p.query_row + (query / p.ratio) * p.query_node +
+                       (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
   }
   if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    if (p.rotate) {
+      hadamard_butterflies(v[i], group);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[i][j] *= kInvSqrt128;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (fabsf(v[i][j]) < INFINITY) amax = fmaxf(amax, fabsf(v[i][j]));
+  }
   amax = warp_max(amax);
   if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
   bar_sync(barrier, THREADS);
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) amax = fmaxf(amax, sm.q_max[w]);
-  return scale_to<10>(amax, inverse);
-}
-
-// The tile's queries into shared memory, by eight threads each: as FP4 terms for pages, as FP16 for BF16 steps.
-template <int NT, int THREADS, typename Smem>
-__device__ __forceinline__ void load_queries(const TreeParams& p, Smem& sm, const Unit& u, int thread, float scale, bool terms) {
-  constexpr int kTermCodes = NT * 64;
-  const int group = thread & 7;
-#pragma unroll 1
-  for (int r = thread >> 3; r < (NT < THREADS / 8 ? THREADS / 8 : NT); r += THREADS / 8) {
-    float v[16];
-    load_query16<NT>(p, u, r, group, v);
-    if (r >= NT) continue;
+  for (int i = 0; i < THREADS / 32; ++i) amax = fmaxf(amax, sm.q_max[i]);
+  float inverse;
+  const float scale = scale_to<10>(amax, &inverse);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] *= scale;
-    if (terms) {
-      const int at = r * 64 + group * 8;
-#pragma unroll 1
-      for (int term = 0; term < kTerms; ++term) {
-        float largest = 0.0f;
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = i * kPerPass + (thread >> 3);
+    if (kPasses * kPerPass > NT && r >= NT) break;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(v[j]));
-        const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
-        GroupCodes codes;
-        codes.scale = e4m3_to_float(byte);
-        // (an approximate reciprocal: what it rounds otherwise is left to the next term)
-        float inverse_scale;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse_scale) : "f"(fmaxf(codes.scale, 1.0e-30f)));
-        float scaled[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) scaled[j] = v[j] * inverse_scale;
-        codes.lo = pack_e2m1x8(scaled);
-        codes.hi = pack_e2m1x8(scaled + 8);
-        *reinterpret_cast<uint2*>(sm.q + term * kTermCodes + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
-        sm.q[kTerms * kTermCodes + term * 1024 + scale_tile_offset(r, group)] = (uint8_t)byte;
-        float rest[16];
-        group_residual16(v, codes, rest);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = rest[j];
-      }
-    } else {
-      uint8_t* row = sm.q + (group >> 2) * NT * 128 + r * 128;
+    for (int j = 0; j < 16; ++j) v[i][j] *= scale;
+    {
+      uint8_t* row = sm.q[group >> 2] + r * 128;
       uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
+      for (int j = 0; j < 8; ++j) w[j] = h2(__floats2half2_rn(v[i][2 * j], v[i][2 * j + 1]));
       const int chunk = (group & 3) * 2;
       *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
       *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) * 16)) = make_uint4(w[4], w[5], w[6], w[7]);
     }
+    const int at = r * 64 + group * 8;
+#pragma unroll 1
+    for (int term = 0; term < kTerms; ++term) {
+      float largest = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) largest = fmaxf(largest, fabsf(v[i][j]));
+      const uint32_t byte = cvt_e4m3(largest * (1.0f / 6.0f));
+      GroupCodes codes;
+      codes.scale = e4m3_to_float(byte);
+      // (an approximate reciprocal: what it rounds otherwise is left to the next term)
+      float inverse_scale;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse_scale) : "f"(fmaxf(codes.scale, 1.0e-30f)));
+      float scaled[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) scaled[j] = v[i][j] * inverse_scale;
+      codes.lo = pack_e2m1x8(scaled);
+      codes.hi = pack_e2m1x8(scaled + 8);
+      *reinterpret_cast<uint2*>(sm.q_codes[term] + (at ^ (((at >> 7) & 3) << 4))) = make_uint2(codes.lo, codes.hi);
+      sm.q_scales[term][scale_tile_offset(r, group)] = (uint8_t)byte;
+      float rest[16];
+      group_residual16(v[i], codes, rest);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[i][j] = rest[j];
+    }
   }
   tc::fence_proxy_async_smem();
+  return inverse;
 }
 
 // One stage's release, by a whole warp. A page's stage waits for its score product too; for a BF16 step's one

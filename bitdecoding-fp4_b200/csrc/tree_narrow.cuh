@@ -50,8 +50,6 @@ struct Shape {
   // (the keys of a BF16 step lie where a page's product had its scales: pages come first in a unit)
   static constexpr int kS = 0, kO = NT, kV = 2 * NT, kK = kV + 64, kKs = kK, kQs = kKs + 8;
   static_assert(kK + 64 <= kTmemColumns && kQs + 8 * kTerms <= kTmemColumns, "tensor memory");
-  // shared memory of the queries: FP4 terms (codes, then two scale atoms each) for the pages, then FP16
-  static constexpr int kTermCodes = NT * 64, kQueries = NT * 256 + kTerms * 1024;
 };
 
 template <int NT>
@@ -59,9 +57,9 @@ struct Smem {
   using Sh = Shape<NT>;
   static constexpr int kStages = 4;  // as many as two CTAs' shared memory holds
   alignas(1024) uint8_t ring[kStages][kStage];
-  // The queries. Against pages, kTerms tiles of FP4 codes (K-major, 64-byte swizzle), then as many pairs of scale
-  // atoms; against BF16 steps, FP16 in two halves of 64 channels (K-major, 128-byte swizzle).
-  alignas(1024) uint8_t q[Sh::kQueries];
+  alignas(1024) uint8_t q[2][NT * 128];            // FP16 queries: two halves of 64 channels, K-major, 128-byte swizzle
+  alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
+  alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
   alignas(1024) uint8_t p[16384];        // MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum, 0 while there is none
@@ -87,7 +85,8 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
   constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const uint32_t q = tc::smem_u32(sm.q), ring = tc::smem_u32(sm.ring);
-  const uint64_t q_codes = tc::fp4_tile_desc(q, 0), q_scales = tc::sf_atom_desc(q + kTerms * Sh::kTermCodes);
+  const uint64_t q_codes = tc::fp4_tile_desc(tc::smem_u32(sm.q_codes), 0);
+  const uint64_t q_scales = tc::sf_atom_desc(tc::smem_u32(sm.q_scales));
   const uint64_t tile = tc::smem_desc(tc::smem_u32(sm.p), tc::kSwizzle128B, 1024, 16384);
   uint32_t k_parity = 0, p_parity = 0;
   Place<Smem<NT>::kStages> at;
@@ -119,7 +118,7 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
             for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
 #pragma unroll
               for (int term = 0; term < kTerms; ++term)
-                tc::mma_nvf4(tmem + Sh::kS, codes + 2 * s, q_codes + term * (Sh::kTermCodes / 16) + 2 * s, kFp4,
+                tc::mma_nvf4(tmem + Sh::kS, codes + 2 * s, q_codes + term * NT * 4 + 2 * s, kFp4,
                              tmem + Sh::kKs + 4 * s, tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
             }
             tc::commit(&sm.s_full);
@@ -193,9 +192,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
   bool known = false;
 #pragma unroll 1
   for (; walker.next(u, known); known = true) {
-    float q_inverse;
-    const float q_scale = query_scale<NT, kWorkers>(p, sm, kWorkBarrier, u, thread, &q_inverse);
-    if (u.begin < u.info.pages) load_queries<NT, kWorkers>(p, sm, u, thread, q_scale, true);
+    const float q_inverse = load_queries<NT, kWorkers>(p, sm, kWorkBarrier, u, thread);
     if (t < C) {
       top[t] = kNoMax;
       base[t] = 0.0f;  // scores as they are
@@ -216,13 +213,11 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     bar_sync(barrier, 128);
     const float page_factor = p.scale_log2 * q_inverse * p.key_scale;
     // Lets the scores of a step be taken: those of the step before are in registers. `keys`: where a BF16 step's
-    // keys are; they go into their operand first, and before a unit's first such step the queries change their
-    // form. Returns what turns the step's scores into log2 units.
+    // keys are; they go into their operand first. Returns what turns the step's scores into log2 units.
     auto let_scores = [&](int step, Place<Smem<NT>::kStages> keys) -> float {
       const StepKind kind = step_kind(u.info, step);
       float f = page_factor;
       if (kind != kStepPage) {
-        if (step == max(u.begin, u.info.pages)) load_queries<NT, kWorkers>(p, sm, u, thread, q_scale, false);
         f = p.scale_log2 * q_inverse * bf16_keys(p, sm, kWorkBarrier, u, kind, keys, k_operand, thread);
         tc::tmem_wait_st();
       }

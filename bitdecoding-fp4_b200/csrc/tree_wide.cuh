@@ -21,7 +21,7 @@ struct Shape {
   static constexpr int kGroups = NT / kColumns;             // softmax groups of 128 threads
   static constexpr int kBlocks = (NT + 63) / 64;            // 128-byte rows of P per token
   static constexpr int kVBuffers = NT > 96 ? 1 : 2;         // operand buffers in tensor memory, as many as it holds
-  static constexpr int kStages = NT > 64 ? 6 : 8;
+  static constexpr int kStages = NT > 96 ? 4 : NT > 64 ? 5 : 7;
   static constexpr int kSoftmaxThreads = 128 * kGroups;
   static constexpr int kThreads = kCacheThreads + kSoftmaxThreads + 128;  // cache side, softmax, control (two of its warps idle)
   // Registers per thread at launch and after the warpgroups have traded them: the sum over the warpgroups
@@ -37,8 +37,6 @@ struct Shape {
   // (the keys of a BF16 step lie where the pages' products had their scales: pages come first in a unit)
   static constexpr int kS = 0, kO = 2 * NT, kV = 3 * NT, kK = kV + 64 * kVBuffers, kKs = kK, kQs = kKs + 16;
   static_assert(kK + 64 <= 512 && kQs + 8 * kTerms <= kK + 64, "tensor memory");
-  // shared memory of the queries: FP4 terms (codes, then two scale atoms each) for the pages, then FP16
-  static constexpr int kTermCodes = NT * 64, kQueries = NT * 256 + kTerms * 1024;
 };
 
 template <int FROM, int TO>
@@ -52,9 +50,9 @@ struct Smem {
   using Sh = Shape<NT>;
   static constexpr int kStages = Sh::kStages;
   alignas(1024) uint8_t ring[kStages][kStage];
-  // The queries. Against pages, kTerms tiles of FP4 codes (K-major, 64-byte swizzle), then as many pairs of scale
-  // atoms; against BF16 steps, FP16 in two halves of 64 channels (K-major, 128-byte swizzle).
-  alignas(1024) uint8_t q[Sh::kQueries];
+  alignas(1024) uint8_t q[2][NT * 128];            // FP16 queries: two halves of 64 channels, K-major, 128-byte swizzle
+  alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
+  alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
   alignas(1024) uint8_t p[2][Sh::kBlocks * 16384];  // MN-major: 128-byte rows of 64 queries per token, swizzled
   uint64_t family[NT];  // draft nodes each query sees
   float base[NT];       // kShift - maximum
@@ -83,9 +81,10 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
   constexpr uint32_t kPages = f16_idesc(NT, 0, true), kBf16 = f16_idesc(NT, 1, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const uint32_t q = tc::smem_u32(sm.q), prob = tc::smem_u32(sm.p), ring = tc::smem_u32(sm.ring);
-  const uint64_t q_codes = tc::fp4_tile_desc(q, 0), q_scales = tc::sf_atom_desc(q + kTerms * Sh::kTermCodes);
+  const uint64_t q_codes = tc::fp4_tile_desc(tc::smem_u32(sm.q_codes), 0);
+  const uint64_t q_scales = tc::sf_atom_desc(tc::smem_u32(sm.q_scales));
   int n = 0, unit = 0;
-  uint32_t q_turn = 0, ka_turn = 0;
+  uint32_t ka_turn = 0;
   Place<Sh::kStages> at;
   Unit u;
   bool known = false;
@@ -116,13 +115,10 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
       }
       __syncwarp();
     };
+    wait(&sm.q_full, unit & 1, &sm.abort_flag);
 #pragma unroll 1
     for (int step = u.begin; step < u.end; ++step, ++n) {
       const StepKind kind = step_kind(u.info, step);
-      if (step == u.begin || step == u.info.pages) {  // the queries come in the form of the step, and once more for BF16
-        wait(&sm.q_full, q_turn, &sm.abort_flag);
-        q_turn ^= 1;
-      }
       const uint32_t scores = tmem + Sh::kS + (n & 1) * NT;
       wait(&sm.s_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
       if (kind == kStepPage) {
@@ -143,7 +139,7 @@ __device__ __forceinline__ void issue(Smem<NT>& sm, Walker walker, int lane) {
           for (int s = 0; s < 2; ++s) {  // 64 channels further: 32 bytes of codes, one atom of scales
 #pragma unroll
             for (int term = 0; term < kTerms; ++term)
-              tc::mma_nvf4(scores, codes + 2 * s, q_codes + term * (Sh::kTermCodes / 16) + 2 * s, kFp4, scales + 4 * s,
+              tc::mma_nvf4(scores, codes + 2 * s, q_codes + term * NT * 4 + 2 * s, kFp4, scales + 4 * s,
                            tmem + Sh::kQs + term * 8 + 4 * s, s + term > 0);
           }
           tc::commit(&sm.s_full[n & 1]);
@@ -235,15 +231,12 @@ __device__ __forceinline__ void cache(const TreeParams& p, Smem<NT>& sm, Walker 
   }
 }
 
-// The queries of a unit's first step into shared memory. Returns their scale, and what undoes it.
 template <int NT>
-__device__ __forceinline__ float first_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread, float* inverse) {
-  constexpr int kThreads = Shape<NT>::kSoftmaxThreads;
-  const float scale = query_scale<NT, kThreads>(p, sm, kSoftmaxBarrier, u, thread, inverse);
-  load_queries<NT, kThreads>(p, sm, u, thread, scale, u.begin < u.info.pages);
+__device__ __forceinline__ float bring_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
+  const float inverse = load_queries<NT, Shape<NT>::kSoftmaxThreads>(p, sm, kSoftmaxBarrier, u, thread);
   __syncwarp();
   if ((thread & 31) == 0) tc::mbar_arrive(&sm.q_full);
-  return scale;
+  return inverse;
 }
 
 template <int NT>
@@ -260,8 +253,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
   Unit u;
   if (!walker.next(u, false)) return;
   bool more = true;
-  float q_inverse;
-  float q_scale = first_queries<NT>(p, sm, u, thread, &q_inverse);
+  float q_inverse = bring_queries<NT>(p, sm, u, thread);
   while (more) {
     for (int j = t; j < C; j += 128) {
       top[j] = kNoMax;
@@ -289,11 +281,6 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
       const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
       const int node = t - BDFP4_MAX_SINK;
-      if (step == u.info.pages && step > u.begin) {  // (the pages' last scores have been waited for)
-        load_queries<NT, Sh::kSoftmaxThreads>(p, sm, u, thread, q_scale, false);
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.q_full);
-      }
       wait(&sm.s_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
       tc::fence_after_sync();
       float f = page_factor;
@@ -436,9 +423,9 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     // the next unit's queries go in while this one's last product runs: all its scores are done
     Unit following = u;
     more = walker.next(following, true);
-    float next_inverse = 1.0f, next_scale = 1.0f;
+    float next_inverse = 1.0f;
     bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);  // both groups have seen their last scores; the parents are free
-    if (more) next_scale = first_queries<NT>(p, sm, following, thread, &next_inverse);
+    if (more) next_inverse = bring_queries<NT>(p, sm, following, thread);
     bar_sync(barrier, 128);
     const bool whole = u.begin == 0 && u.end == u.info.steps;
     // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
@@ -492,7 +479,6 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       p.splits[blockIdx.x] = split;
     }
     q_inverse = next_inverse;
-    q_scale = next_scale;
     u = following;
     ++unit;
   }
