@@ -264,6 +264,93 @@ __device__ __forceinline__ void reduce_columns(float* v, int lane, int column, S
   }
 }
 
+// The launch's steps in a row, cut into equal runs, one per CTA: who does which.
+//
+// A cut within `snap` steps of a unit's end moves there. A unit that straddles a cut costs a second set-up, parts
+// through memory and the merge, together about as much as that many steps.
+struct Plan {
+  long long steps;  // all of them
+  long long per;    // of one CTA, before a cut moves
+  int snap;
+
+  // Where the cut at `x` within the unit [begin, end) goes.
+  __device__ __forceinline__ long long moved(long long x, long long begin, long long end) const {
+    const long long down = x - begin, up = end - x;
+    if (min(down, up) > snap) return x;
+    return down <= up ? begin : end;
+  }
+  // The CTA that does the last step of the unit [begin, end).
+  __device__ __forceinline__ int owner_of_last(long long begin, long long end) const {
+    long long cta = (end - 1) / per;
+    while (cta * per > begin && moved(cta * per, begin, end) >= end) --cta;
+    return (int)cta;
+  }
+};
+
+// All threads of a CTA. Fills sm.plan, sm.start_row, sm.start_offset, sm.first and sm.last (valid after the next
+// barrier of the CTA).
+template <int PT, int THREADS, int SNAP, typename Smem>
+__device__ __forceinline__ void make_plan(const TreeParams& p, Smem& sm, int thread) {
+  const int lane = thread & 31, warp = thread >> 5;
+  long long mine = 0;
+#pragma unroll 1
+  for (int row = thread; row < p.rows; row += THREADS) {
+    const RowInfo r = row_info(p, row, PT);
+    mine += (long long)r.steps * r.tiles * p.heads_kv;
+  }
+#pragma unroll
+  for (int step = 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
+  if (lane == 0) sm.sums[warp] = mine;
+  __syncthreads();
+  if (warp != 0) return;
+  Plan plan;
+  plan.steps = 0;
+  for (int w = 0; w < THREADS / 32; ++w) plan.steps += sm.sums[w];
+  plan.per = max((plan.steps + gridDim.x - 1) / gridDim.x, 1ll);
+  plan.snap = (int)min((long long)SNAP, plan.per - 1);
+  const long long cut[2] = {min(plan.per * blockIdx.x, plan.steps), min(plan.per * (blockIdx.x + 1), plan.steps)};
+  if (lane == 0) {
+    sm.plan = plan;
+    sm.first = sm.last = plan.steps;
+    sm.start_row = p.rows;
+    sm.start_offset = 0;
+  }
+  __syncwarp();
+  long long before = 0;
+#pragma unroll 1
+  for (int row0 = 0; row0 < p.rows && before <= cut[1] && cut[0] < plan.steps; row0 += 32) {
+    RowInfo r;
+    long long steps = 0;
+    if (row0 + lane < p.rows) {
+      r = row_info(p, row0 + lane, PT);
+      steps = (long long)r.steps * r.tiles * p.heads_kv;
+    }
+    long long upto = steps;
+#pragma unroll
+    for (int step = 1; step < 32; step <<= 1) {
+      const long long left = __shfl_up_sync(0xffffffffu, upto, step);
+      if (lane >= step) upto += left;
+    }
+    const long long begin = before + upto - steps;  // of this lane's row
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (steps > 0 && cut[i] >= begin && cut[i] < begin + steps) {
+        const long long unit = begin + (cut[i] - begin) / r.steps * r.steps;
+        const long long at = plan.moved(cut[i], unit, unit + r.steps);
+        if (i == 0) {
+          sm.first = at;
+          sm.start_row = row0 + lane;
+          sm.start_offset = at - begin;  // (the walk goes on to the next row from a row's end)
+        } else {
+          sm.last = at;
+        }
+      }
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  __syncwarp();
+}
+
 constexpr int kTerms = 4;  // FP4 terms of a query
 constexpr int kCacheThreads = 256;  // that bring the cache side: two halves of 128
 

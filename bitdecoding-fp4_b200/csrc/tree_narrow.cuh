@@ -39,6 +39,7 @@ namespace narrow {
 
 // Named barriers: one per half, and all eight working warps.
 constexpr int kHalfBarrier = 1, kWorkBarrier = 3;
+constexpr int kSnap = 4;                   // steps
 constexpr int kWorkers = kCacheThreads;    // two halves of 128
 constexpr int kThreads = kWorkers + 64;    // and a warp each for copies and products
 constexpr int kTmemColumns = 256;          // half of what an SM has
@@ -71,8 +72,9 @@ struct Smem {
   uint64_t full[kStages], empty[kStages];
   uint64_t s_ready, s_full, p_full, o_full, drained;  // s_ready: the scores before are read, BF16 keys in their operand
   long long sums[kThreads / 32];
+  Plan plan;
   int start_row;
-  long long start_offset, first, last, per_cta;
+  long long start_offset, first, last;
   uint32_t tmem;
   int abort_flag, ignored_flag;
 };
@@ -188,6 +190,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
   Place<Smem<NT>::kStages> v_at;
   uint32_t parity = 0;
   bool any = false;  // a step has been taken
+  long long done = sm.first;
   Unit u;
   bool known = false;
 #pragma unroll 1
@@ -362,6 +365,8 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     }
     bar_sync(barrier, 128);
     const bool whole = u.begin == 0 && u.end == u.info.steps;
+    const long long at_step = done - u.begin;  // where the unit begins in the launch's steps
+    done += u.end - u.begin;
     // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
     const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
     if (t < C) {
@@ -405,8 +410,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
       split.row = u.row;
       split.head = u.head;
       split.tile = u.tile;
-      // the unit's last step, counted over the whole launch, names the CTA it ends in
-      split.last = (int)((sm.last + (u.info.steps - u.end) - 1) / sm.per_cta);
+      split.last = sm.plan.owner_of_last(at_step, at_step + u.info.steps);
       p.splits[blockIdx.x] = split;
     }
   }
@@ -421,15 +425,6 @@ tree_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
   dependents_may_launch();
 
-  // all steps of the launch, and where this CTA's run begins
-  long long mine = 0;
-#pragma unroll 1
-  for (int row = thread; row < p.rows; row += kThreads) {
-    const RowInfo r = row_info(p, row, PT);
-    mine += (long long)r.steps * r.tiles * p.heads_kv;
-  }
-  for (int step = 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
-  if (lane == 0) sm.sums[warp] = mine;
   if (thread == 0) {
 #pragma unroll 1
     for (int i = 0; i < Smem<NT>::kStages; ++i) {
@@ -448,41 +443,8 @@ tree_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_const
     none.head = none.tile = none.last = 0;
     p.splits[blockIdx.x] = none;
   }
-  __syncthreads();
+  make_plan<PT, kThreads, kSnap>(p, sm, thread);
   if (warp == 0) {
-    long long all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) all += sm.sums[w];
-    const long long per = max((all + gridDim.x - 1) / gridDim.x, 1ll);
-    const long long first = per * blockIdx.x, last = min(first + per, all);
-    if (lane == 0) {
-      sm.per_cta = per;
-      sm.first = first;
-      sm.last = last;
-    }
-    long long before = 0;
-#pragma unroll 1
-    for (int row0 = 0; row0 < p.rows && first < last; row0 += 32) {
-      long long steps = 0;
-      if (row0 + lane < p.rows) {
-        const RowInfo r = row_info(p, row0 + lane, PT);
-        steps = (long long)r.steps * r.tiles * p.heads_kv;
-      }
-      long long upto = steps;
-      for (int step = 1; step < 32; step <<= 1) {
-        const long long left = __shfl_up_sync(0xffffffffu, upto, step);
-        if (lane >= step) upto += left;
-      }
-      const unsigned holds = __ballot_sync(0xffffffffu, before + upto > first);
-      if (holds) {
-        if (lane == __ffs(holds) - 1) {
-          sm.start_row = row0 + lane;
-          sm.start_offset = first - (before + upto - steps);
-        }
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    __syncwarp();
     tc::tmem_alloc(&sm.tmem, kTmemColumns);
     tc::tmem_relinquish();
     tc::fence_before_sync();

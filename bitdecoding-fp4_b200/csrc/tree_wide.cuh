@@ -11,6 +11,7 @@ namespace wide {
 
 // Named barriers: one per softmax group (four at most), all softmax threads, the key threads.
 constexpr int kCtas = kTreeWideCtas;
+constexpr int kSnap = 6;  // steps
 constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kCacheBarrier = 6;
 
 // A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (128
@@ -67,8 +68,9 @@ struct Smem {
   uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
   uint64_t q_full, o_full, o_empty, drained;
   long long sums[Sh::kThreads / 32];
+  Plan plan;
   int start_row;
-  long long start_offset, first, last, per_cta;
+  long long start_offset, first, last;
   uint32_t tmem;
   int abort_flag, ignored_flag;
 };
@@ -250,6 +252,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
   float* base = sm.base + first_column;
   float* top = sm.top + first_column;
   int n = 0, unit = 0;
+  long long done = sm.first;
   Unit u;
   if (!walker.next(u, false)) return;
   bool more = true;
@@ -428,6 +431,8 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     if (more) next_inverse = bring_queries<NT>(p, sm, following, thread);
     bar_sync(barrier, 128);
     const bool whole = u.begin == 0 && u.end == u.info.steps;
+    const long long at_step = done - u.begin;  // where the unit begins in the launch's steps
+    done += u.end - u.begin;
     // a part that begins a unit goes to the CTA's second slot, one that continues it to the first
     const int part = 2 * blockIdx.x + (u.begin == 0 ? 1 : 0);
     for (int j = t; j < C; j += 128) {
@@ -474,8 +479,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       split.row = u.row;
       split.head = u.head;
       split.tile = u.tile;
-      // the unit's last step, counted over the whole launch, names the CTA it ends in
-      split.last = (int)((sm.last + (u.info.steps - u.end) - 1) / sm.per_cta);
+      split.last = sm.plan.owner_of_last(at_step, at_step + u.info.steps);
       p.splits[blockIdx.x] = split;
     }
     q_inverse = next_inverse;
@@ -493,14 +497,6 @@ tree_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
   dependents_may_launch();
 
-  // all steps of the launch, and where this CTA's run begins
-  long long mine = 0;
-  for (int row = thread; row < p.rows; row += Sh::kThreads) {
-    const RowInfo r = row_info(p, row, PT);
-    mine += (long long)r.steps * r.tiles * p.heads_kv;
-  }
-  for (int step = 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
-  if (lane == 0) sm.sums[warp] = mine;
   if (thread == 0) {
 #pragma unroll 1
     for (int i = 0; i < Sh::kStages; ++i) {
@@ -529,40 +525,8 @@ tree_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     none.head = none.tile = none.last = 0;
     p.splits[blockIdx.x] = none;
   }
-  __syncthreads();
+  make_plan<PT, Sh::kThreads, kSnap>(p, sm, thread);
   if (warp == 0) {
-    long long all = 0;
-    for (int w = 0; w < Sh::kThreads / 32; ++w) all += sm.sums[w];
-    const long long per = max((all + gridDim.x - 1) / gridDim.x, 1ll);
-    const long long first = per * blockIdx.x, last = min(first + per, all);
-    if (lane == 0) {
-      sm.per_cta = per;
-      sm.first = first;
-      sm.last = last;
-    }
-    long long before = 0;
-    for (int row0 = 0; row0 < p.rows && first < last; row0 += 32) {
-      long long steps = 0;
-      if (row0 + lane < p.rows) {
-        const RowInfo r = row_info(p, row0 + lane, PT);
-        steps = (long long)r.steps * r.tiles * p.heads_kv;
-      }
-      long long upto = steps;
-      for (int step = 1; step < 32; step <<= 1) {
-        const long long left = __shfl_up_sync(0xffffffffu, upto, step);
-        if (lane >= step) upto += left;
-      }
-      const unsigned holds = __ballot_sync(0xffffffffu, before + upto > first);
-      if (holds) {
-        if (lane == __ffs(holds) - 1) {
-          sm.start_row = row0 + lane;
-          sm.start_offset = first - (before + upto - steps);
-        }
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    __syncwarp();
     tc::tmem_alloc(&sm.tmem, 512);
     tc::tmem_relinquish();
     tc::fence_before_sync();
