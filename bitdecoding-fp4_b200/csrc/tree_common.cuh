@@ -561,6 +561,63 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem& sm, int
   return inverse;
 }
 
+// Channel t of a tile's queries out of tensor memory: `columns` of them from column `at` (of the tile's
+// `first_column`) on, normalised to the output when the unit is whole, as they are to its part when not.
+template <typename Smem>
+__device__ __forceinline__ void store_output(const TreeParams& p, const Smem& sm, const Unit& u, uint32_t at, int tile,
+                                             int first_column, int columns, bool whole, int part, int t) {
+  const int query = u.tile * tile + first_column;
+  int head = query % p.ratio;
+  columns = min(columns, u.info.count * p.ratio - query);
+  __nv_bfloat16* out = p.out + u.row * p.out_row + (query / p.ratio) * p.out_node +
+                       ((int64_t)u.head * p.ratio + head) * kHeadDim + t;
+  float* partial = p.partial + ((int64_t)part * tile + first_column) * kHeadDim + t;
+  const int64_t next_node = p.out_node - (int64_t)(p.ratio - 1) * kHeadDim;
+#pragma unroll 1
+  for (int j = 0; j < columns; j += 8) {
+    float o[8];
+    tc::tmem_ld8(at + j, o);
+    tc::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (j + i >= columns) break;
+      if (whole) {
+        *out = __float2bfloat16_rn(o[i] * sm.factor[first_column + j + i]);
+        const bool wraps = ++head == p.ratio;
+        out += wraps ? next_node : (int64_t)kHeadDim;
+        if (wraps) head = 0;
+      } else {
+        *partial = o[i];
+        partial += kHeadDim;
+      }
+    }
+  }
+}
+
+// Which of up to 32 columns see each draft node: bit j of seen_by[node] is column j's. By one warp, lane j for
+// column j of the tile's queries from `query` on. A column sees its own node and that node's ancestors.
+__device__ __forceinline__ void make_masks(const TreeParams& p, const Unit& u, const int* parents, uint32_t* seen_by, int query,
+                                           int lane) {
+  uint64_t seen = 0;
+#pragma unroll 1
+  for (int node = min((query + lane) / p.ratio, u.info.count - 1); node >= 0;) {
+    seen |= 1ull << node;
+    const int parent = parents[node];
+    node = parent < node ? parent : -1;
+  }
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t word = (uint32_t)(seen >> (32 * half));
+    uint32_t mine = 0;
+#pragma unroll 4
+    for (int node = 0; node < 32; ++node) {
+      const uint32_t all = __ballot_sync(0xffffffffu, (word >> node) & 1);
+      if (lane == node) mine = all;
+    }
+    seen_by[32 * half + lane] = mine;
+  }
+}
+
 // One stage's release, by a whole warp. A page's stage waits for its score product too; for a BF16 step's one
 // warp arrives in its place.
 template <typename Smem>

@@ -62,7 +62,7 @@ struct Smem {
   alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
   alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
   alignas(1024) uint8_t p[16384];        // MN-major: 128-byte rows of 64 queries per token, swizzled
-  uint64_t family[NT];  // draft nodes each query sees
+  uint32_t seen_by[2][BDFP4_MAX_TREE_NODES];  // [half] which of its columns see a draft node
   float base[NT];       // kShift - maximum, 0 while there is none
   float top[NT];        // maximum, log2 units
   float factor[NT], shift[NT];  // what a renewal does to sums and scores (at a unit's end: 1 / weight)
@@ -199,17 +199,8 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     if (t < C) {
       top[t] = kNoMax;
       base[t] = 0.0f;  // scores as they are
-      // the draft nodes the query of column t sees
-      const int query = u.tile * NT + first_column + t;
-      uint64_t seen = 0;
-#pragma unroll 1
-      for (int node = min(query / p.ratio, u.info.count - 1); node >= 0;) {
-        seen |= 1ull << node;
-        const int parent = sm.parents[node];
-        node = parent < node ? parent : -1;
-      }
-      sm.family[first_column + t] = seen;
     }
+    if (warp == 0) make_masks(p, u, sm.parents, sm.seen_by[half], u.tile * NT + first_column, lane);
     float2 sum[C / 2];
 #pragma unroll
     for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
@@ -245,11 +236,11 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
         if (kind == kStepPage) dead = t < u.info.sink;
         else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
         else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
-        const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
-        const int node = t - BDFP4_MAX_SINK;
+        uint32_t seen = dead ? 0u : ~0u;
+        if (kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead) seen = sm.seen_by[half][t - BDFP4_MAX_SINK];
 #pragma unroll
         for (int j = 0; j < C; ++j)
-          if (dead || (masked && !((sm.family[first_column + j] >> node) & 1))) s[j] = -INFINITY;
+          if (!((seen >> j) & 1)) s[j] = -INFINITY;
       }
       // scores -> log2 units above the maxima, plus kShift
       const float2 f2 = make_float2(f, f);
@@ -382,28 +373,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     bar_sync(barrier, 128);
     wait(&sm.o_full, parity ^ 1, &sm.abort_flag);
     tc::fence_after_sync();
-    const int queries = min(u.info.count * p.ratio - u.tile * NT - first_column, C);
-    const int query = u.tile * NT + first_column;
-    int out_node = query / p.ratio, out_head = query % p.ratio;
-    __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
-    float* partial = p.partial + ((int64_t)part * NT + first_column) * kHeadDim + t;
-#pragma unroll 1
-    for (int j = 0; j < C; j += 8) {
-      float o[8];
-      tc::tmem_ld8(lanes + Sh::kO + first_column + j, o);
-      tc::tmem_wait_ld();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (j + i < queries) {
-          if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.factor[first_column + j + i]);
-            if (++out_head == p.ratio) out_head = 0, ++out_node;
-          } else {
-            partial[(int64_t)(j + i) * kHeadDim] = o[i];
-          }
-        }
-      }
-    }
+    store_output(p, sm, u, lanes + Sh::kO + first_column, NT, first_column, C, whole, part, t);
     tc::fence_before_sync();
     if (!whole && u.begin == 0 && thread == 0) {
       TreeSplit split;

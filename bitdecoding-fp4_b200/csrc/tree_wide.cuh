@@ -55,7 +55,7 @@ struct Smem {
   alignas(1024) uint8_t q_codes[kTerms][NT * 64];  // FP4 terms, K-major, 64-byte swizzle
   alignas(1024) uint8_t q_scales[kTerms][1024];    // two atoms each
   alignas(1024) uint8_t p[2][Sh::kBlocks * 16384];  // MN-major: 128-byte rows of 64 queries per token, swizzled
-  uint64_t family[NT];  // draft nodes each query sees
+  uint32_t seen_by[Sh::kGroups][BDFP4_MAX_TREE_NODES];  // which of a group's columns see a draft node
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
   float factor[NT];     // what a renewal does to sums (at a unit's end: 1 / weight)
@@ -261,16 +261,8 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     for (int j = t; j < C; j += 128) {
       top[j] = kNoMax;
       base[j] = kShift - kNoMax;
-      // the draft nodes the query of column j sees
-      const int query = u.tile * NT + first_column + j;
-      uint64_t seen = 0;
-      for (int node = min(query / p.ratio, u.info.count - 1); node >= 0;) {
-        seen |= 1ull << node;
-        const int parent = sm.parents[node];
-        node = parent < node ? parent : -1;
-      }
-      sm.family[first_column + j] = seen;
     }
+    if (warp == 0) make_masks(p, u, sm.parents, sm.seen_by[group], u.tile * NT + first_column, lane);
     float2 sum[C / 2];
 #pragma unroll
     for (int j = 0; j < C / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
@@ -283,7 +275,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
       else dead = t < BDFP4_MAX_SINK ? t >= u.info.sink : t - BDFP4_MAX_SINK >= u.info.count;
       const bool masked = kind == kStepDraft && t >= BDFP4_MAX_SINK && !dead;
-      const int node = t - BDFP4_MAX_SINK;
+      const uint32_t seen = masked ? sm.seen_by[group][t - BDFP4_MAX_SINK] : ~0u;
       wait(&sm.s_full[n & 1], (n >> 1) & 1, &sm.abort_flag);
       tc::fence_after_sync();
       float f = page_factor;
@@ -293,10 +285,10 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       auto load16 = [&](int j, float* s) {
         tc::tmem_ld16(scores + j, s);
         tc::tmem_wait_ld();
-        if (masked) {
+        if (kind == kStepDraft) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (!((sm.family[first_column + j + i] >> node) & 1)) s[i] = -INFINITY;
+            if (!((seen >> (j + i)) & 1)) s[i] = -INFINITY;
         }
       };
       // scores -> log2 units above the maxima, plus kShift
@@ -448,28 +440,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     bar_sync(barrier, 128);
     wait(&sm.o_full, unit & 1, &sm.abort_flag);
     tc::fence_after_sync();
-    const int queries = min(u.info.count * p.ratio - u.tile * NT - first_column, C);
-    int query = u.tile * NT + first_column;
-    int out_node = query / p.ratio, out_head = query % p.ratio;
-    __nv_bfloat16* out = p.out + u.row * p.out_row + (int64_t)u.head * p.ratio * kHeadDim + t;
-    float* partial = p.partial + ((int64_t)part * NT + first_column) * kHeadDim + t;
-#pragma unroll
-    for (int j = 0; j < C; j += 16) {
-      float o[16];
-      tc::tmem_ld16(sm.tmem + Sh::kO + first_column + j + lanes, o);
-      tc::tmem_wait_ld();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (j + i < queries) {
-          if (whole) {
-            out[out_node * p.out_node + out_head * kHeadDim] = __float2bfloat16_rn(o[i] * sm.factor[first_column + j + i]);
-            if (++out_head == p.ratio) out_head = 0, ++out_node;
-          } else {
-            partial[(int64_t)(j + i) * kHeadDim] = o[i];
-          }
-        }
-      }
-    }
+    store_output(p, sm, u, sm.tmem + Sh::kO + first_column + lanes, NT, first_column, C, whole, part, t);
     tc::fence_before_sync();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sm.o_empty);
