@@ -283,12 +283,15 @@ def _own(op, s):
         v = tree.verify_drafts(s["target"], s["tokens"], s["parents"], s["uniforms"], draft_probs=s["draft"])
         return dict(accepted=v.accepted, counts=v.accepted_counts, next_tokens=v.next_tokens)
     if "committer" not in s:  # what a serving program builds once
-        regions = [_cache_views(b, case["heads_kv"], PAGE) for b in s["blocks"]] if case["crossing"] else None
+        regions = None
+        if s["filled"]:  # a path that ends on a page boundary fills a page too; layers that are not compared seal theirs aside
+            aside = [torch.zeros_like(s["blocks"][0]) for _ in range(case["layers"] - len(s["blocks"]))]
+            regions = [_cache_views(b, case["heads_kv"], PAGE) for b in s["blocks"] + aside]
         s["committer"] = tree.DraftCommitter(
             tail_key=s["tail_key"], tail_value=s["tail_value"], sink_tokens=SINK, rotate_key=case["rotate"],
             key_shift=s["shift"], regions=regions)
     new = s["committer"](s["draft_key"], s["draft_value"], s["accepted"], s["counts"], seq_lens=s["seq_lens"],
-                         row_to_slot=s["slots"], block_table=s["table"] if case["crossing"] else None)
+                         row_to_slot=s["slots"], block_table=s["table"] if s["filled"] else None)
     return _commit_outputs(s, new.seq_lens, new.seqused_fp4, new.seqused_residual, new.seqused_sink)
 
 
