@@ -34,52 +34,49 @@ MAX_TREE_NODES = 64
 ROTATIONS = ("none", "hadamard")
 
 
-class _on_device:
-    """Launches go to the current device's context; the tensors' device is made current if it is not. Entering
-    gives the device's current stream (its handle alone: making a stream object costs 4 us)."""
-
-    def __init__(self, device: torch.device) -> None:
-        self._index = device.index
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self) -> int:
-        if self._guard is not None:
-            self._guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self._index)
-
-    def __exit__(self, *error):
-        if self._guard is not None:
-            self._guard.__exit__(*error)
+def _launch(call, args, device: torch.device) -> None:
+    """``call`` on the device's current stream; the tensors' device is made current if it is not. (The stream's
+    handle alone: making a stream object costs 4 us.)"""
+    if device.index == torch.cuda.current_device():
+        call(args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            call(args, torch._C._cuda_getCurrentRawStream(device.index))
 
 
-def _int32(tensor, name: str, shape: tuple, device) -> None:
+# The checks give the address back, so that a call asks each tensor once.
+
+
+def _int32(tensor, name: str, shape: tuple, device) -> int:
     if (
         not isinstance(tensor, torch.Tensor) or tensor.dtype is not torch.int32 or tensor.device != device
         or tensor.shape != shape or (shape[-1] > 1 and tensor.stride(-1) != 1)
     ):
         raise ValueError(f"{name} must be INT32 {list(shape)} on {device}, dense along its last axis")
+    return tensor.data_ptr()
 
 
-def _tree_tensor(tensor, name: str, shape: tuple, device) -> None:
-    """BF16 ``[..., nodes, heads, 128]`` with free leading strides."""
-    ok = (isinstance(tensor, torch.Tensor) and tensor.dtype is torch.bfloat16 and tensor.device == device
-          and tensor.shape == shape and tensor.data_ptr() % 16 == 0)
-    if ok:
-        *outer, head, inner = tensor.stride()
-        ok = inner == 1 and (head == HEAD_DIM or shape[-2] == 1)
+def _tree_tensor(tensor, name: str, shape: tuple, device) -> tuple:
+    """BF16 ``[..., nodes, heads, 128]`` with free leading strides: its address, then those strides."""
+    if (
+        isinstance(tensor, torch.Tensor) and tensor.dtype is torch.bfloat16 and tensor.device == device
+        and tensor.shape == shape
+    ):
+        address, (*outer, head, inner) = tensor.data_ptr(), tensor.stride()
+        ok = inner == 1 and (head == HEAD_DIM or shape[-2] == 1) and address % 16 == 0
         for stride, size in zip(outer, shape):
             if stride % 8 and size > 1:
                 ok = False
-    if not ok:
-        raise ValueError(f"{name} must be BF16 {list(shape)} on {device}, dense within a node and 16-byte aligned")
+        if ok:
+            return address, *outer
+    raise ValueError(f"{name} must be BF16 {list(shape)} on {device}, dense within a node and 16-byte aligned")
 
 
-def _parents(parents, rows: int, nodes: int, device) -> torch.Tensor:
-    """``[rows, nodes]``, or ``[nodes]`` for one tree that every row shares."""
+def _parents(parents, rows: int, nodes: int, device) -> tuple[int, int]:
+    """``[rows, nodes]``, or ``[nodes]`` for one tree that every row shares: its address and row stride."""
     if isinstance(parents, torch.Tensor) and parents.ndim == 1 and nodes == parents.shape[0]:
         parents = parents.expand(rows, nodes)
-    _int32(parents, "parents", (rows, nodes), device)
-    return parents
+    return _int32(parents, "parents", (rows, nodes), device), parents.stride(0)
 
 
 def _cuda_device(tensor, name: str) -> torch.device:
@@ -93,8 +90,8 @@ def _check_values(bad: torch.Tensor, message: str) -> None:
         raise ValueError(message)
 
 
-def _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, device) -> tuple[int, int, int]:
-    """(pages, page tokens, KV heads) of the four regions of an NVFP4 cache."""
+def _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, device) -> tuple:
+    """(pages, page tokens, KV heads, addresses, page pitches) of the four regions of an NVFP4 cache."""
     packed, scales = (torch.uint8, torch.float4_e2m1fn_x2), (torch.uint8, torch.float8_e4m3fn)
     if not isinstance(key_pages_fp4, torch.Tensor) or key_pages_fp4.device != device:
         raise ValueError(f"key_pages_fp4 must be a CUDA tensor on {device}")
@@ -112,6 +109,7 @@ def _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, dev
     else:
         raise ValueError("key_pages_fp4 must be packed FP4 with shape [pages, 128, heads_kv, 64]")
     half = page // 2
+    addresses, pitches = [], []
     for tensor, name, kinds, shape, inner in (
         (key_pages_fp4, "key_pages_fp4", packed, (pages, page, heads, 64), key_inner),
         (key_scales, "key_scales", scales, scale_shape, key_sf),
@@ -123,10 +121,12 @@ def _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, dev
         if tensor.shape != shape or tensor.dtype not in kinds:
             held = "packed FP4" if kinds is packed else "E4M3 scale bytes"
             raise ValueError(f"{name} must hold {held} with shape {shape}")
-        pitch, *within = tensor.stride()
-        if tuple(within) != inner or pitch % 16 or tensor.data_ptr() % 16:
+        strides, address = tensor.stride(), tensor.data_ptr()
+        if strides[1:] != inner or strides[0] % 16 or address % 16:
             raise ValueError(f"{name} must be in the quantizer's layout, dense within a page, with a 16-byte page pitch")
-    return pages, page, heads
+        addresses.append(address)
+        pitches.append(strides[0])
+    return pages, page, heads, addresses, pitches
 
 
 @functools.lru_cache(maxsize=1024)
@@ -199,19 +199,30 @@ def tree_decode(
         raise ValueError("tree decode needs at least one row and one node")
     if nodes > MAX_TREE_NODES:
         raise NotImplementedError(f"a tree holds at most {MAX_TREE_NODES} nodes, got {nodes}")
-    pages, page_tokens, heads_kv = _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, device)
+    pages, page_tokens, heads_kv, addresses, pitches = _check_regions(
+        key_pages_fp4, key_scales, value_pages_fp4, value_scales, device)
     if heads_q % heads_kv or heads_q < 1:
         raise ValueError("heads_q must be divisible by heads_kv")
-    _tree_tensor(query, "query", (rows, nodes, heads_q, HEAD_DIM), device)
-    _tree_tensor(draft_key, "draft_key", (rows, nodes, heads_kv, HEAD_DIM), device)
-    _tree_tensor(draft_value, "draft_value", (rows, nodes, heads_kv, HEAD_DIM), device)
-    parents = _parents(parents, rows, nodes, device)
+    a = bdfp4.TreeArgs()
+    a.rows, a.nodes, a.heads_q, a.heads_kv = rows, nodes, heads_q, heads_kv
+    a.key_codes, a.key_scales, a.value_codes, a.value_scales = addresses
+    a.key_codes_pitch, a.key_scales_pitch, a.value_codes_pitch, a.value_scales_pitch = pitches
+    a.pages, a.page_tokens = pages, page_tokens
+    shape = (rows, nodes, heads_q, HEAD_DIM)
+    a.query, a.query_row_stride, a.query_node_stride = _tree_tensor(query, "query", shape, device)
+    draft_shape = (rows, nodes, heads_kv, HEAD_DIM)
+    a.draft_key, a.draft_key_row_stride, a.draft_key_node_stride = _tree_tensor(draft_key, "draft_key", draft_shape, device)
+    a.draft_value, a.draft_value_row_stride, a.draft_value_node_stride = _tree_tensor(
+        draft_value, "draft_value", draft_shape, device)
+    a.parents, a.parents_row_stride = _parents(parents, rows, nodes, device)
     if node_counts is not None:
-        _int32(node_counts, "node_counts", (rows,), device)
+        a.node_counts = _int32(node_counts, "node_counts", (rows,), device)
     if fp4_page_table.ndim != 2:
         raise ValueError("fp4_page_table must be row-major INT32 with shape [rows, max_pages]")
-    _int32(fp4_page_table, "fp4_page_table", (rows, fp4_page_table.shape[1]), device)
-    _int32(seqused_fp4, "seqused_fp4", (rows,), device)
+    columns = fp4_page_table.shape[1]
+    a.page_table = _int32(fp4_page_table, "fp4_page_table", (rows, columns), device)
+    a.page_table_stride, a.max_pages_per_row = fp4_page_table.stride(0), columns
+    a.seqused_fp4 = _int32(seqused_fp4, "seqused_fp4", (rows,), device)
     if query_rotation not in ROTATIONS:
         raise ValueError(f"query_rotation must be one of {list(ROTATIONS)}, got {query_rotation!r}")
     if key_shift is not None and (
@@ -219,12 +230,14 @@ def tree_decode(
         or tuple(key_shift.shape) != (heads_kv, HEAD_DIM)
     ):
         raise ValueError(f"key_shift must be contiguous FP32 [{heads_kv}, {HEAD_DIM}] on {device}")
+    a.rotate, a.key_shift = int(query_rotation == "hadamard"), bdfp4.ptr(key_shift)
     scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not math.isfinite(scale) or scale <= 0.0:
         raise ValueError("softmax_scale must be finite and positive")
     key_ts, value_ts = (1.0, 1.0) if tensor_scales is None else map(float, tensor_scales)
     if not (0.0 < key_ts < math.inf and 0.0 < value_ts < math.inf):
         raise ValueError("tensor_scales must be finite and positive")
+    a.softmax_scale, a.key_tensor_scale, a.value_tensor_scale = scale, key_ts, value_ts
 
     residual = (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual)
     has_residual = residual[0] is not None
@@ -235,27 +248,30 @@ def tree_decode(
         raise ValueError("seqused_sink needs the BF16 residual arguments")
     slots = 0
     if has_residual:
-        slots, least = residual[0].shape[0], PAGE_SIZE + (SINK_TOKENS if seqused_sink is not None else 0)
+        tail_shape = residual[0].shape
+        slots, least = tail_shape[0], PAGE_SIZE + (SINK_TOKENS if seqused_sink is not None else 0)
         for tensor, name in ((residual[0], "residual_key_pages_bf16"), (residual[1], "residual_value_pages_bf16")):
             if (
                 tensor.dtype is not torch.bfloat16 or tensor.device != device or not tensor.is_contiguous()
-                or tensor.ndim != 4 or tensor.shape[1] < least or tensor.shape[2:] != (heads_kv, HEAD_DIM)
-                or tensor.shape != residual[0].shape
+                or tensor.shape != tail_shape or len(tail_shape) != 4 or tail_shape[1] < least
+                or tail_shape[2:] != (heads_kv, HEAD_DIM)
             ):
                 raise ValueError(f"{name} must be contiguous BF16 [slots, {least}, {heads_kv}, {HEAD_DIM}] on {device}")
-        for tensor, name in ((residual_page_ids, "residual_page_ids"), (seqused_residual, "seqused_residual"),
-                             (seqused_sink, "seqused_sink")):
-            if tensor is not None:
-                _int32(tensor, name, (rows,), device)
+        a.tail_key, a.tail_value = residual[0].data_ptr(), residual[1].data_ptr()
+        a.tail_slot_stride, a.tail_slots = residual[0].stride(0), slots
+        a.tail_slot_ids = _int32(residual_page_ids, "residual_page_ids", (rows,), device)
+        a.seqused_residual = _int32(seqused_residual, "seqused_residual", (rows,), device)
+        if seqused_sink is not None:
+            a.seqused_sink = _int32(seqused_sink, "seqused_sink", (rows,), device)
     if error_word is not None:
-        _int32(error_word, "error_word", (1,), device)
+        a.error_word = _int32(error_word, "error_word", (1,), device)
     if not trusted_metadata:
         per_step = PAGE_SIZE // page_tokens
-        most = fp4_page_table.shape[1] // per_step * PAGE_SIZE
+        most = columns // per_step * PAGE_SIZE
         _check_values((seqused_fp4 < 0) | (seqused_fp4 > most) | (seqused_fp4 % PAGE_SIZE != 0),
                       f"seqused_fp4 values must be page-aligned and in [0, {most}]")
-        columns = torch.arange(fp4_page_table.shape[1], device=device)[None]
-        _check_values((columns < (seqused_fp4 // page_tokens)[:, None]) & ((fp4_page_table < 0) | (fp4_page_table >= pages)),
+        entry = torch.arange(columns, device=device)[None]
+        _check_values((entry < (seqused_fp4 // page_tokens)[:, None]) & ((fp4_page_table < 0) | (fp4_page_table >= pages)),
                       f"fp4_page_table entries a row consumes must lie in [0, {pages})")
         if node_counts is not None:
             _check_values((node_counts < 0) | (node_counts > nodes), f"node_counts values must lie in [0, {nodes}]")
@@ -269,48 +285,16 @@ def tree_decode(
                               f"seqused_sink values must lie in [0, {SINK_TOKENS}]")
     if out is None:
         make = torch.empty if node_counts is None else torch.zeros
-        out = make(rows, nodes, heads_q, HEAD_DIM, dtype=torch.bfloat16, device=device)
-    else:
-        _tree_tensor(out, "out", (rows, nodes, heads_q, HEAD_DIM), device)
+        out = make(shape, dtype=torch.bfloat16, device=device)
+    a.out, a.out_row_stride, a.out_node_stride = _tree_tensor(out, "out", shape, device)
     need = tree_workspace_bytes(rows, nodes, heads_q, heads_kv)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     elif (workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous()
           or workspace.numel() < need or workspace.data_ptr() % 16):
         raise ValueError(f"workspace must be a contiguous, 16-byte aligned uint8 buffer of at least {need} bytes on {device}")
-
-    a = bdfp4.TreeArgs()
-    a.rows, a.nodes, a.heads_q, a.heads_kv = rows, nodes, heads_q, heads_kv
-    a.query = query.data_ptr()
-    a.query_row_stride, a.query_node_stride = query.stride()[:2]
-    a.draft_key, a.draft_value = draft_key.data_ptr(), draft_value.data_ptr()
-    a.draft_key_row_stride, a.draft_key_node_stride = draft_key.stride()[:2]
-    a.draft_value_row_stride, a.draft_value_node_stride = draft_value.stride()[:2]
-    a.parents, a.parents_row_stride = parents.data_ptr(), parents.stride(0)
-    a.node_counts = bdfp4.ptr(node_counts)
-    a.key_codes, a.key_scales = key_pages_fp4.data_ptr(), key_scales.data_ptr()
-    a.value_codes, a.value_scales = value_pages_fp4.data_ptr(), value_scales.data_ptr()
-    a.key_codes_pitch, a.key_scales_pitch = key_pages_fp4.stride(0), key_scales.stride(0)
-    a.value_codes_pitch, a.value_scales_pitch = value_pages_fp4.stride(0), value_scales.stride(0)
-    a.pages, a.page_tokens = pages, page_tokens
-    a.page_table, a.page_table_stride = fp4_page_table.data_ptr(), fp4_page_table.stride(0)
-    a.max_pages_per_row = fp4_page_table.shape[1]
-    a.rotate = int(query_rotation == "hadamard")
-    a.seqused_fp4 = seqused_fp4.data_ptr()
-    if has_residual:
-        a.tail_key, a.tail_value = residual[0].data_ptr(), residual[1].data_ptr()
-        a.tail_slot_stride, a.tail_slots = residual[0].stride(0), slots
-        a.tail_slot_ids, a.seqused_residual = residual_page_ids.data_ptr(), seqused_residual.data_ptr()
-        a.seqused_sink = bdfp4.ptr(seqused_sink)
-    a.softmax_scale = scale
-    a.key_shift = bdfp4.ptr(key_shift)
-    a.key_tensor_scale, a.value_tensor_scale = key_ts, value_ts
-    a.out = out.data_ptr()
-    a.out_row_stride, a.out_node_stride = out.stride()[:2]
     a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    a.error_word = bdfp4.ptr(error_word)
-    with _on_device(device) as stream:
-        bdfp4.tree_decode(a, stream)
+    _launch(bdfp4.tree_decode, a, device)
     return out
 
 
@@ -360,36 +344,31 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, parents: tor
         ):
             raise ValueError(f"{name} must be {target_probs.dtype} [{rows}, {nodes}, {vocab}] on {device}, dense along "
                              "the vocabulary")
-    _int32(tokens, "tokens", (rows, nodes), device)
-    parents = _parents(parents, rows, nodes, device)
+    a = bdfp4.VerifyArgs()
+    a.rows, a.nodes, a.vocab, a.bf16 = rows, nodes, vocab, int(target_probs.dtype is torch.bfloat16)
+    a.tokens, a.tokens_row_stride = _int32(tokens, "tokens", (rows, nodes), device), tokens.stride(0)
+    a.parents, a.parents_row_stride = _parents(parents, rows, nodes, device)
     if (not isinstance(uniforms, torch.Tensor) or uniforms.dtype is not torch.float32 or uniforms.device != device
             or tuple(uniforms.shape) != (rows, nodes) or (nodes > 1 and uniforms.stride(1) != 1)):
         raise ValueError(f"uniforms must be FP32 [{rows}, {nodes}] on {device}, dense along its last axis")
+    a.uniforms, a.uniforms_row_stride = uniforms.data_ptr(), uniforms.stride(0)
     if node_counts is not None:
-        _int32(node_counts, "node_counts", (rows,), device)
+        a.node_counts = _int32(node_counts, "node_counts", (rows,), device)
     if out is None:
-        flat = torch.empty(rows * (nodes + 2), dtype=torch.int32, device=device)
-        out = DraftVerdict(flat[:rows * nodes].view(rows, nodes), flat[rows * nodes:rows * (nodes + 1)],
-                           flat[rows * (nodes + 1):])
+        path, number, token = torch.empty(rows * (nodes + 2), dtype=torch.int32, device=device).split((rows * nodes, rows, rows))
+        out = DraftVerdict(path.view(rows, nodes), number, token)
     else:
         for tensor, name, shape in zip(out, DraftVerdict._fields, ((rows, nodes), (rows,), (rows,))):
             _int32(tensor, f"out.{name}", shape, device)
             if not tensor.is_contiguous():
                 raise ValueError(f"out.{name} must be contiguous")
-    a = bdfp4.VerifyArgs()
-    a.rows, a.nodes, a.vocab, a.bf16 = rows, nodes, vocab, int(target_probs.dtype is torch.bfloat16)
     a.target_probs = target_probs.data_ptr()
-    a.target_row_stride, a.target_node_stride = target_probs.stride()[:2]
+    a.target_row_stride, a.target_node_stride, _ = target_probs.stride()
     if draft_probs is not None:
         a.draft_probs = draft_probs.data_ptr()
-        a.draft_row_stride, a.draft_node_stride = draft_probs.stride()[:2]
-    a.tokens, a.tokens_row_stride = tokens.data_ptr(), tokens.stride(0)
-    a.parents, a.parents_row_stride = parents.data_ptr(), parents.stride(0)
-    a.uniforms, a.uniforms_row_stride = uniforms.data_ptr(), uniforms.stride(0)
-    a.node_counts = bdfp4.ptr(node_counts)
+        a.draft_row_stride, a.draft_node_stride, _ = draft_probs.stride()
     a.accepted, a.accepted_counts, a.next_tokens = (t.data_ptr() for t in out)
-    with _on_device(device) as stream:
-        bdfp4.verify_drafts(a, stream)
+    _launch(bdfp4.verify_drafts, a, device)
     return out
 
 
@@ -480,46 +459,45 @@ class DraftCommitter:
         if nodes > MAX_TREE_NODES:
             raise NotImplementedError(f"a tree holds at most {MAX_TREE_NODES} nodes, got {nodes}")
         shape = (self.layers, rows, nodes, self.heads, HEAD_DIM)
-        _tree_tensor(draft_key, "draft_key", shape, device)
-        _tree_tensor(draft_value, "draft_value", shape, device)
-        _int32(accepted, "accepted", (rows, nodes), device)
-        for tensor, name in ((accepted_counts, "accepted_counts"), (seq_lens, "seq_lens"), (row_to_slot, "row_to_slot")):
-            _int32(tensor, name, (rows,), device)
+        a = bdfp4.CommitArgs()
+        a.layers, a.rows, a.nodes, a.heads_kv = self.layers, rows, nodes, self.heads
+        a.draft_key, a.key_layer_stride, a.key_row_stride, a.key_node_stride = _tree_tensor(
+            draft_key, "draft_key", shape, device)
+        a.draft_value, a.value_layer_stride, a.value_row_stride, a.value_node_stride = _tree_tensor(
+            draft_value, "draft_value", shape, device)
+        a.accepted, a.accepted_row_stride = _int32(accepted, "accepted", (rows, nodes), device), accepted.stride(0)
+        a.accepted_counts = _int32(accepted_counts, "accepted_counts", (rows,), device)
+        a.seq_lens = _int32(seq_lens, "seq_lens", (rows,), device)
+        a.row_to_slot = _int32(row_to_slot, "row_to_slot", (rows,), device)
         if (block_table is not None) != (self._seal is not None):
             raise ValueError("block_table goes with a committer that was built with regions, and only with one")
         lengths = torch.empty(4, rows, dtype=torch.int32, device=device)
-        a = bdfp4.CommitArgs()
-        a.layers, a.rows, a.nodes, a.heads_kv = self.layers, rows, nodes, self.heads
-        a.draft_key, a.draft_value = draft_key.data_ptr(), draft_value.data_ptr()
-        a.key_layer_stride, a.key_row_stride, a.key_node_stride = draft_key.stride()[:3]
-        a.value_layer_stride, a.value_row_stride, a.value_node_stride = draft_value.stride()[:3]
-        a.accepted, a.accepted_row_stride = accepted.data_ptr(), accepted.stride(0)
-        a.accepted_counts, a.seq_lens = accepted_counts.data_ptr(), seq_lens.data_ptr()
-        a.row_to_slot = row_to_slot.data_ptr()
         a.tail_key, a.tail_value = self._tail_key.data_ptr(), self._tail_value.data_ptr()
         a.tail_layer_stride, a.tail_slot_stride = self._tail_key.stride(0), self._tail_key.stride(1)
         a.tail_slots, a.sink_tokens, a.rotate = self.slots, self.sink_tokens, int(self._rotate)
         a.key_shift = bdfp4.ptr(self._shift)
-        a.new_seq_lens, a.seqused_fp4, a.seqused_residual, a.seqused_sink = (t.data_ptr() for t in lengths)
+        address = lengths.data_ptr()
+        a.new_seq_lens, a.seqused_fp4, a.seqused_residual, a.seqused_sink = range(address, address + 16 * rows, 4 * rows)
         a.error_word = bdfp4.ptr(self._error_word)
-        with _on_device(device) as stream:
-            if self._seal is None:
-                a.part = bdfp4.COMMIT_ALL
-                bdfp4.commit_drafts(a, stream)
-                return CommittedLengths(*lengths)
-            if block_table.ndim != 2:
-                raise ValueError("block_table must be row-major INT32 with shape [rows, columns]")
-            _int32(block_table, "block_table", (rows, block_table.shape[1]), device)
-            work = torch.empty(2, rows * (PAGE_SIZE // self.page_tokens), dtype=torch.int32, device=device)
-            a.page_table, a.page_table_stride = block_table.data_ptr(), block_table.stride(0)
-            a.max_pages_per_row, a.pages, a.page_tokens = block_table.shape[1], self.pages, self.page_tokens
-            a.source_tokens, a.destination_pages = work[0].data_ptr(), work[1].data_ptr()
-            # the tokens behind a page boundary reuse tail rows that the seal reads, so they wait for it
+        if self._seal is None:
+            a.part = bdfp4.COMMIT_ALL
+            _launch(bdfp4.commit_drafts, a, device)
+            return CommittedLengths(*lengths.unbind())
+        if block_table.ndim != 2:
+            raise ValueError("block_table must be row-major INT32 with shape [rows, columns]")
+        columns = block_table.shape[1]
+        a.page_table = _int32(block_table, "block_table", (rows, columns), device)
+        a.page_table_stride = block_table.stride(0)
+        work = torch.empty(2, rows * (PAGE_SIZE // self.page_tokens), dtype=torch.int32, device=device)
+        a.max_pages_per_row, a.pages, a.page_tokens = columns, self.pages, self.page_tokens
+        a.source_tokens, a.destination_pages = work[0].data_ptr(), work[1].data_ptr()
+        # the tokens behind a page boundary reuse tail rows that the seal reads, so they wait for it
+        with torch.cuda.device(device):
             a.part = bdfp4.COMMIT_HEAD
-            bdfp4.commit_drafts(a, stream)
+            _launch(bdfp4.commit_drafts, a, device)
             writer, regions, _ = self._seal
             writer(self._tail_key.view(-1, self.heads, HEAD_DIM), self._tail_value.view(-1, self.heads, HEAD_DIM), regions,
                    work[0], work[1])
             a.part = bdfp4.COMMIT_REST
-            bdfp4.commit_drafts(a, stream)
-        return CommittedLengths(*lengths)
+            _launch(bdfp4.commit_drafts, a, device)
+        return CommittedLengths(*lengths.unbind())
