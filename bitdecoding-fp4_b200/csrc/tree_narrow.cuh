@@ -1,34 +1,16 @@
-// Attention of a tree of drafted tokens over the paged NVFP4 cache, on the tensor cores.
+// The tree attention for tiles of at most 32 queries.
 //
-// Per (row, KV head) the queries are one matrix of nodes x ratio rows, cut into tiles of NT. Against 128
-// tokens at a time,
-//     S^T [token, query]   = K   [token, channel]  * Q^T
-//     O^T [channel, query] = V^T [channel, token] * P^T
-// both as tcgen05.mma.kind::f16 with the cache operand A in tensor memory and the query-side operand B in
-// shared memory. E2M1 x E4M3 has at most six significant bits and lies in [2^-10, 2688], so a page's values
-// are exact in FP16: a thread reads its own token's (K) or channel's (V) code bytes, converts and scales
-// them in registers and stores them straight into its tensor-memory lane; the dequantized tile never passes
-// through shared memory. P is stored as the softmax threads hold it, one token per thread with its queries
-// contiguous, which is the MN-major form of B.
+// Two CTAs share an SM, and within a CTA the same eight warps convert V and take the softmax, one after the other;
+// only the copies and the products have a warp of their own each. What one CTA waits for (a product, a barrier,
+// tensor memory) the other fills. With warps of one role each, side by side on every scheduler and one CTA per SM,
+// 16 rows x 8 KV heads x 65536 tokens under 32 queries took 430 us; this form took 331.
 //
-// Two CTAs share an SM, and within a CTA the same eight warps convert K, convert V and take the softmax, one
-// after the other; only the copies and the products have warps of their own. What one CTA waits for (a product,
-// a barrier, tensor memory) the other fills. Warps of one role each (keys, values, softmax, side by side on
-// every scheduler) were built first: they waited for instructions a third of the time, since the sum of their
-// loops is larger than a scheduler's instruction cache.
-//
-// Thread r (of 128, twice: each half has half of the channels, tokens or queries) owns token r of S^T. Maxima
-// are per query, in shared memory, and lazy: probabilities are formed against them at once, and only when one
-// comes out more than 2^8 above its maximum (the barrier that ends a step carries that vote) are the maxima
-// taken anew, O^T rescaled and the step formed again. Sums stay per thread until the unit ends. Probabilities
-// carry a factor 2^7, so in FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
-//
-// The rolling tail and the drafts with the sink are two more steps of the same form over BF16 values: K is
-// scaled per token by a power of two into FP16's range (the softmax thread of the token undoes it), V and
-// P are BF16. Queries are scaled per tile the same way.
-//
-// Work is the sequence of all steps of all (row, head, tile) units, cut into equal runs, one per CTA, so any
-// mix of lengths is balanced; a unit that straddles CTAs leaves unnormalised parts that a second kernel adds.
+// Thread r (of 128, twice: each half has half of the channels, tokens or queries) owns token r of S^T and channel r
+// of V. A step: its scores into registers (the next step's are taken meanwhile), its half of V into tensor memory,
+// the vote, the exponentials, P. Now (same case) 325 us, 3.7 TB/s of FP4 cache, 0.57 of a plain copy's rate: 1500
+// cycles a step and SM of which the tensor cores work 15% and the schedulers issue half. What bounds it is the chain
+// of a step's waits (scores, output, vote; 150 to 250 cycles each), of which an SM has only two to overlap; a third
+// CTA's operands do not fit the tensor memory.
 #pragma once
 
 #include "tree_common.cuh"

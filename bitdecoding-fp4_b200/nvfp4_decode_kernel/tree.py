@@ -177,8 +177,10 @@ def tree_decode(
 
     The cache regions, ``fp4_page_table``, ``seqused_fp4`` and the ``residual_*`` / ``seqused_*`` arguments are
     those of :func:`nvfp4_decode_kernel.fp4_decode`; MXFP4 caches are not served. Unlike there, neither the
-    query nor the probabilities are rounded to FP4: cache values enter the products exactly and probabilities
-    as FP16 or BF16, so the result is that of attention over the dequantized cache to BF16 rounding.
+    query nor the probabilities are rounded to one FP4 value: cache values enter the products exactly, queries as
+    four FP4 terms (or FP16, against BF16 tokens) and probabilities as FP16 or BF16, so the result is that of
+    attention over the dequantized cache to BF16 rounding. A draft value that is not finite may reach every node
+    of its row: its weight elsewhere is zero, not absent.
 
     Keys in the cache are rotated and shifted; ``query_rotation="hadamard"`` rotates the queries and the draft
     keys alike, and ``key_shift`` (FP32 ``[heads_kv, 128]``, already rotated) is subtracted from the draft keys,
