@@ -155,9 +155,10 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
   if (a->out_node_stride < (int64_t)a->heads_q * kHeadDim || a->parents_row_stride < 0) return BDFP4_E_ARG;
   const int page_tokens = a->page_tokens == 0 ? kPage : a->page_tokens;
   if (page_tokens != 128 && page_tokens != 64) return BDFP4_E_UNSUPPORTED;
-  // the kernel counts one row's steps (128 tokens of one head and tile of queries) in 32 bits
+  // the kernel counts one row's and one CTA's steps (128 tokens of one head and tile of queries) in 32 bits
   const int64_t tiles = ((int64_t)a->nodes * (a->heads_q / a->heads_kv) + 15) / 16;
-  if (((int64_t)a->max_pages_per_row * page_tokens / kPage + 2) * tiles * a->heads_kv > INT32_MAX) return BDFP4_E_UNSUPPORTED;
+  const int64_t row_steps = ((int64_t)a->max_pages_per_row * page_tokens / kPage + 2) * tiles * a->heads_kv;
+  if (row_steps > INT32_MAX || row_steps * a->rows / kTreeWideCtas >= INT32_MAX) return BDFP4_E_UNSUPPORTED;
   const int64_t head_codes = (int64_t)page_tokens * 64, head_scales = (int64_t)page_tokens * 8;
   if (a->key_codes_pitch % 16 || a->key_scales_pitch % 16 || a->value_codes_pitch % 16 || a->value_scales_pitch % 16 ||
       a->key_codes_pitch < a->heads_kv * head_codes || a->value_codes_pitch < a->heads_kv * head_codes ||

@@ -402,6 +402,20 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem& sm, Walker wa
   constexpr int kEntries = kPage / PT;
   const int64_t tail_row = (int64_t)p.heads_kv * kHeadDim;
   Place<Smem::kStages> at;
+  // No CTA may end under copies in flight, also when nobody waits for them any more. (A stage that was never filled,
+  // or whose last use is over, is in a phase whose predecessor has ended.)
+  auto drain = [&] {
+#pragma unroll 1
+    for (int i = 0; i < Smem::kStages; ++i) {
+      wait(&sm.full[at.slot], at.turn ^ 1, &sm.ignored_flag);
+      at.advance();
+    }
+  };
+  // A stage's turn to be filled. False once somebody has given up: no barrier may be armed twice in a phase.
+  auto emptied = [&]() -> bool {
+    wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
+    return __all_sync(0xffffffffu, *static_cast<volatile int*>(&sm.abort_flag) == 0);
+  };
   Unit u;
   bool known = false;
 #pragma unroll 1
@@ -425,7 +439,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem& sm, Walker wa
         int page[kEntries];
 #pragma unroll
         for (int e = 0; e < kEntries; ++e) page[e] = __shfl_sync(0xffffffffu, mine, i * kEntries + e);
-        wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
+        if (!emptied()) return drain();
         uint64_t* const full = &sm.full[at.slot];
         if (elect_one()) {
           uint8_t* stage = sm.ring[at.slot];
@@ -462,7 +476,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem& sm, Walker wa
 #pragma unroll 1
         for (int first = 0; first < places; first += kBf16Rows) {
           const int end = min(first + kBf16Rows, places);
-          wait(&sm.empty[at.slot], at.turn ^ 1, &sm.abort_flag);
+          if (!emptied()) return drain();
           uint64_t* const full = &sm.full[at.slot];
           // the sink's places behind its length stay empty
           const int absent = kind == kStepDraft && first == 0 ? BDFP4_MAX_SINK - u.info.sink : 0;
@@ -482,15 +496,7 @@ __device__ __forceinline__ void produce(const TreeParams& p, Smem& sm, Walker wa
       }
     }
   }
-  // After an abort nobody else waits for the copies still in flight: no CTA may end under them. (A stage that was
-  // never filled, or whose last use is over, is in a phase whose predecessor has ended.)
-  if (*static_cast<volatile int*>(&sm.abort_flag)) {
-#pragma unroll 1
-    for (int i = 0; i < Smem::kStages; ++i) {
-      wait(&sm.full[at.slot], at.turn ^ 1, &sm.ignored_flag);
-      at.advance();
-    }
-  }
+  drain();
   __syncwarp();
 }
 
