@@ -21,7 +21,7 @@ constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kCacheBarrier = 6;
 // threads for NT = 64, 256 for 128) the kernel spilled, into an L1 that shared memory has left 24 KB of.
 template <int NT>
 struct Shape {
-  static constexpr int kColumns = NT < 32 ? NT : 32;        // queries per softmax thread
+  static constexpr int kColumns = NT < 96 ? 16 : 32;        // queries per softmax thread
   static constexpr int kGroups = NT / kColumns;             // softmax groups of 128 threads
   static constexpr int kBlocks = (NT + 63) / 64;            // 128-byte rows of P per token
   static constexpr int kVBuffers = NT > 96 ? 1 : 2;         // operand buffers in tensor memory, as many as it holds
@@ -36,7 +36,7 @@ struct Shape {
   static constexpr int kControlRegs = kGroups == 4 ? 40 : kGroups == 3 ? 40 : kGroups == 2 ? 56 : 88;
   static_assert(kSoftmaxRegs * kGroups + 2 * kCacheRegs + kControlRegs <= kLaunchRegs * (3 + kGroups), "registers");
   static_assert(kLaunchRegs * kThreads <= 65536, "registers");
-  static constexpr bool kHold = kGroups <= 2;  // a thread's scores stay in registers between the vote and the exponentials
+  static constexpr bool kHold = kColumns <= 16;  // a thread's scores stay in registers between the vote and the exponentials
   // tensor memory columns
   // (the keys of a BF16 step lie where the pages' products had their scales: pages come first in a unit)
   static constexpr int kS = 0, kO = 2 * NT, kV = 3 * NT, kK = kV + 64 * kVBuffers, kKs = kK, kQs = kKs + 16;
