@@ -13,7 +13,7 @@ namespace bdfp4 {
 // The query rows of one KV head are cut into as few tiles as hold them, and those made as even as the built
 // widths allow: a wider tile converts the cache for more queries at once, an empty column costs its share of the
 // products and exponentials. Up to 32 queries go to the kernel of two CTAs per SM (331 us against 430 for 16 rows x
-// 65536 tokens under 32 queries per KV head), wider tiles to the one of one (99 against 120 us for 16 rows x 8192
+// 65536 tokens under 32 queries per KV head), wider tiles to the one of one (82 against 120 us for 16 rows x 8192
 // under 64).
 static int tree_tile(int queries) {
   const int tiles = (queries + kTreeMaxTile - 1) / kTreeMaxTile;

@@ -3,7 +3,7 @@
 // query on an SM) and their surroundings, up to four groups of 128 threads with at most 32 queries per thread. One
 // row of 262145 tokens under 256 query rows per KV head takes 390 us, 705 TFLOP/s of FP16 products or 0.44 of a
 // library product's rate: 2900 cycles a step of 128 queries, tensor cores 31% busy, issue slots 60%. With 64 queries
-// (16 rows x 16 nodes x 8192) 90 us; by two CTAs per SM (tree_narrow.cuh's form) 120.
+// (16 rows x 16 nodes x 8192) 82 us; by two CTAs per SM (tree_narrow.cuh's form) 120.
 #pragma once
 
 #include "tree_common.cuh"
@@ -17,8 +17,11 @@ constexpr int kCtas = kTreeWideCtas;
 constexpr int kSnap = 6;  // steps
 constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kCacheBarrier = 6;
 
-// A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (128
-// threads for NT = 64, 256 for 128) the kernel spilled, into an L1 that shared memory has left 24 KB of.
+// A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (256 threads
+// for NT = 128) the kernel spilled, into an L1 that shared memory has left little of. Sixteen, as many threads as a
+// tile of 64 leaves, let it keep the scores too (82 us for 16 rows x 16 nodes x 8192 against 87 with 32). With 32 they
+// are read twice, once for the vote: forming the probabilities first and keeping them, packed, until the vote is over
+// took 413 us for one row x 262145 against 388.
 template <int NT>
 struct Shape {
   static constexpr int kColumns = NT < 96 ? 16 : 32;        // queries per softmax thread
