@@ -7,7 +7,7 @@
 // FP64: acceptance and the drawn index are decisions next to borders, and at 4 to 8 bytes read per value the
 // FP64 adds (64 per clock and SM) stay well under the time of the reads.
 //
-// Small batches are bound by the launch (19 us a call); 32 rows x 131072 with a drafter take 34 us, five times
+// Small batches are bound by the launch (8 us on the device); 32 rows x 131072 with a drafter take 25 us, five times
 // the reads' time: what counts is the chain of a cluster's passes, one per refusal, each a read, a reduction and an
 // exchange.
 //
@@ -177,8 +177,9 @@ struct Verifier {
   }
 };
 
+// (Two CTAs per SM: with one, at 100 registers, 32 rows in clusters of eight were two waves, 35 us instead of 25.)
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
   const int row = blockIdx.x / parts;
