@@ -37,7 +37,7 @@ ROTATIONS = ("none", "hadamard")
 def _launch(call, args, device: torch.device) -> None:
     """``call`` on the device's current stream; the tensors' device is made current if it is not. (The stream's
     handle alone: making a stream object costs 4 us.)"""
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         call(args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
@@ -195,7 +195,7 @@ def tree_decode(
     if query.ndim != 4 or query.shape[3] != HEAD_DIM:
         raise ValueError("query must be BF16 [rows, nodes, heads_q, 128]")
     rows, nodes, heads_q, _ = query.shape
-    if scale_format(scale_mode) != "nvfp4":
+    if scale_mode != DEFAULT_SCALE_MODE and scale_format(scale_mode) != "nvfp4":
         raise NotImplementedError("tree decode is built for NVFP4 caches only")
     if rows < 1 or nodes < 1:
         raise ValueError("tree decode needs at least one row and one node")
@@ -232,18 +232,23 @@ def tree_decode(
         or tuple(key_shift.shape) != (heads_kv, HEAD_DIM)
     ):
         raise ValueError(f"key_shift must be contiguous FP32 [{heads_kv}, {HEAD_DIM}] on {device}")
-    a.rotate, a.key_shift = int(query_rotation == "hadamard"), bdfp4.ptr(key_shift)
+    a.rotate = int(query_rotation == "hadamard")
+    if key_shift is not None:
+        a.key_shift = key_shift.data_ptr()
     scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not math.isfinite(scale) or scale <= 0.0:
         raise ValueError("softmax_scale must be finite and positive")
-    key_ts, value_ts = (1.0, 1.0) if tensor_scales is None else map(float, tensor_scales)
-    if not (0.0 < key_ts < math.inf and 0.0 < value_ts < math.inf):
-        raise ValueError("tensor_scales must be finite and positive")
+    key_ts = value_ts = 1.0
+    if tensor_scales is not None:
+        key_ts, value_ts = map(float, tensor_scales)
+        if not (0.0 < key_ts < math.inf and 0.0 < value_ts < math.inf):
+            raise ValueError("tensor_scales must be finite and positive")
     a.softmax_scale, a.key_tensor_scale, a.value_tensor_scale = scale, key_ts, value_ts
 
     residual = (residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, seqused_residual)
     has_residual = residual[0] is not None
-    if any((part is not None) != has_residual for part in residual):
+    if has_residual != (residual[1] is not None) or has_residual != (residual[2] is not None) or has_residual != (
+            residual[3] is not None):
         raise ValueError("residual_key_pages_bf16, residual_value_pages_bf16, residual_page_ids, and "
                          "seqused_residual must be provided together")
     if seqused_sink is not None and not has_residual:
