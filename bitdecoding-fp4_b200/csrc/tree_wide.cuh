@@ -361,12 +361,10 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
           }
           tc::tmem_wait_st();
         }
-        if constexpr (Sh::kHold) {
 #pragma unroll
-          for (int j = 0; j < C; j += 16) {
-            load16(j, held + j);
-            above16(j, held + j);
-          }
+        for (int j = Sh::kHold ? 0 : C - 16; j < C; j += 16) {
+          load16(j, held + (Sh::kHold ? j : 0));
+          above16(j, held + (Sh::kHold ? j : 0));
         }
       }
       if constexpr (Sh::kHold) {  // the scores are in registers: the next but one may come
@@ -377,9 +375,9 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       // P of this step goes where the one before the last was
       wait(&sm.p_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.abort_flag);
 #pragma unroll
-      for (int j = 0; j < C; j += 16) {
+      for (int j = C - 16; j >= 0; j -= 16) {  // (the last sixteen are there in any case)
         float* s = Sh::kHold ? held + j : held;
-        if constexpr (!Sh::kHold) {
+        if (!Sh::kHold && j < C - 16) {
           load16(j, s);
           above16(j, s);
         }

@@ -203,7 +203,7 @@ def tree_decode(
         raise NotImplementedError(f"a tree holds at most {MAX_TREE_NODES} nodes, got {nodes}")
     pages, page_tokens, heads_kv, addresses, pitches = _check_regions(
         key_pages_fp4, key_scales, value_pages_fp4, value_scales, device)
-    if heads_q % heads_kv or heads_q < 1:
+    if heads_kv < 1 or heads_q < 1 or heads_q % heads_kv:
         raise ValueError("heads_q must be divisible by heads_kv")
     a = bdfp4.TreeArgs()
     a.rows, a.nodes, a.heads_q, a.heads_kv = rows, nodes, heads_q, heads_kv
