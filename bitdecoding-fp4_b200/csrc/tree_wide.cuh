@@ -1,8 +1,8 @@
 // The tree attention for tiles of 64 to 128 queries: warps of one role each, one CTA per SM. A step's values are
 // converted once for up to 128 queries, so what bounds it is the softmax: 128 x NT exponentials (8 cycles a step and
 // query on an SM) and their surroundings, up to four groups of 128 threads with at most 32 queries per thread. One
-// row of 262145 tokens under 256 query rows per KV head takes 390 us, 705 TFLOP/s of FP16 products or 0.44 of a
-// library product's rate: 2900 cycles a step of 128 queries, tensor cores 31% busy, issue slots 60%. With 64 queries
+// row of 262145 tokens under 256 query rows per KV head takes 367 us, 750 TFLOP/s of FP16 products or 0.47 of a
+// library product's rate: 2750 cycles a step of 128 queries, tensor cores 31% busy, issue slots 60%. With 64 queries
 // (16 rows x 16 nodes x 8192) 82 us; by two CTAs per SM (tree_narrow.cuh's form) 120.
 #pragma once
 
@@ -19,9 +19,9 @@ constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kCacheBarrier = 6;
 
 // A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (256 threads
 // for NT = 128) the kernel spilled, into an L1 that shared memory has left little of. Sixteen, as many threads as a
-// tile of 64 leaves, let it keep the scores too (82 us for 16 rows x 16 nodes x 8192 against 87 with 32). With 32 they
-// are read twice, once for the vote: forming the probabilities first and keeping them, packed, until the vote is over
-// took 413 us for one row x 262145 against 388.
+// tile of 64 leaves, let it keep the scores too (82 us for 16 rows x 16 nodes x 8192 against 87 with 32). With 32,
+// half of them are read twice, for the vote and after it (all of them: 385 us for one row x 262145 against 367; forming
+// the probabilities first and keeping them, packed, until the vote is over: 413).
 template <int NT>
 struct Shape {
   static constexpr int kColumns = NT < 96 ? 16 : 32;        // queries per softmax thread
