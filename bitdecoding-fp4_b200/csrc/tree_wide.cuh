@@ -3,7 +3,7 @@
 // query on an SM) and their surroundings, up to four groups of 128 threads with at most 32 queries per thread. One
 // row of 262145 tokens under 256 query rows per KV head takes 367 us, 750 TFLOP/s of FP16 products or 0.47 of a
 // library product's rate: 2750 cycles a step of 128 queries, tensor cores 31% busy, issue slots 60%. With 64 queries
-// (16 rows x 16 nodes x 8192) 82 us; by two CTAs per SM (tree_narrow.cuh's form) 120.
+// (16 rows x 16 nodes, up to 8192) 82 us; by two CTAs per SM (tree_narrow.cuh's form) 120.
 #pragma once
 
 #include "tree_common.cuh"
@@ -14,7 +14,9 @@ namespace wide {
 
 // Named barriers: one per softmax group (four at most), all softmax threads, the key threads.
 constexpr int kCtas = kTreeWideCtas;
-constexpr int kSnap = 6;  // steps
+// How near a unit's end a cut moves there, in steps (3, 6, 10, 16 measured: 16 rows x 16 nodes x 2048 51, 49, 41, 41 us,
+// 24 rows x 61 nodes x 2048 218, 214, 201, 201, a ragged batch of 16 rows up to 8192 80, 82, 84, 89).
+constexpr int kSnap = 10;
 constexpr int kGroupBarrier = 1, kSoftmaxBarrier = 5, kCacheBarrier = 6;
 
 // A softmax thread holds at most 32 queries: their sums stay in registers for a whole unit, and with 64 (256 threads
