@@ -54,7 +54,8 @@ __device__ __forceinline__ void commit_lengths(const CommitParams& p, int row, i
   p.residual[row] = total - fp4;
   p.sink_out[row] = min(total, p.sink);
   const bool fills = live && total / kPage > n / kPage;
-  if (!p.table) return;
+  if (!p.source_tokens) return;
+  // (every entry is written, whatever the table holds: the page writers follow what stands here)
   const int entries = kPage / p.page_tokens;
   for (int e = 0; e < entries; ++e) {
     const int column = (total / kPage - 1) * entries + e;
@@ -180,7 +181,9 @@ extern "C" int bdfp4_commit_drafts(const bdfp4_commit_args* a, void* stream_hand
     return BDFP4_E_ARG;
   const int page_tokens = a->page_tokens == 0 ? kPage : a->page_tokens;
   if (page_tokens != 128 && page_tokens != 64) return BDFP4_E_UNSUPPORTED;
-  if (a->page_table && (!a->source_tokens || !a->destination_pages || a->max_pages_per_row < 0 || a->pages < 1))
+  if (!a->source_tokens != !a->destination_pages) return BDFP4_E_ARG;
+  if (a->source_tokens ? a->max_pages_per_row < 0 || a->pages < 1 || (!a->page_table && a->max_pages_per_row > 0)
+                       : a->page_table != nullptr)
     return BDFP4_E_ARG;
   CommitParams p{};
   p.layers = a->layers;

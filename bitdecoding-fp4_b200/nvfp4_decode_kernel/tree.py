@@ -455,7 +455,9 @@ class DraftCommitter:
         same tensors :func:`tree_decode` read, all layers). Token ``p`` goes to row ``p % 128`` of slot
         ``row_to_slot[r]`` and, below ``sink_tokens``, to the sink; a negative slot leaves its row alone.
         ``block_table`` INT32 ``[rows, columns]`` names the pages that filled tails are sealed into and is required
-        when the committer was built with ``regions``. Returns the new lengths; ``seq_lens`` is not changed.
+        when the committer was built with ``regions``; a page without a valid entry there (or behind the last
+        column) is not sealed and sets ``bdfp4.DEV_BAD_PAGE`` in the error word. Returns the new lengths;
+        ``seq_lens`` is not changed.
         """
         device = self._device
         if not isinstance(draft_key, torch.Tensor) or draft_key.ndim != 5:

@@ -692,14 +692,14 @@ typedef struct bdfp4_commit_args {
   int64_t tail_layer_stride, tail_slot_stride;
   int32_t tail_slots, sink_tokens, rotate, part;
   const float* key_shift;
-  const int32_t* page_table; /* or null: no page is sealed */
+  const int32_t* page_table; /* null when max_pages_per_row is 0: no row has a place for a page */
   int64_t page_table_stride;
   int32_t max_pages_per_row, pages, page_tokens, reserved;
   int32_t* new_seq_lens;    /* [rows] each */
   int32_t* seqused_fp4;
   int32_t* seqused_residual;
   int32_t* seqused_sink;
-  int32_t* source_tokens;   /* or null without page_table */
+  int32_t* source_tokens;   /* both null: no page is sealed (and there is no page_table) */
   int32_t* destination_pages;
   int32_t* error_word;
 } bdfp4_commit_args;

@@ -1,0 +1,33 @@
+"""Arguments that the C entries of the speculative-decoding operators have to tell apart. Every call here ends in a
+refusal of its own kind, so none is launched wherever this runs; addresses are never followed."""
+
+import ctypes
+
+import pytest
+
+
+def _commit_args():
+    import bdfp4
+
+    a = bdfp4.CommitArgs()
+    a.layers, a.rows, a.nodes, a.heads_kv, a.tail_slots, a.page_tokens, a.pages = 1, 2, 5, 2, 3, 128, 4
+    for name in ("draft_key", "draft_value", "accepted", "accepted_counts", "seq_lens", "row_to_slot", "tail_key",
+                 "tail_value", "page_table", "new_seq_lens", "seqused_fp4", "seqused_residual", "seqused_sink",
+                 "source_tokens", "destination_pages"):
+        setattr(a, name, 1 << 20)
+    a.max_pages_per_row, a.page_table_stride = 2, 2
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(source_tokens=0), dict(destination_pages=0), dict(source_tokens=0, destination_pages=0),
+    dict(page_table=0), dict(pages=0), dict(max_pages_per_row=-1), dict(page_table=0, max_pages_per_row=0, pages=0),
+])
+def test_commit_work_table_goes_with_a_page_table(change):
+    """Both halves of the work table or neither; a table of no columns may have no address, one of some may not."""
+    import bdfp4
+
+    a = _commit_args()
+    for name, value in change.items():
+        setattr(a, name, value)
+    assert bdfp4.library().bdfp4_commit_drafts(ctypes.byref(a), None) == bdfp4.E_ARG
