@@ -12,7 +12,9 @@
 // exchange.
 //
 // A row is one cluster of CTAs that share the vocabulary; every CTA does the same walk from the same
-// numbers, and the passes' sums are exchanged through distributed shared memory.
+// numbers, and the passes' sums are exchanged through distributed shared memory. A CTA may only store into
+// another's once that one runs: all arrive on the cluster's barrier as they start, and wait for it before their
+// first store, behind the gather, the walk and the first pass.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -177,6 +179,10 @@ struct Verifier {
   }
 };
 
+// All threads of every CTA of the cluster, once each; the warps converged.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // (Two CTAs per SM: with one, at 100 registers, 32 rows in clusters of eight were two waves, 35 us instead of 25.)
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyParams p) {
@@ -204,6 +210,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     }
     return;
   }
+  if (parts > 1) cluster_arrive();
   const T* target = static_cast<const T*>(p.target) + row * p.target_row;
   const T* draft = DRAFT ? static_cast<const T*>(p.draft) + row * p.draft_row : nullptr;
   if ((int)threadIdx.x < count) {
@@ -231,6 +238,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
   if (part == 0 && threadIdx.x == 0) accepted[0] = 0;
   const int g = part * kVerifyWarps + warp, warps = parts * kVerifyWarps;
   bool summed = false;  // s_totals[buffer] holds the current weights' sums
+  bool started = parts == 1;  // every CTA of the cluster is known to run
   double total = 0.0;
   while (true) {
     if (warp == 0) {  // the walk, up to its end or to a refusal that needs a pass
@@ -303,6 +311,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
       const Verifier<T, DRAFT> verifier{p, s_refusals, lane};
       const double mine = verifier.slice_total(target_row, draft_row, g);
       buffer ^= 1;
+      if (!started) cluster_wait();
+      started = true;
       if (lane < parts) cluster.map_shared_rank(&s_totals[buffer][0], lane)[g] = mine;
       if (parts > 1) cluster.sync();
       else __syncthreads();

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from test_gpu_commit_drafts import _commit, _expect, _setup
+from test_gpu_verify_drafts import _case as _verify_case, _check as _verify_check, _run as _verify_run
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +33,22 @@ def test_commit_with_a_table_of_no_columns(page_tokens):
     s["seq_lens"] = torch.tensor([100, 5, 200], dtype=torch.int32)
     _commit(s, True, error=error, block_table=s["table"][:, :0].cuda())
     assert int(error) == 0 and all(torch.equal(a, b) for a, b in zip(s["blocks"], before))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("drafter", [False, True])
+def test_verify_clusters_that_start_one_by_one(dtype, drafter):
+    """Rows of eight CTAs each while another stream's products keep every SM busy, so that the CTAs of a row start as
+    places come free; every sum that crosses between them counts."""
+    c = _verify_case(18, 5, 70000, dtype, drafter, seed=71)
+    cuda = {k: None if v is None else v.cuda() for k, v in c.items()}
+    want = _verify_run(cuda)
+    _verify_check(c, want)
+    busy, side = torch.randn(2048, 2048, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                busy @ busy
+        for a, b in zip(_verify_run(cuda), want):
+            assert torch.equal(a, b)
