@@ -214,7 +214,16 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
       float s[C];
       tmem_load<C>(scores, s);
       tc::tmem_wait_ld();
-      if (special) {
+      // scores -> log2 units above the maxima, plus kShift
+      const float2 f2 = make_float2(f, f);
+#pragma unroll
+      for (int j = 0; j < C; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(base + j);
+        const float2 y0 = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, make_float2(b.x, b.y));
+        const float2 y1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), f2, make_float2(b.z, b.w));
+        s[j] = y0.x, s[j + 1] = y0.y, s[j + 2] = y1.x, s[j + 3] = y1.y;
+      }
+      if (special) {  // (masked behind the scaling: a factor may underflow to zero, and its product with -inf is NaN)
         bool dead;  // no query sees this thread's token
         if (kind == kStepPage) dead = t < u.info.sink;
         else if (kind == kStepTail) dead = t >= u.info.residual || (u.info.pages == 0 && t < u.info.sink);
@@ -225,17 +234,9 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
         for (int j = 0; j < C; ++j)
           if (!((seen >> j) & 1)) s[j] = -INFINITY;
       }
-      // scores -> log2 units above the maxima, plus kShift
-      const float2 f2 = make_float2(f, f);
       float highest = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < C; j += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(base + j);
-        const float2 y0 = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, make_float2(b.x, b.y));
-        const float2 y1 = __ffma2_rn(make_float2(s[j + 2], s[j + 3]), f2, make_float2(b.z, b.w));
-        s[j] = y0.x, s[j + 1] = y0.y, s[j + 2] = y1.x, s[j + 3] = y1.y;
-        highest = fmaxf(fmaxf(highest, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
-      }
+      for (int j = 0; j < C; j += 4) highest = fmaxf(fmaxf(highest, fmaxf(s[j], s[j + 1])), fmaxf(s[j + 2], s[j + 3]));
       // the next step's scores are taken while this one's probabilities are formed
       float next_f = f;
       if (step + 1 < u.end) {

@@ -293,6 +293,9 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       auto load16 = [&](int j, float* s) {
         tc::tmem_ld16(scores + j, s);
         tc::tmem_wait_ld();
+      };
+      // (behind the scaling: a factor may underflow to zero, and its product with -inf is NaN)
+      auto mask16 = [&](int j, float* s) {
         if (kind == kStepDraft) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -308,6 +311,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
           const float2 y1 = __ffma2_rn(make_float2(s[i + 2], s[i + 3]), f2, make_float2(b.z, b.w));
           s[i] = y0.x, s[i + 1] = y0.y, s[i + 2] = y1.x, s[i + 3] = y1.y;
         }
+        mask16(j, s);
       };
       float held[Sh::kHold ? C : 16];
       float highest = -INFINITY;
@@ -324,10 +328,13 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
         for (int j = 0; j < C; j += 16) {
           float s[16];
           load16(j, s);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] *= f;
+          mask16(j, s);
           float mine = 0.0f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float m = warp_max(dead ? -INFINITY : s[i] * f);
+            const float m = warp_max(dead ? -INFINITY : s[i]);
             if (lane == i) mine = m;
           }
           if (lane < 16) sm.col[warp][first_column + j + lane] = mine;

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from test_gpu_commit_drafts import _commit, _expect, _setup
+from test_gpu_tree_decode import _call as _tree_call, _check as _tree_check, _inputs as _tree_inputs
 from test_gpu_verify_drafts import _case as _verify_case, _check as _verify_check, _run as _verify_run
 
 pytestmark = pytest.mark.gpu
@@ -52,3 +53,15 @@ def test_verify_clusters_that_start_one_by_one(dtype, drafter):
                 busy @ busy
         for a, b in zip(_verify_run(cuda), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("nodes,heads", [(3, (4, 1)), (9, (8, 2)), (13, (8, 2)), (23, (8, 2)), (30, (8, 2))])
+@pytest.mark.parametrize("rotate", [False, True])
+def test_products_below_the_smallest_number(nodes, heads, rotate):
+    """Queries, tail keys and draft keys of 2^-70: every score is zero to FP32, every token a node sees counts alike,
+    and no masked one reaches it. (The tile widths of both kernels.)"""
+    w, x = _tree_inputs([20, 300, 150], nodes, *heads, seed=72, rotate=rotate)
+    w.tail_key.mul_(2.0 ** -70)
+    tiny = dict(x, query=(x["query"].double() * 2.0 ** -70).to(torch.bfloat16),
+                draft_key=(x["draft_key"].double() * 2.0 ** -70).to(torch.bfloat16))
+    _tree_check(w, tiny, _tree_call(w, tiny, query_rotation="hadamard" if rotate else "none"), rotate=rotate)
