@@ -288,14 +288,12 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       tc::fence_after_sync();
       float f = page_factor;
       if (kind != kStepPage) f = p.scale_log2 * q_inverse * sm.key_factor[n & 7][t];
+      f = fmaxf(f, 1.0e-38f);  // (where it underflows to zero, its product with a mask's -inf would be NaN)
       const float2 f2 = make_float2(f, f);
       const uint32_t scores = sm.tmem + Sh::kS + (n & 1) * NT + first_column + lanes;
       auto load16 = [&](int j, float* s) {
         tc::tmem_ld16(scores + j, s);
         tc::tmem_wait_ld();
-      };
-      // (behind the scaling: a factor may underflow to zero, and its product with -inf is NaN)
-      auto mask16 = [&](int j, float* s) {
         if (kind == kStepDraft) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -311,7 +309,6 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
           const float2 y1 = __ffma2_rn(make_float2(s[i + 2], s[i + 3]), f2, make_float2(b.z, b.w));
           s[i] = y0.x, s[i + 1] = y0.y, s[i + 2] = y1.x, s[i + 3] = y1.y;
         }
-        mask16(j, s);
       };
       float held[Sh::kHold ? C : 16];
       float highest = -INFINITY;
@@ -328,13 +325,10 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
         for (int j = 0; j < C; j += 16) {
           float s[16];
           load16(j, s);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] *= f;
-          mask16(j, s);
           float mine = 0.0f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float m = warp_max(dead ? -INFINITY : s[i]);
+            const float m = warp_max(dead ? -INFINITY : s[i] * f);
             if (lane == i) mine = m;
           }
           if (lane < 16) sm.col[warp][first_column + j + lane] = mine;
