@@ -273,15 +273,21 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
         if (lane < C) sm.col[warp][first_column + lane] = mine;
         bar_sync(barrier, 128);
         if (t < C) {
+          // The new maximum is taken from the scores as they stand, above the old one, and all move by the same
+          // difference: between a score and a maximum that were rounded apart, differences beyond FP16's range open
+          // up as soon as scores exceed 2^27.
           const int col = first_column + t;
-          const float before = top[t], was = base[t];
-          const float now = fmaxf(fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]),
-                                        fmaxf(sm.col[2][col], sm.col[3][col])) - was, before);
-          const float is = now == kNoMax ? 0.0f : kShift - now;
-          top[t] = now;
-          base[t] = is;
-          sm.shift[col] = is - was;
-          sm.factor[col] = ex2(before - now);
+          const float m = fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]), fmaxf(sm.col[2][col], sm.col[3][col]));
+          const bool none = top[t] == kNoMax;
+          float move = 0.0f, factor = 1.0f;
+          if (none ? m > -INFINITY : m > kShift) {
+            move = kShift - m;
+            factor = none ? 0.0f : ex2(move);
+            base[t] += move;
+            top[t] = kShift - base[t];
+          }
+          sm.shift[col] = move;
+          sm.factor[col] = factor;
         }
         bar_sync(barrier, 128);
 #pragma unroll

@@ -67,6 +67,9 @@ struct Smem {
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
   float factor[NT];     // what a renewal does to sums (at a unit's end: 1 / weight)
+  float level[NT];      // power of two that a column's scores are brought down by, where a group has any
+  float lower[NT];      // ... by the last renewal
+  bool leveled[Sh::kGroups], lowered[Sh::kGroups];
   float col[4][NT];     // a warp's maxima, then sums
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
   float q_max[16];
@@ -269,7 +272,10 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     for (int j = t; j < C; j += 128) {
       top[j] = kNoMax;
       base[j] = kShift - kNoMax;
+      sm.level[first_column + j] = 1.0f;
     }
+    if (t == 0) sm.leveled[group] = false;
+    bool leveled = false;
     if (warp == 0) make_masks(p, u, sm.parents, sm.seen_by[group], u.tile * NT + first_column, lane);
     float2 sum[C / 2];
 #pragma unroll
@@ -291,6 +297,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       f = fmaxf(f, 1.0e-38f);  // (where it underflows to zero, its product with a mask's -inf would be NaN)
       const float2 f2 = make_float2(f, f);
       const uint32_t scores = sm.tmem + Sh::kS + (n & 1) * NT + first_column + lanes;
+      if (leveled) scale_columns<C>(scores, sm.level + first_column);
       auto load16 = [&](int j, float* s) {
         tc::tmem_ld16(scores + j, s);
         tc::tmem_wait_ld();
@@ -333,17 +340,35 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
           }
           if (lane < 16) sm.col[warp][first_column + j + lane] = mine;
         }
+        if (t == 0) sm.lowered[group] = false;
         bar_sync(barrier, 128);
         for (int j = t; j < C; j += 128) {
           const int col = first_column + j;
           const float before = top[j];
-          const float now = fmaxf(fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]),
-                                        fmaxf(sm.col[2][col], sm.col[3][col])), before);
+          float now = fmaxf(fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]),
+                                  fmaxf(sm.col[2][col], sm.col[3][col])), before);
+          sm.factor[col] = ex2((before - now) / sm.level[col]);
+          // A score's product is not rounded before the maximum, which was, is taken off: above 2^27 the two stand
+          // further apart than FP16's exponents reach. Such a query's scores are brought down to 2^22 by a power of two:
+          // what then differs by less than 64 (log2) did so by less than 2^-16 of the scores, which is what the
+          // rounding of their products and sums may come to.
+          float lower = 1.0f;
+          if (fabsf(now) >= 8388608.0f && now > kNoMax) {
+            float ignored;
+            lower = scale_to<22>(fabsf(now), &ignored);
+            now *= lower;
+            sm.level[col] *= lower;
+            sm.leveled[group] = sm.lowered[group] = true;
+          }
+          sm.lower[col] = lower;
           top[j] = now;
           base[j] = kShift - now;
-          sm.factor[col] = ex2(before - now);
         }
         bar_sync(barrier, 128);
+        if (sm.lowered[group]) {
+          leveled = true;
+          scale_columns<C>(scores, sm.lower + first_column);
+        }
 #pragma unroll
         for (int j = 0; j < C / 2; ++j) {
           sum[j].x *= sm.factor[first_column + 2 * j];
@@ -440,7 +465,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       if (whole) {
         sm.factor[col] = total > 0.0f ? p.value_scale / total : 0.0f;
       } else {
-        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[j];
+        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[j] / sm.level[col];
         p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
       }
     }

@@ -65,3 +65,69 @@ def test_products_below_the_smallest_number(nodes, heads, rotate):
     tiny = dict(x, query=(x["query"].double() * 2.0 ** -70).to(torch.bfloat16),
                 draft_key=(x["draft_key"].double() * 2.0 ** -70).to(torch.bfloat16))
     _tree_check(w, tiny, _tree_call(w, tiny, query_rotation="hadamard" if rotate else "none"), rotate=rotate)
+
+
+def _needles(w, nodes, heads_q, seed, loud):
+    """Inputs whose every query asks for one token: along that token's key, with the workload's outlier channels evened
+    out, so that its score stands far above all others. Query by query the token lies in the pages (spread over them),
+    the tail, the sink, among the node's ancestors. Returns the inputs and the values asked for."""
+    from oracle import tree_oracle as oracle
+    from test_gpu_tree_decode import _trees
+
+    gen = torch.Generator().manual_seed(seed)
+    rows, heads = w.rows, w.heads_kv
+    even = w.outlier_scale.cpu().double() ** -2
+    x = dict(draft_key=(torch.randn(rows, nodes, heads, 128, generator=gen) * w.outlier_scale.cpu()).to(torch.bfloat16),
+             draft_value=torch.randn(rows, nodes, heads, 128, generator=gen).to(torch.bfloat16),
+             parents=_trees(rows, nodes, gen))
+    key, value = oracle.cache_values(w.blocks, heads, w.page_tokens)
+    query = torch.zeros(rows, nodes, heads_q, 128, dtype=torch.bfloat16)
+    want = torch.zeros(rows, nodes, heads_q, 128, dtype=torch.float64)
+    for r in range(rows):
+        fp4, residual, sink = (int(t[r]) for t in (w.seqused_fp4, w.seqused_residual, w.seqused_sink))
+        ids = w.page_table[r, :fp4 // w.page_tokens].cpu().long()
+        tail_key, tail_value = w.tail_key[0, r].cpu().double(), w.tail_value[0, r].cpu().double()
+        k = torch.cat([key[ids].reshape(-1, heads, 128), tail_key[:residual], tail_key[128:128 + sink], x["draft_key"][r].double()])
+        v = torch.cat([value[ids].reshape(-1, heads, 128), tail_value[:residual], tail_value[128:128 + sink],
+                       x["draft_value"][r].double()])
+        first = [0, fp4, fp4 + residual, fp4 + residual + sink]
+        cached = torch.ones(first[3], dtype=torch.bool)
+        cached[:sink] = False
+        cached[first[2]:] = True
+        asked = []  # (node, head, token)
+        for i, family in enumerate(oracle.ancestors(x["parents"][r].tolist())):
+            for h in range(heads_q):
+                n = i * heads_q + h
+                choices = [torch.nonzero(cached[a:b])[:, 0] + a for a, b in zip(first, first[1:])] + [torch.nonzero(family)[:, 0] + first[3]]
+                part = choices[(n + r) % 4]
+                if not len(part):
+                    part = choices[3]
+                spread = (n * 0.6180339887) % 1.0
+                asked.append((i, h, int(part[int(spread * len(part))]), family))
+        for i, h, t, family in asked:
+            kv = h * heads // heads_q
+            direction = loud * k[t, kv] * even[kv]
+            query[r, i, h] = direction.to(torch.bfloat16)
+            want[r, i, h] = v[t, kv]
+            score = query[r, i, h].double() @ k[:, kv].T * 128 ** -0.5 * 1.4427
+            score[:first[3]][~cached] = -float("inf")
+            score[first[3]:][~family] = -float("inf")
+            best = float(score[t])
+            score[t] = -float("inf")
+            assert best - float(score.max()) > 40 + 0.05 * best, "an input that does not single out its token: choose another"
+    return dict(x, query=query), want
+
+
+def _check_needles(got, want):
+    # the token's probability is rounded to BF16 at most (2^-8) against a sum that is not, and so is the result
+    assert bool(((got.cpu().double() - want).abs() <= 1.05 * 2.0 ** -7 * want.abs() + 1e-6).all())
+
+
+@pytest.mark.parametrize("nodes,heads", [(3, (4, 1)), (9, (6, 2)), (13, (8, 2)), (23, (8, 2)), (30, (8, 2))])
+@pytest.mark.parametrize("factor", [1.0, 2.0 ** 22, 2.0 ** 60, 2.0 ** 100])
+def test_scores_beyond_the_fraction_of_a_float(nodes, heads, factor):
+    """Scores whose rounding is larger than any difference that FP16's exponents can hold: the token with the highest
+    one is still the answer."""
+    w, _ = _tree_inputs([700, 130, 20, 1300], 1, *heads, seed=74)
+    x, want = _needles(w, nodes, heads[0], 75, 16.0 * factor)
+    _check_needles(_tree_call(w, x), want)
