@@ -535,9 +535,13 @@ __device__ __forceinline__ void interleave_scales(uint8_t* scales, int lane) {
 
 // The tile's queries into shared memory, a group of sixteen values per thread and pass: as kTerms FP4 terms for the
 // pages, and as FP16 for the BF16 steps. Rotated if asked, and scaled by one power of two: a query whose largest
-// value is 2^-8 of the tile's still has all four terms above E4M3's smallest scale. Returns what undoes the scale.
+// value is 2^-5 of the tile's still has all four terms above E4M3's smallest normal scale. Where one's is less, every
+// query is scaled by its own power of two instead (`uneven`), and its scores are brought down to the tile's
+// (query_level): what is lost of a query goes by its own values, whatever the others of its tile are. Returns what
+// undoes the tile's scale. sm.own: each query's largest value.
 template <int NT, int THREADS, typename Smem>
-__device__ __forceinline__ float load_queries(const TreeParams& p, Smem& sm, int barrier, const Unit& u, int thread) {
+__device__ __forceinline__ float load_queries(const TreeParams& p, Smem& sm, int barrier, const Unit& u, int thread,
+                                              bool& uneven) {
   constexpr int kPerPass = THREADS / 8, kPasses = (NT + kPerPass - 1) / kPerPass;
   const int group = thread & 7;
   const int queries = min(u.info.count * p.ratio - u.tile * NT, NT);
@@ -552,31 +556,45 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem& sm, int
                        (int64_t)(u.head * p.ratio + query % p.ratio) * kHeadDim + group * kGroup, v[i]);
   }
   if (thread < BDFP4_MAX_TREE_NODES) sm.parents[thread] = thread < u.info.count ? p.parents[u.row * p.parents_row + thread] : -1;
-  float amax = 0.0f;
+  float amax = 0.0f, amin = INFINITY;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
+    const int r = i * kPerPass + (thread >> 3);
     if (p.rotate) {
       hadamard_butterflies(v[i], group);
 #pragma unroll
       for (int j = 0; j < 16; ++j) v[i][j] *= kInvSqrt128;
     }
+    float own = 0.0f;
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (fabsf(v[i][j]) < INFINITY) amax = fmaxf(amax, fabsf(v[i][j]));
+      if (fabsf(v[i][j]) < INFINITY) own = fmaxf(own, fabsf(v[i][j]));
+#pragma unroll
+    for (int step = 4; step > 0; step >>= 1) own = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, step));
+    if (group == 0 && r < NT) sm.own[r] = own;
+    amax = fmaxf(amax, own);
+    if (own > 0.0f) amin = fminf(amin, own);
   }
   amax = warp_max(amax);
-  if ((thread & 31) == 0) sm.q_max[thread >> 5] = amax;
+  amin = -warp_max(-amin);
+  if ((thread & 31) == 0) sm.q_range[thread >> 5] = make_float2(amax, amin);
   bar_sync(barrier, THREADS);
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) amax = fmaxf(amax, sm.q_max[i]);
+  for (int i = 0; i < THREADS / 32; ++i) {
+    amax = fmaxf(amax, sm.q_range[i].x);
+    amin = fminf(amin, sm.q_range[i].y);
+  }
+  uneven = amin * 32.0f < amax;
   float inverse;
   const float scale = scale_to<10>(amax, &inverse);
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int r = i * kPerPass + (thread >> 3);
     if (kPasses * kPerPass > NT && r >= NT) break;
+    float by = scale, ignored;
+    if (uneven) by = scale_to<10>(sm.own[min(r, NT - 1)], &ignored);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[i][j] *= scale;
+    for (int j = 0; j < 16; ++j) v[i][j] *= by;
     {
       uint8_t* row = sm.q[group >> 2] + r * 128;
       uint32_t w[8];
@@ -613,6 +631,14 @@ __device__ __forceinline__ float load_queries(const TreeParams& p, Smem& sm, int
   }
   tc::fence_proxy_async_smem();
   return inverse;
+}
+
+// What brings the scores of a query of an uneven tile, whose largest value is `own`, down to the tile's scale, which
+// `inverse` undoes.
+__device__ __forceinline__ float query_level(float own, float inverse) {
+  float mine;
+  scale_to<10>(own, &mine);
+  return own > 0.0f ? mine / inverse : 1.0f;
 }
 
 // Channel t of a tile's queries out of tensor memory: `columns` of them from column `at` (of the tile's

@@ -50,7 +50,9 @@ struct Smem {
   float top[NT];        // maximum, log2 units
   float factor[NT], shift[NT];  // what a renewal does to sums and scores (at a unit's end: 1 / weight)
   float col[4][NT];             // a warp's maxima, then sums
-  float q_max[8];
+  float level[NT];              // what brings a query's scores down to the tile's scale (in uneven tiles)
+  float own[NT];
+  float2 q_range[8];
   int parents[BDFP4_MAX_TREE_NODES];
   uint64_t full[kStages], empty[kStages];
   uint64_t s_ready, s_full, p_full, o_full, drained;  // s_ready: the scores before are read, BF16 keys in their operand
@@ -178,8 +180,10 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
   bool known = false;
 #pragma unroll 1
   for (; walker.next(u, known); known = true) {
-    const float q_inverse = load_queries<NT, kWorkers>(p, sm, kWorkBarrier, u, thread);
+    bool uneven;
+    const float q_inverse = load_queries<NT, kWorkers>(p, sm, kWorkBarrier, u, thread, uneven);
     if (t < C) {
+      sm.level[first_column + t] = query_level(sm.own[first_column + t], q_inverse);
       top[t] = kNoMax;
       base[t] = 0.0f;  // scores as they are
     }
@@ -211,6 +215,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
       wait(&sm.s_full, parity, &sm.abort_flag);
       tc::fence_after_sync();
 
+      if (uneven) scale_columns<C>(scores, sm.level + first_column);
       float s[C];
       tmem_load<C>(scores, s);
       tc::tmem_wait_ld();

@@ -67,12 +67,14 @@ struct Smem {
   float base[NT];       // kShift - maximum
   float top[NT];        // maximum, log2 units
   float factor[NT];     // what a renewal does to sums (at a unit's end: 1 / weight)
-  float level[NT];      // power of two that a column's scores are brought down by, where a group has any
-  float lower[NT];      // ... by the last renewal
-  bool leveled[Sh::kGroups], lowered[Sh::kGroups];
+  float level[NT];      // power of two that a column's scores are multiplied by as they come, where a group has any
+  float squeeze[NT];    // undoes what renewals made of it
+  float lower[NT];      // what the last renewal did
+  bool lowered[Sh::kGroups];
   float col[4][NT];     // a warp's maxima, then sums
   float key_factor[8][128];  // what undoes the scaling of a BF16 step's keys, by step number
-  float q_max[16];
+  float own[NT];
+  float2 q_range[16];
   int parents[BDFP4_MAX_TREE_NODES];
   uint64_t full[kStages], empty[kStages];
   uint64_t ka_full, ka_empty, va_full[2], va_empty[2];  // operands: BF16 keys, values
@@ -245,8 +247,8 @@ __device__ __forceinline__ void cache(const TreeParams& p, Smem<NT>& sm, Walker 
 }
 
 template <int NT>
-__device__ __forceinline__ float bring_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread) {
-  const float inverse = load_queries<NT, Shape<NT>::kSoftmaxThreads>(p, sm, kSoftmaxBarrier, u, thread);
+__device__ __forceinline__ float bring_queries(const TreeParams& p, Smem<NT>& sm, const Unit& u, int thread, bool& uneven) {
+  const float inverse = load_queries<NT, Shape<NT>::kSoftmaxThreads>(p, sm, kSoftmaxBarrier, u, thread, uneven);
   __syncwarp();
   if ((thread & 31) == 0) tc::mbar_arrive(&sm.q_full);
   return inverse;
@@ -267,15 +269,15 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
   Unit u;
   if (!walker.next(u, false)) return;
   bool more = true;
-  float q_inverse = bring_queries<NT>(p, sm, u, thread);
+  bool leveled;  // the group's scores are brought down as they come
+  float q_inverse = bring_queries<NT>(p, sm, u, thread, leveled);
   while (more) {
     for (int j = t; j < C; j += 128) {
       top[j] = kNoMax;
       base[j] = kShift - kNoMax;
-      sm.level[first_column + j] = 1.0f;
+      sm.level[first_column + j] = leveled ? query_level(sm.own[first_column + j], q_inverse) : 1.0f;
+      sm.squeeze[first_column + j] = 1.0f;
     }
-    if (t == 0) sm.leveled[group] = false;
-    bool leveled = false;
     if (warp == 0) make_masks(p, u, sm.parents, sm.seen_by[group], u.tile * NT + first_column, lane);
     float2 sum[C / 2];
 #pragma unroll
@@ -347,18 +349,19 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
           const float before = top[j];
           float now = fmaxf(fmaxf(fmaxf(sm.col[0][col], sm.col[1][col]),
                                   fmaxf(sm.col[2][col], sm.col[3][col])), before);
-          sm.factor[col] = ex2((before - now) / sm.level[col]);
+          sm.factor[col] = ex2((before - now) * sm.squeeze[col]);
           // A score's product is not rounded before the maximum, which was, is taken off: above 2^27 the two stand
           // further apart than FP16's exponents reach. Such a query's scores are brought down to 2^22 by a power of two:
           // what then differs by less than 64 (log2) did so by less than 2^-16 of the scores, which is what the
           // rounding of their products and sums may come to.
           float lower = 1.0f;
           if (fabsf(now) >= 8388608.0f && now > kNoMax) {
-            float ignored;
-            lower = scale_to<22>(fabsf(now), &ignored);
+            float back;
+            lower = scale_to<22>(fabsf(now), &back);
             now *= lower;
             sm.level[col] *= lower;
-            sm.leveled[group] = sm.lowered[group] = true;
+            sm.squeeze[col] *= back;
+            sm.lowered[group] = true;
           }
           sm.lower[col] = lower;
           top[j] = now;
@@ -451,8 +454,9 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
     Unit following = u;
     more = walker.next(following, true);
     float next_inverse = 1.0f;
+    bool next_leveled = false;
     bar_sync(kSoftmaxBarrier, Sh::kSoftmaxThreads);  // both groups have seen their last scores; the parents are free
-    if (more) next_inverse = bring_queries<NT>(p, sm, following, thread);
+    if (more) next_inverse = bring_queries<NT>(p, sm, following, thread, next_leveled);
     bar_sync(barrier, 128);
     const bool whole = u.begin == 0 && u.end == u.info.steps;
     const long long at_step = done - u.begin;  // where the unit begins in the launch's steps
@@ -465,7 +469,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       if (whole) {
         sm.factor[col] = total > 0.0f ? p.value_scale / total : 0.0f;
       } else {
-        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[j] / sm.level[col];
+        p.partial_stat[(int64_t)(2 * part) * NT + col] = top[j] * sm.squeeze[col];
         p.partial_stat[(int64_t)(2 * part + 1) * NT + col] = total;
       }
     }
@@ -486,6 +490,7 @@ __device__ __forceinline__ void softmax(const TreeParams& p, Smem<NT>& sm, Walke
       p.splits[blockIdx.x] = split;
     }
     q_inverse = next_inverse;
+    leveled = next_leveled;
     u = following;
     ++unit;
   }

@@ -52,9 +52,10 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
     query is rounded to FP16 (2^-11), so its scores carry 2^-11 A more. Against FP4 pages a query is four FP4
     terms, each the rounding of what is left: the E4M3 scale of a group is at most 2^-4 off amax / 6, and half
     the widest E2M1 step is one scale, so a term leaves at most 17/16 / 6 < 0.178 of the group's largest value (a
-    value clipped at six scales leaves less), four leave 0.178^4. Scaled so that the head's largest query value
-    lies in [2^10, 2^11), a term whose scale falls below E4M3's smallest (2^-9) leaves at most 6 x 2^-9, under
-    2^-16 of that value. An error d in a score is a relative error d of its probability, and sum p v / sum p
+    value clipped at six scales leaves less), four leave 0.178^4. Scaled so that the largest query value
+    of its tile lies in [2^10, 2^11), or its own where that is below 2^-5 of the tile's, a term whose scale falls to
+    E4M3's smallest (2^-9) or below leaves at most 3 x 2^-9, under 2^-16 of that value: of the head's largest, and of 32
+    times the query's own. An error d in a score is a relative error d of its probability, and sum p v / sum p
     moves by at most sum p_t (d_t + mean d) |v_t|."""
     nodes, hq, _ = query.shape
     h = draft_key.shape[1]
@@ -83,9 +84,10 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
             torch.ones(nodes, sink, dtype=torch.bool))
     add(dk, draft_value.double(), ancestors(parents))
     k, v, mask = torch.cat(keys), torch.cat(values), torch.cat(seen, 1)
-    tile = q.abs().reshape(nodes, h, -1).amax((0, 2))  # the largest query value of each KV head
     left = q.abs().reshape(nodes, hq, 8, 16).amax(3) * 0.178 ** 4
-    left = torch.maximum(left, 2.0 ** -16 * tile.repeat_interleave(g)[None, :, None])
+    own = q.abs().amax(2)  # each query's largest value; below, the largest of each KV head
+    tile = own.reshape(nodes, h, g).amax((0, 2)).repeat_interleave(g)
+    left = torch.maximum(left, 2.0 ** -16 * torch.minimum(tile[None], 32 * own)[:, :, None])
     out = torch.empty(nodes, hq, 128, dtype=torch.float64)
     allowed = torch.empty_like(out)
     for head in range(hq):

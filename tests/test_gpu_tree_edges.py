@@ -131,3 +131,17 @@ def test_scores_beyond_the_fraction_of_a_float(nodes, heads, factor):
     w, _ = _tree_inputs([700, 130, 20, 1300], 1, *heads, seed=74)
     x, want = _needles(w, nodes, heads[0], 75, 16.0 * factor)
     _check_needles(_tree_call(w, x), want)
+
+
+@pytest.mark.parametrize("nodes,heads", [(3, (4, 1)), (9, (6, 2)), (13, (8, 2)), (23, (8, 2)), (30, (8, 2))])
+@pytest.mark.parametrize("factor", [2.0 ** 10, 2.0 ** 20, 2.0 ** 60])
+@pytest.mark.parametrize("rotate", [False, True])
+def test_a_loud_query_leaves_the_others_alone(nodes, heads, factor, rotate):
+    """One node, and one head of another, far louder than the rest of their tile: what is lost of a query goes by its
+    own values (the allowance's terms are each query's own), not by the loudest."""
+    w, x = _tree_inputs([700, 130, 20], nodes, *heads, seed=73, loud=4.0, rotate=rotate)
+    loud = x["query"].double()
+    loud[:, 1] *= factor
+    loud[:, 2, -1] *= factor
+    loud = dict(x, query=loud.to(torch.bfloat16))
+    _tree_check(w, loud, _tree_call(w, loud, query_rotation="hadamard" if rotate else "none"), rotate=rotate)
