@@ -141,8 +141,9 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
   if (a->rows < 1 || a->nodes < 1 || a->heads_q < 1 || a->heads_kv < 1 || a->heads_q % a->heads_kv) return BDFP4_E_ARG;
   if (a->nodes > BDFP4_MAX_TREE_NODES || a->rows > 65535 || a->heads_kv > 65535) return BDFP4_E_UNSUPPORTED;
   if (!a->query || !a->draft_key || !a->draft_value || !a->parents || !a->out) return BDFP4_E_ARG;
-  if (!a->key_codes || !a->key_scales || !a->value_codes || !a->value_scales || a->pages < 1 || !a->page_table ||
-      !a->seqused_fp4 || a->max_pages_per_row < 0 || a->page_table_stride < a->max_pages_per_row)
+  if (!a->key_codes || !a->key_scales || !a->value_codes || !a->value_scales || a->pages < 1 ||
+      (!a->page_table && a->max_pages_per_row > 0) || !a->seqused_fp4 || a->max_pages_per_row < 0 ||
+      a->page_table_stride < a->max_pages_per_row)
     return BDFP4_E_ARG;
   auto misaligned = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) != 0; };
   for (const void* ptr : {a->query, a->draft_key, a->draft_value, a->key_codes, a->key_scales, a->value_codes,

@@ -603,7 +603,7 @@ typedef struct bdfp4_tree_args {
   const void* value_scales;
   int64_t key_codes_pitch, key_scales_pitch, value_codes_pitch, value_scales_pitch;
   int32_t pages, page_tokens; /* page_tokens 128 or 64 (0 means 128) */
-  const int32_t* page_table;
+  const int32_t* page_table; /* null when max_pages_per_row is 0: no row reads a page */
   int64_t page_table_stride;
   int32_t max_pages_per_row;
   int32_t rotate;

@@ -145,3 +145,13 @@ def test_a_loud_query_leaves_the_others_alone(nodes, heads, factor, rotate):
     loud[:, 2, -1] *= factor
     loud = dict(x, query=loud.to(torch.bfloat16))
     _tree_check(w, loud, _tree_call(w, loud, query_rotation="hadamard" if rotate else "none"), rotate=rotate)
+
+
+@pytest.mark.parametrize("page_tokens", [128, 64])
+@pytest.mark.parametrize("trusted", [False, True])
+def test_tree_with_a_table_of_no_columns(page_tokens, trusted):
+    """A batch whose rows have no page yet, the first steps of every sequence."""
+    w, x = _tree_inputs([1, 20, 128], 5, 8, 2, seed=76, page_tokens=page_tokens)
+    assert not bool(w.seqused_fp4.any())
+    w.page_table = w.page_table[:, :0]
+    _tree_check(w, x, _tree_call(w, x, trusted_metadata=trusted))

@@ -31,3 +31,15 @@ def test_commit_work_table_goes_with_a_page_table(change):
     for name, value in change.items():
         setattr(a, name, value)
     assert bdfp4.library().bdfp4_commit_drafts(ctypes.byref(a), None) == bdfp4.E_ARG
+
+
+def test_tree_takes_a_table_of_no_columns():
+    """No row reads a page: the check behind the table's is the one that refuses this call."""
+    import bdfp4
+    from test_tree_cpu import _tree_args
+
+    a = _tree_args()
+    a.page_table, a.page_table_stride, a.max_pages_per_row, a.page_tokens = 0, 1, 0, 32
+    assert bdfp4.library().bdfp4_tree_decode(ctypes.byref(a), None) == bdfp4.E_UNSUPPORTED
+    a.max_pages_per_row = 1
+    assert bdfp4.library().bdfp4_tree_decode(ctypes.byref(a), None) == bdfp4.E_ARG
