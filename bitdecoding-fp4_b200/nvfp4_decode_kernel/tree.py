@@ -57,15 +57,18 @@ def _int32(tensor, name: str, shape: tuple, device) -> int:
 
 
 def _tree_tensor(tensor, name: str, shape: tuple, device) -> tuple:
-    """BF16 ``[..., nodes, heads, 128]`` with free leading strides: its address, then those strides."""
+    """BF16 ``[..., nodes, heads, 128]`` with free leading strides: its address, then those strides (where a dimension
+    has one entry its stride means nothing: that of a dense node stands in)."""
     if (
         isinstance(tensor, torch.Tensor) and tensor.dtype is torch.bfloat16 and tensor.device == device
         and tensor.shape == shape
     ):
         address, (*outer, head, inner) = tensor.data_ptr(), tensor.stride()
         ok = inner == 1 and (head == HEAD_DIM or shape[-2] == 1) and address % 16 == 0
-        for stride, size in zip(outer, shape):
-            if stride % 8 and size > 1:
+        for i, size in enumerate(shape[:-2]):
+            if size == 1:
+                outer[i] = shape[-2] * HEAD_DIM
+            elif outer[i] % 8:
                 ok = False
         if ok:
             return address, *outer
@@ -122,10 +125,11 @@ def _check_regions(key_pages_fp4, key_scales, value_pages_fp4, value_scales, dev
             held = "packed FP4" if kinds is packed else "E4M3 scale bytes"
             raise ValueError(f"{name} must hold {held} with shape {shape}")
         strides, address = tensor.stride(), tensor.data_ptr()
-        if strides[1:] != inner or strides[0] % 16 or address % 16:
+        pitch = strides[0] if pages > 1 else tensor.numel()
+        if strides[1:] != inner or pitch % 16 or address % 16:
             raise ValueError(f"{name} must be in the quantizer's layout, dense within a page, with a 16-byte page pitch")
         addresses.append(address)
-        pitches.append(strides[0])
+        pitches.append(pitch)
     return pages, page, heads, addresses, pitches
 
 
@@ -223,7 +227,9 @@ def tree_decode(
         raise ValueError("fp4_page_table must be row-major INT32 with shape [rows, max_pages]")
     columns = fp4_page_table.shape[1]
     a.page_table = _int32(fp4_page_table, "fp4_page_table", (rows, columns), device)
-    a.page_table_stride, a.max_pages_per_row = fp4_page_table.stride(0), columns
+    a.page_table_stride, a.max_pages_per_row = fp4_page_table.stride(0) if rows > 1 else columns, columns
+    if a.page_table_stride < columns:
+        raise ValueError("fp4_page_table must be row-major INT32 with shape [rows, max_pages]")
     a.seqused_fp4 = _int32(seqused_fp4, "seqused_fp4", (rows,), device)
     if query_rotation not in ROTATIONS:
         raise ValueError(f"query_rotation must be one of {list(ROTATIONS)}, got {query_rotation!r}")
@@ -265,7 +271,7 @@ def tree_decode(
             ):
                 raise ValueError(f"{name} must be contiguous BF16 [slots, {least}, {heads_kv}, {HEAD_DIM}] on {device}")
         a.tail_key, a.tail_value = residual[0].data_ptr(), residual[1].data_ptr()
-        a.tail_slot_stride, a.tail_slots = residual[0].stride(0), slots
+        a.tail_slot_stride, a.tail_slots = tail_shape[1] * heads_kv * HEAD_DIM, slots
         a.tail_slot_ids = _int32(residual_page_ids, "residual_page_ids", (rows,), device)
         a.seqused_residual = _int32(seqused_residual, "seqused_residual", (rows,), device)
         if seqused_sink is not None:
@@ -482,7 +488,8 @@ class DraftCommitter:
             raise ValueError("block_table goes with a committer that was built with regions, and only with one")
         lengths = torch.empty(4, rows, dtype=torch.int32, device=device)
         a.tail_key, a.tail_value = self._tail_key.data_ptr(), self._tail_value.data_ptr()
-        a.tail_layer_stride, a.tail_slot_stride = self._tail_key.stride(0), self._tail_key.stride(1)
+        a.tail_slot_stride = (PAGE_SIZE + self.sink_tokens) * self.heads * HEAD_DIM
+        a.tail_layer_stride = self.slots * a.tail_slot_stride
         a.tail_slots, a.sink_tokens, a.rotate = self.slots, self.sink_tokens, int(self._rotate)
         a.key_shift = bdfp4.ptr(self._shift)
         address = lengths.data_ptr()

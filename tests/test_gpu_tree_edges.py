@@ -155,3 +155,36 @@ def test_tree_with_a_table_of_no_columns(page_tokens, trusted):
     assert not bool(w.seqused_fp4.any())
     w.page_table = w.page_table[:, :0]
     _tree_check(w, x, _tree_call(w, x, trusted_metadata=trusted))
+
+
+@pytest.mark.parametrize("rows,nodes", [(1, 1), (1, 4), (3, 1)])
+def test_single_entries_of_any_stride(rows, nodes):
+    """What broadcasting, slicing and transposing leave behind in dimensions of one entry."""
+    def odd(t):  # every single entry's stride a 3
+        return t.as_strided(t.shape, [3 if size == 1 and i < t.ndim - 1 else stride
+                                      for i, (size, stride) in enumerate(zip(t.shape, t.stride()))])
+
+    w, x = _tree_inputs([200, 20, 700][:rows], nodes, 4, 2, seed=77)
+    want = _tree_call(w, x)
+    device = {k: odd(v.cuda()) for k, v in x.items()}
+    w.page_table = odd(w.page_table)
+    w.tail_key, w.tail_value = w.tail_key.contiguous(), w.tail_value.contiguous()
+    got = _tree_call(w, device, residual_key_pages_bf16=odd(w.tail_key[0]), residual_value_pages_bf16=odd(w.tail_value[0]),
+                     out=odd(torch.zeros_like(want)))
+    assert torch.equal(got, want)
+    s = _setup(rows, 1, nodes, 2, [126, 5, 250][:rows], [1] * rows, seed=78)
+    tails, lengths = _commit(s, True)
+    s = dict(s, **{k: _Held(odd(s[k].cuda())) for k in ("key", "value", "accepted", "table")})
+    again, others = _commit(s, True)
+    assert all(torch.equal(a, b) for a, b in zip(tails, again))
+    assert all(torch.equal(a, b) for a, b in zip(lengths, others))
+
+
+class _Held:
+    """A stand-in whose ``.cuda()`` hands out the tensor as it is, strides and all."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def cuda(self):
+        return self.t

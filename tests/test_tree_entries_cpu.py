@@ -43,3 +43,21 @@ def test_tree_takes_a_table_of_no_columns():
     assert bdfp4.library().bdfp4_tree_decode(ctypes.byref(a), None) == bdfp4.E_UNSUPPORTED
     a.max_pages_per_row = 1
     assert bdfp4.library().bdfp4_tree_decode(ctypes.byref(a), None) == bdfp4.E_ARG
+
+
+def test_strides_of_single_entries_mean_nothing():
+    """A dimension of one entry may carry any stride; what reaches the kernels is that of a dense node."""
+    import torch
+    from nvfp4_decode_kernel.tree import _tree_tensor
+
+    flat = torch.zeros(5000, dtype=torch.bfloat16)
+    flat = flat[(-flat.data_ptr() % 16) // 2:]
+    cpu = torch.device("cpu")
+    for shape, strides, want in (
+        ((1, 3, 2, 128), (1, 264, 128, 1), (256, 264)), ((3, 1, 2, 128), (512, 3, 128, 1), (512, 256)),
+        ((1, 1, 1, 128), (7, 5, 3, 1), (128, 128)), ((2, 1, 2, 1, 128), (1024, 9, 136, 77, 1), (1024, 128, 136)),
+    ):
+        assert _tree_tensor(flat.as_strided(shape, strides), "x", shape, cpu)[1:] == want
+    for shape, strides in (((2, 3, 2, 128), (771, 256, 128, 1)), ((1, 3, 2, 128), (8, 257, 128, 1))):
+        with pytest.raises(ValueError):
+            _tree_tensor(flat.as_strided(shape, strides), "x", shape, cpu)
