@@ -1,6 +1,7 @@
 // C ABI of the tree attention: argument checks, the tile and its instantiation (tree_p128.cu, tree_p64.cu),
 // and the kernel that adds the parts of units that straddle CTAs. The attention itself is
 // tree_narrow.cuh and tree_wide.cuh.
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
@@ -166,7 +167,7 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
       a->key_scales_pitch < a->heads_kv * head_scales || a->value_scales_pitch < a->heads_kv * head_scales)
     return BDFP4_E_ARG;
   if (a->tail_key && (!a->tail_value || !a->tail_slot_ids || !a->seqused_residual || a->tail_slots < 1 ||
-                      a->tail_slot_stride < (int64_t)(kPage + (a->seqused_sink ? BDFP4_MAX_SINK : 0)) * a->heads_kv * kHeadDim))
+                      a->tail_slot_stride < (int64_t)kPage * a->heads_kv * kHeadDim))
     return BDFP4_E_ARG;
   if (!(a->softmax_scale > 0.0f) || !std::isfinite(a->softmax_scale)) return BDFP4_E_ARG;
   auto bad_scale = [](float s) { return s != 0.0f && !(s > 0.0f && std::isfinite(s)); };
@@ -213,6 +214,7 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
   p.slot_ids = a->tail_slot_ids;
   p.residual = a->seqused_residual;
   p.sink = a->tail_key ? a->seqused_sink : nullptr;
+  p.sink_rows = a->tail_key ? (int)std::min<int64_t>(a->tail_slot_stride / ((int64_t)a->heads_kv * kHeadDim) - kPage, BDFP4_MAX_SINK) : 0;
   p.key_shift = a->key_shift;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.key_scale = a->key_tensor_scale == 0.0f ? 1.0f : a->key_tensor_scale;

@@ -166,7 +166,7 @@ __device__ __forceinline__ RowInfo row_info(const TreeParams& p, int row, int pa
     r.slot = p.slot_ids[row];
     if (r.slot >= 0 && r.slot < p.tail_slots) {
       r.residual = min(max(p.residual[row], 0), kPage);
-      if (p.sink) r.sink = min(max(p.sink[row], 0), BDFP4_MAX_SINK);
+      if (p.sink) r.sink = min(max(p.sink[row], 0), p.sink_rows);
     } else {
       r.slot = 0;
     }

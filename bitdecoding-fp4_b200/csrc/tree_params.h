@@ -50,6 +50,7 @@ struct TreeParams {
   const int32_t* slot_ids;
   const int32_t* residual;
   const int32_t* sink;
+  int sink_rows;  // of a slot, 0 to 16
   const float* key_shift;
   float scale_log2;  // softmax scale in log2 units
   float key_scale;   // key tensor scale of the pages

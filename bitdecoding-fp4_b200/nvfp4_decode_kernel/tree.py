@@ -180,7 +180,8 @@ def tree_decode(
     its output is left as it was (zeros without ``out``).
 
     The cache regions, ``fp4_page_table``, ``seqused_fp4`` and the ``residual_*`` / ``seqused_*`` arguments are
-    those of :func:`nvfp4_decode_kernel.fp4_decode`; MXFP4 caches are not served. Unlike there, neither the
+    those of :func:`nvfp4_decode_kernel.fp4_decode`; MXFP4 caches are not served. A tail may have any number of sink
+    rows from 0 to 16 behind its 128 (``fp4_decode`` takes 16 with ``seqused_sink``, none without). Unlike there, neither the
     query nor the probabilities are rounded to one FP4 value: cache values enter the products exactly, queries as
     four FP4 terms (or FP16, against BF16 tokens) and probabilities as FP16 or BF16, so the result is that of
     attention over the dequantized cache to BF16 rounding. A draft value that is not finite may reach every node
@@ -262,14 +263,16 @@ def tree_decode(
     slots = 0
     if has_residual:
         tail_shape = residual[0].shape
-        slots, least = tail_shape[0], PAGE_SIZE + (SINK_TOKENS if seqused_sink is not None else 0)
+        slots = tail_shape[0]
         for tensor, name in ((residual[0], "residual_key_pages_bf16"), (residual[1], "residual_value_pages_bf16")):
             if (
                 tensor.dtype is not torch.bfloat16 or tensor.device != device or not tensor.is_contiguous()
-                or tensor.shape != tail_shape or len(tail_shape) != 4 or tail_shape[1] < least
+                or tensor.shape != tail_shape or len(tail_shape) != 4 or tail_shape[1] < PAGE_SIZE
                 or tail_shape[2:] != (heads_kv, HEAD_DIM)
             ):
-                raise ValueError(f"{name} must be contiguous BF16 [slots, {least}, {heads_kv}, {HEAD_DIM}] on {device}")
+                raise ValueError(f"{name} must be contiguous BF16 [slots, {PAGE_SIZE} + sink tokens, {heads_kv}, {HEAD_DIM}] "
+                                 f"on {device}")
+        sink_rows = min(tail_shape[1] - PAGE_SIZE, SINK_TOKENS)
         a.tail_key, a.tail_value = residual[0].data_ptr(), residual[1].data_ptr()
         a.tail_slot_stride, a.tail_slots = tail_shape[1] * heads_kv * HEAD_DIM, slots
         a.tail_slot_ids = _int32(residual_page_ids, "residual_page_ids", (rows,), device)
@@ -294,8 +297,8 @@ def tree_decode(
             _check_values((residual_page_ids < 0) | (residual_page_ids >= slots),
                           "residual_page_ids contains an out-of-range physical page ID")
             if seqused_sink is not None:
-                _check_values((seqused_sink < 0) | (seqused_sink > SINK_TOKENS),
-                              f"seqused_sink values must lie in [0, {SINK_TOKENS}]")
+                _check_values((seqused_sink < 0) | (seqused_sink > sink_rows),
+                              f"seqused_sink values must lie in [0, {sink_rows}]")
     if out is None:
         make = torch.empty if node_counts is None else torch.zeros
         out = make(shape, dtype=torch.bfloat16, device=device)
@@ -387,7 +390,7 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, parents: tor
 
 class CommittedLengths(NamedTuple):
     """Each row's lengths after a commit, INT32 ``[rows]`` on the device: what the next step's
-    :func:`tree_decode` (or ``fp4_decode``) takes."""
+    :func:`tree_decode` takes (or ``fp4_decode``, whose sink is the whole 16 rows or, without ``seqused_sink``, none)."""
 
     seq_lens: torch.Tensor
     seqused_fp4: torch.Tensor

@@ -615,7 +615,7 @@ typedef struct bdfp4_tree_args {
   float softmax_scale;
   const int32_t* tail_slot_ids;
   const int32_t* seqused_residual;
-  const int32_t* seqused_sink; /* or null */
+  const int32_t* seqused_sink; /* or null; the sink's rows are those of a slot behind its 128, at most 16 */
   const float* key_shift;   /* or null */
   float key_tensor_scale, value_tensor_scale; /* of the pages; 0 means 1 */
   void* out;                /* BF16 [rows][nodes][heads_q][128], dense within a node */

@@ -188,3 +188,41 @@ class _Held:
 
     def cuda(self):
         return self.t
+
+
+@pytest.mark.parametrize("sink", [0, 1, 4, 15])
+@pytest.mark.parametrize("nodes", [3, 20])
+def test_what_a_commit_with_a_short_sink_left(sink, nodes):
+    """The lengths and tails of a committer with any sink are what the next step's attention takes."""
+    from nvfp4_decode_kernel import tree
+    from oracle import tree_oracle as oracle
+
+    lens, counts = [0, 2, 100], [3, 3, 2]
+    s = _setup(3, 1, 6, 2, lens, counts, seed=79, sink=sink, seal=False, shift=False)
+    tails, lengths = _commit(s, False, sink=sink)
+    w, x = _tree_inputs([1, 1, 1], nodes, 8, 2, seed=80)
+    device = {k: v.cuda() for k, v in x.items()}
+    for trusted in (False, True):
+        out = tree.tree_decode(
+            device["query"], device["draft_key"], device["draft_value"], device["parents"], *w.regions, w.page_table,
+            lengths.seqused_fp4, residual_key_pages_bf16=tails[0][0], residual_value_pages_bf16=tails[1][0],
+            residual_page_ids=s["row_to_slot"].cuda(), seqused_residual=lengths.seqused_residual,
+            seqused_sink=lengths.seqused_sink, trusted_metadata=trusted).cpu().double()
+        for r in range(3):
+            n, slot = lens[r] + counts[r], int(s["row_to_slot"][r])
+            want, allowed = oracle.tree_attention(
+                query=x["query"][r], draft_key=x["draft_key"][r], draft_value=x["draft_value"][r],
+                parents=x["parents"][r].tolist(), key=None, value=None, page_ids=None, fp4=0,
+                tail_key=tails[0][0, slot].cpu(), tail_value=tails[1][0, slot].cpu(), residual=n, sink=min(n, sink),
+                softmax_scale=128 ** -0.5)
+            assert bool(((out[r] - want).abs() <= allowed).all()), f"row {r}"
+    # a sink length beyond the rows there are is refused, and never followed
+    args = (device["query"], device["draft_key"], device["draft_value"], device["parents"], *w.regions, w.page_table,
+            lengths.seqused_fp4)
+    more = dict(residual_key_pages_bf16=tails[0][0], residual_value_pages_bf16=tails[1][0],
+                residual_page_ids=s["row_to_slot"].cuda(), seqused_residual=lengths.seqused_residual)
+    with pytest.raises(ValueError):
+        tree.tree_decode(*args, **more, seqused_sink=lengths.seqused_sink + sink + 1)
+    over = tree.tree_decode(*args, **more, seqused_sink=torch.full_like(lengths.seqused_sink, 16), trusted_metadata=True)
+    full = tree.tree_decode(*args, **more, seqused_sink=torch.full_like(lengths.seqused_sink, sink), trusted_metadata=True)
+    assert torch.equal(over, full)
