@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libbdfp4.so"
 
 OK, E_ARG, E_UNSUPPORTED, E_CUDA, E_DEVICE, E_TOO_LARGE = 0, -1, -2, -3, -4, -5
 STATIC_SCRATCH_BYTES = 8 << 20
-DEV_WAIT_TIMEOUT, DEV_BAD_PAGE = 1, 2
+DEV_WAIT_TIMEOUT, DEV_BAD_PAGE, DEV_BAD_NODE = 1, 2, 4
 SCALE_MODE_IDS = {"amax6": 0, "four_six": 1, "four_six_sixhalf": 2,
                   "mxfp4_ocp": 3, "mxfp4_round_up": 4, "mxfp4_search": 5}
 FORMAT_NVFP4, FORMAT_MXFP4 = 0, 1

@@ -78,9 +78,21 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitPara
   const int slot = p.row_to_slot[row];
   const int n = p.seq_lens[row];
   const bool live = slot >= 0 && slot < p.slots && n >= 0;
-  const int count = min(max(p.counts[row], 0), p.nodes);
-  if (blockIdx.x == 0 && layer == 0 && threadIdx.x == 0 && p.part != BDFP4_COMMIT_REST)
+  // The path ends at the first entry that is not a node's number: the tokens behind it have nothing to be written
+  // from, and a length that counted them would make old rows of the tail part of the sequence. (Every warp looks for it.)
+  const int claimed = min(max(p.counts[row], 0), p.nodes);
+  int count = claimed;
+#pragma unroll
+  for (int half = 1; half >= 0; --half) {
+    const int i = 32 * half + (threadIdx.x & 31);
+    const int node = i < p.nodes ? p.accepted[(int64_t)row * p.accepted_stride + i] : 0;
+    const unsigned bad = __ballot_sync(0xffffffffu, i < claimed && (node < 0 || node >= p.nodes));
+    if (bad) count = 32 * half + __ffs(bad) - 1;
+  }
+  if (blockIdx.x == 0 && layer == 0 && threadIdx.x == 0 && p.part != BDFP4_COMMIT_REST) {
     commit_lengths(p, row, n, count, live, slot);
+    if (live && count < claimed && p.error_word) atomicOr(p.error_word, (int)BDFP4_DEV_BAD_NODE);
+  }
   if (!live) return;
   const int boundary = (n + count) / kPage * kPage;
   const bool fills = boundary > n / kPage * kPage;
@@ -108,15 +120,13 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitPara
       const bool is_key = within < groups;
       const int channel = (is_key ? within : within - groups) * kGroup;  // head and channel in one
       const int node = p.accepted[(int64_t)row * p.accepted_stride + token];
-      if (node >= 0 && node < p.nodes) {
-        const __nv_bfloat16* src = is_key ? p.key + layer * p.key_layer + row * p.key_row + node * p.key_node
-                                          : p.value + layer * p.value_layer + row * p.value_row + node * p.value_node;
-        raw[k][0] = __ldg(reinterpret_cast<const uint4*>(src + channel));
-        raw[k][1] = __ldg(reinterpret_cast<const uint4*>(src + channel) + 1);
-        const int position = n + token;
-        to[k] = (int64_t)slot * p.tail_slot + (position % kPage) * row_elems + channel;
-        to_sink[k] = position < p.sink ? kPage + position - position % kPage : 0;  // rows between the two places
-      }
+      const __nv_bfloat16* src = is_key ? p.key + layer * p.key_layer + row * p.key_row + node * p.key_node
+                                        : p.value + layer * p.value_layer + row * p.value_row + node * p.value_node;
+      raw[k][0] = __ldg(reinterpret_cast<const uint4*>(src + channel));
+      raw[k][1] = __ldg(reinterpret_cast<const uint4*>(src + channel) + 1);
+      const int position = n + token;
+      to[k] = (int64_t)slot * p.tail_slot + (position % kPage) * row_elems + channel;
+      to_sink[k] = position < p.sink ? kPage + position - position % kPage : 0;  // rows between the two places
     }
   }
 #pragma unroll

@@ -458,7 +458,8 @@ class DraftCommitter:
                  accepted_counts: torch.Tensor, *, seq_lens: torch.Tensor, row_to_slot: torch.Tensor,
                  block_table: torch.Tensor | None = None) -> CommittedLengths:
         """Append each row's accepted nodes (``accepted`` INT32 ``[rows, nodes]``, the first ``accepted_counts[r]``
-        entries) to its sequence of ``seq_lens[r]`` tokens.
+        entries) to its sequence of ``seq_lens[r]`` tokens. A path ends before an entry that is not a node's number, and
+        sets ``bdfp4.DEV_BAD_NODE`` in the error word.
 
         ``draft_key`` / ``draft_value`` are BF16 ``[layers, rows, nodes, heads, 128]`` as the model made them (the
         same tensors :func:`tree_decode` read, all layers). Token ``p`` goes to row ``p % 128`` of slot

@@ -38,6 +38,7 @@ extern "C" {
 /* bits a kernel may OR into *error_word */
 #define BDFP4_DEV_WAIT_TIMEOUT 1u /* a bounded mbarrier wait gave up */
 #define BDFP4_DEV_BAD_PAGE 2u     /* a page id outside [0, pages) was clamped */
+#define BDFP4_DEV_BAD_NODE 4u     /* an accepted path was cut at an entry outside [0, nodes) */
 
 /* NVFP4 scale-candidate sets (src/nvfp4_decode_kernel/scale_mode.py:18-22) */
 #define BDFP4_SCALE_AMAX6 0            /* (6) */
@@ -670,7 +671,8 @@ int bdfp4_verify_drafts(const bdfp4_verify_args* args, void* stream);
  * where it fills none), BDFP4_COMMIT_REST the others: between the two a caller seals the filled pages out of
  * the tail with the work table (source_tokens, destination_pages: [rows * 128 / page_tokens], -1 where the row
  * fills no page). ALL and HEAD also write the new lengths. A row with a negative slot is left alone (its
- * lengths are those of seq_lens). A filled page without a valid destination sets BDFP4_DEV_BAD_PAGE.
+ * lengths are those of seq_lens). A path ends at its first entry that is not a node's number, which
+ * sets BDFP4_DEV_BAD_NODE. A filled page without a valid destination sets BDFP4_DEV_BAD_PAGE.
  */
 #define BDFP4_COMMIT_ALL 0
 #define BDFP4_COMMIT_HEAD 1

@@ -226,3 +226,24 @@ def test_what_a_commit_with_a_short_sink_left(sink, nodes):
     over = tree.tree_decode(*args, **more, seqused_sink=torch.full_like(lengths.seqused_sink, 16), trusted_metadata=True)
     full = tree.tree_decode(*args, **more, seqused_sink=torch.full_like(lengths.seqused_sink, sink), trusted_metadata=True)
     assert torch.equal(over, full)
+
+
+def test_a_commit_ends_at_a_number_that_is_no_node():
+    """The row grows by what was written; nothing of the entries behind is, valid ones included, and it is reported."""
+    import bdfp4
+
+    s = _setup(4, 2, 40, 2, [10, 126, 126, 300], [5, 6, 38, 40], seed=81)
+    s["accepted"][1, 1] = 40
+    s["accepted"][2, 35] = -4
+    s["accepted"][3, 0] = 1 << 30
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    before = [b.clone() for b in s["blocks"]]
+    tails, lengths = _commit(s, True, error=error)
+    assert int(error) == bdfp4.DEV_BAD_NODE
+    cut = dict(s, counts=torch.tensor([5, 1, 35, 0], dtype=torch.int32))
+    want_tails, sealed, want_lengths = _expect(cut, True)
+    for got, want in zip(tails, want_tails):
+        assert torch.equal(got.cpu().view(torch.int16), want.view(torch.int16))
+    assert torch.stack([t.cpu() for t in lengths], 1).tolist() == [list(x) for x in want_lengths]
+    for block, old in zip(s["blocks"], before):
+        assert (block != old).any(1).nonzero()[:, 0].tolist() == sorted(int(s["table"][r, c]) for r, c, _ in sealed)
