@@ -126,8 +126,9 @@ def check_supported(vllm_config) -> None:
          lambda: f"long_prefill_token_threshold={scheduler.long_prefill_token_threshold} splits long prompts "
                  "even with chunked prefill disabled. Leave it at 0."),
         (vllm_config.speculative_config is not None,
-         lambda: "speculative decoding is not supported by the NVFP4 KV cache: it verifies several draft tokens "
-                 "per step, and the decode kernel attends one query token per sequence."),
+         lambda: "speculative decoding is not supported by the NVFP4 plugin: its attention step takes one query token "
+                 "per sequence. Leave speculative_config unset; nvfp4_decode_kernel.tree has the operators (attention of "
+                 "drafted trees, verification, commit) for a loop of one's own over this cache."),
         (bool(getattr(cache, "kv_cache_dtype_skip_layers", None)),
          lambda: f"kv_cache_dtype_skip_layers={cache.kv_cache_dtype_skip_layers} leaves some layers on a "
                  "different cache dtype, which splits the model into KV cache groups with their own metadata "

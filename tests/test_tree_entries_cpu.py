@@ -61,3 +61,11 @@ def test_strides_of_single_entries_mean_nothing():
     for shape, strides in (((2, 3, 2, 128), (771, 256, 128, 1)), ((1, 3, 2, 128), (8, 257, 128, 1))):
         with pytest.raises(ValueError):
             _tree_tensor(flat.as_strided(shape, strides), "x", shape, cpu)
+
+
+def test_the_plugin_says_where_speculative_decoding_is():
+    from nvfp4_vllm import guards
+    from test_vllm_plugin import _config
+
+    with pytest.raises(guards.UnsupportedConfigError, match="nvfp4_decode_kernel.tree"):
+        guards.check_supported(_config(speculative_config=object()))
