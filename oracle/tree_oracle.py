@@ -40,7 +40,7 @@ def cache_values(blocks: torch.Tensor, heads: int, page_tokens: int):
 
 
 def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_ids, fp4, tail_key, tail_value,
-                   residual, sink, softmax_scale, rotate=False, shift=None):
+                   residual, sink, softmax_scale, rotate=False, shift=None, typical=False):
     """One row: ``query [nodes, Hq, 128]``, drafts ``[nodes, H, 128]`` (BF16), ``key`` / ``value`` the FP64 cache pages
     (tensor scales multiplied in), ``page_ids`` the row's pages, ``tail_* [>= 128, H, 128]`` BF16 (sink behind row
     128). Returns the FP64 result ``[nodes, Hq, 128]`` and how far a kernel may be from it.
@@ -56,7 +56,11 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
     of its tile lies in [2^10, 2^11), or its own where that is below 2^-5 of the tile's, a term whose scale falls to
     E4M3's smallest (2^-9) or below leaves at most 3 x 2^-9, under 2^-16 of that value: of the head's largest, and of 32
     times the query's own. An error d in a score is a relative error d of its probability, and sum p v / sum p
-    moves by at most sum p_t (d_t + mean d) |v_t|."""
+    moves by at most sum p_t (d_t + mean d) |v_t|.
+
+    That adds every token's error to every other's, so over thousands of tokens it exceeds the result. With ``typical``
+    the second return is instead the root mean square error per (node, head) that independent roundings come to: the
+    same bounds, a token's 128 products and the tokens added in squares, page probabilities by FP16's 2^-11."""
     nodes, hq, _ = query.shape
     h = draft_key.shape[1]
     g = hq // h
@@ -90,6 +94,7 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
     left = torch.maximum(left, 2.0 ** -16 * torch.minimum(tile[None], 32 * own)[:, :, None])
     out = torch.empty(nodes, hq, 128, dtype=torch.float64)
     allowed = torch.empty_like(out)
+    rms = torch.empty(nodes, hq, dtype=torch.float64)
     for head in range(hq):
         kh, vh = k[:, head // g], v[:, head // g]
         s = (q[:, head] @ kh.T * softmax_scale).masked_fill(~mask, -math.inf)
@@ -101,7 +106,15 @@ def tree_attention(*, query, draft_key, draft_value, parents, key, value, page_i
         out[:, head] = p @ vh
         weight = p * (d + (p * d).sum(1, keepdim=True) + 2.0 ** -8)
         allowed[:, head] = 1.05 * (weight @ vh.abs() + 2.0 ** -8 * out[:, head].abs()) + 1e-7
-    return out, allowed
+        if typical:
+            e = (terms * 2.0 ** -16) ** 2
+            if rotate:
+                e += (2.0 ** -11 * softmax_scale) ** 2 * (q[:, head] ** 2 @ kh.T ** 2)
+            e[:, :fp4] += softmax_scale ** 2 * (left[:, head] ** 2 @ (kh[:fp4] ** 2).reshape(fp4, 8, 16).sum(2).T)
+            e += torch.where(torch.arange(len(kh)) < fp4, 2.0 ** -22, 2.0 ** -16)
+            variance = (p ** 2 * e) @ vh ** 2 + (2.0 ** -8 * out[:, head]) ** 2
+            rms[:, head] = variance.mean(1).sqrt()
+    return out, rms if typical else allowed
 
 
 def base_rotate(x):
@@ -165,3 +178,12 @@ def verify(target, tokens, parents, uniforms, draft=None, count=None):
 def commit_positions(n, count):
     """(token number, tail row) of each accepted token of a row of ``n`` committed ones, and whether a page fills."""
     return [(n + i, (n + i) % PAGE) for i in range(count)], (n + count) // PAGE > n // PAGE
+
+
+def outside_typical(got, want, typical):
+    """How many (node, head) results of a row lie further from the FP64 one than three times what independent
+    roundings come to. (Over a head's 128 channels and many tokens the root mean square is within a few percent of its
+    expectation, and the roundings' bounds are taken for their spread, 1.7 times it for evenly spread errors: a right
+    result stays below one.)"""
+    off = ((got - want) ** 2).mean(-1).sqrt()
+    return int((off > 3 * typical).sum())
