@@ -8,9 +8,10 @@
 // S^T over a page is the block-scaled FP4 product of the codes as they lie in the cache (kind::mxf4nvf4, no
 // conversion) with the query written as a sum of four FP4 terms, each the rounding of what the ones before left: a
 // term leaves at most 0.178 of its group's largest value (half the widest E2M1 step of amax / 6, with the E4M3
-// scale's rounding), four leave 10^-3, a quarter of the BF16 rounding the query came with. Four terms of K = 64 take
-// the tensor time of FP16's K = 16. (Converting K to FP16 instead cost a third of the conversions and a chain of
-// waits: 350 us where the terms take 331, 120 against 99 for tiles of 64.)
+// scale's rounding), four leave 10^-3 of it: a quarter of what BF16 rounding may cost the group's largest value, four
+// times what it may cost one a sixteenth as large. Four terms of K = 64 take the tensor time of FP16's K = 16.
+// (Converting K to FP16 instead cost a third of the conversions and a chain of waits: 350 us where the terms take 331,
+// 120 against 99 for tiles of 64.)
 //
 // O^T over a page is a kind::f16 product with V^T in tensor memory: E2M1 x E4M3 has at most six significant bits and
 // lies in [2^-10, 2688], so a page's values are exact in FP16. A thread reads its own channel's code bytes, converts
@@ -21,12 +22,16 @@
 // Softmax maxima are per query, in shared memory, and lazy: probabilities are formed against them at once, and only
 // when a score exceeds its query's by more than 8 (log2; the step's barrier carries that vote) are the maxima taken
 // anew and O^T rescaled. (Where scores are so large that what rounding does to a maximum counts, above 2^24, the two
-// kernels see to it in their own ways that the largest still gets its weight and no more.) Sums are FP32, per thread until the unit ends. Probabilities carry a factor 2^7, so in FP16
-// they stay below 2^15 and lose nothing above 2^-31 of the largest.
+// kernels see to it in their own ways that the largest still gets its weight and no more.) Sums are FP32, per thread
+// until the unit ends, of the probabilities as they are before their rounding. Probabilities carry a factor 2^7, so in
+// FP16 they stay below 2^15 and lose nothing above 2^-31 of the largest.
 //
 // The rolling tail and the drafts with the sink are two more steps over BF16 values, both products kind::f16 with the
 // cache side in tensor memory: K is scaled per token by a power of two into FP16's range (the softmax thread of the
-// token undoes it), V and P are BF16.
+// token undoes it), V and P are BF16. P has to have V's type, and V has no scale that would bring it into FP16's
+// range: one per channel cannot be undone in a sum that runs on over the pages, one per step would cost a channel that
+// is quiet beside another its values. So the probabilities of these up to 208 tokens are rounded to 2^-8, the pages' to
+// 2^-11; for short rows that is as much as the output's own rounding.
 //
 // Work is the sequence of all steps of all (row, head, tile) units, cut into runs, one per CTA, so any mix of lengths
 // is balanced; a unit that straddles CTAs leaves unnormalised parts that a second kernel adds.

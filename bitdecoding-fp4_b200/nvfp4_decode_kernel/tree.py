@@ -181,20 +181,20 @@ def tree_decode(
 
     The cache regions, ``fp4_page_table``, ``seqused_fp4`` and the ``residual_*`` / ``seqused_*`` arguments are
     those of :func:`nvfp4_decode_kernel.fp4_decode`; MXFP4 caches are not served. A tail may have any number of sink
-    rows from 0 to 16 behind its 128 (``fp4_decode`` takes 16 with ``seqused_sink``, none without). Unlike there, neither the
-    query nor the probabilities are rounded to one FP4 value: cache values enter the products exactly, queries as
-    four FP4 terms (or FP16, against BF16 tokens) and probabilities as FP16 or BF16, so the result is that of
-    attention over the dequantized cache to BF16 rounding. A draft value that is not finite may reach every node
-    of its row: its weight elsewhere is zero, not absent.
+    rows from 0 to 16 behind its 128 (``fp4_decode`` takes 16 with ``seqused_sink``, none without). Unlike there,
+    neither the query nor the probabilities are rounded to one FP4 value: cache values enter the products exactly,
+    queries as four FP4 terms (up to 1.0e-3 of the largest of 16 channels is lost; FP16 against BF16 tokens) and
+    probabilities as FP16 (BF16 against BF16 tokens). A draft value that is not finite may reach every node of its
+    row: its weight elsewhere is zero, not absent.
 
     Keys in the cache are rotated and shifted; ``query_rotation="hadamard"`` rotates the queries and the draft
     keys alike, and ``key_shift`` (FP32 ``[heads_kv, 128]``, already rotated) is subtracted from the draft keys,
     which are then rounded to BF16, as the tail writer does. ``tensor_scales`` is ``(key, value)`` of the pages.
 
     ``workspace`` (uint8, at least :func:`tree_workspace_bytes`, 16-byte aligned) makes the call allocation-free
-    together with ``out`` (BF16 ``[rows, nodes, heads_q, 128]``, dense within a node); calls that may overlap on
-    the GPU, captured ones included, need a workspace each. ``error_word`` (INT32 ``[1]``) collects
-    ``bdfp4.DEV_*`` bits. ``trusted_metadata`` skips the checks that read device values.
+    together with ``out`` (BF16 ``[rows, nodes, heads_q, 128]``, dense within a node, apart from the inputs); calls
+    that may overlap on the GPU, captured ones included, need a workspace each. ``error_word`` (INT32 ``[1]``)
+    collects ``bdfp4.DEV_*`` bits. ``trusted_metadata`` skips the checks that read device values.
     """
     device = _cuda_device(query, "query")
     if query.ndim != 4 or query.shape[3] != HEAD_DIM:
@@ -463,7 +463,8 @@ class DraftCommitter:
 
         ``draft_key`` / ``draft_value`` are BF16 ``[layers, rows, nodes, heads, 128]`` as the model made them (the
         same tensors :func:`tree_decode` read, all layers). Token ``p`` goes to row ``p % 128`` of slot
-        ``row_to_slot[r]`` and, below ``sink_tokens``, to the sink; a negative slot leaves its row alone.
+        ``row_to_slot[r]`` and, below ``sink_tokens``, to the sink; a negative slot (or one the tail does not have)
+        leaves its row alone, and no two rows may name one slot.
         ``block_table`` INT32 ``[rows, columns]`` names the pages that filled tails are sealed into and is required
         when the committer was built with ``regions``; a page without a valid entry there (or behind the last
         column) is not sealed and sets ``bdfp4.DEV_BAD_PAGE`` in the error word. Returns the new lengths;

@@ -580,13 +580,16 @@ int bdfp4_mla_combine(const float* partial_out, const float* partial_lse, int32_
  * Attention of `nodes` drafted tokens per row. Node i sees the row's cache (FP4 pages, BF16 rolling tail,
  * BF16 sink, as bdfp4_decode sees them) and, among the drafts, itself and its ancestors: parents[i] < i is
  * the parent's number, anything else makes node i a root. The result is that of attention over the
- * dequantized cache to BF16 rounding: K and V enter the MMAs exactly (FP4 codes with their scales, V as the
- * FP16 values they stand for; tail, sink and drafts keep BF16 values), queries as a sum of four FP4 terms
- * (pages; less than BF16's own rounding is lost) or as FP16, probabilities as FP16 (pages) or BF16. A draft
- * value that is not finite may reach every node of its row (its weight elsewhere is zero, not absent). `rotate` applies the Hadamard rotation to the queries and to the
- * draft keys, and `key_shift` (FP32 [heads_kv][128], in the rotated basis) is subtracted from the draft
- * keys, which are then rounded to BF16: what the cache would hold of them. Rows of node_counts[r] nodes
- * (0..nodes) leave the output of the nodes behind them as it was. A node that sees nothing gets zeros.
+ * dequantized cache, with these roundings. K and V enter the MMAs exactly (FP4 codes with their scales, V as
+ * the FP16 values they stand for; tail, sink and drafts keep BF16 values). Against pages a query is a sum of four
+ * FP4 terms, which lose up to 1.0e-3 of the largest magnitude of a value's group of 16 channels, or, if that is
+ * more, 2^-16 of the largest of up to 128 query rows that share a tile (of 32 times the query's own largest where
+ * that is less); against BF16 tokens it is FP16. Probabilities are FP16 (pages) or BF16, sums FP32, the output
+ * BF16. A draft value that is not finite may reach every node of its row (its weight elsewhere is zero, not absent).
+ * `rotate` applies the Hadamard rotation to the queries and to the draft keys, and `key_shift` (FP32
+ * [heads_kv][128], in the rotated basis) is subtracted from the draft keys, which are then rounded to BF16: what
+ * the cache would hold of them. Rows of node_counts[r] nodes (0..nodes) leave the output of the nodes behind them
+ * as it was. The output must not overlap any input.
  */
 typedef struct bdfp4_tree_args {
   int32_t rows, nodes, heads_q, heads_kv;
