@@ -24,6 +24,8 @@ static int tree_tile(int queries) {
   return kTreeMaxTile;
 }
 
+constexpr int kMaxHeads = 65535;  // what a row's query rows are counted in 32 bits for
+
 static int tree_ctas(int tile) { return tile <= kTreeNarrowTile ? kTreeNarrowCtas : kTreeWideCtas; }
 
 // One block per (CTA that a straddling unit begins in, eight query rows). First the parts' weights 2^(their
@@ -132,7 +134,9 @@ static cudaError_t launch_merge(const TreeParams& p, cudaStream_t stream) {
 using namespace bdfp4;
 
 extern "C" int64_t bdfp4_tree_workspace_bytes(int32_t rows, int32_t nodes, int32_t heads_q, int32_t heads_kv) {
-  if (rows < 1 || nodes < 1 || nodes > BDFP4_MAX_TREE_NODES || heads_kv < 1 || heads_q < 1 || heads_q % heads_kv) return 0;
+  if (rows < 1 || nodes < 1 || nodes > BDFP4_MAX_TREE_NODES || heads_kv < 1 || heads_q < 1 || heads_q % heads_kv ||
+      heads_q > kMaxHeads)
+    return 0;
   const int64_t tile = tree_tile(nodes * (heads_q / heads_kv));
   return (int64_t)tree_ctas((int)tile) * (2 * tile * (kHeadDim + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(TreeSplit));
 }
@@ -140,7 +144,7 @@ extern "C" int64_t bdfp4_tree_workspace_bytes(int32_t rows, int32_t nodes, int32
 extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) {
   if (!a) return BDFP4_E_ARG;
   if (a->rows < 1 || a->nodes < 1 || a->heads_q < 1 || a->heads_kv < 1 || a->heads_q % a->heads_kv) return BDFP4_E_ARG;
-  if (a->nodes > BDFP4_MAX_TREE_NODES || a->rows > 65535 || a->heads_kv > 65535) return BDFP4_E_UNSUPPORTED;
+  if (a->nodes > BDFP4_MAX_TREE_NODES || a->rows > 65535 || a->heads_q > kMaxHeads) return BDFP4_E_UNSUPPORTED;
   if (!a->query || !a->draft_key || !a->draft_value || !a->parents || !a->out) return BDFP4_E_ARG;
   if (!a->key_codes || !a->key_scales || !a->value_codes || !a->value_scales || a->pages < 1 ||
       (!a->page_table && a->max_pages_per_row > 0) || !a->seqused_fp4 || a->max_pages_per_row < 0 ||
@@ -160,7 +164,7 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
   // the kernel counts one row's and one CTA's steps (128 tokens of one head and tile of queries) in 32 bits
   const int64_t tiles = ((int64_t)a->nodes * (a->heads_q / a->heads_kv) + 15) / 16;
   const int64_t row_steps = ((int64_t)a->max_pages_per_row * page_tokens / kPage + 2) * tiles * a->heads_kv;
-  if (row_steps > INT32_MAX || row_steps * a->rows / kTreeWideCtas >= INT32_MAX) return BDFP4_E_UNSUPPORTED;
+  if (row_steps > INT32_MAX || row_steps * a->rows / kTreeWideCtas >= INT32_MAX - 64) return BDFP4_E_UNSUPPORTED;
   const int64_t head_codes = (int64_t)page_tokens * 64, head_scales = (int64_t)page_tokens * 8;
   if (a->key_codes_pitch % 16 || a->key_scales_pitch % 16 || a->value_codes_pitch % 16 || a->value_scales_pitch % 16 ||
       a->key_codes_pitch < a->heads_kv * head_codes || a->value_codes_pitch < a->heads_kv * head_codes ||

@@ -69,3 +69,17 @@ def test_the_plugin_says_where_speculative_decoding_is():
 
     with pytest.raises(guards.UnsupportedConfigError, match="nvfp4_decode_kernel.tree"):
         guards.check_supported(_config(speculative_config=object()))
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Query rows are counted in 32 bits: 64 nodes x 2^27 heads are none, or a tile of the wrong width."""
+    import bdfp4
+    from test_tree_cpu import _tree_args
+
+    lib = bdfp4.library()
+    for heads in (1 << 16, 1 << 26, 1 << 27, (1 << 31) - 1):
+        assert lib.bdfp4_tree_workspace_bytes(1, 64, heads, 1) == 0
+        a = _tree_args()
+        a.heads_q, a.heads_kv, a.nodes, a.page_tokens = heads, 1, 64, 32
+        assert lib.bdfp4_tree_decode(ctypes.byref(a), None) == bdfp4.E_UNSUPPORTED
+    assert lib.bdfp4_tree_workspace_bytes(1, 64, 65535, 1) > 0
