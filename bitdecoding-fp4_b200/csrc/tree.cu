@@ -3,6 +3,7 @@
 // tree_narrow.cuh and tree_wide.cuh.
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "common.cuh"
 #include "decode_params.h"
@@ -141,6 +142,13 @@ extern "C" int64_t bdfp4_tree_workspace_bytes(int32_t rows, int32_t nodes, int32
   return (int64_t)tree_ctas((int)tile) * (2 * tile * (kHeadDim + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(TreeSplit));
 }
 
+// Whether the blocks of `size` elements of a two-dimensional grid share none, one dimension wholly inside the other.
+static bool apart(int64_t n0, int64_t stride0, int64_t n1, int64_t stride1, int64_t size) {
+  if (n0 == 1 || n1 == 1) return n0 * n1 == 1 || (n0 == 1 ? stride1 : stride0) >= size;
+  if (stride0 < stride1) std::swap(n0, n1), std::swap(stride0, stride1);
+  return stride1 >= size && stride0 >= (n1 - 1) * stride1 + size;
+}
+
 extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) {
   if (!a) return BDFP4_E_ARG;
   if (a->rows < 1 || a->nodes < 1 || a->heads_q < 1 || a->heads_kv < 1 || a->heads_q % a->heads_kv) return BDFP4_E_ARG;
@@ -158,7 +166,9 @@ extern "C" int bdfp4_tree_decode(const bdfp4_tree_args* a, void* stream_handle) 
                          a->draft_value_row_stride, a->draft_value_node_stride, a->tail_slot_stride, a->out_row_stride,
                          a->out_node_stride})
     if (stride % 8 || stride < 0) return BDFP4_E_ARG;
-  if (a->out_node_stride < (int64_t)a->heads_q * kHeadDim || a->parents_row_stride < 0) return BDFP4_E_ARG;
+  if (a->parents_row_stride < 0 ||
+      !apart(a->rows, a->out_row_stride, a->nodes, a->out_node_stride, (int64_t)a->heads_q * kHeadDim))
+    return BDFP4_E_ARG;
   const int page_tokens = a->page_tokens == 0 ? kPage : a->page_tokens;
   if (page_tokens != 128 && page_tokens != 64) return BDFP4_E_UNSUPPORTED;
   // the kernel counts one row's and one CTA's steps (128 tokens of one head and tile of queries) in 32 bits

@@ -303,6 +303,11 @@ def tree_decode(
         make = torch.empty if node_counts is None else torch.zeros
         out = make(shape, dtype=torch.bfloat16, device=device)
     a.out, a.out_row_stride, a.out_node_stride = _tree_tensor(out, "out", shape, device)
+    extent = heads_q * HEAD_DIM
+    for stride, size in sorted(((a.out_row_stride, rows), (a.out_node_stride, nodes))):
+        if size > 1 and stride < extent:
+            raise ValueError("out must have an element of its own for every result")
+        extent += stride * (size - 1)
     need = tree_workspace_bytes(rows, nodes, heads_q, heads_kv)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)

@@ -247,3 +247,18 @@ def test_a_commit_ends_at_a_number_that_is_no_node():
     assert torch.stack([t.cpu() for t in lengths], 1).tolist() == [list(x) for x in want_lengths]
     for block, old in zip(s["blocks"], before):
         assert (block != old).any(1).nonzero()[:, 0].tolist() == sorted(int(s["table"][r, c]) for r, c, _ in sealed)
+
+
+def test_outputs_that_share_memory_are_refused():
+    w, x = _tree_inputs([20, 300], 3, 4, 2, seed=82)
+    want = _tree_call(w, x)
+    for out in (torch.zeros(1, 3, 4, 128).expand(2, 3, 4, 128), torch.zeros(2, 1, 4, 128).expand(2, 3, 4, 128),
+                torch.zeros(4096).as_strided((2, 3, 4, 128), (1024, 512, 128, 1))):
+        with pytest.raises(ValueError):
+            _tree_call(w, x, out=out.to(torch.bfloat16).cuda() if out.is_contiguous() else _like(out))
+    by_node = torch.zeros(3, 2, 4, 128, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    assert torch.equal(_tree_call(w, x, out=by_node), want)
+
+
+def _like(t):
+    return torch.zeros(4096, dtype=torch.bfloat16, device="cuda").as_strided(t.shape, t.stride())

@@ -83,3 +83,19 @@ def test_sizes_past_32_bits_are_refused():
         a.heads_q, a.heads_kv, a.nodes, a.page_tokens = heads, 1, 64, 32
         assert lib.bdfp4_tree_decode(ctypes.byref(a), None) == bdfp4.E_UNSUPPORTED
     assert lib.bdfp4_tree_workspace_bytes(1, 64, 65535, 1) > 0
+
+
+@pytest.mark.parametrize("rows,nodes,row,node,fine", [
+    (2, 5, 5120, 1024, True), (2, 5, 1024, 2048, True), (2, 5, 0, 1024, False), (2, 5, 1024, 1024, False), (2, 5, 5120, 0, False),
+    (2, 5, 4096, 1024, False), (1, 5, 8, 1024, True), (2, 1, 1024, 8, True), (2, 1, 1016, 8, False), (1, 1, 0, 0, True),
+    (1, 5, 8, 1016, False), (3, 5, 1024, 2048, False),
+])
+def test_tree_output_has_its_own_elements(rows, nodes, row, node, fine):
+    """Rows and nodes of the output that share memory would be written in any order. (The call's page size is one that is
+    refused later, so none is launched.)"""
+    import bdfp4
+    from test_tree_cpu import _tree_args
+
+    a = _tree_args()
+    a.rows, a.nodes, a.out_row_stride, a.out_node_stride, a.page_tokens = rows, nodes, row, node, 32
+    assert bdfp4.library().bdfp4_tree_decode(ctypes.byref(a), None) == (bdfp4.E_UNSUPPORTED if fine else bdfp4.E_ARG)
