@@ -224,7 +224,7 @@ def tree_decode(
     a.parents, a.parents_row_stride = _parents(parents, rows, nodes, device)
     if node_counts is not None:
         a.node_counts = _int32(node_counts, "node_counts", (rows,), device)
-    if fp4_page_table.ndim != 2:
+    if not isinstance(fp4_page_table, torch.Tensor) or fp4_page_table.ndim != 2:
         raise ValueError("fp4_page_table must be row-major INT32 with shape [rows, max_pages]")
     columns = fp4_page_table.shape[1]
     a.page_table = _int32(fp4_page_table, "fp4_page_table", (rows, columns), device)
@@ -235,7 +235,7 @@ def tree_decode(
     if query_rotation not in ROTATIONS:
         raise ValueError(f"query_rotation must be one of {list(ROTATIONS)}, got {query_rotation!r}")
     if key_shift is not None and (
-        key_shift.dtype is not torch.float32 or key_shift.device != device or not key_shift.is_contiguous()
+        not isinstance(key_shift, torch.Tensor) or key_shift.dtype is not torch.float32 or key_shift.device != device or not key_shift.is_contiguous()
         or tuple(key_shift.shape) != (heads_kv, HEAD_DIM)
     ):
         raise ValueError(f"key_shift must be contiguous FP32 [{heads_kv}, {HEAD_DIM}] on {device}")
@@ -262,12 +262,12 @@ def tree_decode(
         raise ValueError("seqused_sink needs the BF16 residual arguments")
     slots = 0
     if has_residual:
-        tail_shape = residual[0].shape
-        slots = tail_shape[0]
+        tail_shape = residual[0].shape if isinstance(residual[0], torch.Tensor) else ()
+        slots = tail_shape[0] if tail_shape else 0
         for tensor, name in ((residual[0], "residual_key_pages_bf16"), (residual[1], "residual_value_pages_bf16")):
             if (
-                tensor.dtype is not torch.bfloat16 or tensor.device != device or not tensor.is_contiguous()
-                or tensor.shape != tail_shape or len(tail_shape) != 4 or tail_shape[1] < PAGE_SIZE
+                not isinstance(tensor, torch.Tensor) or tensor.dtype is not torch.bfloat16 or tensor.device != device
+                or not tensor.is_contiguous() or tensor.shape != tail_shape or len(tail_shape) != 4 or tail_shape[1] < PAGE_SIZE
                 or tail_shape[2:] != (heads_kv, HEAD_DIM)
             ):
                 raise ValueError(f"{name} must be contiguous BF16 [slots, {PAGE_SIZE} + sink tokens, {heads_kv}, {HEAD_DIM}] "
@@ -311,7 +311,7 @@ def tree_decode(
     need = tree_workspace_bytes(rows, nodes, heads_q, heads_kv)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif (workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous()
+    elif (not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous()
           or workspace.numel() < need or workspace.data_ptr() % 16):
         raise ValueError(f"workspace must be a contiguous, 16-byte aligned uint8 buffer of at least {need} bytes on {device}")
     a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
@@ -360,7 +360,7 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, parents: tor
         raise NotImplementedError(f"a tree holds at most {MAX_TREE_NODES} nodes, got {nodes}")
     for tensor, name in ((target_probs, "target_probs"), (draft_probs, "draft_probs")):
         if tensor is not None and (
-            tensor.dtype is not target_probs.dtype or tensor.device != device or tensor.shape != target_probs.shape
+            not isinstance(tensor, torch.Tensor) or tensor.dtype is not target_probs.dtype or tensor.device != device or tensor.shape != target_probs.shape
             or (vocab > 1 and tensor.stride(2) != 1)
         ):
             raise ValueError(f"{name} must be {target_probs.dtype} [{rows}, {nodes}, {vocab}] on {device}, dense along "
@@ -423,15 +423,15 @@ class DraftCommitter:
             raise ValueError(f"sink_tokens must lie in [0, {SINK_TOKENS}], got {sink_tokens}")
         for tensor, name in ((tail_key, "tail_key"), (tail_value, "tail_value")):
             if (
-                tensor.dtype is not torch.bfloat16 or tensor.device != device or not tensor.is_contiguous()
-                or tensor.ndim != 5 or tensor.shape[2] != PAGE_SIZE + sink_tokens or tensor.shape[4] != HEAD_DIM
+                not isinstance(tensor, torch.Tensor) or tensor.dtype is not torch.bfloat16 or tensor.device != device
+                or not tensor.is_contiguous() or tensor.ndim != 5 or tensor.shape[2] != PAGE_SIZE + sink_tokens or tensor.shape[4] != HEAD_DIM
                 or tensor.shape != tail_key.shape
             ):
                 raise ValueError(f"{name} must be contiguous BF16 [layers, slots, {PAGE_SIZE + sink_tokens}, heads, 128] "
                                  f"on {device}")
         layers, slots, _, heads, _ = tail_key.shape
         if key_shift is not None and (
-            key_shift.dtype is not torch.float32 or key_shift.device != device or not key_shift.is_contiguous()
+            not isinstance(key_shift, torch.Tensor) or key_shift.dtype is not torch.float32 or key_shift.device != device or not key_shift.is_contiguous()
             or tuple(key_shift.shape) != (layers, heads, HEAD_DIM)
         ):
             raise ValueError(f"key_shift must be contiguous FP32 [{layers}, {heads}, {HEAD_DIM}] on {device}")
@@ -509,7 +509,7 @@ class DraftCommitter:
             a.part = bdfp4.COMMIT_ALL
             _launch(bdfp4.commit_drafts, a, device)
             return CommittedLengths(*lengths.unbind())
-        if block_table.ndim != 2:
+        if not isinstance(block_table, torch.Tensor) or block_table.ndim != 2:
             raise ValueError("block_table must be row-major INT32 with shape [rows, columns]")
         columns = block_table.shape[1]
         a.page_table = _int32(block_table, "block_table", (rows, columns), device)

@@ -262,3 +262,31 @@ def test_outputs_that_share_memory_are_refused():
 
 def _like(t):
     return torch.zeros(4096, dtype=torch.bfloat16, device="cuda").as_strided(t.shape, t.stride())
+
+
+def test_what_is_no_tensor_is_refused_as_such():
+    from nvfp4_decode_kernel import tree
+
+    w, x = _tree_inputs([20, 300], 3, 4, 2, seed=83)
+    device = {k: v.cuda() for k, v in x.items()}
+    args = [device["query"], device["draft_key"], device["draft_value"], device["parents"], *w.regions, w.page_table, w.seqused_fp4]
+    tail = dict(residual_key_pages_bf16=w.tail_key[0], residual_value_pages_bf16=w.tail_value[0],
+                residual_page_ids=w.slot_ids, seqused_residual=w.seqused_residual)
+    for at in range(len(args)):
+        with pytest.raises(ValueError):
+            tree.tree_decode(*args[:at], None, *args[at + 1:], **tail)
+    for name in (*tail, "key_shift", "workspace", "out", "node_counts", "seqused_sink", "error_word"):
+        with pytest.raises(ValueError):
+            tree.tree_decode(*args, **{**tail, name: [1]})
+    probs, tokens = torch.full((2, 3, 8), 0.125, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    uniforms = torch.rand(2, 3, device="cuda")
+    for change in (dict(tokens=None), dict(parents=[0]), dict(uniforms=None), dict(draft_probs=[1])):
+        with pytest.raises(ValueError):
+            tree.verify_drafts(**{**dict(target_probs=probs, tokens=tokens, parents=tokens, uniforms=uniforms), **change})
+    s = _setup(2, 1, 3, 2, [3, 4], [2, 2], seed=84)
+    key, value = s["tail_key"].cuda(), s["tail_value"].cuda()
+    for change in (dict(tail_value=None), dict(key_shift=[0.0])):
+        with pytest.raises(ValueError):
+            tree.DraftCommitter(**{**dict(tail_key=key, tail_value=value), **change})
+    with pytest.raises(ValueError):
+        _commit(s, True, block_table=[1])
