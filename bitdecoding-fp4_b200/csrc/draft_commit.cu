@@ -3,7 +3,7 @@
 // Token p of a sequence lives at row p % 128 of its slot's rolling page, so the a accepted nodes of a row of
 // n committed tokens go to rows n % 128 .. (n + a - 1) % 128: a gather of whole K/V rows by node number, with
 // K brought into the cache's basis on the way. Bound by HBM (2 x 512 bytes read and written per token and
-// head; 64 rows x 32 layers x 8 heads of up to 16 tokens: 26 us, 0.84 of a plain copy's rate), or by the launch for
+// head; 64 rows x 32 layers x 8 heads of up to 16 tokens: 27 us, 0.81 of a plain copy's rate), or by the launch for
 // small batches. At most 64 nodes make at most one page boundary per row; the
 // page that fills is sealed by the page writers between a HEAD and a REST call, since the tokens behind the
 // boundary reuse the rows that the seal still has to read.

@@ -7,8 +7,8 @@
 //
 // Thread r (of 128, twice: each half has half of the channels, tokens or queries) owns token r of S^T and channel r
 // of V. A step: its scores into registers (the next step's are taken meanwhile), its half of V into tensor memory,
-// the vote, the exponentials, P. Now (same case) 325 us, 3.7 TB/s of FP4 cache, 0.57 of a plain copy's rate: 1500
-// cycles a step and SM of which the tensor cores work 15% and the schedulers issue half. What bounds it is the chain
+// the vote, the exponentials, P. Now (same case, by box) 321 to 370 us, 3.3 to 3.8 TB/s of FP4 cache, 0.50 to 0.58 of a
+// plain copy's rate: some 1500 cycles a step and SM of which the tensor cores work 15% and the schedulers issue half. What bounds it is the chain
 // of a step's waits (scores, output, vote; 150 to 250 cycles each), of which an SM has only two to overlap; a third
 // CTA's operands do not fit the tensor memory.
 #pragma once

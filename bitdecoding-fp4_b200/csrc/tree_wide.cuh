@@ -1,9 +1,10 @@
 // The tree attention for tiles of 64 to 128 queries: warps of one role each, one CTA per SM. A step's values are
 // converted once for up to 128 queries, so what bounds it is the softmax: 128 x NT exponentials (8 cycles a step and
 // query on an SM) and their surroundings, up to four groups of 128 threads with at most 32 queries per thread. One
-// row of 262145 tokens under 256 query rows per KV head takes 367 us, 750 TFLOP/s of FP16 products or 0.47 of a
-// library product's rate: 2750 cycles a step of 128 queries, tensor cores 31% busy, issue slots 60%. With 64 queries
-// (16 rows x 16 nodes, up to 8192) 82 us; by two CTAs per SM (tree_narrow.cuh's form) 120.
+// row of 262145 tokens under 256 query rows per KV head takes 418 to 425 us, 650 TFLOP/s of FP16 products or 0.41 of a
+// library product's rate: tensor cores 31% busy, issue slots 57%. (Before scores of any magnitude were served, 403 to
+// 420 on the same boxes, and 367 on another: 2750 cycles a step of 128 queries.) With 64 queries (16 rows x 16 nodes, up
+// to 8192) 87 us; by two CTAs per SM (tree_narrow.cuh's form) 120.
 #pragma once
 
 #include "tree_common.cuh"
