@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import tree_oracle as oracle
-from test_gpu_tree_decode import _call, _inputs
+from test_gpu_tree_decode import _call, _check, _inputs
 from test_gpu_tree_edges import _check_needles, _needles
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +41,28 @@ def test_single_tokens_are_found(lens, nodes, heads, page_tokens):
     w, _ = _inputs(lens, 1, *heads, seed=92, page_tokens=page_tokens)
     x, want = _needles(w, nodes, heads[0], 93, 16.0)
     _check_needles(_call(w, x), want)
+
+
+@pytest.mark.parametrize("lens,nodes,heads,page_tokens", CASES)
+def test_single_tokens_at_any_magnitude(lens, nodes, heads, page_tokens):
+    """Each query by a power of two of its own: quiet beside loud in every tile, scores beyond 2^27 next to ordinary ones,
+    in rows that straddle CTAs and in CTAs that hold many units."""
+    w, _ = _inputs(lens, 1, *heads, seed=94, page_tokens=page_tokens)
+    x, want = _needles(w, nodes, heads[0], 95, 16.0)
+    power = torch.randint(0, 4, x["query"].shape[:3], generator=torch.Generator().manual_seed(96))
+    by = torch.tensor([1.0, 2.0 ** 9, 2.0 ** 26, 2.0 ** 70], dtype=torch.float64)[power]
+    x["query"] = (x["query"].double() * by[..., None]).to(torch.bfloat16)
+    _check_needles(_call(w, x), want)
+
+
+@pytest.mark.parametrize("nodes,heads", [(3, (8, 2)), (7, (8, 2)), (15, (8, 2)), (22, (8, 2)), (31, (8, 2))])
+@pytest.mark.parametrize("page_tokens", [128, 64])
+def test_many_units_per_cta_some_with_loud_queries(nodes, heads, page_tokens):
+    """Hundreds of short units, so that a CTA goes from tiles of one scale to uneven ones and back."""
+    lens = [1 + (211 * i) % 520 for i in range(220)]
+    w, x = _inputs(lens, nodes, *heads, seed=97, page_tokens=page_tokens)
+    loud = x["query"].double()
+    loud[::3, nodes // 2] *= 2.0 ** 20
+    loud[1::5, 0, 1] *= 2.0 ** -20
+    x["query"] = loud.to(torch.bfloat16)
+    _check(w, x, _call(w, x), rows=range(0, 220, 7))
