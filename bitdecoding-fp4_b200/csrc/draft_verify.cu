@@ -7,9 +7,9 @@
 // FP64: acceptance and the drawn index are decisions next to borders, and at 4 to 8 bytes read per value the
 // FP64 adds (64 per clock and SM) stay well under the time of the reads.
 //
-// Small batches are bound by the launch (8 us on the device); 32 rows x 131072 with a drafter take 28 to 31 us, five
-// to six times the reads' time: what counts is the chain of a cluster's passes, one per refusal, each a read, a reduction and an
-// exchange.
+// Small batches are bound by the launch (8 us on the device); 32 rows x 131072 with a drafter take 28 to 31 us, five to
+// six times the reads' time: what counts is the chain of a cluster's passes, one per refusal, each a read, a reduction
+// and an exchange.
 //
 // A row is one cluster of CTAs that share the vocabulary; every CTA does the same walk from the same
 // numbers, and the passes' sums are exchanged through distributed shared memory. A CTA may only store into

@@ -8,9 +8,9 @@
 // Thread r (of 128, twice: each half has half of the channels, tokens or queries) owns token r of S^T and channel r
 // of V. A step: its scores into registers (the next step's are taken meanwhile), its half of V into tensor memory,
 // the vote, the exponentials, P. Now (same case, by box) 321 to 370 us, 3.3 to 3.8 TB/s of FP4 cache, 0.50 to 0.58 of a
-// plain copy's rate: some 1500 cycles a step and SM of which the tensor cores work 15% and the schedulers issue half. What bounds it is the chain
-// of a step's waits (scores, output, vote; 150 to 250 cycles each), of which an SM has only two to overlap; a third
-// CTA's operands do not fit the tensor memory.
+// plain copy's rate: some 1500 cycles a step and SM of which the tensor cores work 15% and the schedulers issue half.
+// What bounds it is the chain of a step's waits (scores, output, vote; 150 to 250 cycles each), of which an SM has only
+// two to overlap; a third CTA's operands do not fit the tensor memory.
 #pragma once
 
 #include "tree_common.cuh"
@@ -183,7 +183,7 @@ __device__ __forceinline__ void work(const TreeParams& p, Smem<NT>& sm, Walker w
     bool uneven;
     const float q_inverse = load_queries<NT, kWorkers>(p, sm, kWorkBarrier, u, thread, uneven);
     if (t < C) {
-      sm.level[first_column + t] = query_level(sm.own[first_column + t], q_inverse);
+      if (uneven) sm.level[first_column + t] = query_level(sm.own[first_column + t], q_inverse);
       top[t] = kNoMax;
       base[t] = 0.0f;  // scores as they are
     }

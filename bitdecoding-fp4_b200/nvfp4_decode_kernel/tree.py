@@ -302,12 +302,14 @@ def tree_decode(
     if out is None:
         make = torch.empty if node_counts is None else torch.zeros
         out = make(shape, dtype=torch.bfloat16, device=device)
-    a.out, a.out_row_stride, a.out_node_stride = _tree_tensor(out, "out", shape, device)
+    a.out, by_row, by_node = _tree_tensor(out, "out", shape, device)
     extent = heads_q * HEAD_DIM
-    for stride, size in sorted(((a.out_row_stride, rows), (a.out_node_stride, nodes))):
-        if size > 1 and stride < extent:
-            raise ValueError("out must have an element of its own for every result")
-        extent += stride * (size - 1)
+    if by_node < extent or by_row < (nodes - 1) * by_node + extent:  # not rows of nodes: nodes of rows, or they overlap
+        for stride, size in sorted(((by_row, rows), (by_node, nodes))):
+            if size > 1 and stride < extent:
+                raise ValueError("out must have an element of its own for every result")
+            extent += stride * (size - 1)
+    a.out_row_stride, a.out_node_stride = by_row, by_node
     need = tree_workspace_bytes(rows, nodes, heads_q, heads_kv)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
